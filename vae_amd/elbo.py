@@ -20,6 +20,14 @@ def nll(x, recon_x, nll_type):
     return F_.nll(x, recon_x, nll_type)
 
 
+def distillation(recon_x, teacher_logits, teacher_ids, temperature=1.0):
+    """[B] distillation term of a categorical decoder: sum over each sample's positions of the KL from the teacher's top
+    logits to softmax(recon_x / temperature) (functional.distill_top_logits), in recon_x's dtype.  Meant for
+    loss_function's extra loss terms: loss_function(recon_x, x, params, distill=distillation(...))."""
+    kl, _ = F_.distill_top_logits(recon_x, teacher_logits, teacher_ids, temperature, fuse_backward=False)
+    return F_.sample_sums(kl, recon_x.dtype)
+
+
 def _pack(loss, elbo, means, kl_beta, dtype):
     means = means.to(dtype)
     return {

@@ -334,7 +334,10 @@ def _flat_pixels(x, recon, nll_type):
 
 
 def nll(x, recon_x, nll_type):
-    """Per-sample negative log-likelihood [B] (abstract_vae.py:461-471; definitions: oracle/cpu_ref.py)."""
+    """Per-sample negative log-likelihood [B] (abstract_vae.py:461-471; definitions: oracle/cpu_ref.py).
+    nll_type 'categorical': x holds integer tokens [B, ...] (negative: padding), recon_x their logits [B, ..., V]."""
+    if _is_categorical(nll_type):
+        return _TokenNllElbo.apply(*_token_rows(x, recon_x), None, None, None, 0.0, 0.0, False, False)[0]
     code, xf, rf = _flat_pixels(x, recon_x, nll_type)
     return _NllElbo.apply(xf, rf, None, None, None, code, 0.0, 0.0, False)[0]
 
@@ -343,7 +346,17 @@ def nll_elbo(x, recon_x, nll_type, kld=None, add=None, mi=None, kl_beta=1.0, inv
     """Fused nll + ELBO combine: returns (nll, loss, elbo) [B] and means float32[6]
     ordered (loss, elbo, nll, kld, additional, mut_info).  abstract_vae.py:344-388 with K == 1.
     `fuse_backward`: also form d(loss_mean)/d(recon) in the same pass (one read of x and recon per training
-    step instead of two); results are identical, the gradient buffer is simply allocated a step earlier."""
+    step instead of two); results are identical, the gradient buffer is simply allocated a step earlier.
+    nll_type 'categorical': integer tokens and logits, as in nll()."""
+    if _is_categorical(nll_type):
+        rows, tokens, B = _token_rows(x, recon_x)
+        if inv_count is None:
+            inv_count = 1.0 / max(B, 1)
+        # fp16: two passes, for the reason given below
+        fuse = (fuse_backward and rows.dtype != torch.float16 and rows.requires_grad and torch.is_grad_enabled()
+                and rows.numel() > 0)
+        kld, add, mi = (None if t is None else t.to(rows.dtype).contiguous() for t in (kld, add, mi))
+        return _TokenNllElbo.apply(rows, tokens, B, kld, add, mi, float(kl_beta), float(inv_count), True, fuse)
     code, xf, rf = _flat_pixels(x, recon_x, nll_type)
     if inv_count is None:
         inv_count = 1.0 / max(xf.shape[0], 1)
@@ -497,6 +510,333 @@ def categorical_kl(log_q, log_p):
     """sum softmax(q) * (log_softmax(q) - log_softmax(p)) over the last dim (gumbel.py:222-254)."""
     shape = log_q.shape[:-1]
     return _CategoricalKL.apply(_rows(log_q), _rows(log_p.expand_as(log_q))).reshape(shape)
+
+
+# --------------------------------------------------------------------------------------
+# Categorical observations: tokens of a vocabulary (no reference counterpart: its likelihoods are
+# Bernoulli, Gaussian and the discretized logistic, abstract_vae.py:461-471)
+# --------------------------------------------------------------------------------------
+MAX_TOP = 64        # VAE_MAX_TOP in include/vae_amd.h
+MAX_TEACHER = 256   # VAE_MAX_TEACHER
+
+
+def _is_categorical(nll_type):
+    return nll_type.strip().lower() == 'categorical'
+
+
+def _id_bytes(t, what):
+    if t.dtype == torch.int64:
+        return 8
+    if t.dtype == torch.int32:
+        return 4
+    raise TypeError("%s: ids must be int32 or int64, got %s" % (what, t.dtype))
+
+
+def _vocab_rows(logits, what):
+    if logits.dim() < 1 or logits.shape[-1] < 1:
+        raise ValueError("%s: logits need a last dimension over the vocabulary, got %s" % (what, tuple(logits.shape)))
+    return _rows(logits)
+
+
+def _token_rows(x, recon):
+    """(logits rows [B*T, V], tokens [B*T], B) of tokens x [B, ...] and their logits recon [B, ..., V]."""
+    _id_bytes(x, "nll 'categorical'")
+    if x.dim() < 1 or recon.dim() < 2 or recon.shape[0] != x.shape[0] or recon.shape[:-1].numel() != x.numel():
+        raise ValueError("nll 'categorical': logits %s do not fit tokens %s (a last dimension over the vocabulary)"
+                         % (tuple(recon.shape), tuple(x.shape)))
+    return _vocab_rows(recon, "nll 'categorical'"), x.reshape(-1).contiguous(), x.shape[0]
+
+
+def _row_sums(rows, scale, B, dtype):
+    """[B] = scale * sum over each of B equal runs of `rows` (fp32, summed in double)."""
+    out = torch.empty((B,), dtype=dtype, device=rows.device)
+    call('vae_row_sums', ptr(rows), scale, ptr(out), B, rows.numel() // max(B, 1), dtype_code(out),
+         stream_ptr(rows.device))
+    return out
+
+
+class _TokenLogProbs(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, tokens, top_k, want_entropy):
+        ctx.set_materialize_grads(False)
+        logp, entropy, top, ids, stats = _token_fwd(logits, tokens, top_k, want_entropy, True)
+        ctx.save_for_backward(logits, tokens, entropy, ids, stats)
+        outs, nd = [], []
+        for t in (logp, entropy, top, ids):
+            if t is None:
+                t = logits.new_empty((0,))
+                nd.append(t)
+            outs.append(t)
+        if ids is not None:
+            nd.append(ids)
+        if nd:
+            ctx.mark_non_differentiable(*nd)
+        return tuple(outs)
+
+    @staticmethod
+    def backward(ctx, glogp, gentropy, gtop, gids):
+        logits, tokens, entropy, ids, stats = ctx.saved_tensors
+        glogp = None if tokens is None else glogp
+        gentropy = None if entropy is None else gentropy
+        gtop = None if ids is None else gtop
+        if glogp is None and gentropy is None and gtop is None:
+            return None, None, None, None
+        return _token_bwd(logits, None if glogp is None else tokens, tokens, entropy, ids, stats, _dense(glogp), 1, 1.0,
+                          _dense(gentropy), _dense(gtop)), None, None, None
+
+
+def _token_fwd(logits, tokens, top_k, want_entropy, want_stats):
+    dev = check_device(logits, tokens)
+    N, V = logits.shape
+    new = lambda *s: torch.empty(s, dtype=torch.float32, device=dev)
+    logp = new(N) if tokens is not None else None
+    entropy = new(N) if want_entropy else None
+    stats = new(N, 2) if want_stats else None
+    top = new(N, top_k) if top_k else None
+    ids = torch.empty((N, top_k), dtype=torch.int64, device=dev) if top_k else None
+    with _Guard(dev):
+        call('vae_token_logp_fwd', ptr(logits), logits.stride(0), ptr(tokens),
+             0 if tokens is None else tokens.element_size(), ptr(logp), ptr(entropy), ptr(stats), ptr(top), ptr(ids),
+             top_k, N, V, dtype_code(logits), stream_ptr(dev))
+    return logp, entropy, top, ids, stats
+
+
+def token_log_probs(logits, tokens=None, top_k=0, want_entropy=True):
+    """logits [..., V], tokens [...] (int32 / int64) -> (log_prob [...], entropy [...], top_log_probs [..., top_k],
+    top_ids [..., top_k] int64) of softmax(logits), float32, in one read of the logits; an output that is not asked for
+    (tokens None, want_entropy False, top_k 0) is None.  The alternatives are the top_k <= 64 largest entries, by value,
+    ties by the lower id.  log_prob, entropy and top_log_probs are differentiable with respect to the logits.
+
+    A negative token marks a padded row: its logits are not read; log_prob 0, entropy 0, alternatives -inf / -1,
+    gradient 0.  A token beyond the vocabulary gives NaN (log_prob and the row's gradient).  Logits of -inf are masked
+    out; a row of nothing else has log_prob -inf, entropy 0 and gradient 0."""
+    shape = logits.shape[:-1]
+    rows = _vocab_rows(logits, 'token_log_probs')
+    top_k = int(top_k)
+    if not 0 <= top_k <= min(MAX_TOP, rows.shape[1]):
+        raise ValueError("token_log_probs: top_k must be in 0..min(%d, V = %d), got %d"
+                         % (MAX_TOP, rows.shape[1], top_k))
+    if tokens is not None:
+        _id_bytes(tokens, 'token_log_probs')
+        if tokens.shape != shape:
+            raise ValueError("token_log_probs: tokens %s do not fit logits %s"
+                             % (tuple(tokens.shape), tuple(logits.shape)))
+        tokens = tokens.reshape(-1).contiguous()
+    want_entropy = bool(want_entropy)
+    if rows.requires_grad and torch.is_grad_enabled():
+        logp, entropy, top, ids = _TokenLogProbs.apply(rows, tokens, top_k, want_entropy)
+    else:
+        logp, entropy, top, ids, _ = _token_fwd(rows, tokens, top_k, want_entropy, False)
+    return (logp.reshape(shape) if tokens is not None else None, entropy.reshape(shape) if want_entropy else None,
+            top.reshape(shape + (top_k,)) if top_k else None, ids.reshape(shape + (top_k,)) if top_k else None)
+
+
+class _TokenNllElbo(torch.autograd.Function):
+    """Categorical nll [B] of B samples with T tokens each, with the ELBO combine (with_elbo) and d(loss_mean)/d(logits)
+    out of the same launch (fuse), as in _NllElboFused."""
+
+    @staticmethod
+    def forward(ctx, logits, tokens, B, kld, add, mi, kl_beta, inv_count, with_elbo, fuse):
+        ctx.set_materialize_grads(False)
+        dev = check_device(logits, tokens, kld, add, mi)
+        N, V = logits.shape
+        code, st = dtype_code(logits), stream_ptr(dev)
+        rows = torch.empty((N,), dtype=torch.float32, device=dev)
+        stats = torch.empty((N, 2), dtype=torch.float32, device=dev)
+        grad = torch.empty((N, V), dtype=logits.dtype, device=dev) if fuse else None
+        loss = elbo = means = None
+        with _Guard(dev):
+            if fuse:
+                call('vae_token_nll_fused', ptr(logits), logits.stride(0), ptr(tokens), tokens.element_size(), ptr(rows),
+                     ptr(stats), ptr(grad), inv_count, N, V, code, st)
+            else:
+                call('vae_token_logp_fwd', ptr(logits), logits.stride(0), ptr(tokens), tokens.element_size(), ptr(rows),
+                     None, ptr(stats), None, None, 0, N, V, code, st)
+            nll = _row_sums(rows, -1.0, B, logits.dtype)
+            if with_elbo:
+                loss, elbo = torch.empty_like(nll), torch.empty_like(nll)
+                means = _scalars(6, dev, B)
+                call('vae_elbo_combine_fwd', ptr(nll), ptr(kld), ptr(add), ptr(mi), kl_beta, inv_count, ptr(loss),
+                     ptr(elbo), ptr(means), ptr(workspace(dev)), B, code, st)
+        ctx.save_for_backward(logits, tokens, stats)
+        ctx.grad = grad
+        ctx.cfg = (B, kl_beta, inv_count, kld is not None, add is not None, mi is not None)
+        if not with_elbo:
+            loss, elbo, means = nll.new_empty((0,)), nll.new_empty((0,)), rows.new_empty((0,))
+            ctx.mark_non_differentiable(loss, elbo, means)
+        return nll, loss, elbo, means
+
+    @staticmethod
+    def backward(ctx, gnll, gloss, gelbo, gmeans):
+        logits, tokens, stats = ctx.saved_tensors
+        B, kl_beta, inv_count, has_kld, has_add, has_mi = ctx.cfg
+        dev = logits.device
+        need = [ctx.needs_input_grad[i] and has for i, has in ((3, has_kld), (4, has_add), (5, has_mi))]
+        gmeans = None if gmeans is None else gmeans.contiguous().float()
+        grad, ctx.grad = ctx.grad, None
+        with _Guard(dev):
+            if gnll is None and gloss is None and gelbo is None and gmeans is not None and grad is not None:
+                terms = [torch.empty((B,), dtype=logits.dtype, device=dev) if n else None for n in need]
+                call('vae_nll_fused_backward', ptr(grad), grad.numel(), ptr(gmeans), kl_beta, inv_count, ptr(terms[0]),
+                     ptr(terms[1]), ptr(terms[2]), B, dtype_code(logits), stream_ptr(dev))
+            else:
+                # the per-sample upstream gradient is formed in fp32: 1/B of a mean is a subnormal of fp16
+                f32 = lambda t: None if t is None else t.contiguous().float()
+                gloss, gelbo = f32(gloss), f32(gelbo)
+                g = torch.empty((B,), dtype=torch.float32, device=dev)
+                terms = [torch.empty_like(g) if n else None for n in need]
+                call('vae_elbo_combine_bwd', ptr(gloss), ptr(gelbo), ptr(gmeans), kl_beta, inv_count, ptr(g),
+                     ptr(terms[0]), ptr(terms[1]), ptr(terms[2]), B, _lib.VAE_F32, stream_ptr(dev))
+                if gnll is not None:
+                    g = g + f32(gnll)
+                terms = [None if t is None else t.to(logits.dtype) for t in terms]
+                grad = None
+                if ctx.needs_input_grad[0]:
+                    grad = _token_bwd(logits, tokens, tokens, None, None, stats, g, tokens.numel() // max(B, 1), -1.0,
+                                      None, None)
+        return (grad, None, None) + tuple(terms) + (None, None, None, None)
+
+
+def _token_bwd(logits, g_tokens, tokens, entropy, ids, stats, glogp, rows_per_g, g_scale, gentropy, gtop):
+    """d(logits).  `tokens` says which rows are padding; `g_tokens` is None when no gradient reached their log probs."""
+    dev = logits.device
+    N, V = logits.shape
+    grad = torch.empty((N, V), dtype=logits.dtype, device=dev)
+    if g_tokens is None and tokens is not None:
+        glogp, rows_per_g, g_scale = torch.zeros((1,), dtype=torch.float32, device=dev), max(N, 1), 0.0
+    with _Guard(dev):
+        call('vae_token_logp_bwd', ptr(logits), logits.stride(0), ptr(tokens),
+             0 if tokens is None else tokens.element_size(), ptr(stats), ptr(entropy), ptr(glogp), max(rows_per_g, 1),
+             g_scale, ptr(gentropy), ptr(gtop), ptr(ids) if gtop is not None else None,
+             ids.shape[1] if gtop is not None else 0, ptr(grad), N, V, dtype_code(logits), stream_ptr(dev))
+    return grad
+
+
+def _token_steps_elbo(xs, recons, kld, add, mi, kl_beta, inv_count, with_lse):
+    """nll_steps_elbo for nll_type 'categorical': one scoring launch per step, one combine over the T*B entries."""
+    T, B = len(recons), recons[0].shape[0]
+    if isinstance(kl_beta, (list, tuple)):
+        if len(kl_beta) != T:
+            raise ValueError("nll_steps_elbo: %d KL weights for %d steps" % (len(kl_beta), T))
+        if any(float(b) != float(kl_beta[0]) for b in kl_beta):
+            raise NotImplementedError("nll_steps_elbo: 'categorical' takes one KL weight for all steps (a host model "
+                                      "with an annealer scores its steps one by one: vae_amd.vrnn.loss_function)")
+        kl_beta = kl_beta[0]
+    for name, v in (('kld', kld), ('add', add), ('mi', mi)):
+        if v is not None and v.numel() != T * B:
+            raise ValueError("nll_steps_elbo: %s must hold T*B = %d values, got %d" % (name, T * B, v.numel()))
+    nll_ = torch.cat([nll(x, r, 'categorical') for x, r in zip(xs, recons)], 0)
+    if nll_.numel() != T * B:
+        raise ValueError("nll_steps_elbo: every step must have the same shapes and dtype")
+    loss, elbo, means = elbo_combine(nll_, kld=kld, add=add, mi=mi, kl_beta=float(kl_beta),
+                                     inv_count=1.0 / max(T * B, 1) if inv_count is None else inv_count)
+    out = (nll_, loss, elbo, means, loss.view(T, B).mean(0), elbo.view(T, B).mean(0))
+    return out + (torch.logsumexp(elbo.detach().view(T, B), 0),) if with_lse else out
+
+
+class _Distill(torch.autograd.Function):
+    """kl [N] and mean = inv_count * sum(kl); fuse: d(mean)/d(logits) out of the forward launch, handed out by
+    backward() when only the mean's gradient arrives (rescaled on the device when that is not 1)."""
+
+    @staticmethod
+    def forward(ctx, logits, teacher, ids, temperature, inv_count, fuse):
+        ctx.set_materialize_grads(False)
+        kl, mean, stats, grad = _distill_fwd(logits, teacher, ids, temperature, inv_count, True, fuse)
+        ctx.save_for_backward(logits, teacher, ids, stats)
+        ctx.grad = grad
+        ctx.cfg = (temperature, inv_count)
+        return kl, mean
+
+    @staticmethod
+    def backward(ctx, gkl, gmean):
+        if gkl is None and gmean is None:
+            return (None,) * 6
+        logits, teacher, ids, stats = ctx.saved_tensors
+        temperature, inv_count = ctx.cfg
+        dev = logits.device
+        N, V = logits.shape
+        grad, ctx.grad = ctx.grad, None
+        gkl, gmean = _dense(gkl), _dense(gmean)
+        with _Guard(dev):
+            if gkl is None and grad is not None:
+                call('vae_grad_scale', ptr(grad), ptr(gmean), grad.numel(), dtype_code(grad), stream_ptr(dev))
+            else:
+                grad = torch.empty((N, V), dtype=logits.dtype, device=dev)
+                call('vae_distill_bwd', ptr(logits), logits.stride(0), ptr(teacher), teacher.stride(0),
+                     dtype_code(teacher), ptr(ids), ids.stride(0), ids.element_size(), ids.shape[1], temperature,
+                     ptr(stats), ptr(gkl), ptr(gmean), inv_count, ptr(grad), N, V, dtype_code(logits), stream_ptr(dev))
+        return grad, None, None, None, None, None
+
+
+def _distill_fwd(logits, teacher, ids, temperature, inv_count, want_stats, fuse):
+    dev = check_device(logits, teacher, ids)
+    N, V = logits.shape
+    kl = torch.empty((N,), dtype=torch.float32, device=dev)
+    stats = torch.empty((N, 2), dtype=torch.float32, device=dev) if want_stats else None
+    grad = torch.empty((N, V), dtype=logits.dtype, device=dev) if fuse else None
+    with _Guard(dev):
+        call('vae_distill_fwd', ptr(logits), logits.stride(0), ptr(teacher), teacher.stride(0), dtype_code(teacher),
+             ptr(ids), ids.stride(0), ids.element_size(), ids.shape[1], temperature, ptr(kl), ptr(stats), ptr(grad),
+             inv_count, N, V, dtype_code(logits), stream_ptr(dev))
+        mean = _row_sums(kl, inv_count, 1, torch.float32).reshape(())
+    return kl, mean, stats, grad
+
+
+def distill_top_logits(logits, teacher_logits, teacher_ids, temperature=1.0, inv_count=None, fuse_backward=True):
+    """Distillation from a teacher's K <= 256 largest logits: student logits [..., V], teacher_logits [..., K] and
+    teacher_ids [..., K] (int32 / int64) -> (kl [...], mean), float32:  kl = sum_k q_k (ln q_k - ln p[id_k]),
+    q = softmax(teacher_logits / temperature) over the K entries, p = softmax(logits / temperature) over the vocabulary;
+    mean = inv_count * sum(kl), inv_count = 1 / rows unless given (1 / unpadded rows, times temperature^2 where the
+    loss is to be weighted so).  Differentiable with respect to `logits` only.
+
+    A negative id or a teacher logit of -inf is no entry; a row without entries has kl 0 and gradient 0 and is not read;
+    an id may come twice; an id beyond the vocabulary gives NaN.  `fuse_backward`: d(mean)/d(logits) is formed by the
+    forward launch (one read of the logits per step instead of two); a gradient on `kl` takes the general kernel."""
+    shape = logits.shape[:-1]
+    rows = _vocab_rows(logits, 'distill_top_logits')
+    _id_bytes(teacher_ids, 'distill_top_logits')
+    if teacher_logits.shape != teacher_ids.shape or teacher_ids.shape[:-1] != shape or teacher_ids.dim() < 1:
+        raise ValueError("distill_top_logits: teacher logits %s / ids %s do not fit logits %s"
+                         % (tuple(teacher_logits.shape), tuple(teacher_ids.shape), tuple(logits.shape)))
+    if not 1 <= teacher_ids.shape[-1] <= MAX_TEACHER:
+        raise ValueError("distill_top_logits: 1..%d teacher logits a row, got %d" % (MAX_TEACHER, teacher_ids.shape[-1]))
+    temperature = float(temperature)
+    if not 0.0 < temperature < float('inf'):
+        raise ValueError("distill_top_logits: temperature must be positive and finite, got %r" % temperature)
+    if teacher_logits.requires_grad and torch.is_grad_enabled():
+        raise ValueError("distill_top_logits: no gradient is formed for the teacher; pass teacher_logits.detach()")
+    teacher, ids = _rows(teacher_logits), _rows(teacher_ids)
+    inv_count = 1.0 / max(rows.shape[0], 1) if inv_count is None else float(inv_count)
+    if rows.requires_grad and torch.is_grad_enabled():
+        # fp16: two passes, for the reason given in nll_elbo
+        fuse = bool(fuse_backward) and rows.dtype != torch.float16 and rows.numel() > 0
+        kl, mean = _Distill.apply(rows, teacher, ids, temperature, inv_count, fuse)
+    else:
+        kl, mean, _, _ = _distill_fwd(rows, teacher, ids, temperature, inv_count, False, False)
+    return kl.reshape(shape), mean
+
+
+class _SampleSums(torch.autograd.Function):
+    """[B] sums of B equal runs of float32 row values, in `dtype`."""
+
+    @staticmethod
+    def forward(ctx, rows, B, dtype):
+        dev = check_device(rows)
+        ctx.n = rows.numel()
+        with _Guard(dev):
+            return _row_sums(rows, 1.0, B, dtype)
+
+    @staticmethod
+    def backward(ctx, g):
+        B = g.shape[0]
+        return g.float()[:, None].expand(B, ctx.n // max(B, 1)).reshape(-1), None, None
+
+
+def sample_sums(rows, dtype=torch.float32):
+    """Per-sample totals [B] of float32 per-position values [B, ...] (token_log_probs, distill_top_logits), in `dtype`."""
+    if rows.dtype != torch.float32:
+        raise TypeError("sample_sums takes float32 row values, got %s" % rows.dtype)
+    return _SampleSums.apply(rows.reshape(-1).contiguous(), rows.shape[0], dtype)
 
 
 # --------------------------------------------------------------------------------------
@@ -1107,8 +1447,18 @@ MAX_SAMPLES = 8  # VAE_MAX_SAMPLES in include/vae_amd.h
 def nll_multi_elbo(x, recons, nll_type, kld=None, add=None, mi=None, kl_beta=1.0, inv_count=None, with_elbo=True):
     """nll [B] = mean over the S decoder outputs in `recons` of nll(x, recon_s) (abstract_vae.py:344-354), fused
     with the ELBO combine (:356-388).  Returns (nll, loss, elbo, means[6]); x is read once per launch.
-    More than MAX_SAMPLES outputs: one launch per group, the group NLLs averaged, then the combine kernel."""
+    More than MAX_SAMPLES outputs: one launch per group, the group NLLs averaged, then the combine kernel.
+    nll_type 'categorical': one launch per output, then the same."""
     S = len(recons)
+    if _is_categorical(nll_type):
+        total = None
+        for r in recons:
+            part = nll(x, r, nll_type) / S
+            total = part if total is None else total + part
+        if not with_elbo:
+            return total, None, None, None
+        loss, elbo, means = elbo_combine(total, kld=kld, add=add, mi=mi, kl_beta=kl_beta, inv_count=inv_count)
+        return total, loss, elbo, means
     flat = [_flat_pixels(x, r, nll_type) for r in recons]
     code, xf = flat[0][0], flat[0][1]
     rfs = [f[2] for f in flat]
@@ -1195,6 +1545,8 @@ def nll_steps_elbo(xs, recons, nll_type, kld=None, add=None, mi=None, kl_beta=1.
     posterior per sample, AbstractVAE.likelihood's estimate (abstract_vae.py:301-315)."""
     T = len(recons)
     assert 1 <= T <= MAX_STEPS and len(xs) == T
+    if _is_categorical(nll_type):
+        return _token_steps_elbo(xs, recons, kld, add, mi, kl_beta, inv_count, with_lse)
     flat = [_flat_pixels(x, r, nll_type) for x, r in zip(xs, recons)]
     code = flat[0][0]
     xf, rf = [f[1] for f in flat], [f[2] for f in flat]

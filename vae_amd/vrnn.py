@@ -129,7 +129,8 @@ def loss_function(reparameterizer, config, recon_x, x, params, K=1, kl_beta=None
     VRNNMixin-style host object) supplies kld / mut_info / compute_kl_beta and they are called once per step, in step
     order; without a model the same terms come from `config` (`kl_beta`: one float or T floats overrides
     config['kl_beta']).  The T steps are then scored by ONE launch pair over [T*B] rows that reads the T tensors where
-    they are.  A model that overrides `nll`, or T > 128 steps, takes the reference's own per-step loop."""
+    they are.  A model that overrides `nll`, T > 128 steps or a 'categorical' likelihood take the reference's own per-step
+    loop."""
     assert len(recon_x) == len(params)
     assert K == 1, "Monte carlo sampling for decoding not implemented for VRNN"
     T = len(recon_x)
@@ -137,7 +138,7 @@ def loss_function(reparameterizer, config, recon_x, x, params, K=1, kl_beta=None
         x = [x for _ in range(T)]
         if additive:
             recon_x = [recon_x[-1] for _ in range(T)]
-    if model is not None and (T > F_.MAX_STEPS or model._own_nll()):
+    if model is not None and (T > F_.MAX_STEPS or model._own_nll() or F_._is_categorical(config['nll_type'])):
         return vrnn_loss_function([ELBOMixin.loss_function(model, r, xi, p, K=K) for r, xi, p in zip(recon_x, x, params)])
     B = recon_x[0].shape[0]
     klds, mis, betas = [], [], []
@@ -177,8 +178,11 @@ def loss_function(reparameterizer, config, recon_x, x, params, K=1, kl_beta=None
         if not uniform:
             raise NotImplementedError("vae_amd.vrnn.loss_function: more than %d steps with a per-step KL weight needs "
                                       "a host model (model=...) for the per-step loop" % F_.MAX_STEPS)
-        recon_all = torch.cat([r.reshape(B, -1) for r in recon_x], 0)                  # [T*B, D or 2D]
-        x_all = torch.cat([xi.reshape(B, -1) for xi in x], 0)
+        if F_._is_categorical(config['nll_type']):
+            recon_all, x_all = torch.cat(list(recon_x), 0), torch.cat(list(x), 0)      # [T*B, ..., V], [T*B, ...]
+        else:
+            recon_all = torch.cat([r.reshape(B, -1) for r in recon_x], 0)              # [T*B, D or 2D]
+            x_all = torch.cat([xi.reshape(B, -1) for xi in x], 0)
         _, loss, elbo, means = F_.nll_elbo(x_all, recon_all, config['nll_type'], kld=klds, mi=mis, kl_beta=betas[0],
                                            inv_count=inv_count)
         out = _pack(loss.view(T, B).mean(0), elbo.view(T, B).mean(0), means, beta_scalar, loss.dtype)
