@@ -478,11 +478,14 @@ int vae_bnflow_bwd_apply(const void* x, const void* gy, float* stats, void* gx, 
  * vae_token_logp_fwd: logp[r] = ln softmax(logits[r])[token[r]] (needs tokens; may be NULL), entropy[r] of the row's
  * distribution (may be NULL), stats [N, 2] = (max, sum of exponentials), what the backward wants (may be NULL), and the
  * top_k <= VAE_MAX_TOP largest entries, top_logp / top_ids [N, top_k]: by value, ties by the lower id.  tokens == NULL:
- * no row is padding.                                                                                             */
+ * no row is padding.  `scratch` (here and below): vae_token_scratch_bytes(N, V, top_k, dtype) bytes, 8-byte aligned,
+ * contents free, not shared with a call that may run at the same time; NULL where that is 0 (few rows are cut into
+ * pieces whose results a second launch joins).                                                                   */
 #define VAE_MAX_TOP 64
+size_t vae_token_scratch_bytes(int64_t N, int64_t V, int64_t top_k, int dtype);
 int vae_token_logp_fwd(const void* logits, int64_t row_stride, const void* tokens, int token_bytes, float* logp,
-                       float* entropy, float* stats, float* top_logp, int64_t* top_ids, int64_t top_k, int64_t N,
-                       int64_t V, int dtype, vae_stream_t stream);
+                       float* entropy, float* stats, float* top_logp, int64_t* top_ids, int64_t top_k, void* scratch,
+                       int64_t N, int64_t V, int dtype, vae_stream_t stream);
 /* glogits [N, V] (contiguous, every element written) from glogp (one value per `rows_per_g` consecutive rows, times
  * g_scale; NULL with tokens: g_scale itself on every row), gentropy [N] (with the forward's `entropy`) and gtop
  * [N, top_k] (with the forward's top_ids); each may be NULL.                                                     */
@@ -492,7 +495,7 @@ int vae_token_logp_bwd(const void* logits, int64_t row_stride, const void* token
                        int64_t N, int64_t V, int dtype, vae_stream_t stream);
 /* logp and stats as above together with glogits = grad_scale * d(-logp) / d logits, the training step's form.      */
 int vae_token_nll_fused(const void* logits, int64_t row_stride, const void* tokens, int token_bytes, float* logp,
-                        float* stats, void* glogits, float grad_scale, int64_t N, int64_t V, int dtype,
+                        float* stats, void* glogits, float grad_scale, void* scratch, int64_t N, int64_t V, int dtype,
                         vae_stream_t stream);
 /* out[b] (dtype) = scale * sum of rows[b T .. b T + T), summed in double in a fixed order.                         */
 int vae_row_sums(const float* rows, float scale, void* out, int64_t B, int64_t T, int dtype, vae_stream_t stream);
@@ -501,13 +504,13 @@ int vae_grad_scale(void* buf, const float* factor, int64_t n, int dtype, vae_str
 /* Distillation from a teacher's K <= VAE_MAX_TEACHER largest logits per row (t_logits in t_dtype, t_ids; rows t_stride /
  * id_stride apart), both sides at `temperature` > 0:  q = softmax(t_logits / temperature) over the entries that are
  * there (id >= 0 and logit > -inf), p = softmax(logits / temperature) over V,
- * kl[r] = sum_k q_k (ln q_k - ln p[id_k]).  An id may come more than once.  No entry there: kl 0, gradient 0, the row's
- * logits are not read.  An id >= V: NaN, nothing is read out of range.  stats [N, 2] for the backward (may be NULL
- * without glogits); glogits != NULL: also grad_scale * d kl / d logits.                                            */
+ * kl[r] = sum_k q_k (ln q_k - ln p[id_k]).  An id may come more than once.  No entry there: kl 0, gradient 0, whatever the
+ * row's logits hold.  An id >= V: NaN, nothing is read out of range.  stats [N, 2] for the backward (may be NULL
+ * without glogits); glogits != NULL: also grad_scale * d kl / d logits.  scratch: as above with top_k = 0.          */
 #define VAE_MAX_TEACHER 256
 int vae_distill_fwd(const void* logits, int64_t row_stride, const void* t_logits, int64_t t_stride, int t_dtype,
                     const void* t_ids, int64_t id_stride, int id_bytes, int64_t K, float temperature, float* kl,
-                    float* stats, void* glogits, float grad_scale, int64_t N, int64_t V, int dtype,
+                    float* stats, void* glogits, float grad_scale, void* scratch, int64_t N, int64_t V, int dtype,
                     vae_stream_t stream);
 /* glogits[r] = (gkl[r] + *gmean * mean_scale) * d kl[r] / d logits[r]; gkl [N], gmean (one float): each may be NULL
  * (both NULL: mean_scale on every row).                                                                          */

@@ -64,10 +64,11 @@ P = ctypes.c_void_p(4096)   # never read: every call below is refused, or has no
 
 
 def fwd(**kw):
-    a = dict(logits=P, stride=10, tokens=P, tb=8, logp=P, ent=P, stats=P, top=P, ids=P, k=3, N=2, V=10, dtype=0)
+    a = dict(logits=P, stride=10, tokens=P, tb=8, logp=P, ent=P, stats=P, top=P, ids=P, k=3, scratch=P, N=2, V=10,
+             dtype=0)
     a.update(kw)
     return _call('vae_token_logp_fwd', [a[n] for n in ('logits', 'stride', 'tokens', 'tb', 'logp', 'ent', 'stats', 'top',
-                                                       'ids', 'k', 'N', 'V', 'dtype')] + [None])
+                                                       'ids', 'k', 'scratch', 'N', 'V', 'dtype')] + [None])
 
 
 def bwd(**kw):
@@ -80,18 +81,20 @@ def bwd(**kw):
 
 
 def fused(**kw):
-    a = dict(logits=P, stride=10, tokens=P, tb=8, logp=P, stats=P, out=P, scale=1.0, N=2, V=10, dtype=0)
+    a = dict(logits=P, stride=10, tokens=P, tb=8, logp=P, stats=P, out=P, scale=1.0, scratch=P, N=2, V=10,
+             dtype=0)
     a.update(kw)
     return _call('vae_token_nll_fused', [a[n] for n in ('logits', 'stride', 'tokens', 'tb', 'logp', 'stats', 'out',
-                                                        'scale', 'N', 'V', 'dtype')] + [None])
+                                                        'scale', 'scratch', 'N', 'V', 'dtype')] + [None])
 
 
 def dfwd(**kw):
-    a = dict(logits=P, stride=10, y=P, ys=2, yt=0, ids=P, ids_s=2, ib=8, K=2, tau=1.0, kl=P, stats=P, out=P, scale=1.0, N=2,
-             V=10, dtype=0)
+    a = dict(logits=P, stride=10, y=P, ys=2, yt=0, ids=P, ids_s=2, ib=8, K=2, tau=1.0, kl=P, stats=P, out=P, scale=1.0,
+             scratch=P, N=2, V=10, dtype=0)
     a.update(kw)
     return _call('vae_distill_fwd', [a[n] for n in ('logits', 'stride', 'y', 'ys', 'yt', 'ids', 'ids_s', 'ib', 'K', 'tau',
-                                                    'kl', 'stats', 'out', 'scale', 'N', 'V', 'dtype')] + [None])
+                                                    'kl', 'stats', 'out', 'scale', 'scratch', 'N', 'V', 'dtype')]
+                 + [None])
 
 
 def dbwd(**kw):
@@ -113,7 +116,8 @@ def test_c_entry_points_refuse_bad_shapes(f, bad):
 
 @pytest.mark.parametrize('f,bad', [
     (fwd, dict(k=-1)), (fwd, dict(k=65, V=100, stride=100)), (fwd, dict(k=11)), (fwd, dict(tb=2)),
-    (fwd, dict(tokens=None)), (fwd, dict(top=None)), (fwd, dict(ids=None)),
+    (fwd, dict(scratch=None, V=65536, stride=65536)), (dfwd, dict(out=None, scratch=None, V=65536, stride=65536)),
+    (fused, dict(scratch=None, V=65536, stride=65536)), (fwd, dict(tokens=None)), (fwd, dict(top=None)), (fwd, dict(ids=None)),
     (bwd, dict(k=65)), (bwd, dict(k=-1)), (bwd, dict(per=0)), (bwd, dict(stats=None)), (bwd, dict(out=None)),
     (bwd, dict(tb=1)), (bwd, dict(ent=None)), (bwd, dict(gtop=None)), (bwd, dict(ids=None)), (bwd, dict(tokens=None)),
     (fused, dict(tokens=None)), (fused, dict(logp=None)), (fused, dict(stats=None)), (fused, dict(out=None)),

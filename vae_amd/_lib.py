@@ -92,14 +92,18 @@ SIGNATURES = {
     'vae_bnflow_bwd': [_p, _p, _p, _p, _p, _i64, _i64, _i, _i, _i, _p],
     'vae_bnflow_bwd_sums': [_p, _p, _p, _p, _i64, _i64, _i, _i, _p],
     'vae_bnflow_bwd_apply': [_p, _p, _p, _p, _i64, _i64, _i64, _i, _i, _p],
-    'vae_token_logp_fwd': [_p, _i64, _p, _i, _p, _p, _p, _p, _p, _i64, _i64, _i64, _i, _p],
+    'vae_token_scratch_bytes': [_i64, _i64, _i64, _i],
+    'vae_token_logp_fwd': [_p, _i64, _p, _i, _p, _p, _p, _p, _p, _i64, _p, _i64, _i64, _i, _p],
     'vae_token_logp_bwd': [_p, _i64, _p, _i, _p, _p, _p, _i64, _f, _p, _p, _p, _i64, _p, _i64, _i64, _i, _p],
-    'vae_token_nll_fused': [_p, _i64, _p, _i, _p, _p, _p, _f, _i64, _i64, _i, _p],
+    'vae_token_nll_fused': [_p, _i64, _p, _i, _p, _p, _p, _f, _p, _i64, _i64, _i, _p],
     'vae_row_sums': [_p, _f, _p, _i64, _i64, _i, _p],
     'vae_grad_scale': [_p, _p, _i64, _i, _p],
-    'vae_distill_fwd': [_p, _i64, _p, _i64, _i, _p, _i64, _i, _i64, _f, _p, _p, _p, _f, _i64, _i64, _i, _p],
+    'vae_distill_fwd': [_p, _i64, _p, _i64, _i, _p, _i64, _i, _i64, _f, _p, _p, _p, _f, _p, _i64, _i64, _i, _p],
     'vae_distill_bwd': [_p, _i64, _p, _i64, _i, _p, _i64, _i, _i64, _f, _p, _p, _p, _f, _p, _i64, _i64, _i, _p],
 }
+
+# entry points that return a size_t
+SIZES = ('vae_workspace_bytes', 'vae_bnflow_stats_floats', 'vae_token_scratch_bytes')
 
 _lib = None
 
@@ -118,7 +122,7 @@ def load():
     for name, argtypes in SIGNATURES.items():
         fn = getattr(lib, name)  # AttributeError if the ABI lost a symbol
         fn.argtypes = argtypes
-        fn.restype = ctypes.c_size_t if name in ('vae_workspace_bytes', 'vae_bnflow_stats_floats') else ctypes.c_int
+        fn.restype = ctypes.c_size_t if name in SIZES else ctypes.c_int
     if lib.vae_abi_version() != ABI_VERSION:
         raise RuntimeError("vae_amd: libvae_amd.so has ABI %d, the binding expects %d; rebuild"
                            % (lib.vae_abi_version(), ABI_VERSION))

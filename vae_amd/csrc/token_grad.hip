@@ -1,0 +1,548 @@
+// Gradients with respect to rows of logits [N, V]: of log probs, entropy and alternatives (token_logp_bwd), of the
+// distillation KL (distill_bwd), and both losses together with their gradient in one pass (token_nll_fused,
+// distill_fwd with glogits).  Formulas and the conventions for masks: token_row.hpp.
+//
+// Every one of them is   g_j = e_j (A + B d_j) + sum over a few entries (id, g) with id = j,   d = (x - m) c, e = 2^d:
+//   tokens:   A = -(sum_i g_i + g_H (H - ln s)) / s,  B = -g_H ln2 / s,  entries: the token and the alternatives
+//   teacher:  A = w / (tau s),  B = 0,  entries: (id_k, -w q_k / tau)
+// The entries are owned by the thread whose vector holds them and added before the vector is stored: no atomics on the
+// gradient, no second write, one rounding.
+#include "token_row.hpp"
+
+namespace vae {
+
+// A piece's entries in LDS: each thread's own in a list.  Entries of one id are merged first, in entry order, so what
+// a gradient element receives does not depend on the order of the list.
+constexpr int kMaxEntries = VAE_MAX_TEACHER;
+template <int BT>
+struct Entries {
+  static constexpr int R = (kMaxEntries + BT - 1) / BT;
+  int head[BT];
+  int next[kMaxEntries], id[kMaxEntries];
+  float g[kMaxEntries];
+
+  // id[0..n), g[0..n) have been written by the workgroup (id < 0: none)
+  template <typename T, int VN>
+  __device__ __forceinline__ void link(int n, const RowCut<T, VN>& cut, int v0, int v1) {
+    int own[R];
+    float sum[R];
+    head[threadIdx.x] = -1;
+    lds_barrier();
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      const int k = threadIdx.x + r * BT;
+      own[r] = k < n ? id[k] : -1;
+      sum[r] = 0.f;
+      if (own[r] >= 0) {
+        bool first = true;
+        for (int q = 0; q < n; ++q)
+          if (id[q] == own[r]) {
+            first &= q >= k;
+            sum[r] += g[q];
+          }
+        if (!first) own[r] = -1;
+      }
+    }
+    lds_barrier();
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      const int k = threadIdx.x + r * BT;
+      if (own[r] < 0) continue;
+      g[k] = sum[r];
+      const int off = own[r] - cut.head;
+      int owner = -1;
+      if (off < 0) owner = own[r];                                      // RowCut::edge
+      else if (off >= cut.nvec * VN) owner = 16 + off - cut.nvec * VN;
+      else if (off / VN >= v0 && off / VN < v1) owner = (off / VN - v0) % BT;
+      if (owner >= 0) next[k] = atomicExch(&head[owner], k);
+    }
+    lds_barrier();
+  }
+};
+
+// What a thread adds to its elements: one entry known to all (ONE), or the workgroup's lists.
+template <typename T, int VN, int BT, bool LIST>
+struct Adds {
+  const Entries<BT>* lds;
+  int one_id;        // -1: none
+  float one_g;
+  uint32_t mask;     // bit u: the thread's u-th vector of the piece holds an entry (at most 32 vectors)
+
+  __device__ __forceinline__ void prepare(const RowCut<T, VN>& cut, int v0, int v1) {
+    mask = 0;
+    auto note = [&](int id) {
+      const int off = id - cut.head, vec = off / VN;
+      if (off >= 0 && vec < cut.nvec && vec >= v0 && vec < v1 && (vec - v0) % BT == (int)threadIdx.x)
+        mask |= 1u << ((vec - v0) / BT);
+    };
+    if constexpr (LIST) {
+      for (int k = lds->head[threadIdx.x]; k >= 0; k = lds->next[k]) note(lds->id[k]);
+    } else if (one_id >= 0) {
+      note(one_id);
+    }
+  }
+  template <int W>
+  __device__ __forceinline__ void to(int index, float (&v)[W]) const {
+    auto add = [&](int id, float g) {
+      const int e = id - index;
+#pragma unroll
+      for (int i = 0; i < W; ++i)
+        if (e == i) v[i] += g;
+    };
+    if constexpr (LIST) {
+      for (int k = lds->head[threadIdx.x]; k >= 0; k = lds->next[k]) add(lds->id[k], lds->g[k]);
+    } else {
+      add(one_id, one_g);
+    }
+  }
+};
+
+struct GradArgs {
+  const void* logits;
+  int64_t row_stride;
+  void* glogits;
+  int64_t N;
+  int V, parts, part_vecs;
+  bool nts;
+  float scale2, inv_tau;
+  const float* stats_in;
+  // tokens
+  const void* tokens;
+  int token_bytes;
+  const float *entropy, *glogp;
+  int64_t rows_per_g;
+  float g_scale;
+  const float *gentropy, *gtop;
+  const int64_t* top_ids;
+  int top_k;
+  // teacher
+  TeacherArgs teacher;
+  const float *gkl, *gmean;
+  float mean_scale;
+  // fused
+  float *out, *stats_out;            // logp or kl, and the statistics
+};
+
+template <typename T, int VN, int BT>
+__device__ __forceinline__ void fill_row(T* __restrict__ gx, const RowCut<T, VN>& cut, int v0, int v1, int edge,
+                                         float value, bool nts) {
+  float v[VN];
+#pragma unroll
+  for (int i = 0; i < VN; ++i) v[i] = value;
+  for (int j = v0 + (int)threadIdx.x; j < v1; j += BT) store_vec<T, VN>(nts, gx + cut.index(j), v);
+  if (edge >= 0) gx[edge] = from_f32<T>(value);
+}
+
+// ---------------------------------------------------------------------------------------------------------------
+// from given statistics: one read, one write; a row is cut into pieces of at most 32 vectors a thread
+// ---------------------------------------------------------------------------------------------------------------
+template <typename T, int VN, int BT, bool ENT, bool LIST, bool DIST>
+__global__ __launch_bounds__(BT) void token_bwd_kernel(GradArgs a) {
+  constexpr int U = 4;
+  __shared__ struct {
+    Entries<BT> entries[LIST ? 1 : 0];
+    TeacherRow<BT> teacher[DIST ? 1 : 0];
+  } lds;
+  for (int64_t item = blockIdx.x; item < a.N * a.parts; item += gridDim.x) {
+    const int64_t row = a.parts == 1 ? item : item / a.parts;
+    const int part = a.parts == 1 ? 0 : (int)(item - row * a.parts);
+    const T* x = (const T*)a.logits + row * a.row_stride;
+    T* gx = (T*)a.glogits + row * (int64_t)a.V;
+    const RowCut<T, VN> cut(x, a.V);
+    const int v0 = part * a.part_vecs;
+    int v1 = v0 + a.part_vecs;
+    v1 = v1 < cut.nvec ? v1 : cut.nvec;
+    int ei = cut.edge(threadIdx.x);
+    if (ei >= 0 && (ei < cut.head ? part != 0 : part != a.parts - 1)) ei = -1;
+    const float m = a.stats_in[2 * row], s = a.stats_in[2 * row + 1];
+    Adds<T, VN, BT, LIST> adds;
+    if constexpr (LIST) adds.lds = lds.entries;
+    float A, B = 0.f;
+    bool zero, bad = false;
+    const float inv = 1.0f / s;
+    if constexpr (DIST) {
+      const int state = lds.teacher[0].load(a.teacher, row, a.V, a.inv_tau, a.scale2);
+      const float g0 = a.gmean ? a.gmean[0] * a.mean_scale : (a.gkl ? 0.f : a.mean_scale);
+      const float w = ((a.gkl ? a.gkl[row] : 0.f) + g0) * a.inv_tau;
+      zero = state == kRowEmpty || (state == kRowFine && s == 0.f);
+      bad = state == kRowBad;
+      A = w * inv;
+      if (!zero && !bad)
+        for (int k = threadIdx.x; k < a.teacher.K; k += BT) {
+          lds.entries[0].id[k] = lds.teacher[0].id[k];
+          lds.entries[0].g[k] = -w * lds.teacher[0].q[k];
+        }
+    } else {
+      const int64_t tok = a.tokens ? load_id(a.tokens, a.token_bytes, row) : 0;
+      zero = tok < 0 || s == 0.f;
+      float gt = a.tokens ? (a.glogp ? a.glogp[row / a.rows_per_g] * a.g_scale : a.g_scale) : 0.f;
+      const bool inside = a.tokens && tok >= 0 && tok < a.V;
+      if (tok >= a.V && (!a.glogp || a.g_scale != 0.f)) gt = nan_f();
+      float sum = gt;
+      adds.one_id = inside ? (int)tok : -1;
+      adds.one_g = gt;
+      if constexpr (LIST) {
+        for (int k = 0; k < a.top_k; ++k) sum += a.gtop[row * a.top_k + k];
+        lds_barrier();  // the row before this one has been read
+        if (!zero)
+          for (int k = threadIdx.x; k <= a.top_k; k += BT) {
+            lds.entries[0].id[k] = k == 0 ? adds.one_id : (int)a.top_ids[row * a.top_k + k - 1];
+            lds.entries[0].g[k] = k == 0 ? gt : a.gtop[row * a.top_k + k - 1];
+          }
+      }
+      if constexpr (ENT) {
+        const float gh = a.gentropy[row];
+        sum += gh * (a.entropy[row] - kLn2 * log2f(s));
+        B = -gh * kLn2 * inv;
+      }
+      A = -sum * inv;
+    }
+    if (zero || bad) {
+      fill_row<T, VN, BT>(gx, cut, v0, v1, ei, zero ? 0.f : nan_f(), a.nts);
+      continue;
+    }
+    if constexpr (LIST) lds.entries[0].template link<T, VN>(DIST ? a.teacher.K : a.top_k + 1, cut, v0, v1);
+    adds.prepare(cut, v0, v1);
+    auto grad = [&](float v) {
+      const float d = (v - m) * a.scale2;
+      const float e = exp2_raw(d);
+      return ENT ? e * __builtin_fmaf(B, max_raw(d, -300.f), A) : e * A;
+    };
+    int j = v0 + (int)threadIdx.x, bit = 0;
+    const int full = (v1 - v0) / (U * BT);
+    for (int it = 0; it < full; ++it, j += U * BT, bit += U) {
+      Packet<T, VN> p[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) p[u].load(x + cut.index(j + u * BT));
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        float v[VN];
+        p[u].get(v);
+#pragma unroll
+        for (int i = 0; i < VN; ++i) v[i] = grad(v[i]);
+        if (adds.mask >> (bit + u) & 1u) adds.to(cut.index(j + u * BT), v);
+        store_vec<T, VN>(a.nts, gx + cut.index(j + u * BT), v);
+      }
+    }
+    for (; j < v1; j += BT, ++bit) {
+      Packet<T, VN> p;
+      p.load(x + cut.index(j));
+      float v[VN];
+      p.get(v);
+#pragma unroll
+      for (int i = 0; i < VN; ++i) v[i] = grad(v[i]);
+      if (adds.mask >> bit & 1u) adds.to(cut.index(j), v);
+      store_vec<T, VN>(a.nts, gx + cut.index(j), v);
+    }
+    if (ei >= 0) {
+      float v[1] = {grad(to_f32(x[ei]))};
+      adds.to(ei, v);
+      gx[ei] = from_f32<T>(v[0]);
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------------------------------------------
+// loss and gradient in one pass: a workgroup holds its row in registers (U vectors a thread), as the 16-byte packets it
+// was read in: 4 registers a vector whatever the type
+// ---------------------------------------------------------------------------------------------------------------
+template <typename T, int BT, int U, bool DIST>
+__global__ __launch_bounds__(BT) void token_fused_kernel(GradArgs a) {
+  constexpr int VN = VecOf<T>::n;
+  __shared__ struct {
+    Entries<BT> entries[DIST ? 1 : 0];
+    TeacherRow<BT> teacher[DIST ? 1 : 0];
+  } lds;
+  for (int64_t row = blockIdx.x; row < a.N; row += gridDim.x) {
+    const T* x = (const T*)a.logits + row * a.row_stride;
+    T* gx = (T*)a.glogits + row * (int64_t)a.V;
+    const RowCut<T, VN> cut(x, a.V);
+    const int ei = cut.edge(threadIdx.x);
+    int64_t tok = 0;
+    int state = kRowFine;
+    if constexpr (DIST) {
+      state = lds.teacher[0].load(a.teacher, row, a.V, a.inv_tau, a.scale2);
+    } else {
+      tok = load_id(a.tokens, a.token_bytes, row);
+      state = tok < 0 ? kRowEmpty : (tok >= a.V ? kRowBad : kRowFine);
+    }
+    if (state != kRowFine) {
+      const float v = state == kRowEmpty ? 0.f : nan_f();
+      fill_row<T, VN, BT>(gx, cut, 0, cut.nvec, ei, v, a.nts);
+      if (threadIdx.x == 0) {
+        a.out[row] = v;
+        a.stats_out[2 * row] = 0.f;
+        a.stats_out[2 * row + 1] = DIST ? 0.f : v;
+      }
+      continue;
+    }
+    Packet<T, VN> p[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int j = threadIdx.x + u * BT;
+      if (j < cut.nvec) p[u].load(x + cut.index(j));
+    }
+    const float edge = ei >= 0 ? to_f32(x[ei]) : -INFINITY;
+    float m = max_raw(edge, kLowest);
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if ((int)threadIdx.x + u * BT < cut.nvec) {
+        float v[VN];
+        p[u].get(v);
+        m = vec_max(v, m);
+      }
+    m = block_max<BT>(m);
+    float s = ei >= 0 ? exp2_raw((edge - m) * a.scale2) : 0.f;
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if ((int)threadIdx.x + u * BT < cut.nvec) {
+        asm volatile("" : "+v"(p[u].raw));   // unpack again: the packets, not their elements, stay in registers
+        float v[VN];
+        p[u].get(v);
+#pragma unroll
+        for (int i = 0; i < VN; ++i) s += exp2_raw((v[i] - m) * a.scale2);
+      }
+    s = block_sum<BT>(s);
+    Adds<T, VN, BT, DIST> adds;
+    const float w = DIST ? a.mean_scale * a.inv_tau : a.g_scale;   // of p; the entries have the other sign
+    if constexpr (DIST) {
+      adds.lds = lds.entries;
+      float kl = 0.f;
+      for (int k = threadIdx.x; k < a.teacher.K; k += BT) {
+        const int id = lds.teacher[0].id[k];
+        const float q = lds.teacher[0].q[k];
+        if (id >= 0) kl += q * (lds.teacher[0].logq[k] - row_log_prob(to_f32(x[id]), m, s, a.inv_tau));
+        lds.entries[0].id[k] = id;
+        lds.entries[0].g[k] = -w * q;
+      }
+      kl = block_sum<BT>(kl);
+      if (threadIdx.x == 0) a.out[row] = kl;
+      lds.entries[0].template link<T, VN>(a.teacher.K, cut, 0, cut.nvec);
+    } else {
+      adds.one_id = (int)tok;
+      adds.one_g = -w;
+      if (threadIdx.x == 0) a.out[row] = row_log_prob(to_f32(x[tok]), m, s, 1.0f);
+    }
+    if (threadIdx.x == 0) {
+      a.stats_out[2 * row] = m;
+      a.stats_out[2 * row + 1] = s;
+    }
+    if (s == 0.f) {
+      fill_row<T, VN, BT>(gx, cut, 0, cut.nvec, ei, 0.f, a.nts);
+      continue;
+    }
+    adds.prepare(cut, 0, cut.nvec);
+    const float A = w / s;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int j = threadIdx.x + u * BT;
+      if (j < cut.nvec) {
+        asm volatile("" : "+v"(p[u].raw));
+        float v[VN];
+        p[u].get(v);
+#pragma unroll
+        for (int i = 0; i < VN; ++i) v[i] = A * exp2_raw((v[i] - m) * a.scale2);
+        if (adds.mask >> u & 1u) adds.to(cut.index(j), v);
+        store_vec<T, VN>(a.nts, gx + cut.index(j), v);
+      }
+    }
+    if (ei >= 0) {
+      float v[1] = {A * exp2_raw((edge - m) * a.scale2)};
+      adds.to(ei, v);
+      gx[ei] = from_f32<T>(v[0]);
+    }
+  }
+}
+
+template <typename T, int V>
+__global__ __launch_bounds__(kBlock) void grad_scale_kernel(T* __restrict__ buf, const float* __restrict__ factor,
+                                                            int64_t items) {
+  const float c = factor[0];
+  if (c == 1.0f) return;
+  for (int64_t j = (int64_t)blockIdx.x * kBlock + threadIdx.x; j < items; j += (int64_t)gridDim.x * kBlock) {
+    float v[V];
+    load_vec<T, V, false>(buf + j * V, v);
+#pragma unroll
+    for (int i = 0; i < V; ++i) v[i] *= c;
+    store_vec<T, V>(buf + j * V, v);
+  }
+}
+
+// ---------------------------------------------------------------------------------------------------------------
+// host
+// ---------------------------------------------------------------------------------------------------------------
+static bool type_ok(int d) { return d == VAE_F32 || d == VAE_BF16 || d == VAE_F16; }
+static bool bad_rows(int64_t N, int64_t V, int64_t row_stride, int dtype) {
+  return N < 0 || V < 1 || V > VAE_MAX_ROW || (N > 1 && row_stride < V) || !type_ok(dtype);
+}
+static int launched() { return hipGetLastError() == hipSuccess ? VAE_OK : VAE_ERR_LAUNCH; }
+static int grid_for(int64_t items) { return (int)(items < kMaxGrid ? items : kMaxGrid); }
+
+// logits and gradient rows start at the same offset from a 16-byte boundary, all of them
+template <typename T>
+static bool same_phase(const GradArgs& a) {
+  const int64_t by = (int64_t)reinterpret_cast<uintptr_t>(a.logits) - (int64_t)reinterpret_cast<uintptr_t>(a.glogits);
+  return by % 16 == 0 && (a.N <= 1 || (a.row_stride - a.V) * (int64_t)sizeof(T) % 16 == 0);
+}
+
+template <typename T, int VN, int BT, bool ENT, bool LIST, bool DIST>
+static int bwd_launch(GradArgs a, hipStream_t st) {
+  // pieces of at most 32 vectors a thread (Adds::mask), more of them while the rows alone do not fill the chip
+  const int64_t nvec = ((int64_t)a.V + VN - 1) / VN;
+  int64_t parts = (nvec + 32 * BT - 1) / (32 * BT);
+  const int64_t most = (nvec + 4 * BT - 1) / (4 * BT);
+  while (parts < most && a.N * parts < 2048) parts *= 2;
+  parts = parts < most ? parts : most;
+  const int64_t per = (nvec + parts - 1) / parts;
+  a.parts = (int)((nvec + per - 1) / per);
+  a.part_vecs = (int)per;
+  a.nts = (int64_t)sizeof(T) * a.N * a.V >= kNtStoreMinBytes;
+  hipLaunchKernelGGL((token_bwd_kernel<T, VN, BT, ENT, LIST, DIST>), dim3(grid_for(a.N * a.parts)), dim3(BT), 0, st, a);
+  return launched();
+}
+template <typename T, int VN, bool ENT, bool LIST, bool DIST>
+static int bwd_block(const GradArgs& a, hipStream_t st) {
+  if (((int64_t)a.V + VN - 1) / VN <= 512) return bwd_launch<T, VN, 64, ENT, LIST, DIST>(a, st);
+  return bwd_launch<T, VN, kBlock, ENT, LIST, DIST>(a, st);
+}
+template <typename T, int VN, bool DIST>
+static int bwd_kind(const GradArgs& a, hipStream_t st) {
+  if constexpr (DIST) return bwd_block<T, VN, false, true, true>(a, st);
+  else {
+    const bool list = a.gtop != nullptr;
+    if (a.gentropy) return list ? bwd_block<T, VN, true, true, false>(a, st) : bwd_block<T, VN, true, false, false>(a, st);
+    return list ? bwd_block<T, VN, false, true, false>(a, st) : bwd_block<T, VN, false, false, false>(a, st);
+  }
+}
+template <typename T, bool DIST>
+static int bwd_type(const GradArgs& a, hipStream_t st) {
+  return same_phase<T>(a) ? bwd_kind<T, VecOf<T>::n, DIST>(a, st) : bwd_kind<T, 1, DIST>(a, st);
+}
+
+template <typename T, int BT, int U, bool DIST>
+static int fused_launch(GradArgs a, hipStream_t st) {
+  a.nts = (int64_t)sizeof(T) * a.N * a.V >= kNtStoreMinBytes;
+  hipLaunchKernelGGL((token_fused_kernel<T, BT, U, DIST>), dim3(grid_for(a.N)), dim3(BT), 0, st, a);
+  return launched();
+}
+// true when the one-pass kernel takes this call: the row fits a workgroup's registers, and there are rows enough
+template <typename T, bool DIST>
+static bool fused_type(const GradArgs& a, hipStream_t st, int* rc) {
+  const int64_t nvec = (int64_t)a.V / VecOf<T>::n;
+  if (!same_phase<T>(a) || nvec > 16384 || (a.N < 256 && nvec > 4096)) return false;
+  if (nvec <= 512) *rc = fused_launch<T, 64, 8, DIST>(a, st);
+  else if (nvec <= 1024) *rc = fused_launch<T, 256, 4, DIST>(a, st);
+  else if (nvec <= 2048) *rc = fused_launch<T, 256, 8, DIST>(a, st);
+  else if (nvec <= 4096) *rc = fused_launch<T, 256, 16, DIST>(a, st);
+  else if (nvec <= 8192) *rc = fused_launch<T, 512, 16, DIST>(a, st);
+  else *rc = fused_launch<T, 1024, 16, DIST>(a, st);
+  return true;
+}
+
+static bool bad_teacher(const TeacherArgs& t, int64_t N, float temperature) {
+  return !type_ok(t.dtype) || t.K < 1 || t.K > VAE_MAX_TEACHER || (N > 1 && (t.stride < t.K || t.id_stride < t.K)) ||
+         (t.id_bytes != 4 && t.id_bytes != 8) || !(temperature > 0.f) || !(temperature < INFINITY);
+}
+static void set_temperature(GradArgs& a, float temperature) {
+  a.scale2 = (float)(1.4426950408889634 / (double)temperature);
+  a.inv_tau = (float)(1.0 / (double)temperature);
+}
+
+}  // namespace vae
+
+using namespace vae;
+
+extern "C" {
+
+int vae_token_logp_bwd(const void* logits, int64_t row_stride, const void* tokens, int token_bytes, const float* stats,
+                       const float* entropy, const float* glogp, int64_t rows_per_g, float g_scale,
+                       const float* gentropy, const float* gtop, const int64_t* top_ids, int64_t top_k, void* glogits,
+                       int64_t N, int64_t V, int dtype, vae_stream_t stream) {
+  if (bad_rows(N, V, row_stride, dtype) || top_k < 0 || top_k > VAE_MAX_TOP || rows_per_g < 1) return VAE_ERR_ARG;
+  if (N == 0) return VAE_OK;
+  if (!logits || !stats || !glogits || (tokens && token_bytes != 4 && token_bytes != 8)) return VAE_ERR_ARG;
+  if ((gentropy && !entropy) || (top_k > 0 && (!gtop || !top_ids)) || (glogp && !tokens)) return VAE_ERR_ARG;
+  GradArgs a = {};
+  a.logits = logits; a.row_stride = row_stride; a.glogits = glogits; a.N = N; a.V = (int)V;
+  a.scale2 = kLog2e; a.inv_tau = 1.0f; a.stats_in = stats;
+  a.tokens = tokens; a.token_bytes = token_bytes; a.entropy = entropy; a.glogp = glogp; a.rows_per_g = rows_per_g;
+  a.g_scale = g_scale; a.gentropy = gentropy; a.gtop = top_k ? gtop : nullptr; a.top_ids = top_ids; a.top_k = (int)top_k;
+  VAE_BY_TYPE(dtype, return (bwd_type<T, false>(a, (hipStream_t)stream)));
+  return VAE_ERR_ARG;
+}
+
+int vae_token_nll_fused(const void* logits, int64_t row_stride, const void* tokens, int token_bytes, float* logp,
+                        float* stats, void* glogits, float grad_scale, void* scratch, int64_t N, int64_t V, int dtype,
+                        vae_stream_t stream) {
+  if (bad_rows(N, V, row_stride, dtype)) return VAE_ERR_ARG;
+  if (N == 0) return VAE_OK;
+  if (!logits || !tokens || !logp || !stats || !glogits || (token_bytes != 4 && token_bytes != 8)) return VAE_ERR_ARG;
+  GradArgs a = {};
+  a.logits = logits; a.row_stride = row_stride; a.glogits = glogits; a.N = N; a.V = (int)V;
+  a.scale2 = kLog2e; a.inv_tau = 1.0f;
+  a.tokens = tokens; a.token_bytes = token_bytes; a.g_scale = grad_scale; a.out = logp; a.stats_out = stats;
+  int rc = VAE_ERR_ARG;
+  VAE_BY_TYPE(dtype, if (fused_type<T, false>(a, (hipStream_t)stream, &rc)) return rc);
+  rc = vae_token_logp_fwd(logits, row_stride, tokens, token_bytes, logp, nullptr, stats, nullptr, nullptr, 0, scratch, N,
+                          V, dtype, stream);
+  if (rc != VAE_OK) return rc;
+  return vae_token_logp_bwd(logits, row_stride, tokens, token_bytes, stats, nullptr, nullptr, 1, -grad_scale, nullptr,
+                            nullptr, nullptr, 0, glogits, N, V, dtype, stream);
+}
+
+int vae_distill_bwd(const void* logits, int64_t row_stride, const void* t_logits, int64_t t_stride, int t_dtype,
+                    const void* t_ids, int64_t id_stride, int id_bytes, int64_t K, float temperature,
+                    const float* stats, const float* gkl, const float* gmean, float mean_scale, void* glogits,
+                    int64_t N, int64_t V, int dtype, vae_stream_t stream) {
+  if (K > VAE_MAX_TEACHER) return VAE_ERR_ARG;
+  GradArgs a = {};
+  a.teacher = {t_logits, t_ids, t_stride, id_stride, t_dtype, id_bytes, (int)K};
+  if (bad_rows(N, V, row_stride, dtype) || bad_teacher(a.teacher, N, temperature)) return VAE_ERR_ARG;
+  if (N == 0) return VAE_OK;
+  if (!logits || !t_logits || !t_ids || !stats || !glogits) return VAE_ERR_ARG;
+  a.logits = logits; a.row_stride = row_stride; a.glogits = glogits; a.N = N; a.V = (int)V;
+  a.stats_in = stats; a.gkl = gkl; a.gmean = gmean; a.mean_scale = mean_scale;
+  set_temperature(a, temperature);
+  VAE_BY_TYPE(dtype, return (bwd_type<T, true>(a, (hipStream_t)stream)));
+  return VAE_ERR_ARG;
+}
+
+int vae_distill_fwd(const void* logits, int64_t row_stride, const void* t_logits, int64_t t_stride, int t_dtype,
+                    const void* t_ids, int64_t id_stride, int id_bytes, int64_t K, float temperature, float* kl,
+                    float* stats, void* glogits, float grad_scale, void* scratch, int64_t N, int64_t V, int dtype,
+                    vae_stream_t stream) {
+  if (K > VAE_MAX_TEACHER) return VAE_ERR_ARG;
+  GradArgs a = {};
+  a.teacher = {t_logits, t_ids, t_stride, id_stride, t_dtype, id_bytes, (int)K};
+  if (bad_rows(N, V, row_stride, dtype) || bad_teacher(a.teacher, N, temperature)) return VAE_ERR_ARG;
+  if (N == 0) return VAE_OK;
+  if (!logits || !t_logits || !t_ids || !kl || (glogits && !stats)) return VAE_ERR_ARG;
+  if (glogits) {
+    a.logits = logits; a.row_stride = row_stride; a.glogits = glogits; a.N = N; a.V = (int)V;
+    a.mean_scale = grad_scale; a.out = kl; a.stats_out = stats;
+    set_temperature(a, temperature);
+    int rc = VAE_ERR_ARG;
+    VAE_BY_TYPE(dtype, if (fused_type<T, true>(a, (hipStream_t)stream, &rc)) return rc);
+  }
+  const int rc = distill_stats(logits, row_stride, a.teacher, temperature, kl, stats, scratch, N, V, dtype,
+                               (hipStream_t)stream);
+  if (rc != VAE_OK || !glogits) return rc;
+  return vae_distill_bwd(logits, row_stride, t_logits, t_stride, t_dtype, t_ids, id_stride, id_bytes, K, temperature,
+                         stats, nullptr, nullptr, grad_scale, glogits, N, V, dtype, stream);
+}
+
+int vae_grad_scale(void* buf, const float* factor, int64_t n, int dtype, vae_stream_t stream) {
+  if (n < 0) return VAE_ERR_ARG;
+  if (n == 0) return VAE_OK;
+  if (!buf || !factor) return VAE_ERR_ARG;
+  hipStream_t st = (hipStream_t)stream;
+  VAE_BY_TYPE(dtype, constexpr int VN = VecOf<T>::n; const bool vec = n % VN == 0 && aligned16(buf);
+              const int64_t items = vec ? n / VN : n; const int64_t blocks = (items + kBlock - 1) / kBlock;
+              const int grid = (int)(blocks < 4096 ? blocks : 4096);
+              if (vec) hipLaunchKernelGGL((grad_scale_kernel<T, VN>), dim3(grid), dim3(kBlock), 0, st, (T*)buf, factor, items);
+              else hipLaunchKernelGGL((grad_scale_kernel<T, 1>), dim3(grid), dim3(kBlock), 0, st, (T*)buf, factor, items);
+              return launched());
+  return VAE_ERR_ARG;
+}
+
+}  // extern "C"

@@ -1,6 +1,6 @@
-// What the token kernels (token.hip, distill.hip) share: a row of logits over a vocabulary, its softmax statistics and
-// the ids that index it.  No reference counterpart: the reference's likelihoods are Bernoulli, Gaussian and the
-// discretized logistic (abstract_vae.py:461-471); this is the categorical one.
+// What the token kernels (token.hip, token_grad.hip) share: a row of logits over a vocabulary, its softmax statistics,
+// the ids that index it and the teacher's entries.  No reference counterpart: the reference's likelihoods are Bernoulli,
+// Gaussian and the discretized logistic (abstract_vae.py:461-471); this is the categorical one.
 //
 // Statistics of a row x[V] at scale c = log2(e) / temperature:  m = max x,  s = sum 2^((x - m) c).
 //   p_j = 2^((x_j - m) c) / s,   ln p_j = ln2 ((x_j - m) c - log2 s).
@@ -9,18 +9,32 @@
 // entropy 0, gradient 0.  A NaN or +inf logit makes s NaN and with it everything the row returns.
 #pragma once
 #include "common.hpp"
+#include "../../include/vae_amd.h"
 
 namespace vae {
+
+constexpr int kMaxGrid = 1 << 20;  // blocks of a launch; items beyond are grid-strided
 
 // ids come as int32 or int64
 __device__ __forceinline__ int64_t load_id(const void* __restrict__ ids, int id_bytes, int64_t i) {
   return id_bytes == 4 ? (int64_t) reinterpret_cast<const int32_t*>(ids)[i] : reinterpret_cast<const int64_t*>(ids)[i];
 }
+__device__ __forceinline__ float load_any(const void* __restrict__ p, int dtype, int64_t i) {
+  if (dtype == VAE_F32) return reinterpret_cast<const float*>(p)[i];
+  if (dtype == VAE_BF16) return to_f32(reinterpret_cast<const bf16_t*>(p)[i]);
+  return to_f32(reinterpret_cast<const f16_t*>(p)[i]);
+}
 
-// the largest finite-or-minus-infinite value a statistic is taken against: -inf would make x - m NaN
+// the least value a statistic is taken against: -inf would make x - m NaN
 constexpr float kLowest = -3.402823466e38f;
 
 __device__ __forceinline__ float nan_f() { return __builtin_nanf(""); }
+__device__ __forceinline__ float exp2_raw(float x) { return __builtin_amdgcn_exp2f(x); }
+__device__ __forceinline__ float max3_raw(float a, float b, float c) {
+  float r;
+  asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+  return r;
+}
 
 // ln p of a value with statistics (m, s); s == 0: an empty row.  In natural units: x - m of the type's range does not
 // overflow here, times log2(e) it could.
@@ -37,24 +51,197 @@ __device__ __forceinline__ float order_value(uint32_t o) {
   return __uint_as_float((o & 0x80000000u) ? (o ^ 0x80000000u) : ~o);
 }
 __device__ __forceinline__ uint64_t order_key(float x, uint32_t index) {
-  return ((uint64_t)order_bits(x) << 32) | (uint32_t)(~index);
+  const uint32_t o = order_bits(x);
+  return o ? ((uint64_t)o << 32) | (uint32_t)(~index) : 0;  // 0: no entry
 }
+__device__ __forceinline__ float key_value(uint64_t key) { return order_value((uint32_t)(key >> 32)); }
+__device__ __forceinline__ int64_t key_index(uint64_t key) { return (int64_t)(uint32_t)~(uint32_t)key; }
 
-// sum / max over a workgroup of 256 in a fixed order; every thread gets the result
-__device__ __forceinline__ uint64_t block_max_u64(uint64_t v) {
-  __shared__ uint64_t lds_k[kBlock / 64];
+// Sum / max over a workgroup of BT threads, in a fixed order; every thread gets the result.  Uniform control flow.
+template <int BT>
+__device__ __forceinline__ float block_sum(float v) {
+  v = group_sum(v, 64);
+  if constexpr (BT > 64) {
+    __shared__ float lds[BT / 64];
+    lds_barrier();  // the readers of the last one are done
+    if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
+    lds_barrier();
+    v = 0.f;
+#pragma unroll
+    for (int w = 0; w < BT / 64; ++w) v += lds[w];
+  }
+  return v;
+}
+template <int BT>
+__device__ __forceinline__ float block_max(float v) {
+  v = group_max(v, 64);
+  if constexpr (BT > 64) {
+    __shared__ float lds[BT / 64];
+    lds_barrier();
+    if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
+    lds_barrier();
+    v = lds[0];
+#pragma unroll
+    for (int w = 1; w < BT / 64; ++w) v = max_raw(v, lds[w]);
+  }
+  return v;
+}
+template <int BT>
+__device__ __forceinline__ uint64_t block_max_key(uint64_t v) {
 #pragma unroll
   for (int o = 32; o >= 1; o >>= 1) {
     const uint64_t w = __shfl_xor(v, o, 64);
     v = w > v ? w : v;
   }
-  lds_barrier();
-  if ((threadIdx.x & 63) == 0) lds_k[threadIdx.x >> 6] = v;
-  lds_barrier();
-  uint64_t r = lds_k[0];
+  if constexpr (BT > 64) {
+    __shared__ uint64_t lds[BT / 64];
+    lds_barrier();
+    if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
+    lds_barrier();
+    v = lds[0];
 #pragma unroll
-  for (int w = 1; w < kBlock / 64; ++w) r = lds_k[w] > r ? lds_k[w] : r;
-  return r;
+    for (int w = 1; w < BT / 64; ++w) v = lds[w] > v ? lds[w] : v;
+  }
+  return v;
 }
+
+// A row as a workgroup reads it: up to VN - 1 scalars in front of the first 16-byte boundary (threads 0..7 hold one
+// each), `nvec` whole vectors, up to VN - 1 scalars behind them (threads 16..23).  Nothing outside the row is touched,
+// whatever its alignment.  VN == 1: every element is a "vector" of its own.
+template <typename T, int VN>
+struct RowCut {
+  int head, nvec, tail;
+  __device__ __forceinline__ RowCut(const T* row, int V) {
+    if constexpr (VN == 1) {
+      head = tail = 0;
+      nvec = V;
+    } else {
+      const int off = (int)((reinterpret_cast<uintptr_t>(row) & 15u) / sizeof(T));
+      head = off ? VN - off : 0;
+      head = head < V ? head : V;
+      nvec = (V - head) / VN;
+      tail = V - head - nvec * VN;
+    }
+  }
+  // the scalar that thread `tid` holds, or -1
+  __device__ __forceinline__ int edge(int tid) const {
+    if (tid < head) return tid;
+    if (tid >= 16 && tid < 16 + tail) return head + nvec * VN + (tid - 16);
+    return -1;
+  }
+  __device__ __forceinline__ int index(int vec) const { return head + vec * VN; }
+};
+
+// raw 16-byte packet of a row and its elements as floats
+template <typename T, int VN>
+struct Packet {
+  typename PackOf<T, VN>::type raw;
+  __device__ __forceinline__ void load(const T* __restrict__ p) {
+    raw = __builtin_nontemporal_load(reinterpret_cast<const typename PackOf<T, VN>::type*>(p));
+  }
+  __device__ __forceinline__ void get(float (&v)[VN]) const {
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+      for (int i = 0; i < VN; ++i) v[i] = raw[i];
+    } else if constexpr (DTypeCode<T>::value == 2) {
+#pragma unroll
+      for (int i = 0; i < VN / 2; ++i) {
+        v[2 * i] = (float)__builtin_bit_cast(_Float16, (uint16_t)(raw[i] & 0xffffu));
+        v[2 * i + 1] = (float)__builtin_bit_cast(_Float16, (uint16_t)(raw[i] >> 16));
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < VN / 2; ++i) {
+        v[2 * i] = __uint_as_float(raw[i] << 16);
+        v[2 * i + 1] = __uint_as_float(raw[i] & 0xffff0000u);
+      }
+    }
+  }
+};
+template <typename T>
+struct Packet<T, 1> {
+  T raw;
+  __device__ __forceinline__ void load(const T* __restrict__ p) { raw = *p; }
+  __device__ __forceinline__ void get(float (&v)[1]) const { v[0] = to_f32(raw); }
+};
+template <int VN>
+__device__ __forceinline__ float vec_max(const float (&v)[VN], float m) {
+  if constexpr (VN == 1) return max_raw(v[0], m);
+#pragma unroll
+  for (int i = 0; i + 1 < VN; i += 2) m = max3_raw(v[i], v[i + 1], m);
+  return m;
+}
+
+// ---------------------------------------------------------------------------------------------------------------
+// The teacher's row of a distillation, in LDS: q = softmax(y / tau) over the entries that are there.  Entries with the
+// same id are merged into the first of them (in index order: the sums do not depend on timing), the others get id -1.
+// ---------------------------------------------------------------------------------------------------------------
+struct TeacherArgs {
+  const void* logits;
+  const void* ids;
+  int64_t stride, id_stride;
+  int dtype, id_bytes, K;
+};
+// kl [N] and stats [N, 2] of a distillation (token.hip); the arguments have been checked
+int distill_stats(const void* logits, int64_t row_stride, const TeacherArgs& teacher, float temperature, float* kl,
+                  float* stats, void* scratch, int64_t N, int64_t V, int dtype, hipStream_t stream);
+enum { kRowFine = 0, kRowEmpty = 1, kRowBad = 2 };  // nothing there | an id beyond the vocabulary
+
+template <int BT>
+struct TeacherRow {
+  static constexpr int R = (VAE_MAX_TEACHER + BT - 1) / BT;
+  int id[VAE_MAX_TEACHER];
+  float q[VAE_MAX_TEACHER], logq[VAE_MAX_TEACHER];
+
+  __device__ __forceinline__ int load(const TeacherArgs& a, int64_t row, int V, float inv_tau, float scale2) {
+    float y[R];
+    int ids[R];
+    bool bad = false;
+    float m = kLowest;
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      const int k = threadIdx.x + r * BT;
+      y[r] = -INFINITY;
+      ids[r] = -1;
+      if (k < a.K) {
+        const int64_t i = load_id(a.ids, a.id_bytes, row * a.id_stride + k);
+        bad |= i >= V;
+        if (i >= 0 && i < V) {
+          y[r] = load_any(a.logits, a.dtype, row * a.stride + k);
+          ids[r] = (int)i;
+        }
+      }
+      m = max_raw(m, y[r]);
+    }
+    m = block_max<BT>(m);
+    float e[R], s = 0.f;
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      e[r] = ids[r] >= 0 ? exp2_raw((y[r] - m) * scale2) : 0.f;
+      s += e[r];
+    }
+    s = block_sum<BT>(s);
+    const float any_bad = block_sum<BT>(bad ? 1.f : 0.f);
+    lds_barrier();  // the row before this one has been read
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      const int k = threadIdx.x + r * BT;
+      if (k < a.K) {
+        q[k] = e[r] / s;
+        logq[k] = row_log_prob(y[r], m, s, inv_tau);
+        id[k] = e[r] == 0.f ? -1 : ids[r];   // e NaN keeps its id: the row comes out NaN
+      }
+    }
+    lds_barrier();
+    return any_bad > 0.f ? kRowBad : (s == 0.f ? kRowEmpty : kRowFine);
+  }
+};
+
+#define VAE_BY_TYPE(dtype_, ...)                                        \
+  switch (dtype_) {                                                     \
+    case VAE_F32: { using T = float; __VA_ARGS__; } break;              \
+    case VAE_BF16: { using T = bf16_t; __VA_ARGS__; } break;            \
+    case VAE_F16: { using T = f16_t; __VA_ARGS__; } break;              \
+  }
 
 }  // namespace vae

@@ -547,6 +547,13 @@ def _token_rows(x, recon):
     return _vocab_rows(recon, "nll 'categorical'"), x.reshape(-1).contiguous(), x.shape[0]
 
 
+def _token_scratch(logits, top_k, dev):
+    """The pieces of split rows (few rows): the caller's own memory each call, so that calls on several streams and
+    captured graphs share nothing."""
+    n = _lib.load().vae_token_scratch_bytes(logits.shape[0], logits.shape[1], top_k, dtype_code(logits))
+    return torch.empty((n,), dtype=torch.uint8, device=dev) if n else None
+
+
 def _row_sums(rows, scale, B, dtype):
     """[B] = scale * sum over each of B equal runs of `rows` (fp32, summed in double)."""
     out = torch.empty((B,), dtype=dtype, device=rows.device)
@@ -594,10 +601,11 @@ def _token_fwd(logits, tokens, top_k, want_entropy, want_stats):
     stats = new(N, 2) if want_stats else None
     top = new(N, top_k) if top_k else None
     ids = torch.empty((N, top_k), dtype=torch.int64, device=dev) if top_k else None
+    scratch = _token_scratch(logits, top_k, dev)
     with _Guard(dev):
         call('vae_token_logp_fwd', ptr(logits), logits.stride(0), ptr(tokens),
              0 if tokens is None else tokens.element_size(), ptr(logp), ptr(entropy), ptr(stats), ptr(top), ptr(ids),
-             top_k, N, V, dtype_code(logits), stream_ptr(dev))
+             top_k, ptr(scratch), N, V, dtype_code(logits), stream_ptr(dev))
     return logp, entropy, top, ids, stats
 
 
@@ -645,13 +653,14 @@ class _TokenNllElbo(torch.autograd.Function):
         stats = torch.empty((N, 2), dtype=torch.float32, device=dev)
         grad = torch.empty((N, V), dtype=logits.dtype, device=dev) if fuse else None
         loss = elbo = means = None
+        scratch = _token_scratch(logits, 0, dev)
         with _Guard(dev):
             if fuse:
                 call('vae_token_nll_fused', ptr(logits), logits.stride(0), ptr(tokens), tokens.element_size(), ptr(rows),
-                     ptr(stats), ptr(grad), inv_count, N, V, code, st)
+                     ptr(stats), ptr(grad), inv_count, ptr(scratch), N, V, code, st)
             else:
                 call('vae_token_logp_fwd', ptr(logits), logits.stride(0), ptr(tokens), tokens.element_size(), ptr(rows),
-                     None, ptr(stats), None, None, 0, N, V, code, st)
+                     None, ptr(stats), None, None, 0, ptr(scratch), N, V, code, st)
             nll = _row_sums(rows, -1.0, B, logits.dtype)
             if with_elbo:
                 loss, elbo = torch.empty_like(nll), torch.empty_like(nll)
@@ -774,10 +783,11 @@ def _distill_fwd(logits, teacher, ids, temperature, inv_count, want_stats, fuse)
     kl = torch.empty((N,), dtype=torch.float32, device=dev)
     stats = torch.empty((N, 2), dtype=torch.float32, device=dev) if want_stats else None
     grad = torch.empty((N, V), dtype=logits.dtype, device=dev) if fuse else None
+    scratch = _token_scratch(logits, 0, dev)
     with _Guard(dev):
         call('vae_distill_fwd', ptr(logits), logits.stride(0), ptr(teacher), teacher.stride(0), dtype_code(teacher),
              ptr(ids), ids.stride(0), ids.element_size(), ids.shape[1], temperature, ptr(kl), ptr(stats), ptr(grad),
-             inv_count, N, V, dtype_code(logits), stream_ptr(dev))
+             inv_count, ptr(scratch), N, V, dtype_code(logits), stream_ptr(dev))
         mean = _row_sums(kl, inv_count, 1, torch.float32).reshape(())
     return kl, mean, stats, grad
 
@@ -789,8 +799,8 @@ def distill_top_logits(logits, teacher_logits, teacher_ids, temperature=1.0, inv
     mean = inv_count * sum(kl), inv_count = 1 / rows unless given (1 / unpadded rows, times temperature^2 where the
     loss is to be weighted so).  Differentiable with respect to `logits` only.
 
-    A negative id or a teacher logit of -inf is no entry; a row without entries has kl 0 and gradient 0 and is not read;
-    an id may come twice; an id beyond the vocabulary gives NaN.  `fuse_backward`: d(mean)/d(logits) is formed by the
+    A negative id or a teacher logit of -inf is no entry; a row without entries has kl 0 and gradient 0 whatever it
+    holds; an id may come twice; an id beyond the vocabulary gives NaN.  `fuse_backward`: d(mean)/d(logits) is formed by the
     forward launch (one read of the logits per step instead of two); a gradient on `kl` takes the general kernel."""
     shape = logits.shape[:-1]
     rows = _vocab_rows(logits, 'distill_top_logits')
