@@ -12,6 +12,7 @@
 namespace vae {
 
 constexpr int kCand = 1024;          // candidates for the alternatives that LDS holds
+constexpr int kVecBytes = 16;
 constexpr float kHuge = 1.0e6f;      // |max| beyond which the shifted exponent is formed as (x - m) c, see row_stats
 
 struct FwdArgs {
@@ -62,7 +63,7 @@ __device__ __forceinline__ void row_stats(const T* __restrict__ x, const RowCut<
                                           float edge, bool has_edge, float c, float& m, float& s, float& t, float& mine,
                                           int& tile) {
   constexpr int VN = VecOf<T>::n, U = 4;
-  const T* body = x + cut.head;
+  const Buffer body(x + cut.head, cut.nvec * kVecBytes);
   RunStats<ENT> st(c);
   tile = -1;
   int j = v0 + (int)threadIdx.x;
@@ -71,7 +72,7 @@ __device__ __forceinline__ void row_stats(const T* __restrict__ x, const RowCut<
   for (int it = 0; it < full; ++it, j += U * BT) {
     Packet<T, VN> p[U];
 #pragma unroll
-    for (int u = 0; u < U; ++u) p[u].load(body + (int64_t)(j + u * BT) * VN);
+    for (int u = 0; u < U; ++u) p[u].load(body, j * kVecBytes, u * BT * kVecBytes);
     float v[U][VN], mt = -INFINITY;
 #pragma unroll
     for (int u = 0; u < U; ++u) {
@@ -87,7 +88,7 @@ __device__ __forceinline__ void row_stats(const T* __restrict__ x, const RowCut<
   }
   for (; j < v1; j += BT) {
     Packet<T, VN> p;
-    p.load(body + (int64_t)j * VN);
+    p.load(body, j * kVecBytes, 0);
     float v[VN];
     p.get(v);
     const float mt = vec_max(v, -INFINITY);
@@ -123,7 +124,7 @@ __device__ __forceinline__ void row_stats(const T* __restrict__ x, const RowCut<
   };
   for (j = v0 + (int)threadIdx.x; j < v1; j += BT) {
     Packet<T, VN> p;
-    p.load(body + (int64_t)j * VN);
+    p.load(body, j * kVecBytes, 0);
     float v[VN];
     p.get(v);
 #pragma unroll
@@ -204,7 +205,7 @@ __device__ __forceinline__ void row_top(TopLds<BT>& lds, const T* __restrict__ x
                                         int v0, int v1, float edge, int edge_index, float mine, int tile, int k,
                                         Emit emit) {
   constexpr int VN = VecOf<T>::n, U = 4;
-  const T* body = x + cut.head;
+  const Buffer body(x + cut.head, cut.nvec * kVecBytes);
   auto vec_key = [&](int j, int i, float v) { return order_key(v, (uint32_t)(cut.index(j) + i)); };
   uint64_t key = edge_index >= 0 ? order_key(edge, (uint32_t)edge_index) : 0;
   if (tile >= 0) {
@@ -215,7 +216,7 @@ __device__ __forceinline__ void row_top(TopLds<BT>& lds, const T* __restrict__ x
       const int j = tile + u * BT;
       if (j < v1) {
         Packet<T, VN> p;
-        p.load(body + (int64_t)j * VN);
+        p.load(body, j * kVecBytes, 0);
         float v[VN];
         p.get(v);
 #pragma unroll
@@ -233,7 +234,7 @@ __device__ __forceinline__ void row_top(TopLds<BT>& lds, const T* __restrict__ x
   for (int q = wave; q < nseg; q += BT / 64) {
     for (int j = v0 + lds.seg[q] + lane * BT; j < v1; j += 64 * BT) {
       Packet<T, VN> p;
-      p.load(body + (int64_t)j * VN);
+      p.load(body, j * kVecBytes, 0);
       float v[VN];
       p.get(v);
 #pragma unroll
@@ -248,7 +249,7 @@ __device__ __forceinline__ void row_top(TopLds<BT>& lds, const T* __restrict__ x
     if (best >= last) best = 0;
     for (int j = v0 + (int)threadIdx.x; j < v1; j += BT) {
       Packet<T, VN> p;
-      p.load(body + (int64_t)j * VN);
+      p.load(body, j * kVecBytes, 0);
       float v[VN];
       p.get(v);
 #pragma unroll
@@ -317,7 +318,7 @@ __global__ __launch_bounds__(BT) void token_fwd_kernel(FwdArgs a) {
         if (state != kRowFine) {
           if (threadIdx.x == 0) {
             a.logp[row] = state == kRowEmpty ? 0.f : nan_f();
-            if (a.stats) a.stats[2 * row] = a.stats[2 * row + 1] = 0.f;
+            if (a.stats) a.stats[2 * row] = 0.f, a.stats[2 * row + 1] = a.logp[row];  // the backward's sign of either
           }
           continue;
         }
@@ -374,7 +375,7 @@ __global__ __launch_bounds__(BT) void token_join_kernel(FwdArgs a) {
       if (state != kRowFine) {
         if (threadIdx.x == 0) {
           a.logp[row] = state == kRowEmpty ? 0.f : nan_f();
-          if (a.stats) a.stats[2 * row] = a.stats[2 * row + 1] = 0.f;
+          if (a.stats) a.stats[2 * row] = 0.f, a.stats[2 * row + 1] = a.logp[row];
         }
         continue;
       }
@@ -528,6 +529,9 @@ int vae_token_logp_fwd(const void* logits, int64_t row_stride, const void* token
   if (N == 0) return VAE_OK;
   if (!logits || (tokens && token_bytes != 4 && token_bytes != 8)) return VAE_ERR_ARG;
   if ((logp && !tokens) || (top_k > 0 && (!top_logp || !top_ids))) return VAE_ERR_ARG;
+  int rc = VAE_OK;
+  ShortArgs sa = {logits, row_stride, tokens, token_bytes, N, (int)V, logp, entropy, stats, top_logp, top_ids, (int)top_k};
+  if (short_rows(sa, dtype, (hipStream_t)stream, &rc)) return rc;
   const Cut cut = cut_rows(N, V, dtype);
   if (cut.parts > 1 && !scratch) return VAE_ERR_ARG;
   const FwdArgs a = {logits, row_stride, tokens, token_bytes, logp, entropy, stats, top_logp, top_ids, (int)top_k, N,

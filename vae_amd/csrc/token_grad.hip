@@ -86,8 +86,7 @@ struct Adds {
     auto add = [&](int id, float g) {
       const int e = id - index;
 #pragma unroll
-      for (int i = 0; i < W; ++i)
-        if (e == i) v[i] += g;
+      for (int i = 0; i < W; ++i) v[i] += e == i ? g : 0.f;   // as a select: v stays in registers
     };
     if constexpr (LIST) {
       for (int k = lds->head[threadIdx.x]; k >= 0; k = lds->next[k]) add(lds->id[k], lds->g[k]);
@@ -102,7 +101,7 @@ struct GradArgs {
   int64_t row_stride;
   void* glogits;
   int64_t N;
-  int V, parts, part_vecs;
+  int V, parts;
   bool nts;
   float scale2, inv_tau;
   const float* stats_in;
@@ -123,22 +122,47 @@ struct GradArgs {
   float *out, *stats_out;            // logp or kl, and the statistics
 };
 
-template <typename T, int VN, int BT>
-__device__ __forceinline__ void fill_row(T* __restrict__ gx, const RowCut<T, VN>& cut, int v0, int v1, int edge,
-                                         float value, bool nts) {
-  float v[VN];
+// A thread's U vectors of a piece of a row, v0 + tid, v0 + tid + BT, ...  `nvec`: vectors of the piece (a piece is at
+// most U * BT vectors, 1 MiB).
+template <typename T, int VN, int BT, int U>
+struct Piece {
+  typedef Packet<T, VN> P;
+  P p[U];
+  const Buffer in, out;
+  const int nvec, byte;
+
+  __device__ __forceinline__ Piece(const T* x, T* gx, const RowCut<T, VN>& cut, int v0, int nvec_)
+      : in(x + cut.index(v0), nvec_ * P::kBytes), out(gx + cut.index(v0), nvec_ * P::kBytes), nvec(nvec_),
+        byte((int)threadIdx.x * P::kBytes) {}
+  __device__ __forceinline__ bool any(int u) const { return u * BT < nvec; }   // the same for all threads
+  __device__ __forceinline__ void load() {
 #pragma unroll
-  for (int i = 0; i < VN; ++i) v[i] = value;
-  for (int j = v0 + (int)threadIdx.x; j < v1; j += BT) store_vec<T, VN>(nts, gx + cut.index(j), v);
-  if (edge >= 0) gx[edge] = from_f32<T>(value);
-}
+    for (int u = 0; u < U; ++u) p[u].load(in, byte, u * BT * P::kBytes);
+  }
+  __device__ __forceinline__ void mask() {       // what is not there counts as masked out
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if ((u + 1) * BT > nvec && (int)threadIdx.x + u * BT >= nvec) p[u].set_masked();
+  }
+  __device__ __forceinline__ void store(bool nts, int u, const float (&v)[VN]) const {
+    P::store(out, nts, byte, u * BT * P::kBytes, v);
+  }
+  __device__ __forceinline__ void fill(bool nts, float value) const {
+    float v[VN];
+#pragma unroll
+    for (int i = 0; i < VN; ++i) v[i] = value;
+#pragma unroll
+    for (int u = 0; u < U; ++u) store(nts, u, v);
+  }
+};
 
 // ---------------------------------------------------------------------------------------------------------------
-// from given statistics: one read, one write; a row is cut into pieces of at most 32 vectors a thread
+// from given statistics: one read, one write.  A workgroup takes one piece of U vectors a thread, all loads in front of
+// all stores: in a loop the loads of a turn wait for the stores of the turn before it (4096 x 32768 bf16: 153 us with
+// a loop over U = 4, see bwd_launch for what one piece takes).
 // ---------------------------------------------------------------------------------------------------------------
-template <typename T, int VN, int BT, bool ENT, bool LIST, bool DIST>
+template <typename T, int VN, int BT, int U, bool ENT, bool LIST, bool DIST>
 __global__ __launch_bounds__(BT) void token_bwd_kernel(GradArgs a) {
-  constexpr int U = 4;
   __shared__ struct {
     Entries<BT> entries[LIST ? 1 : 0];
     TeacherRow<BT> teacher[DIST ? 1 : 0];
@@ -149,34 +173,37 @@ __global__ __launch_bounds__(BT) void token_bwd_kernel(GradArgs a) {
     const T* x = (const T*)a.logits + row * a.row_stride;
     T* gx = (T*)a.glogits + row * (int64_t)a.V;
     const RowCut<T, VN> cut(x, a.V);
-    const int v0 = part * a.part_vecs;
-    int v1 = v0 + a.part_vecs;
-    v1 = v1 < cut.nvec ? v1 : cut.nvec;
+    const int v0 = part * (U * BT);
+    const int left = cut.nvec - v0;
+    const int v1 = v0 + (left < 0 ? 0 : (left < U * BT ? left : U * BT));
     int ei = cut.edge(threadIdx.x);
     if (ei >= 0 && (ei < cut.head ? part != 0 : part != a.parts - 1)) ei = -1;
+    Piece<T, VN, BT, U> piece(x, gx, cut, v0, v1 - v0);
     const float m = a.stats_in[2 * row], s = a.stats_in[2 * row + 1];
+    const int64_t tok = !DIST && a.tokens ? load_id(a.tokens, a.token_bytes, row) : 0;
+    if (tok < 0 || s == 0.f) {
+      piece.fill(a.nts, 0.f);
+      if (ei >= 0) gx[ei] = from_f32<T>(0.f);
+      continue;
+    }
+    piece.load();
+    const float edge = ei >= 0 ? to_f32(x[ei]) : 0.f;
     Adds<T, VN, BT, LIST> adds;
     if constexpr (LIST) adds.lds = lds.entries;
     float A, B = 0.f;
-    bool zero, bad = false;
     const float inv = 1.0f / s;
     if constexpr (DIST) {
-      const int state = lds.teacher[0].load(a.teacher, row, a.V, a.inv_tau, a.scale2);
+      lds.teacher[0].load(a.teacher, row, a.V, a.inv_tau, a.scale2);   // an id beyond the vocabulary: s is NaN
       const float g0 = a.gmean ? a.gmean[0] * a.mean_scale : (a.gkl ? 0.f : a.mean_scale);
       const float w = ((a.gkl ? a.gkl[row] : 0.f) + g0) * a.inv_tau;
-      zero = state == kRowEmpty || (state == kRowFine && s == 0.f);
-      bad = state == kRowBad;
       A = w * inv;
-      if (!zero && !bad)
-        for (int k = threadIdx.x; k < a.teacher.K; k += BT) {
-          lds.entries[0].id[k] = lds.teacher[0].id[k];
-          lds.entries[0].g[k] = -w * lds.teacher[0].q[k];
-        }
+      for (int k = threadIdx.x; k < a.teacher.K; k += BT) {
+        lds.entries[0].id[k] = lds.teacher[0].id[k];
+        lds.entries[0].g[k] = -w * lds.teacher[0].q[k];
+      }
     } else {
-      const int64_t tok = a.tokens ? load_id(a.tokens, a.token_bytes, row) : 0;
-      zero = tok < 0 || s == 0.f;
       float gt = a.tokens ? (a.glogp ? a.glogp[row / a.rows_per_g] * a.g_scale : a.g_scale) : 0.f;
-      const bool inside = a.tokens && tok >= 0 && tok < a.V;
+      const bool inside = a.tokens && tok < a.V;
       if (tok >= a.V && (!a.glogp || a.g_scale != 0.f)) gt = nan_f();
       float sum = gt;
       adds.one_id = inside ? (int)tok : -1;
@@ -184,11 +211,10 @@ __global__ __launch_bounds__(BT) void token_bwd_kernel(GradArgs a) {
       if constexpr (LIST) {
         for (int k = 0; k < a.top_k; ++k) sum += a.gtop[row * a.top_k + k];
         lds_barrier();  // the row before this one has been read
-        if (!zero)
-          for (int k = threadIdx.x; k <= a.top_k; k += BT) {
-            lds.entries[0].id[k] = k == 0 ? adds.one_id : (int)a.top_ids[row * a.top_k + k - 1];
-            lds.entries[0].g[k] = k == 0 ? gt : a.gtop[row * a.top_k + k - 1];
-          }
+        for (int k = threadIdx.x; k <= a.top_k; k += BT) {
+          lds.entries[0].id[k] = k == 0 ? adds.one_id : (int)a.top_ids[row * a.top_k + k - 1];
+          lds.entries[0].g[k] = k == 0 ? gt : a.gtop[row * a.top_k + k - 1];
+        }
       }
       if constexpr (ENT) {
         const float gh = a.gentropy[row];
@@ -197,10 +223,6 @@ __global__ __launch_bounds__(BT) void token_bwd_kernel(GradArgs a) {
       }
       A = -sum * inv;
     }
-    if (zero || bad) {
-      fill_row<T, VN, BT>(gx, cut, v0, v1, ei, zero ? 0.f : nan_f(), a.nts);
-      continue;
-    }
     if constexpr (LIST) lds.entries[0].template link<T, VN>(DIST ? a.teacher.K : a.top_k + 1, cut, v0, v1);
     adds.prepare(cut, v0, v1);
     auto grad = [&](float v) {
@@ -208,34 +230,18 @@ __global__ __launch_bounds__(BT) void token_bwd_kernel(GradArgs a) {
       const float e = exp2_raw(d);
       return ENT ? e * __builtin_fmaf(B, max_raw(d, -300.f), A) : e * A;
     };
-    int j = v0 + (int)threadIdx.x, bit = 0;
-    const int full = (v1 - v0) / (U * BT);
-    for (int it = 0; it < full; ++it, j += U * BT, bit += U) {
-      Packet<T, VN> p[U];
 #pragma unroll
-      for (int u = 0; u < U; ++u) p[u].load(x + cut.index(j + u * BT));
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
+    for (int u = 0; u < U; ++u)
+      if (piece.any(u)) {
         float v[VN];
-        p[u].get(v);
+        piece.p[u].get(v);
 #pragma unroll
         for (int i = 0; i < VN; ++i) v[i] = grad(v[i]);
-        if (adds.mask >> (bit + u) & 1u) adds.to(cut.index(j + u * BT), v);
-        store_vec<T, VN>(a.nts, gx + cut.index(j + u * BT), v);
+        if (adds.mask >> u & 1u) adds.to(cut.index(v0 + u * BT + (int)threadIdx.x), v);
+        piece.store(a.nts, u, v);
       }
-    }
-    for (; j < v1; j += BT, ++bit) {
-      Packet<T, VN> p;
-      p.load(x + cut.index(j));
-      float v[VN];
-      p.get(v);
-#pragma unroll
-      for (int i = 0; i < VN; ++i) v[i] = grad(v[i]);
-      if (adds.mask >> bit & 1u) adds.to(cut.index(j), v);
-      store_vec<T, VN>(a.nts, gx + cut.index(j), v);
-    }
     if (ei >= 0) {
-      float v[1] = {grad(to_f32(x[ei]))};
+      float v[1] = {grad(edge)};
       adds.to(ei, v);
       gx[ei] = from_f32<T>(v[0]);
     }
@@ -243,10 +249,12 @@ __global__ __launch_bounds__(BT) void token_bwd_kernel(GradArgs a) {
 }
 
 // ---------------------------------------------------------------------------------------------------------------
-// loss and gradient in one pass: a workgroup holds its row in registers (U vectors a thread), as the 16-byte packets it
-// was read in: 4 registers a vector whatever the type
+// loss and gradient in one pass: a workgroup holds its row in registers, U vectors a thread.
+//   KEEP: every element's exponential against the thread's own maximum, in float32: one exponential an element, the
+//         gradient is a product.  8 registers a 16-bit vector, 4 an fp32 one.
+//   else: the packets as they were read, 4 registers a vector whatever the type; the exponentials are formed twice.
 // ---------------------------------------------------------------------------------------------------------------
-template <typename T, int BT, int U, bool DIST>
+template <typename T, int BT, int U, bool KEEP, bool DIST>
 __global__ __launch_bounds__(BT) void token_fused_kernel(GradArgs a) {
   constexpr int VN = VecOf<T>::n;
   __shared__ struct {
@@ -258,94 +266,112 @@ __global__ __launch_bounds__(BT) void token_fused_kernel(GradArgs a) {
     T* gx = (T*)a.glogits + row * (int64_t)a.V;
     const RowCut<T, VN> cut(x, a.V);
     const int ei = cut.edge(threadIdx.x);
+    Piece<T, VN, BT, U> piece(x, gx, cut, 0, cut.nvec);
     int64_t tok = 0;
     int state = kRowFine;
+    typename TeacherRow<BT>::Mine mine;
     if constexpr (DIST) {
-      state = lds.teacher[0].load(a.teacher, row, a.V, a.inv_tau, a.scale2);
+      if (!TeacherRow<BT>::fetch(mine, a.teacher, row, a.V)) state = kRowEmpty;
     } else {
       tok = load_id(a.tokens, a.token_bytes, row);
       state = tok < 0 ? kRowEmpty : (tok >= a.V ? kRowBad : kRowFine);
     }
     if (state != kRowFine) {
       const float v = state == kRowEmpty ? 0.f : nan_f();
-      fill_row<T, VN, BT>(gx, cut, 0, cut.nvec, ei, v, a.nts);
+      piece.fill(a.nts, v);
+      if (ei >= 0) gx[ei] = from_f32<T>(v);
       if (threadIdx.x == 0) {
         a.out[row] = v;
         a.stats_out[2 * row] = 0.f;
-        a.stats_out[2 * row + 1] = DIST ? 0.f : v;
+        a.stats_out[2 * row + 1] = v;
       }
       continue;
     }
-    Packet<T, VN> p[U];
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int j = threadIdx.x + u * BT;
-      if (j < cut.nvec) p[u].load(x + cut.index(j));
-    }
+    piece.load();
     const float edge = ei >= 0 ? to_f32(x[ei]) : -INFINITY;
-    float m = max_raw(edge, kLowest);
-#pragma unroll
-    for (int u = 0; u < U; ++u)
-      if ((int)threadIdx.x + u * BT < cut.nvec) {
-        float v[VN];
-        p[u].get(v);
-        m = vec_max(v, m);
-      }
-    m = block_max<BT>(m);
-    float s = ei >= 0 ? exp2_raw((edge - m) * a.scale2) : 0.f;
-#pragma unroll
-    for (int u = 0; u < U; ++u)
-      if ((int)threadIdx.x + u * BT < cut.nvec) {
-        asm volatile("" : "+v"(p[u].raw));   // unpack again: the packets, not their elements, stay in registers
-        float v[VN];
-        p[u].get(v);
-#pragma unroll
-        for (int i = 0; i < VN; ++i) s += exp2_raw((v[i] - m) * a.scale2);
-      }
-    s = block_sum<BT>(s);
     Adds<T, VN, BT, DIST> adds;
     const float w = DIST ? a.mean_scale * a.inv_tau : a.g_scale;   // of p; the entries have the other sign
     if constexpr (DIST) {
-      adds.lds = lds.entries;
-      float kl = 0.f;
+      // while the row is on its way
+      state = lds.teacher[0].finish(mine, a.teacher, a.V, a.inv_tau, a.scale2);
       for (int k = threadIdx.x; k < a.teacher.K; k += BT) {
         const int id = lds.teacher[0].id[k];
-        const float q = lds.teacher[0].q[k];
-        if (id >= 0) kl += q * (lds.teacher[0].logq[k] - row_log_prob(to_f32(x[id]), m, s, a.inv_tau));
+        lds.teacher[0].x[k] = id >= 0 ? to_f32(x[id]) : 0.f;
         lds.entries[0].id[k] = id;
-        lds.entries[0].g[k] = -w * q;
+        lds.entries[0].g[k] = -w * lds.teacher[0].q[k];
       }
-      kl = block_sum<BT>(kl);
-      if (threadIdx.x == 0) a.out[row] = kl;
+      adds.lds = lds.entries;
       lds.entries[0].template link<T, VN>(a.teacher.K, cut, 0, cut.nvec);
     } else {
       adds.one_id = (int)tok;
       adds.one_g = -w;
-      if (threadIdx.x == 0) a.out[row] = row_log_prob(to_f32(x[tok]), m, s, 1.0f);
+    }
+    adds.prepare(cut, 0, cut.nvec);
+    piece.mask();
+    float mt = max_raw(edge, kLowest);
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (piece.any(u)) {
+        float v[VN];
+        piece.p[u].get(v);
+        mt = vec_max(v, mt);
+      }
+    float e[KEEP ? U : 1][VN];
+    float s = exp2_raw((edge - mt) * a.scale2);
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (piece.any(u)) {
+        asm volatile("" : "+v"(piece.p[u].raw));   // unpack again: the packets, not their elements, stay in registers
+        float v[VN];
+        piece.p[u].get(v);
+#pragma unroll
+        for (int i = 0; i < VN; ++i) {
+          const float ev = exp2_raw((v[i] - mt) * a.scale2);
+          s += ev;
+          if constexpr (KEEP) e[u][i] = ev;
+        }
+      }
+    const float m = block_max<BT>(mt);
+    float f = exp2_raw((mt - m) * a.scale2);       // from the thread's maximum to the row's
+    s = block_sum<BT>(s * f);
+    if (DIST && state == kRowBad) s = nan_f();
+    if constexpr (DIST) {
+      float kl = 0.f;
+      for (int k = threadIdx.x; k < a.teacher.K; k += BT)
+        if (lds.teacher[0].id[k] >= 0)
+          kl += lds.teacher[0].q[k] * (lds.teacher[0].logq[k] - row_log_prob(lds.teacher[0].x[k], m, s, a.inv_tau));
+      kl = block_sum<BT>(kl);
+      if (threadIdx.x == 0) a.out[row] = state == kRowBad ? nan_f() : kl;
+    } else if (threadIdx.x == 0) {
+      a.out[row] = row_log_prob(to_f32(x[tok]), m, s, 1.0f);
     }
     if (threadIdx.x == 0) {
       a.stats_out[2 * row] = m;
       a.stats_out[2 * row + 1] = s;
     }
     if (s == 0.f) {
-      fill_row<T, VN, BT>(gx, cut, 0, cut.nvec, ei, 0.f, a.nts);
+      piece.fill(a.nts, 0.f);
+      if (ei >= 0) gx[ei] = from_f32<T>(0.f);
       continue;
     }
-    adds.prepare(cut, 0, cut.nvec);
     const float A = w / s;
+    f *= A;
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int j = threadIdx.x + u * BT;
-      if (j < cut.nvec) {
-        asm volatile("" : "+v"(p[u].raw));
+    for (int u = 0; u < U; ++u)
+      if (piece.any(u)) {
         float v[VN];
-        p[u].get(v);
+        if constexpr (KEEP) {
 #pragma unroll
-        for (int i = 0; i < VN; ++i) v[i] = A * exp2_raw((v[i] - m) * a.scale2);
-        if (adds.mask >> u & 1u) adds.to(cut.index(j), v);
-        store_vec<T, VN>(a.nts, gx + cut.index(j), v);
+          for (int i = 0; i < VN; ++i) v[i] = f * e[u][i];
+        } else {
+          asm volatile("" : "+v"(piece.p[u].raw));
+          piece.p[u].get(v);
+#pragma unroll
+          for (int i = 0; i < VN; ++i) v[i] = A * exp2_raw((v[i] - m) * a.scale2);
+        }
+        if (adds.mask >> u & 1u) adds.to(cut.index(u * BT + (int)threadIdx.x), v);
+        piece.store(a.nts, u, v);
       }
-    }
     if (ei >= 0) {
       float v[1] = {A * exp2_raw((edge - m) * a.scale2)};
       adds.to(ei, v);
@@ -385,25 +411,21 @@ static bool same_phase(const GradArgs& a) {
   return by % 16 == 0 && (a.N <= 1 || (a.row_stride - a.V) * (int64_t)sizeof(T) % 16 == 0);
 }
 
-template <typename T, int VN, int BT, bool ENT, bool LIST, bool DIST>
+template <typename T, int VN, int BT, int U, bool ENT, bool LIST, bool DIST>
 static int bwd_launch(GradArgs a, hipStream_t st) {
-  // pieces of at most 32 vectors a thread (Adds::mask), more of them while the rows alone do not fill the chip
   const int64_t nvec = ((int64_t)a.V + VN - 1) / VN;
-  int64_t parts = (nvec + 32 * BT - 1) / (32 * BT);
-  const int64_t most = (nvec + 4 * BT - 1) / (4 * BT);
-  while (parts < most && a.N * parts < 2048) parts *= 2;
-  parts = parts < most ? parts : most;
-  const int64_t per = (nvec + parts - 1) / parts;
-  a.parts = (int)((nvec + per - 1) / per);
-  a.part_vecs = (int)per;
+  a.parts = (int)((nvec + U * BT - 1) / (U * BT));
   a.nts = (int64_t)sizeof(T) * a.N * a.V >= kNtStoreMinBytes;
-  hipLaunchKernelGGL((token_bwd_kernel<T, VN, BT, ENT, LIST, DIST>), dim3(grid_for(a.N * a.parts)), dim3(BT), 0, st, a);
+  hipLaunchKernelGGL((token_bwd_kernel<T, VN, BT, U, ENT, LIST, DIST>), dim3(grid_for(a.N * a.parts)), dim3(BT), 0, st,
+                     a);
   return launched();
 }
 template <typename T, int VN, bool ENT, bool LIST, bool DIST>
 static int bwd_block(const GradArgs& a, hipStream_t st) {
-  if (((int64_t)a.V + VN - 1) / VN <= 512) return bwd_launch<T, VN, 64, ENT, LIST, DIST>(a, st);
-  return bwd_launch<T, VN, kBlock, ENT, LIST, DIST>(a, st);
+  const int64_t nvec = ((int64_t)a.V + VN - 1) / VN;
+  if (nvec <= 256) return bwd_launch<T, VN, 64, 4, ENT, LIST, DIST>(a, st);
+  // the entries are prepared once a piece: longer pieces where there are many
+  return bwd_launch<T, VN, kBlock, LIST ? 8 : 4, ENT, LIST, DIST>(a, st);
 }
 template <typename T, int VN, bool DIST>
 static int bwd_kind(const GradArgs& a, hipStream_t st) {
@@ -419,23 +441,24 @@ static int bwd_type(const GradArgs& a, hipStream_t st) {
   return same_phase<T>(a) ? bwd_kind<T, VecOf<T>::n, DIST>(a, st) : bwd_kind<T, 1, DIST>(a, st);
 }
 
-template <typename T, int BT, int U, bool DIST>
+template <typename T, int BT, int U, bool KEEP, bool DIST>
 static int fused_launch(GradArgs a, hipStream_t st) {
   a.nts = (int64_t)sizeof(T) * a.N * a.V >= kNtStoreMinBytes;
-  hipLaunchKernelGGL((token_fused_kernel<T, BT, U, DIST>), dim3(grid_for(a.N)), dim3(BT), 0, st, a);
+  hipLaunchKernelGGL((token_fused_kernel<T, BT, U, KEEP, DIST>), dim3(grid_for(a.N)), dim3(BT), 0, st, a);
   return launched();
 }
 // true when the one-pass kernel takes this call: the row fits a workgroup's registers, and there are rows enough
 template <typename T, bool DIST>
 static bool fused_type(const GradArgs& a, hipStream_t st, int* rc) {
+  constexpr int E = 64 / VecOf<T>::n;    // vectors a thread: 64 elements
   const int64_t nvec = (int64_t)a.V / VecOf<T>::n;
   if (!same_phase<T>(a) || nvec > 16384 || (a.N < 256 && nvec > 4096)) return false;
-  if (nvec <= 512) *rc = fused_launch<T, 64, 8, DIST>(a, st);
-  else if (nvec <= 1024) *rc = fused_launch<T, 256, 4, DIST>(a, st);
-  else if (nvec <= 2048) *rc = fused_launch<T, 256, 8, DIST>(a, st);
-  else if (nvec <= 4096) *rc = fused_launch<T, 256, 16, DIST>(a, st);
-  else if (nvec <= 8192) *rc = fused_launch<T, 512, 16, DIST>(a, st);
-  else *rc = fused_launch<T, 1024, 16, DIST>(a, st);
+  if (nvec <= 64 * E) *rc = fused_launch<T, 64, E, true, DIST>(a, st);
+  else if (nvec <= 128 * E) *rc = fused_launch<T, 128, E, true, DIST>(a, st);
+  else if (nvec <= 256 * E) *rc = fused_launch<T, 256, E, true, DIST>(a, st);
+  else if (nvec <= 512 * E) *rc = fused_launch<T, 512, E, true, DIST>(a, st);
+  else if (nvec <= 1024 * E) *rc = fused_launch<T, 1024, E, true, DIST>(a, st);
+  else *rc = fused_launch<T, 1024, 16, false, DIST>(a, st);
   return true;
 }
 
@@ -462,6 +485,10 @@ int vae_token_logp_bwd(const void* logits, int64_t row_stride, const void* token
   if (N == 0) return VAE_OK;
   if (!logits || !stats || !glogits || (tokens && token_bytes != 4 && token_bytes != 8)) return VAE_ERR_ARG;
   if ((gentropy && !entropy) || (top_k > 0 && (!gtop || !top_ids)) || (glogp && !tokens)) return VAE_ERR_ARG;
+  int rc = VAE_OK;
+  ShortArgs sa = {logits, row_stride, tokens, token_bytes, N, (int)V, nullptr, nullptr, nullptr, nullptr, nullptr, 0,
+                  glogits, glogp, rows_per_g, g_scale, gentropy, gtop, top_ids, (int)top_k};
+  if (short_rows(sa, dtype, (hipStream_t)stream, &rc)) return rc;
   GradArgs a = {};
   a.logits = logits; a.row_stride = row_stride; a.glogits = glogits; a.N = N; a.V = (int)V;
   a.scale2 = kLog2e; a.inv_tau = 1.0f; a.stats_in = stats;
@@ -477,11 +504,14 @@ int vae_token_nll_fused(const void* logits, int64_t row_stride, const void* toke
   if (bad_rows(N, V, row_stride, dtype)) return VAE_ERR_ARG;
   if (N == 0) return VAE_OK;
   if (!logits || !tokens || !logp || !stats || !glogits || (token_bytes != 4 && token_bytes != 8)) return VAE_ERR_ARG;
+  int rc = VAE_ERR_ARG;
+  ShortArgs sa = {logits, row_stride, tokens, token_bytes, N, (int)V, logp, nullptr, stats, nullptr, nullptr, 0,
+                  glogits, nullptr, 1, -grad_scale, nullptr, nullptr, nullptr, 0};
+  if (short_rows(sa, dtype, (hipStream_t)stream, &rc)) return rc;
   GradArgs a = {};
   a.logits = logits; a.row_stride = row_stride; a.glogits = glogits; a.N = N; a.V = (int)V;
   a.scale2 = kLog2e; a.inv_tau = 1.0f;
   a.tokens = tokens; a.token_bytes = token_bytes; a.g_scale = grad_scale; a.out = logp; a.stats_out = stats;
-  int rc = VAE_ERR_ARG;
   VAE_BY_TYPE(dtype, if (fused_type<T, false>(a, (hipStream_t)stream, &rc)) return rc);
   rc = vae_token_logp_fwd(logits, row_stride, tokens, token_bytes, logp, nullptr, stats, nullptr, nullptr, 0, scratch, N,
                           V, dtype, stream);

@@ -132,37 +132,71 @@ struct RowCut {
   __device__ __forceinline__ int index(int vec) const { return head + vec * VN; }
 };
 
-// raw 16-byte packet of a row and its elements as floats
+// A run of memory behind a buffer descriptor: the base and the length sit in scalar registers, a lane brings one 32-bit
+// byte offset for all its accesses, and the hardware checks every access against the length: a load beyond it returns
+// zeros and a store beyond it is dropped, without a branch or a predicate.
+struct Buffer {
+  __amdgpu_buffer_rsrc_t rsrc;
+  __device__ __forceinline__ Buffer(const void* base, int bytes)
+      : rsrc(__builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), 0, bytes, 0x00020000)) {}
+};
+constexpr int kNonTemporal = 2;   // cache policy operand of the buffer instructions
+
+// Raw 16-byte packet of a row and its elements as floats.
 template <typename T, int VN>
 struct Packet {
-  typename PackOf<T, VN>::type raw;
-  __device__ __forceinline__ void load(const T* __restrict__ p) {
-    raw = __builtin_nontemporal_load(reinterpret_cast<const typename PackOf<T, VN>::type*>(p));
+  typedef uint32_t Raw __attribute__((ext_vector_type(4)));
+  static constexpr int kBytes = 16;
+  Raw raw;
+  __device__ __forceinline__ void load(const Buffer& b, int lane_byte, int byte) {
+    raw = __builtin_amdgcn_raw_buffer_load_b128(b.rsrc, lane_byte, byte, kNonTemporal);
+  }
+  __device__ __forceinline__ void set_masked() {   // every element -inf
+    const uint32_t inf = sizeof(T) == 4 ? 0xff800000u : (DTypeCode<T>::value == 2 ? 0xfc00fc00u : 0xff80ff80u);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) raw[i] = inf;
   }
   __device__ __forceinline__ void get(float (&v)[VN]) const {
-    if constexpr (sizeof(T) == 4) {
 #pragma unroll
-      for (int i = 0; i < VN; ++i) v[i] = raw[i];
-    } else if constexpr (DTypeCode<T>::value == 2) {
-#pragma unroll
-      for (int i = 0; i < VN / 2; ++i) {
+    for (int i = 0; i < 4; ++i) {
+      if constexpr (sizeof(T) == 4) {
+        v[i] = __uint_as_float(raw[i]);
+      } else if constexpr (DTypeCode<T>::value == 2) {
         v[2 * i] = (float)__builtin_bit_cast(_Float16, (uint16_t)(raw[i] & 0xffffu));
         v[2 * i + 1] = (float)__builtin_bit_cast(_Float16, (uint16_t)(raw[i] >> 16));
-      }
-    } else {
-#pragma unroll
-      for (int i = 0; i < VN / 2; ++i) {
+      } else {
         v[2 * i] = __uint_as_float(raw[i] << 16);
         v[2 * i + 1] = __uint_as_float(raw[i] & 0xffff0000u);
       }
     }
   }
+  __device__ __forceinline__ static void store(const Buffer& b, bool nts, int lane_byte, int byte,
+                                               const float (&v)[VN]) {
+    Raw r;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if constexpr (sizeof(T) == 4) r[i] = __float_as_uint(v[i]);
+      else r[i] = pack2<T>(v[2 * i], v[2 * i + 1]);
+    }
+    if (nts) __builtin_amdgcn_raw_buffer_store_b128(r, b.rsrc, lane_byte, byte, kNonTemporal);
+    else __builtin_amdgcn_raw_buffer_store_b128(r, b.rsrc, lane_byte, byte, 0);
+  }
 };
+// rows whose gradient is not aligned as they are: element by element
 template <typename T>
 struct Packet<T, 1> {
+  static constexpr int kBytes = sizeof(T);
   T raw;
-  __device__ __forceinline__ void load(const T* __restrict__ p) { raw = *p; }
+  __device__ __forceinline__ void load(const Buffer& b, int lane_byte, int byte) {
+    if constexpr (sizeof(T) == 4) raw = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(b.rsrc, lane_byte, byte, 0));
+    else raw.bits = __builtin_amdgcn_raw_buffer_load_b16(b.rsrc, lane_byte, byte, 0);
+  }
+  __device__ __forceinline__ void set_masked() { raw = from_f32<T>(-INFINITY); }
   __device__ __forceinline__ void get(float (&v)[1]) const { v[0] = to_f32(raw); }
+  __device__ __forceinline__ static void store(const Buffer& b, bool, int lane_byte, int byte, const float (&v)[1]) {
+    if constexpr (sizeof(T) == 4) __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(v[0]), b.rsrc, lane_byte, byte, 0);
+    else __builtin_amdgcn_raw_buffer_store_b16(from_f32<T>(v[0]).bits, b.rsrc, lane_byte, byte, 0);
+  }
 };
 template <int VN>
 __device__ __forceinline__ float vec_max(const float (&v)[VN], float m) {
@@ -192,32 +226,48 @@ struct TeacherRow {
   static constexpr int R = (VAE_MAX_TEACHER + BT - 1) / BT;
   int id[VAE_MAX_TEACHER];
   float q[VAE_MAX_TEACHER], logq[VAE_MAX_TEACHER];
+  float x[VAE_MAX_TEACHER];   // the student's logits there, for who keeps them
 
-  __device__ __forceinline__ int load(const TeacherArgs& a, int64_t row, int V, float inv_tau, float scale2) {
+  // A thread's own entries between fetch() and finish(): loads of the row's logits fit in between.
+  struct Mine {
     float y[R];
-    int ids[R];
-    bool bad = false;
-    float m = kLowest;
+    int id[R];
+  };
+
+  // true when the row has an entry, or an id beyond the vocabulary
+  __device__ __forceinline__ static bool fetch(Mine& e, const TeacherArgs& a, int64_t row, int V) {
+    bool any = false;
 #pragma unroll
     for (int r = 0; r < R; ++r) {
       const int k = threadIdx.x + r * BT;
-      y[r] = -INFINITY;
-      ids[r] = -1;
+      e.y[r] = -INFINITY;
+      e.id[r] = -1;
       if (k < a.K) {
         const int64_t i = load_id(a.ids, a.id_bytes, row * a.id_stride + k);
-        bad |= i >= V;
-        if (i >= 0 && i < V) {
-          y[r] = load_any(a.logits, a.dtype, row * a.stride + k);
-          ids[r] = (int)i;
+        const float y = load_any(a.logits, a.dtype, row * a.stride + k);
+        if (i >= V) e.id[r] = V;
+        else if (i >= 0) {
+          e.id[r] = (int)i;
+          e.y[r] = y;
         }
+        any |= i >= V || (i >= 0 && y != -INFINITY);
       }
-      m = max_raw(m, y[r]);
+    }
+    return block_sum<BT>(any ? 1.f : 0.f) > 0.f;
+  }
+  __device__ __forceinline__ int finish(const Mine& mine, const TeacherArgs& a, int V, float inv_tau, float scale2) {
+    float m = kLowest;
+    bool bad = false;
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      m = max_raw(m, mine.y[r]);
+      bad |= mine.id[r] == V;
     }
     m = block_max<BT>(m);
     float e[R], s = 0.f;
 #pragma unroll
     for (int r = 0; r < R; ++r) {
-      e[r] = ids[r] >= 0 ? exp2_raw((y[r] - m) * scale2) : 0.f;
+      e[r] = mine.id[r] >= 0 && mine.id[r] < V ? exp2_raw((mine.y[r] - m) * scale2) : 0.f;
       s += e[r];
     }
     s = block_sum<BT>(s);
@@ -228,14 +278,40 @@ struct TeacherRow {
       const int k = threadIdx.x + r * BT;
       if (k < a.K) {
         q[k] = e[r] / s;
-        logq[k] = row_log_prob(y[r], m, s, inv_tau);
-        id[k] = e[r] == 0.f ? -1 : ids[r];   // e NaN keeps its id: the row comes out NaN
+        logq[k] = row_log_prob(mine.y[r], m, s, inv_tau);
+        id[k] = e[r] == 0.f ? -1 : mine.id[r];   // e NaN keeps its id: the row comes out NaN
       }
     }
     lds_barrier();
     return any_bad > 0.f ? kRowBad : (s == 0.f ? kRowEmpty : kRowFine);
   }
+  __device__ __forceinline__ int load(const TeacherArgs& a, int64_t row, int V, float inv_tau, float scale2) {
+    Mine e;
+    return fetch(e, a, row, V) ? finish(e, a, V, inv_tau, scale2) : kRowEmpty;
+  }
 };
+
+// Short rows (token_short.hip): everything that is asked of a row from one reading of it.  False: the rows are too long
+// for it, nothing was launched.
+struct ShortArgs {
+  const void* logits;
+  int64_t row_stride;
+  const void* tokens;
+  int token_bytes;
+  int64_t N;
+  int V;
+  float *logp, *entropy, *stats, *top_logp;        // each may be NULL
+  int64_t* top_ids;
+  int top_k;
+  void* glogits;                                   // NULL: no gradient
+  const float* glogp;
+  int64_t rows_per_g;
+  float g_scale;
+  const float *gentropy, *gtop;
+  const int64_t* gtop_ids;
+  int gtop_k;
+};
+bool short_rows(const ShortArgs& a, int dtype, hipStream_t st, int* rc);
 
 #define VAE_BY_TYPE(dtype_, ...)                                        \
   switch (dtype_) {                                                     \
