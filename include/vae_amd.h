@@ -497,6 +497,18 @@ int vae_token_logp_bwd(const void* logits, int64_t row_stride, const void* token
 int vae_token_nll_fused(const void* logits, int64_t row_stride, const void* tokens, int token_bytes, float* logp,
                         float* stats, void* glogits, float grad_scale, void* scratch, int64_t N, int64_t V, int dtype,
                         vae_stream_t stream);
+/* The loss of B samples of T tokens each, from logp [B * T]: nll[b] = -sum_t logp[b T + t] (in double, in a fixed
+ * order), loss / elbo / means as vae_elbo_combine_fwd (abstract_vae.py:356-388); loss == elbo == NULL: nll alone.   */
+int vae_token_elbo_fwd(const float* logp, int64_t T, const void* kld, const void* add, const void* mi, float kl_beta,
+                       float inv_count, void* nll, void* loss, void* elbo, float* means, float* workspace, int64_t B,
+                       int dtype, vae_stream_t stream);
+/* Its backward.  gnll / gloss / gelbo [B] (dtype) and gmeans, a HOST array of 6 device pointers to one value each
+ * (gmeans_dtype): every one may be NULL.  grow [B] (float32) = d / d nll[b], what vae_token_logp_bwd takes with
+ * rows_per_g = T and g_scale = -1; or grad [n] = a stored d(loss_mean) / d logits (vae_token_nll_fused), multiplied by
+ * the mean gradients' sum where that is not 1 (gnll, gloss and gelbo NULL).  gkld / gadd / gmi [B] (dtype) or NULL.  */
+int vae_token_elbo_bwd(const void* gnll, const void* gloss, const void* gelbo, const void* const* gmeans,
+                       int gmeans_dtype, float kl_beta, float inv_count, float* grow, void* grad, int64_t n, void* gkld,
+                       void* gadd, void* gmi, int64_t B, int dtype, vae_stream_t stream);
 /* out[b] (dtype) = scale * sum of rows[b T .. b T + T), summed in double in a fixed order.                         */
 int vae_row_sums(const float* rows, float scale, void* out, int64_t B, int64_t T, int dtype, vae_stream_t stream);
 /* buf[n] *= *factor (a device float); returns without touching buf when it is 1.                                   */

@@ -149,3 +149,19 @@ def test_sums_and_scale_refusals():
     assert _call('vae_grad_scale', [P, P, -4, 0, None]) == _lib.VAE_ERR_ARG
     assert _call('vae_grad_scale', [P, P, 4, 7, None]) == _lib.VAE_ERR_ARG
     assert _call('vae_grad_scale', [None, None, 0, 0, None]) == _lib.VAE_OK
+
+
+def test_loss_closing_refusals():
+    f, b = 'vae_token_elbo_fwd', 'vae_token_elbo_bwd'
+    ok = [P, 3, None, None, None, 1.0, 1.0, P, P, P, P, P, 0, 0, None]          # no samples: nothing is launched
+    assert _call(f, ok) == _lib.VAE_OK
+    for i, v in ((12, -1), (1, -1), (13, 5)):
+        assert _call(f, ok[:i] + [v] + ok[i + 1:]) == _lib.VAE_ERR_ARG
+    some = ok[:12] + [2] + ok[13:]
+    for i in (0, 7, 8, 9, 10, 11):
+        assert _call(f, some[:i] + [None] + some[i + 1:]) == _lib.VAE_ERR_ARG
+    ok = [None, None, None, None, 0, 1.0, 1.0, P, None, 0, None, None, None, 0, 0, None]
+    assert _call(b, ok) == _lib.VAE_OK
+    for i, v in ((13, -1), (9, -1), (14, 3), (4, 3)):
+        assert _call(b, ok[:i] + [v] + ok[i + 1:]) == _lib.VAE_ERR_ARG
+    assert _call(b, [P] + ok[1:8] + [P] + ok[9:]) == _lib.VAE_ERR_ARG              # a stored gradient and per-sample ones

@@ -96,6 +96,8 @@ SIGNATURES = {
     'vae_token_logp_fwd': [_p, _i64, _p, _i, _p, _p, _p, _p, _p, _i64, _p, _i64, _i64, _i, _p],
     'vae_token_logp_bwd': [_p, _i64, _p, _i, _p, _p, _p, _i64, _f, _p, _p, _p, _i64, _p, _i64, _i64, _i, _p],
     'vae_token_nll_fused': [_p, _i64, _p, _i, _p, _p, _p, _f, _p, _i64, _i64, _i, _p],
+    'vae_token_elbo_fwd': [_p, _i64, _p, _p, _p, _f, _f, _p, _p, _p, _p, _p, _i64, _i, _p],
+    'vae_token_elbo_bwd': [_p, _p, _p, _pp, _i, _f, _f, _p, _p, _i64, _p, _p, _p, _i64, _i, _p],
     'vae_row_sums': [_p, _f, _p, _i64, _i64, _i, _p],
     'vae_grad_scale': [_p, _p, _i64, _i, _p],
     'vae_distill_fwd': [_p, _i64, _p, _i64, _i, _p, _i64, _i, _i64, _f, _p, _p, _p, _f, _p, _i64, _i64, _i, _p],
@@ -130,14 +132,14 @@ def load():
     return lib
 
 
+DTYPE_CODES = {torch.float32: VAE_F32, torch.bfloat16: VAE_BF16, torch.float16: VAE_F16}
+
+
 def dtype_code(t):
-    if t.dtype == torch.float32:
-        return VAE_F32
-    if t.dtype == torch.bfloat16:
-        return VAE_BF16
-    if t.dtype == torch.float16:
-        return VAE_F16
-    raise TypeError("vae_amd kernels take float32, bfloat16 or float16 tensors, got %s" % t.dtype)
+    code = DTYPE_CODES.get(t.dtype)
+    if code is None:
+        raise TypeError("vae_amd kernels take float32, bfloat16 or float16 tensors, got %s" % t.dtype)
+    return code
 
 
 def check_device(*tensors):
@@ -157,7 +159,8 @@ def check_device(*tensors):
 
 
 def ptr(t):
-    return None if t is None else ctypes.c_void_p(t.data_ptr())
+    """A tensor's device address (ctypes turns an int into the pointer argument; no c_void_p object per argument)."""
+    return None if t is None else t.data_ptr()
 
 
 def float_array(values):
@@ -182,7 +185,7 @@ def _stream_handle(device):
 
 
 def stream_ptr(device):
-    return ctypes.c_void_p(_stream_handle(device))
+    return _stream_handle(device)
 
 
 _workspaces = {}

@@ -431,26 +431,6 @@ __global__ __launch_bounds__(BT) void token_join_kernel(FwdArgs a) {
   }
 }
 
-// out[b] = scale * sum of T consecutive row values, in a fixed order, summed in double
-template <typename O>
-__global__ __launch_bounds__(kBlock) void row_sums_kernel(const float* __restrict__ rows, float scale,
-                                                          O* __restrict__ out, int64_t B, int64_t T) {
-  __shared__ double part[kBlock / 64];
-  for (int64_t b = blockIdx.x; b < B; b += gridDim.x) {
-    double v = 0.0;
-    for (int64_t t = threadIdx.x; t < T; t += kBlock) v += (double)rows[b * T + t];
-    v = wave_sum_d(v);
-    lds_barrier();
-    if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = v;
-    lds_barrier();
-    if (threadIdx.x == 0) {
-      double r = 0.0;
-      for (int w = 0; w < kBlock / 64; ++w) r += part[w];
-      out[b] = from_f32<O>((float)(r * (double)scale));
-    }
-  }
-}
-
 static bool bad_shape(int64_t N, int64_t V, int64_t row_stride, int dtype) {
   return N < 0 || V < 1 || V > VAE_MAX_ROW || (N > 1 && row_stride < V) ||
          (dtype != VAE_F32 && dtype != VAE_BF16 && dtype != VAE_F16);
@@ -537,16 +517,6 @@ int vae_token_logp_fwd(const void* logits, int64_t row_stride, const void* token
   const FwdArgs a = {logits, row_stride, tokens, token_bytes, logp, entropy, stats, top_logp, top_ids, (int)top_k, N,
                      (int)V, cut.parts, cut.part_vecs, (char*)scratch, kLog2e, 1.0f, {}};
   VAE_BY_TYPE(dtype, return (fwd_type<T, false>(a, (hipStream_t)stream)));
-  return VAE_ERR_ARG;
-}
-
-int vae_row_sums(const float* rows, float scale, void* out, int64_t B, int64_t T_, int dtype, vae_stream_t stream) {
-  if (B < 0 || T_ < 0) return VAE_ERR_ARG;
-  if (B == 0) return VAE_OK;
-  if (!out || (T_ > 0 && !rows)) return VAE_ERR_ARG;
-  VAE_BY_TYPE(dtype, hipLaunchKernelGGL((row_sums_kernel<T>), dim3(grid_for(B)), dim3(kBlock), 0, (hipStream_t)stream,
-                                        rows, scale, (T*)out, B, T_);
-              return hipGetLastError() == hipSuccess ? VAE_OK : VAE_ERR_LAUNCH);
   return VAE_ERR_ARG;
 }
 

@@ -1,0 +1,164 @@
+// What closes a categorical likelihood: the samples' sums of their tokens' log probs, the ELBO combine with its six batch
+// means, and the backward of both; sums of row values; a stored gradient times a device scalar.  All of it is [B] or
+// [rows] work of a few microseconds: one launch each.
+#include "token_row.hpp"
+
+namespace vae {
+
+// G lanes a sample (a power of two, up to a wave); samples in order, so a result does not depend on the grid
+template <typename T>
+__global__ __launch_bounds__(kBlock) void token_elbo_fwd_kernel(
+    const float* __restrict__ logp, int64_t len, const T* __restrict__ kld, const T* __restrict__ add,
+    const T* __restrict__ mi, float kl_beta, float inv_count, T* __restrict__ nll, T* __restrict__ loss,
+    T* __restrict__ elbo, float* __restrict__ means, float* __restrict__ ws, int64_t B, int G) {
+  const int rpb = kBlock / G, sub = threadIdx.x % G, rloc = threadIdx.x / G;
+  float acc[6] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+  for (int64_t b0 = (int64_t)blockIdx.x * rpb; b0 < B; b0 += (int64_t)gridDim.x * rpb) {
+    const int64_t b = b0 + rloc;
+    double v = 0.0;
+    if (b < B)
+      for (int64_t t = sub; t < len; t += G) v += (double)logp[b * len + t];
+    for (int o = G >> 1; o >= 1; o >>= 1) v += __shfl_xor(v, o, 64);
+    if (sub != 0 || b >= B) continue;
+    const float n = to_f32(from_f32<T>((float)-v));
+    nll[b] = from_f32<T>(n);
+    if (!loss) continue;
+    const float k = kld ? to_f32(kld[b]) : 0.f;
+    const float ad = add ? to_f32(add[b]) : 0.f;
+    const float m = mi ? to_f32(mi[b]) : 0.f;
+    const float e = to_f32(from_f32<T>(n + k));
+    const float l = to_f32(from_f32<T>((n + ad + kl_beta * k) - m));
+    loss[b] = from_f32<T>(l);
+    elbo[b] = from_f32<T>(e);
+    acc[0] += l; acc[1] += e; acc[2] += n; acc[3] += k; acc[4] += ad; acc[5] += m;
+  }
+  if (loss) grid_reduce<6>(acc, ws, inv_count, means, kNanElbo6);
+}
+
+struct Scalars6 {
+  const void* p[6];
+};
+template <typename T, int V>
+__global__ __launch_bounds__(kBlock) void token_elbo_bwd_kernel(
+    const T* __restrict__ gnll, const T* __restrict__ gloss, const T* __restrict__ gelbo, Scalars6 gmeans,
+    int gmeans_dtype, float kl_beta, float inv_count, float* __restrict__ grow, T* __restrict__ grad, int64_t items,
+    T* __restrict__ gkld, T* __restrict__ gadd, T* __restrict__ gmi, int64_t B) {
+  float gm[6];
+#pragma unroll
+  for (int k = 0; k < 6; ++k) gm[k] = gmeans.p[k] ? load_any(gmeans.p[k], gmeans_dtype, 0) : 0.f;
+  const float c = gm[0] + gm[1] + gm[2];
+  for (int64_t b = (int64_t)blockIdx.x * kBlock + threadIdx.x; b < B; b += (int64_t)gridDim.x * kBlock) {
+    const float gl = (gloss ? to_f32(gloss[b]) : 0.f) + gm[0] * inv_count;
+    const float ge = (gelbo ? to_f32(gelbo[b]) : 0.f) + gm[1] * inv_count;
+    if (grow) grow[b] = gl + ge + gm[2] * inv_count + (gnll ? to_f32(gnll[b]) : 0.f);
+    if (gkld) gkld[b] = from_f32<T>(kl_beta * gl + ge + gm[3] * inv_count);
+    if (gadd) gadd[b] = from_f32<T>(gl + gm[4] * inv_count);
+    if (gmi) gmi[b] = from_f32<T>(gm[5] * inv_count - gl);
+  }
+  if (!grad || c == 1.0f) return;
+  for (int64_t j = (int64_t)blockIdx.x * kBlock + threadIdx.x; j < items; j += (int64_t)gridDim.x * kBlock) {
+    float v[V];
+    load_vec<T, V, false>(grad + j * V, v);
+#pragma unroll
+    for (int i = 0; i < V; ++i) v[i] *= c;
+    store_vec<T, V>(grad + j * V, v);
+  }
+}
+
+// out[b] = scale * sum of `len` consecutive row values, in a fixed order, summed in double: a workgroup a sum
+template <typename O>
+__global__ __launch_bounds__(kBlock) void row_sums_kernel(const float* __restrict__ rows, float scale,
+                                                          O* __restrict__ out, int64_t B, int64_t len) {
+  __shared__ double part[kBlock / 64];
+  for (int64_t b = blockIdx.x; b < B; b += gridDim.x) {
+    double v = 0.0;
+    for (int64_t t = threadIdx.x; t < len; t += kBlock) v += (double)rows[b * len + t];
+    v = wave_sum_d(v);
+    lds_barrier();
+    if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = v;
+    lds_barrier();
+    if (threadIdx.x == 0) {
+      double r = 0.0;
+      for (int w = 0; w < kBlock / 64; ++w) r += part[w];
+      out[b] = from_f32<O>((float)(r * (double)scale));
+    }
+  }
+}
+
+static int launched() { return hipGetLastError() == hipSuccess ? VAE_OK : VAE_ERR_LAUNCH; }
+static bool type_ok(int d) { return d == VAE_F32 || d == VAE_BF16 || d == VAE_F16; }
+
+template <typename T, int V>
+static void elbo_bwd_launch(const void* gnll, const void* gloss, const void* gelbo, const Scalars6& gm, int gmeans_dtype,
+                            float kl_beta, float inv_count, float* grow, void* grad, int64_t items, void* gkld,
+                            void* gadd, void* gmi, int64_t B, hipStream_t st) {
+  // sized for the [B] part; the (rare) rescale walks the gradient with at least 1024 blocks
+  int64_t blocks = (B + kBlock - 1) / kBlock;
+  const int64_t wide = (items + kBlock - 1) / kBlock;
+  if (grad && blocks < 1024) blocks = wide < 1024 ? (wide > blocks ? wide : blocks) : 1024;
+  const int grid = (int)(blocks < 1 ? 1 : (blocks < 4096 ? blocks : 4096));
+  hipLaunchKernelGGL((token_elbo_bwd_kernel<T, V>), dim3(grid), dim3(kBlock), 0, st, (const T*)gnll, (const T*)gloss,
+                     (const T*)gelbo, gm, gmeans_dtype, kl_beta, inv_count, grow, (T*)grad, items, (T*)gkld, (T*)gadd,
+                     (T*)gmi, B);
+}
+
+}  // namespace vae
+
+using namespace vae;
+
+extern "C" {
+
+int vae_token_elbo_fwd(const float* logp, int64_t len, const void* kld, const void* add, const void* mi, float kl_beta,
+                       float inv_count, void* nll, void* loss, void* elbo, float* means, float* workspace, int64_t B,
+                       int dtype, vae_stream_t stream) {
+  if (B < 0 || len < 0 || !type_ok(dtype)) return VAE_ERR_ARG;
+  if (B == 0) return VAE_OK;
+  if (!nll || (len > 0 && !logp) || (loss == nullptr) != (elbo == nullptr) || (loss && (!means || !workspace)))
+    return VAE_ERR_ARG;
+  int G = 1;
+  while (G < 64 && G < len) G <<= 1;
+  const int64_t blocks = (B + kBlock / G - 1) / (kBlock / G);
+  const int grid = (int)(blocks < kGridReduce ? blocks : kGridReduce);
+  VAE_BY_TYPE(dtype, hipLaunchKernelGGL((token_elbo_fwd_kernel<T>), dim3(grid), dim3(kBlock), 0, (hipStream_t)stream,
+                                        logp, len, (const T*)kld, (const T*)add, (const T*)mi, kl_beta, inv_count,
+                                        (T*)nll, (T*)loss, (T*)elbo, means, workspace, B, G));
+  return launched();
+}
+
+int vae_token_elbo_bwd(const void* gnll, const void* gloss, const void* gelbo, const void* const* gmeans,
+                       int gmeans_dtype, float kl_beta, float inv_count, float* grow, void* grad, int64_t n, void* gkld,
+                       void* gadd, void* gmi, int64_t B, int dtype, vae_stream_t stream) {
+  if (B < 0 || n < 0 || !type_ok(dtype) || !type_ok(gmeans_dtype)) return VAE_ERR_ARG;
+  if (grad && (gnll || gloss || gelbo)) return VAE_ERR_ARG;
+  if (B == 0 && (n == 0 || !grad)) return VAE_OK;
+  Scalars6 gm = {};
+  if (gmeans)
+    for (int k = 0; k < 6; ++k) gm.p[k] = gmeans[k];
+  VAE_BY_TYPE(dtype, constexpr int VN = VecOf<T>::n;
+              if (n % VN == 0 && aligned16(grad))
+                elbo_bwd_launch<T, VN>(gnll, gloss, gelbo, gm, gmeans_dtype, kl_beta, inv_count, grow, grad, n / VN,
+                                       gkld, gadd, gmi, B, (hipStream_t)stream);
+              else elbo_bwd_launch<T, 1>(gnll, gloss, gelbo, gm, gmeans_dtype, kl_beta, inv_count, grow, grad, n, gkld,
+                                         gadd, gmi, B, (hipStream_t)stream));
+  return launched();
+}
+
+int vae_grad_scale(void* buf, const float* factor, int64_t n, int dtype, vae_stream_t stream) {
+  if (n < 0) return VAE_ERR_ARG;
+  if (n == 0) return type_ok(dtype) ? VAE_OK : VAE_ERR_ARG;
+  if (!buf || !factor) return VAE_ERR_ARG;
+  const void* g[6] = {factor, nullptr, nullptr, nullptr, nullptr, nullptr};
+  return vae_token_elbo_bwd(nullptr, nullptr, nullptr, g, VAE_F32, 0.f, 0.f, nullptr, buf, n, nullptr, nullptr, nullptr, 0,
+                            dtype, stream);
+}
+
+int vae_row_sums(const float* rows, float scale, void* out, int64_t B, int64_t len, int dtype, vae_stream_t stream) {
+  if (B < 0 || len < 0 || !type_ok(dtype)) return VAE_ERR_ARG;
+  if (B == 0) return VAE_OK;
+  if (!out || (len > 0 && !rows)) return VAE_ERR_ARG;
+  VAE_BY_TYPE(dtype, hipLaunchKernelGGL((row_sums_kernel<T>), dim3((int)(B < kMaxGrid ? B : kMaxGrid)), dim3(kBlock), 0,
+                                        (hipStream_t)stream, rows, scale, (T*)out, B, len));
+  return launched();
+}
+
+}  // extern "C"

@@ -380,20 +380,6 @@ __global__ __launch_bounds__(BT) void token_fused_kernel(GradArgs a) {
   }
 }
 
-template <typename T, int V>
-__global__ __launch_bounds__(kBlock) void grad_scale_kernel(T* __restrict__ buf, const float* __restrict__ factor,
-                                                            int64_t items) {
-  const float c = factor[0];
-  if (c == 1.0f) return;
-  for (int64_t j = (int64_t)blockIdx.x * kBlock + threadIdx.x; j < items; j += (int64_t)gridDim.x * kBlock) {
-    float v[V];
-    load_vec<T, V, false>(buf + j * V, v);
-#pragma unroll
-    for (int i = 0; i < V; ++i) v[i] *= c;
-    store_vec<T, V>(buf + j * V, v);
-  }
-}
-
 // ---------------------------------------------------------------------------------------------------------------
 // host
 // ---------------------------------------------------------------------------------------------------------------
@@ -559,20 +545,6 @@ int vae_distill_fwd(const void* logits, int64_t row_stride, const void* t_logits
   if (rc != VAE_OK || !glogits) return rc;
   return vae_distill_bwd(logits, row_stride, t_logits, t_stride, t_dtype, t_ids, id_stride, id_bytes, K, temperature,
                          stats, nullptr, nullptr, grad_scale, glogits, N, V, dtype, stream);
-}
-
-int vae_grad_scale(void* buf, const float* factor, int64_t n, int dtype, vae_stream_t stream) {
-  if (n < 0) return VAE_ERR_ARG;
-  if (n == 0) return VAE_OK;
-  if (!buf || !factor) return VAE_ERR_ARG;
-  hipStream_t st = (hipStream_t)stream;
-  VAE_BY_TYPE(dtype, constexpr int VN = VecOf<T>::n; const bool vec = n % VN == 0 && aligned16(buf);
-              const int64_t items = vec ? n / VN : n; const int64_t blocks = (items + kBlock - 1) / kBlock;
-              const int grid = (int)(blocks < 4096 ? blocks : 4096);
-              if (vec) hipLaunchKernelGGL((grad_scale_kernel<T, VN>), dim3(grid), dim3(kBlock), 0, st, (T*)buf, factor, items);
-              else hipLaunchKernelGGL((grad_scale_kernel<T, 1>), dim3(grid), dim3(kBlock), 0, st, (T*)buf, factor, items);
-              return launched());
-  return VAE_ERR_ARG;
 }
 
 }  // extern "C"

@@ -29,7 +29,8 @@ def distillation(recon_x, teacher_logits, teacher_ids, temperature=1.0):
 
 
 def _pack(loss, elbo, means, kl_beta, dtype):
-    means = means.to(dtype)
+    if torch.is_tensor(means):
+        means = means.to(dtype)
     return {
         'loss': loss,
         'elbo': elbo,
@@ -68,6 +69,9 @@ def loss_function(recon_x, x, kld, nll_type, kl_beta=1.0, mut_info=None, extra_l
     if nll_given is None and isinstance(recon_x, (list, tuple)):
         _, loss, elbo, means = F_.nll_multi_elbo(x, list(recon_x), nll_type, kld=kld, add=add, mi=mut_info,
                                                  kl_beta=kl_beta, inv_count=inv_count)
+    elif nll_given is None and F_._is_categorical(nll_type):
+        _, loss, elbo, means = F_.token_nll_elbo(x, recon_x, kld, add, mut_info, kl_beta, inv_count, fuse_backward,
+                                                 mean_dtype=recon_x.dtype)
     elif nll_given is None:
         _, loss, elbo, means = F_.nll_elbo(x, recon_x, nll_type, kld=kld, add=add, mi=mut_info, kl_beta=kl_beta,
                                            inv_count=inv_count, fuse_backward=fuse_backward)

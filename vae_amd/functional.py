@@ -5,6 +5,8 @@ current HIP stream through `_lib.call` and never synchronises.  Shapes are flatt
 (`[rows, features]`) here; the module classes in `vae_amd.reparameterizers` restore the
 reference's shapes.
 """
+import ctypes
+
 import torch
 
 from . import _lib
@@ -337,7 +339,8 @@ def nll(x, recon_x, nll_type):
     """Per-sample negative log-likelihood [B] (abstract_vae.py:461-471; definitions: oracle/cpu_ref.py).
     nll_type 'categorical': x holds integer tokens [B, ...] (negative: padding), recon_x their logits [B, ..., V]."""
     if _is_categorical(nll_type):
-        return _TokenNllElbo.apply(*_token_rows(x, recon_x), None, None, None, 0.0, 0.0, False, False)[0]
+        _check_tokens(x, recon_x)
+        return _TokenNllElbo.apply(recon_x, x.contiguous(), None, None, None, 0.0, 0.0, False, False, torch.float32)[0]
     code, xf, rf = _flat_pixels(x, recon_x, nll_type)
     return _NllElbo.apply(xf, rf, None, None, None, code, 0.0, 0.0, False)[0]
 
@@ -349,14 +352,8 @@ def nll_elbo(x, recon_x, nll_type, kld=None, add=None, mi=None, kl_beta=1.0, inv
     step instead of two); results are identical, the gradient buffer is simply allocated a step earlier.
     nll_type 'categorical': integer tokens and logits, as in nll()."""
     if _is_categorical(nll_type):
-        rows, tokens, B = _token_rows(x, recon_x)
-        if inv_count is None:
-            inv_count = 1.0 / max(B, 1)
-        # fp16: two passes, for the reason given below
-        fuse = (fuse_backward and rows.dtype != torch.float16 and rows.requires_grad and torch.is_grad_enabled()
-                and rows.numel() > 0)
-        kld, add, mi = (None if t is None else t.to(rows.dtype).contiguous() for t in (kld, add, mi))
-        return _TokenNllElbo.apply(rows, tokens, B, kld, add, mi, float(kl_beta), float(inv_count), True, fuse)
+        nll_, loss, elbo, means = token_nll_elbo(x, recon_x, kld, add, mi, kl_beta, inv_count, fuse_backward)
+        return nll_, loss, elbo, torch.stack(means)
     code, xf, rf = _flat_pixels(x, recon_x, nll_type)
     if inv_count is None:
         inv_count = 1.0 / max(xf.shape[0], 1)
@@ -532,34 +529,66 @@ def _id_bytes(t, what):
     raise TypeError("%s: ids must be int32 or int64, got %s" % (what, t.dtype))
 
 
-def _vocab_rows(logits, what):
+def _check_vocab(logits, what):
     if logits.dim() < 1 or logits.shape[-1] < 1:
         raise ValueError("%s: logits need a last dimension over the vocabulary, got %s" % (what, tuple(logits.shape)))
-    return _rows(logits)
 
 
-def _token_rows(x, recon):
-    """(logits rows [B*T, V], tokens [B*T], B) of tokens x [B, ...] and their logits recon [B, ..., V]."""
-    _id_bytes(x, "nll 'categorical'")
-    if x.dim() < 1 or recon.dim() < 2 or recon.shape[0] != x.shape[0] or recon.shape[:-1].numel() != x.numel():
-        raise ValueError("nll 'categorical': logits %s do not fit tokens %s (a last dimension over the vocabulary)"
-                         % (tuple(recon.shape), tuple(x.shape)))
-    return _vocab_rows(recon, "nll 'categorical'"), x.reshape(-1).contiguous(), x.shape[0]
+_SPLIT_ROWS = 512   # with fewer rows the library may cut a row into pieces (csrc/token.hip: kFillRows)
 
 
-def _token_scratch(logits, top_k, dev):
+def _token_scratch(rows, top_k, dev):
     """The pieces of split rows (few rows): the caller's own memory each call, so that calls on several streams and
     captured graphs share nothing."""
-    n = _lib.load().vae_token_scratch_bytes(logits.shape[0], logits.shape[1], top_k, dtype_code(logits))
+    if rows.shape[0] >= _SPLIT_ROWS:
+        return None
+    n = _lib.load().vae_token_scratch_bytes(rows.shape[0], rows.shape[1], top_k, dtype_code(rows))
     return torch.empty((n,), dtype=torch.uint8, device=dev) if n else None
 
 
-def _row_sums(rows, scale, B, dtype):
-    """[B] = scale * sum over each of B equal runs of `rows` (fp32, summed in double)."""
-    out = torch.empty((B,), dtype=dtype, device=rows.device)
+def _row_sums(rows, scale, shape, dtype):
+    """scale * sum over equal runs of `rows` (fp32, summed in double), one run for each entry of `shape`."""
+    out = torch.empty(shape, dtype=dtype, device=rows.device)
+    B = out.numel()
     call('vae_row_sums', ptr(rows), scale, ptr(out), B, rows.numel() // max(B, 1), dtype_code(out),
          stream_ptr(rows.device))
     return out
+
+
+# The autograd functions below take the caller's logits as they are and return outputs in their final shape: every view
+# recorded around a custom function is a node of the backward pass, a few microseconds each way.
+def _token_fwd(logits, tokens, top_k, want_entropy, want_stats):
+    dev = check_device(logits, tokens)
+    rows, shape = _rows(logits), logits.shape[:-1]
+    N, V = rows.shape
+    new = lambda s: torch.empty(s, dtype=torch.float32, device=dev)
+    logp = new(shape) if tokens is not None else None
+    entropy = new(shape) if want_entropy else None
+    stats = new((N, 2)) if want_stats else None
+    top = new(shape + (top_k,)) if top_k else None
+    ids = torch.empty(shape + (top_k,), dtype=torch.int64, device=dev) if top_k else None
+    scratch = _token_scratch(rows, top_k, dev)
+    with _Guard(dev):
+        call('vae_token_logp_fwd', ptr(rows), rows.stride(0), ptr(tokens),
+             0 if tokens is None else tokens.element_size(), ptr(logp), ptr(entropy), ptr(stats), ptr(top), ptr(ids),
+             top_k, ptr(scratch), N, V, dtype_code(rows), stream_ptr(dev))
+    return logp, entropy, top, ids, stats
+
+
+def _token_bwd(logits, tokens, entropy, ids, stats, glogp, rows_per_g, g_scale, gentropy, gtop):
+    """d(logits).  glogp None: no gradient reached the log probs (`tokens` still says which rows are padding)."""
+    dev = logits.device
+    rows = _rows(logits)
+    N, V = rows.shape
+    grad = torch.empty(logits.shape, dtype=logits.dtype, device=dev)
+    if glogp is None and tokens is not None:
+        glogp, rows_per_g, g_scale = torch.zeros((1,), dtype=torch.float32, device=dev), N, 0.0
+    with _Guard(dev):
+        call('vae_token_logp_bwd', ptr(rows), rows.stride(0), ptr(tokens),
+             0 if tokens is None else tokens.element_size(), ptr(stats), ptr(entropy), ptr(glogp), max(rows_per_g, 1),
+             g_scale, ptr(gentropy), ptr(gtop), ptr(ids) if gtop is not None else None,
+             ids.shape[-1] if gtop is not None else 0, ptr(grad), N, V, dtype_code(rows), stream_ptr(dev))
+    return grad
 
 
 class _TokenLogProbs(torch.autograd.Function):
@@ -568,45 +597,17 @@ class _TokenLogProbs(torch.autograd.Function):
         ctx.set_materialize_grads(False)
         logp, entropy, top, ids, stats = _token_fwd(logits, tokens, top_k, want_entropy, True)
         ctx.save_for_backward(logits, tokens, entropy, ids, stats)
-        outs, nd = [], []
-        for t in (logp, entropy, top, ids):
-            if t is None:
-                t = logits.new_empty((0,))
-                nd.append(t)
-            outs.append(t)
         if ids is not None:
-            nd.append(ids)
-        if nd:
-            ctx.mark_non_differentiable(*nd)
-        return tuple(outs)
+            ctx.mark_non_differentiable(ids)
+        return logp, entropy, top, ids
 
     @staticmethod
     def backward(ctx, glogp, gentropy, gtop, gids):
-        logits, tokens, entropy, ids, stats = ctx.saved_tensors
-        glogp = None if tokens is None else glogp
-        gentropy = None if entropy is None else gentropy
-        gtop = None if ids is None else gtop
         if glogp is None and gentropy is None and gtop is None:
             return None, None, None, None
-        return _token_bwd(logits, None if glogp is None else tokens, tokens, entropy, ids, stats, _dense(glogp), 1, 1.0,
-                          _dense(gentropy), _dense(gtop)), None, None, None
-
-
-def _token_fwd(logits, tokens, top_k, want_entropy, want_stats):
-    dev = check_device(logits, tokens)
-    N, V = logits.shape
-    new = lambda *s: torch.empty(s, dtype=torch.float32, device=dev)
-    logp = new(N) if tokens is not None else None
-    entropy = new(N) if want_entropy else None
-    stats = new(N, 2) if want_stats else None
-    top = new(N, top_k) if top_k else None
-    ids = torch.empty((N, top_k), dtype=torch.int64, device=dev) if top_k else None
-    scratch = _token_scratch(logits, top_k, dev)
-    with _Guard(dev):
-        call('vae_token_logp_fwd', ptr(logits), logits.stride(0), ptr(tokens),
-             0 if tokens is None else tokens.element_size(), ptr(logp), ptr(entropy), ptr(stats), ptr(top), ptr(ids),
-             top_k, ptr(scratch), N, V, dtype_code(logits), stream_ptr(dev))
-    return logp, entropy, top, ids, stats
+        logits, tokens, entropy, ids, stats = ctx.saved_tensors
+        return _token_bwd(logits, tokens, entropy, ids, stats, _dense(glogp), 1, 1.0, _dense(gentropy),
+                          _dense(gtop)), None, None, None
 
 
 def token_log_probs(logits, tokens=None, top_k=0, want_entropy=True):
@@ -618,107 +619,105 @@ def token_log_probs(logits, tokens=None, top_k=0, want_entropy=True):
     A negative token marks a padded row: its logits are not read; log_prob 0, entropy 0, alternatives -inf / -1,
     gradient 0.  A token beyond the vocabulary gives NaN (log_prob and the row's gradient).  Logits of -inf are masked
     out; a row of nothing else has log_prob -inf, entropy 0 and gradient 0."""
-    shape = logits.shape[:-1]
-    rows = _vocab_rows(logits, 'token_log_probs')
+    _check_vocab(logits, 'token_log_probs')
     top_k = int(top_k)
-    if not 0 <= top_k <= min(MAX_TOP, rows.shape[1]):
+    if not 0 <= top_k <= min(MAX_TOP, logits.shape[-1]):
         raise ValueError("token_log_probs: top_k must be in 0..min(%d, V = %d), got %d"
-                         % (MAX_TOP, rows.shape[1], top_k))
+                         % (MAX_TOP, logits.shape[-1], top_k))
     if tokens is not None:
         _id_bytes(tokens, 'token_log_probs')
-        if tokens.shape != shape:
+        if tokens.shape != logits.shape[:-1]:
             raise ValueError("token_log_probs: tokens %s do not fit logits %s"
                              % (tuple(tokens.shape), tuple(logits.shape)))
-        tokens = tokens.reshape(-1).contiguous()
-    want_entropy = bool(want_entropy)
-    if rows.requires_grad and torch.is_grad_enabled():
-        logp, entropy, top, ids = _TokenLogProbs.apply(rows, tokens, top_k, want_entropy)
-    else:
-        logp, entropy, top, ids, _ = _token_fwd(rows, tokens, top_k, want_entropy, False)
-    return (logp.reshape(shape) if tokens is not None else None, entropy.reshape(shape) if want_entropy else None,
-            top.reshape(shape + (top_k,)) if top_k else None, ids.reshape(shape + (top_k,)) if top_k else None)
+        tokens = tokens.contiguous()
+    if logits.requires_grad and torch.is_grad_enabled():
+        return _TokenLogProbs.apply(logits, tokens, top_k, bool(want_entropy))
+    return _token_fwd(logits, tokens, top_k, want_entropy, False)[:4]
+
+
+def _check_tokens(x, recon):
+    """Tokens x [B, ...] and their logits recon [B, ..., V]."""
+    _id_bytes(x, "nll 'categorical'")
+    if x.dim() < 1 or recon.dim() < 2 or recon.shape[0] != x.shape[0] or recon.shape[:-1].numel() != x.numel():
+        raise ValueError("nll 'categorical': logits %s do not fit tokens %s (a last dimension over the vocabulary)"
+                         % (tuple(recon.shape), tuple(x.shape)))
+    _check_vocab(recon, "nll 'categorical'")
 
 
 class _TokenNllElbo(torch.autograd.Function):
-    """Categorical nll [B] of B samples with T tokens each, with the ELBO combine (with_elbo) and d(loss_mean)/d(logits)
-    out of the same launch (fuse), as in _NllElboFused."""
+    """Categorical nll [B] of B samples with T tokens each, with the ELBO combine (with_elbo; the six means as scalars of
+    their own, in `mean_dtype`) and d(loss_mean)/d(logits) out of the same launch (fuse), as in _NllElboFused."""
 
     @staticmethod
-    def forward(ctx, logits, tokens, B, kld, add, mi, kl_beta, inv_count, with_elbo, fuse):
+    def forward(ctx, logits, tokens, kld, add, mi, kl_beta, inv_count, with_elbo, fuse, mean_dtype):
         ctx.set_materialize_grads(False)
         dev = check_device(logits, tokens, kld, add, mi)
-        N, V = logits.shape
-        code, st = dtype_code(logits), stream_ptr(dev)
-        rows = torch.empty((N,), dtype=torch.float32, device=dev)
+        rows, B = _rows(logits), tokens.shape[0]
+        N, V = rows.shape
+        code, st = dtype_code(rows), stream_ptr(dev)
+        logp = torch.empty((N,), dtype=torch.float32, device=dev)
         stats = torch.empty((N, 2), dtype=torch.float32, device=dev)
-        grad = torch.empty((N, V), dtype=logits.dtype, device=dev) if fuse else None
-        loss = elbo = means = None
-        scratch = _token_scratch(logits, 0, dev)
+        grad = torch.empty(logits.shape, dtype=logits.dtype, device=dev) if fuse else None
+        scratch = _token_scratch(rows, 0, dev)
+        nll = torch.empty((B,), dtype=logits.dtype, device=dev)
+        loss = elbo = means = ws = None
+        if with_elbo:
+            loss, elbo, means, ws = torch.empty_like(nll), torch.empty_like(nll), _scalars(6, dev, B), workspace(dev)
         with _Guard(dev):
             if fuse:
-                call('vae_token_nll_fused', ptr(logits), logits.stride(0), ptr(tokens), tokens.element_size(), ptr(rows),
+                call('vae_token_nll_fused', ptr(rows), rows.stride(0), ptr(tokens), tokens.element_size(), ptr(logp),
                      ptr(stats), ptr(grad), inv_count, ptr(scratch), N, V, code, st)
             else:
-                call('vae_token_logp_fwd', ptr(logits), logits.stride(0), ptr(tokens), tokens.element_size(), ptr(rows),
+                call('vae_token_logp_fwd', ptr(rows), rows.stride(0), ptr(tokens), tokens.element_size(), ptr(logp),
                      None, ptr(stats), None, None, 0, ptr(scratch), N, V, code, st)
-            nll = _row_sums(rows, -1.0, B, logits.dtype)
-            if with_elbo:
-                loss, elbo = torch.empty_like(nll), torch.empty_like(nll)
-                means = _scalars(6, dev, B)
-                call('vae_elbo_combine_fwd', ptr(nll), ptr(kld), ptr(add), ptr(mi), kl_beta, inv_count, ptr(loss),
-                     ptr(elbo), ptr(means), ptr(workspace(dev)), B, code, st)
+            call('vae_token_elbo_fwd', ptr(logp), N // max(B, 1), ptr(kld), ptr(add), ptr(mi), kl_beta, inv_count,
+                 ptr(nll), ptr(loss), ptr(elbo), ptr(means), ptr(ws), B, code, st)
         ctx.save_for_backward(logits, tokens, stats)
         ctx.grad = grad
-        ctx.cfg = (B, kl_beta, inv_count, kld is not None, add is not None, mi is not None)
+        ctx.cfg = (kl_beta, inv_count, kld is not None, add is not None, mi is not None, mean_dtype)
         if not with_elbo:
-            loss, elbo, means = nll.new_empty((0,)), nll.new_empty((0,)), rows.new_empty((0,))
-            ctx.mark_non_differentiable(loss, elbo, means)
-        return nll, loss, elbo, means
+            return (nll,) + (None,) * 8
+        return (nll, loss, elbo) + means.to(mean_dtype).unbind(0)
 
     @staticmethod
-    def backward(ctx, gnll, gloss, gelbo, gmeans):
+    def backward(ctx, gnll, gloss, gelbo, *gmeans):
         logits, tokens, stats = ctx.saved_tensors
-        B, kl_beta, inv_count, has_kld, has_add, has_mi = ctx.cfg
-        dev = logits.device
-        need = [ctx.needs_input_grad[i] and has for i, has in ((3, has_kld), (4, has_add), (5, has_mi))]
-        gmeans = None if gmeans is None else gmeans.contiguous().float()
+        kl_beta, inv_count, has_kld, has_add, has_mi, mean_dtype = ctx.cfg
+        dev, B = logits.device, tokens.shape[0]
+        need = ctx.needs_input_grad
+        terms = [torch.empty((B,), dtype=logits.dtype, device=dev) if has and need[i] else None
+                 for i, has in ((2, has_kld), (3, has_add), (4, has_mi))]
         grad, ctx.grad = ctx.grad, None
+        stored = gnll is None and gloss is None and gelbo is None and grad is not None
+        # otherwise: the per-sample upstream gradient, in fp32 (1/B of a mean is a subnormal of fp16)
+        grow = None if stored else torch.empty((B,), dtype=torch.float32, device=dev)
+        gnll, gloss, gelbo = _dense(gnll), _dense(gloss), _dense(gelbo)
+        at = (ctypes.c_void_p * 6)(*[None if g is None else g.data_ptr() for g in gmeans])
         with _Guard(dev):
-            if gnll is None and gloss is None and gelbo is None and gmeans is not None and grad is not None:
-                terms = [torch.empty((B,), dtype=logits.dtype, device=dev) if n else None for n in need]
-                call('vae_nll_fused_backward', ptr(grad), grad.numel(), ptr(gmeans), kl_beta, inv_count, ptr(terms[0]),
-                     ptr(terms[1]), ptr(terms[2]), B, dtype_code(logits), stream_ptr(dev))
-            else:
-                # the per-sample upstream gradient is formed in fp32: 1/B of a mean is a subnormal of fp16
-                f32 = lambda t: None if t is None else t.contiguous().float()
-                gloss, gelbo = f32(gloss), f32(gelbo)
-                g = torch.empty((B,), dtype=torch.float32, device=dev)
-                terms = [torch.empty_like(g) if n else None for n in need]
-                call('vae_elbo_combine_bwd', ptr(gloss), ptr(gelbo), ptr(gmeans), kl_beta, inv_count, ptr(g),
-                     ptr(terms[0]), ptr(terms[1]), ptr(terms[2]), B, _lib.VAE_F32, stream_ptr(dev))
-                if gnll is not None:
-                    g = g + f32(gnll)
-                terms = [None if t is None else t.to(logits.dtype) for t in terms]
-                grad = None
-                if ctx.needs_input_grad[0]:
-                    grad = _token_bwd(logits, tokens, tokens, None, None, stats, g, tokens.numel() // max(B, 1), -1.0,
-                                      None, None)
-        return (grad, None, None) + tuple(terms) + (None, None, None, None)
+            call('vae_token_elbo_bwd', ptr(gnll), ptr(gloss), ptr(gelbo), at, _lib.DTYPE_CODES[mean_dtype], kl_beta,
+                 inv_count, ptr(grow), ptr(grad) if stored else None, grad.numel() if stored else 0, ptr(terms[0]),
+                 ptr(terms[1]), ptr(terms[2]), B, dtype_code(logits), stream_ptr(dev))
+        if not stored:
+            grad = None
+            if need[0]:
+                grad = _token_bwd(logits, tokens, None, None, stats, grow, tokens.numel() // max(B, 1), -1.0, None, None)
+        return (grad, None) + tuple(terms) + (None, None, None, None, None)
 
 
-def _token_bwd(logits, g_tokens, tokens, entropy, ids, stats, glogp, rows_per_g, g_scale, gentropy, gtop):
-    """d(logits).  `tokens` says which rows are padding; `g_tokens` is None when no gradient reached their log probs."""
-    dev = logits.device
-    N, V = logits.shape
-    grad = torch.empty((N, V), dtype=logits.dtype, device=dev)
-    if g_tokens is None and tokens is not None:
-        glogp, rows_per_g, g_scale = torch.zeros((1,), dtype=torch.float32, device=dev), max(N, 1), 0.0
-    with _Guard(dev):
-        call('vae_token_logp_bwd', ptr(logits), logits.stride(0), ptr(tokens),
-             0 if tokens is None else tokens.element_size(), ptr(stats), ptr(entropy), ptr(glogp), max(rows_per_g, 1),
-             g_scale, ptr(gentropy), ptr(gtop), ptr(ids) if gtop is not None else None,
-             ids.shape[1] if gtop is not None else 0, ptr(grad), N, V, dtype_code(logits), stream_ptr(dev))
-    return grad
+def token_nll_elbo(x, recon_x, kld=None, add=None, mi=None, kl_beta=1.0, inv_count=None, fuse_backward=False,
+                   mean_dtype=torch.float32):
+    """nll_elbo for nll_type 'categorical' with the six means as scalars: (nll, loss, elbo [B], 6 scalars in
+    `mean_dtype`)."""
+    _check_tokens(x, recon_x)
+    if inv_count is None:
+        inv_count = 1.0 / max(x.shape[0], 1)
+    kld, add, mi = (None if t is None else t.to(recon_x.dtype).contiguous() for t in (kld, add, mi))
+    # fp16: two passes, for the reason given in nll_elbo
+    fuse = bool(fuse_backward and recon_x.dtype != torch.float16 and recon_x.requires_grad and torch.is_grad_enabled()
+                and recon_x.numel() > 0)
+    out = _TokenNllElbo.apply(recon_x, x.contiguous(), kld, add, mi, float(kl_beta), float(inv_count), True, fuse,
+                              mean_dtype)
+    return out[0], out[1], out[2], out[3:]
 
 
 def _token_steps_elbo(xs, recons, kld, add, mi, kl_beta, inv_count, with_lse):
@@ -744,7 +743,7 @@ def _token_steps_elbo(xs, recons, kld, add, mi, kl_beta, inv_count, with_lse):
 
 
 class _Distill(torch.autograd.Function):
-    """kl [N] and mean = inv_count * sum(kl); fuse: d(mean)/d(logits) out of the forward launch, handed out by
+    """kl [...] and mean = inv_count * sum(kl); fuse: d(mean)/d(logits) out of the forward launch, handed out by
     backward() when only the mean's gradient arrives (rescaled on the device when that is not 1)."""
 
     @staticmethod
@@ -763,32 +762,34 @@ class _Distill(torch.autograd.Function):
         logits, teacher, ids, stats = ctx.saved_tensors
         temperature, inv_count = ctx.cfg
         dev = logits.device
-        N, V = logits.shape
         grad, ctx.grad = ctx.grad, None
         gkl, gmean = _dense(gkl), _dense(gmean)
         with _Guard(dev):
             if gkl is None and grad is not None:
                 call('vae_grad_scale', ptr(grad), ptr(gmean), grad.numel(), dtype_code(grad), stream_ptr(dev))
             else:
-                grad = torch.empty((N, V), dtype=logits.dtype, device=dev)
-                call('vae_distill_bwd', ptr(logits), logits.stride(0), ptr(teacher), teacher.stride(0),
+                rows = _rows(logits)
+                grad = torch.empty(logits.shape, dtype=logits.dtype, device=dev)
+                call('vae_distill_bwd', ptr(rows), rows.stride(0), ptr(teacher), teacher.stride(0),
                      dtype_code(teacher), ptr(ids), ids.stride(0), ids.element_size(), ids.shape[1], temperature,
-                     ptr(stats), ptr(gkl), ptr(gmean), inv_count, ptr(grad), N, V, dtype_code(logits), stream_ptr(dev))
+                     ptr(stats), ptr(gkl), ptr(gmean), inv_count, ptr(grad), rows.shape[0], rows.shape[1],
+                     dtype_code(rows), stream_ptr(dev))
         return grad, None, None, None, None, None
 
 
 def _distill_fwd(logits, teacher, ids, temperature, inv_count, want_stats, fuse):
     dev = check_device(logits, teacher, ids)
-    N, V = logits.shape
-    kl = torch.empty((N,), dtype=torch.float32, device=dev)
+    rows = _rows(logits)
+    N, V = rows.shape
+    kl = torch.empty(logits.shape[:-1], dtype=torch.float32, device=dev)
     stats = torch.empty((N, 2), dtype=torch.float32, device=dev) if want_stats else None
-    grad = torch.empty((N, V), dtype=logits.dtype, device=dev) if fuse else None
-    scratch = _token_scratch(logits, 0, dev)
+    grad = torch.empty(logits.shape, dtype=logits.dtype, device=dev) if fuse else None
+    scratch = _token_scratch(rows, 0, dev)
     with _Guard(dev):
-        call('vae_distill_fwd', ptr(logits), logits.stride(0), ptr(teacher), teacher.stride(0), dtype_code(teacher),
+        call('vae_distill_fwd', ptr(rows), rows.stride(0), ptr(teacher), teacher.stride(0), dtype_code(teacher),
              ptr(ids), ids.stride(0), ids.element_size(), ids.shape[1], temperature, ptr(kl), ptr(stats), ptr(grad),
-             inv_count, ptr(scratch), N, V, dtype_code(logits), stream_ptr(dev))
-        mean = _row_sums(kl, inv_count, 1, torch.float32).reshape(())
+             inv_count, ptr(scratch), N, V, dtype_code(rows), stream_ptr(dev))
+        mean = _row_sums(kl, inv_count, (), torch.float32)
     return kl, mean, stats, grad
 
 
@@ -800,12 +801,11 @@ def distill_top_logits(logits, teacher_logits, teacher_ids, temperature=1.0, inv
     loss is to be weighted so).  Differentiable with respect to `logits` only.
 
     A negative id or a teacher logit of -inf is no entry; a row without entries has kl 0 and gradient 0 whatever it
-    holds; an id may come twice; an id beyond the vocabulary gives NaN.  `fuse_backward`: d(mean)/d(logits) is formed by the
-    forward launch (one read of the logits per step instead of two); a gradient on `kl` takes the general kernel."""
-    shape = logits.shape[:-1]
-    rows = _vocab_rows(logits, 'distill_top_logits')
+    holds; an id may come twice; an id beyond the vocabulary gives NaN.  `fuse_backward`: d(mean)/d(logits) is formed by
+    the forward launch (one read of the logits per step instead of two); a gradient on `kl` takes the general kernel."""
+    _check_vocab(logits, 'distill_top_logits')
     _id_bytes(teacher_ids, 'distill_top_logits')
-    if teacher_logits.shape != teacher_ids.shape or teacher_ids.shape[:-1] != shape or teacher_ids.dim() < 1:
+    if teacher_logits.shape != teacher_ids.shape or teacher_ids.dim() < 1 or teacher_ids.shape[:-1] != logits.shape[:-1]:
         raise ValueError("distill_top_logits: teacher logits %s / ids %s do not fit logits %s"
                          % (tuple(teacher_logits.shape), tuple(teacher_ids.shape), tuple(logits.shape)))
     if not 1 <= teacher_ids.shape[-1] <= MAX_TEACHER:
@@ -816,14 +816,12 @@ def distill_top_logits(logits, teacher_logits, teacher_ids, temperature=1.0, inv
     if teacher_logits.requires_grad and torch.is_grad_enabled():
         raise ValueError("distill_top_logits: no gradient is formed for the teacher; pass teacher_logits.detach()")
     teacher, ids = _rows(teacher_logits), _rows(teacher_ids)
-    inv_count = 1.0 / max(rows.shape[0], 1) if inv_count is None else float(inv_count)
-    if rows.requires_grad and torch.is_grad_enabled():
+    inv_count = 1.0 / max(logits.shape[:-1].numel(), 1) if inv_count is None else float(inv_count)
+    if logits.requires_grad and torch.is_grad_enabled():
         # fp16: two passes, for the reason given in nll_elbo
-        fuse = bool(fuse_backward) and rows.dtype != torch.float16 and rows.numel() > 0
-        kl, mean = _Distill.apply(rows, teacher, ids, temperature, inv_count, fuse)
-    else:
-        kl, mean, _, _ = _distill_fwd(rows, teacher, ids, temperature, inv_count, False, False)
-    return kl.reshape(shape), mean
+        fuse = bool(fuse_backward) and logits.dtype != torch.float16 and logits.numel() > 0
+        return _Distill.apply(logits, teacher, ids, temperature, inv_count, fuse)
+    return _distill_fwd(logits, teacher, ids, temperature, inv_count, False, False)[:2]
 
 
 class _SampleSums(torch.autograd.Function):
@@ -834,7 +832,7 @@ class _SampleSums(torch.autograd.Function):
         dev = check_device(rows)
         ctx.n = rows.numel()
         with _Guard(dev):
-            return _row_sums(rows, 1.0, B, dtype)
+            return _row_sums(rows, 1.0, (B,), dtype)
 
     @staticmethod
     def backward(ctx, g):
