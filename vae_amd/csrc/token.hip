@@ -11,7 +11,6 @@
 
 namespace vae {
 
-constexpr int kCand = 1024;          // candidates for the alternatives that LDS holds
 constexpr int kVecBytes = 16;
 constexpr float kHuge = 1.0e6f;      // |max| beyond which the shifted exponent is formed as (x - m) c, see row_stats
 
@@ -56,46 +55,44 @@ struct RunStats {
 };
 
 // Statistics of vectors [v0, v1) of a row (and its edges when they belong to this piece), for the whole workgroup.
-// On return m, s, t are the workgroup's, relative to the exact maximum; `tile` is the thread's first vector group that
-// reached its own maximum `mine` (for the alternatives), -1 if it has none.
-template <typename T, int BT, bool ENT>
+// On return m, s, t are the workgroup's, relative to the exact maximum; `mine` is the thread's own maximum (without the
+// edge), for the alternatives.  NT: the row is not read again.
+template <typename T, int BT, bool ENT, bool NT>
 __device__ __forceinline__ void row_stats(const T* __restrict__ x, const RowCut<T, VecOf<T>::n>& cut, int v0, int v1,
-                                          float edge, bool has_edge, float c, float& m, float& s, float& t, float& mine,
-                                          int& tile) {
+                                          float edge, bool has_edge, float c, float& m, float& s, float& t,
+                                          float& mine) {
   constexpr int VN = VecOf<T>::n, U = 4;
   const Buffer body(x + cut.head, cut.nvec * kVecBytes);
   RunStats<ENT> st(c);
-  tile = -1;
-  int j = v0 + (int)threadIdx.x;
-  const int full = (v1 - v0) / (U * BT);
-  if (j < v1) tile = j;
-  for (int it = 0; it < full; ++it, j += U * BT) {
-    Packet<T, VN> p[U];
+  // W vectors of a lane; a running maximum for all of them
+  auto group = [&](auto& p) {
+    constexpr int W = sizeof(p) / sizeof(p[0]);
+    float v[W][VN], mt = -INFINITY;
 #pragma unroll
-    for (int u = 0; u < U; ++u) p[u].load(body, j * kVecBytes, u * BT * kVecBytes);
-    float v[U][VN], mt = -INFINITY;
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
+    for (int u = 0; u < W; ++u) {
       p[u].get(v[u]);
       mt = vec_max(v[u], mt);
     }
-    if (mt > st.m) tile = j;
     st.raise(mt, c);
 #pragma unroll
-    for (int u = 0; u < U; ++u)
+    for (int u = 0; u < W; ++u) {
 #pragma unroll
       for (int i = 0; i < VN; ++i) st.add(v[u][i], c);
+      __builtin_amdgcn_sched_barrier(0);   // vector by vector: interleaved they need half as many registers again
+    }
+  };
+  int j = v0 + (int)threadIdx.x;
+  const int full = (v1 - v0) / (U * BT);
+  for (int it = 0; it < full; ++it, j += U * BT) {
+    Packet<T, VN> p[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) p[u].template load<NT>(body, j * kVecBytes, u * BT * kVecBytes);
+    group(p);
   }
   for (; j < v1; j += BT) {
-    Packet<T, VN> p;
-    p.load(body, j * kVecBytes, 0);
-    float v[VN];
-    p.get(v);
-    const float mt = vec_max(v, -INFINITY);
-    if (mt > st.m) tile = j;
-    st.raise(mt, c);
-#pragma unroll
-    for (int i = 0; i < VN; ++i) st.add(v[i], c);
+    Packet<T, VN> p[1];
+    p[0].template load<NT>(body, j * kVecBytes, 0);
+    group(p);
   }
   mine = st.m;
   if (has_edge) {
@@ -124,7 +121,7 @@ __device__ __forceinline__ void row_stats(const T* __restrict__ x, const RowCut<
   };
   for (j = v0 + (int)threadIdx.x; j < v1; j += BT) {
     Packet<T, VN> p;
-    p.load(body, j * kVecBytes, 0);
+    p.template load<NT>(body, j * kVecBytes, 0);
     float v[VN];
     p.get(v);
 #pragma unroll
@@ -136,45 +133,50 @@ __device__ __forceinline__ void row_stats(const T* __restrict__ x, const RowCut<
 }
 
 // ---------------------------------------------------------------------------------------------------------------
-// The k largest keys of a set.  Every thread brings the largest key of its own share; the k-th largest of those is a
-// lower bound of the k-th largest of all, and only the k threads at or above it can hold any of the k.
+// The k largest keys (order_key: value, then the lower index) of what a workgroup has read.  A bound from below comes
+// from the threads' own maxima: every wave takes the ceil(k / waves)-th largest of its lanes', the least of those has k
+// elements at or above it.  Only the few threads whose maximum reaches the bound can hold any of the k; their vectors
+// are read once more (out of the caches), all lanes side by side.  Measured beside a list kept while reading: the list
+// costs every element a comparison (4096 x 32768, k = 20: 145 us with it, see fwd_type for this one).
 // ---------------------------------------------------------------------------------------------------------------
+constexpr int kCand = 1024;      // candidates that LDS holds
+constexpr int kMostShares = 96;  // threads at the bound beyond which equal values are told apart by their index first
+
 template <int BT>
 struct TopLds {
-  uint64_t keys[BT], cand[kCand];
-  int seg[BT];
-  int nseg, ncand;
-  uint64_t bound;
+  uint64_t cand[kCand];
+  uint64_t wave_bound[BT / 64];
+  int share[BT];
+  int nshare, ncand;
 };
 
-// the k-th largest of the BT keys in lds.keys (0 where fewer than k are there): bit by bit, by the first wave
-template <int BT>
-__device__ __forceinline__ uint64_t kth_key(TopLds<BT>& lds, uint64_t mine, int k) {
-  lds_barrier();
-  lds.keys[threadIdx.x] = mine;
-  if (threadIdx.x == 0) lds.nseg = lds.ncand = 0;
-  lds_barrier();
-  if (threadIdx.x < 64) {
-    uint64_t key[BT / 64];
-#pragma unroll
-    for (int i = 0; i < BT / 64; ++i) key[i] = lds.keys[threadIdx.x + 64 * i];
-    uint64_t b = 0;
-    for (int bit = 63; bit >= 0; --bit) {
-      const uint64_t want = b | (1ull << bit);
-      int n = 0;
-#pragma unroll
-      for (int i = 0; i < BT / 64; ++i) n += __popcll(__ballot(key[i] >= want));
-      if (n >= k) {
-        b = want;
-        if (n == k) break;
-      }
+// the n-th largest of a wave's 64 keys, or a number below it that no more than the n-th largest share down to bit
+// `last`; 0 where there are fewer than n
+__device__ __forceinline__ uint64_t wave_nth(uint64_t key, int n, int last) {
+  uint64_t b = 0;
+  for (int bit = 63; bit >= last; --bit) {
+    const uint64_t want = b | (1ull << bit);
+    const int c = __popcll(__ballot(key >= want));
+    if (c >= n) {
+      b = want;
+      if (c == n) break;
     }
-    if (threadIdx.x == 0) lds.bound = b;
   }
-  lds_barrier();
-  return lds.bound;
+  return b;
 }
-
+template <int BT>
+__device__ __forceinline__ uint64_t block_bound(TopLds<BT>& lds, uint64_t key, int k, int last) {
+  constexpr int NW = BT / 64;
+  const uint64_t mine = wave_nth(key, (k + NW - 1) / NW, last);
+  lds_barrier();   // what the last one left has been read
+  if ((threadIdx.x & 63) == 0) lds.wave_bound[threadIdx.x >> 6] = mine;
+  if (threadIdx.x == 0) lds.nshare = lds.ncand = 0;
+  lds_barrier();
+  uint64_t b = lds.wave_bound[0];
+#pragma unroll
+  for (int w = 1; w < NW; ++w) b = lds.wave_bound[w] < b ? lds.wave_bound[w] : b;
+  return b;
+}
 template <int BT>
 __device__ __forceinline__ void push_key(TopLds<BT>& lds, uint64_t key, uint64_t bound) {
   if (key != 0 && key >= bound) {
@@ -182,7 +184,6 @@ __device__ __forceinline__ void push_key(TopLds<BT>& lds, uint64_t key, uint64_t
     if (at < kCand) lds.cand[at] = key;
   }
 }
-
 // emit(rank, key) for the candidates of rank < k; key 0 for the ranks that are not there.  False: too many candidates.
 template <int BT, typename Emit>
 __device__ __forceinline__ bool emit_ranked(TopLds<BT>& lds, int k, Emit emit) {
@@ -192,6 +193,7 @@ __device__ __forceinline__ bool emit_ranked(TopLds<BT>& lds, int k, Emit emit) {
   for (int i = threadIdx.x; i < n; i += BT) {
     const uint64_t key = lds.cand[i];
     int rank = 0;
+#pragma unroll 4
     for (int q = 0; q < n; ++q) rank += lds.cand[q] > key ? 1 : 0;
     if (rank < k) emit(rank, key);
   }
@@ -199,67 +201,67 @@ __device__ __forceinline__ bool emit_ranked(TopLds<BT>& lds, int k, Emit emit) {
   return true;
 }
 
-// The k largest of vectors [v0, v1) and the edges of a row; `mine`, `tile` from row_stats.
 template <typename T, int BT, typename Emit>
 __device__ __forceinline__ void row_top(TopLds<BT>& lds, const T* __restrict__ x, const RowCut<T, VecOf<T>::n>& cut,
-                                        int v0, int v1, float edge, int edge_index, float mine, int tile, int k,
-                                        Emit emit) {
-  constexpr int VN = VecOf<T>::n, U = 4;
+                                        int v0, int v1, float edge, int edge_index, float mine, int k, Emit emit) {
+  constexpr int VN = VecOf<T>::n;
+  // value bits that tell two numbers of the type apart (fp32: enough of them)
+  constexpr int kLastBit = sizeof(T) == 2 ? 48 : 40;
   const Buffer body(x + cut.head, cut.nvec * kVecBytes);
-  auto vec_key = [&](int j, int i, float v) { return order_key(v, (uint32_t)(cut.index(j) + i)); };
-  uint64_t key = edge_index >= 0 ? order_key(edge, (uint32_t)edge_index) : 0;
-  if (tile >= 0) {
-    // the first element of the thread's share that is its maximum: somewhere in `tile`
+  const int tid = threadIdx.x;
+  auto each = [&](int j, auto f) {   // the elements of vector j
+    Packet<T, VN> p;
+    p.template load<false>(body, j * kVecBytes, 0);
+    float v[VN];
+    p.get(v);
+#pragma unroll
+    for (int i = 0; i < VN; ++i) f(v[i], (uint32_t)(cut.index(j) + i));
+  };
+  const uint64_t edge_key = edge_index >= 0 ? order_key(edge, (uint32_t)edge_index) : 0;
+  uint64_t key = v0 + tid < v1 ? (uint64_t)order_bits(mine) << 32 : 0;
+  const uint64_t edge_top = edge_key >> 32 << 32;
+  key = edge_top > key ? edge_top : key;
+  uint64_t bound = block_bound(lds, key, k, kLastBit);
+  auto take_share = [&]() {
+    if (key != 0 && key >= bound) lds.share[atomicAdd(&lds.nshare, 1)] = tid;
+    lds_barrier();
+    return lds.nshare;
+  };
+  int n = take_share();
+  if (n > kMostShares) {
+    // many equal maxima (a constant row, a mask that leaves little): the first index of each decides
+    key = edge_key;
     uint64_t best = 0;
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int j = tile + u * BT;
-      if (j < v1) {
-        Packet<T, VN> p;
-        p.load(body, j * kVecBytes, 0);
-        float v[VN];
-        p.get(v);
-#pragma unroll
-        for (int i = 0; i < VN; ++i)
-          if (v[i] == mine && best == 0) best = vec_key(j, i, v[i]);
-      }
-    }
+    for (int j = v0 + tid; j < v1 && best == 0; j += BT)
+      each(j, [&](float v, uint32_t at) { best = v == mine && best == 0 ? order_key(v, at) : best; });
     key = best > key ? best : key;
+    bound = block_bound(lds, key, k, 0);
+    n = take_share();
   }
-  const uint64_t bound = kth_key(lds, key, k);
-  if (key != 0 && key >= bound) lds.seg[atomicAdd(&lds.nseg, 1)] = threadIdx.x;
-  if (edge_index >= 0) push_key(lds, order_key(edge, (uint32_t)edge_index), bound);
-  lds_barrier();
-  const int nseg = lds.nseg, wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-  for (int q = wave; q < nseg; q += BT / 64) {
-    for (int j = v0 + lds.seg[q] + lane * BT; j < v1; j += 64 * BT) {
-      Packet<T, VN> p;
-      p.load(body, j * kVecBytes, 0);
-      float v[VN];
-      p.get(v);
-#pragma unroll
-      for (int i = 0; i < VN; ++i) push_key(lds, vec_key(j, i, v[i]), bound);
+  push_key(lds, edge_key, bound);
+  // the shares' vectors, side by side: share q holds v0 + share[q] + i BT
+  const int per = (v1 - v0 + BT - 1) / BT;
+  const float least = (bound >> 32) > order_bits(-INFINITY) ? key_value(bound) : -INFINITY;   // below it lie the NaN
+  for (int q = tid; q < n * per; q += BT) {
+    const int j = v0 + lds.share[q / per] + (q % per) * BT;
+    if (j < v1) {
+      each(j, [&](float v, uint32_t at) {
+        if (v >= least) push_key(lds, order_key(v, at), bound);
+      });
     }
   }
   if (emit_ranked(lds, k, emit)) return;
   // the large values all sit in few threads' shares: one after the other
   uint64_t last = ~0ull;
   for (int r = 0; r < k; ++r) {
-    uint64_t best = edge_index >= 0 ? order_key(edge, (uint32_t)edge_index) : 0;
-    if (best >= last) best = 0;
-    for (int j = v0 + (int)threadIdx.x; j < v1; j += BT) {
-      Packet<T, VN> p;
-      p.load(body, j * kVecBytes, 0);
-      float v[VN];
-      p.get(v);
-#pragma unroll
-      for (int i = 0; i < VN; ++i) {
-        const uint64_t kk = vec_key(j, i, v[i]);
-        if (kk < last && kk > best) best = kk;
-      }
-    }
+    uint64_t best = edge_key < last ? edge_key : 0;
+    for (int j = v0 + tid; j < v1; j += BT)
+      each(j, [&](float v, uint32_t at) {
+        const uint64_t kk = order_key(v, at);
+        best = kk < last && kk > best ? kk : best;
+      });
     last = block_max_key<BT>(best);
-    if (threadIdx.x == 0) emit(r, last);
+    if (tid == 0) emit(r, last);
   }
 }
 
@@ -280,18 +282,18 @@ __device__ __forceinline__ void write_padding(const FwdArgs& a, int64_t row) {
   }
 }
 // what a row's statistics give, once they are whole
-template <typename T, int BT, bool ENT, bool DIST>
-__device__ __forceinline__ void write_row(const FwdArgs& a, int64_t row, const T* __restrict__ x, int64_t tok, float m,
-                                          float s, float t, const TeacherRow<BT>* tr) {
+template <int BT, bool ENT, bool DIST>
+__device__ __forceinline__ void write_row(const FwdArgs& a, int64_t row, int64_t tok, float token_logit, float m, float s,
+                                          float t, const TeacherRow<BT>* tr) {
   float kl = 0.f;
   if constexpr (DIST) {
     for (int k = threadIdx.x; k < a.teacher.K; k += BT)
-      if (tr->id[k] >= 0) kl += tr->q[k] * (tr->logq[k] - row_log_prob(to_f32(x[tr->id[k]]), m, s, a.inv_tau));
+      if (tr->id[k] >= 0) kl += tr->q[k] * (tr->logq[k] - row_log_prob(tr->x[k], m, s, a.inv_tau));
     kl = block_sum<BT>(kl);
   }
   if (threadIdx.x == 0) {
     if constexpr (DIST) a.logp[row] = kl;
-    else if (a.logp) a.logp[row] = tok < a.V ? row_log_prob(to_f32(x[tok]), m, s, 1.0f) : nan_f();
+    else if (a.logp) a.logp[row] = tok < a.V ? row_log_prob(token_logit, m, s, 1.0f) : nan_f();
     if constexpr (ENT) a.entropy[row] = s == 0.f ? 0.f : kLn2 * (log2f(s) - t / s);
     if (a.stats) {
       a.stats[2 * row] = m;
@@ -312,6 +314,7 @@ __global__ __launch_bounds__(BT) void token_fwd_kernel(FwdArgs a) {
     const int part = a.parts == 1 ? 0 : (int)(item - row * a.parts);
     const T* x = (const T*)a.logits + row * a.row_stride;
     int64_t tok = 0;
+    float token_logit = 0.f;       // asked for in front of the row: it is there when the row's sum is
     if constexpr (DIST) {
       if (a.parts == 1) {
         const int state = lds.teacher[0].load(a.teacher, row, a.V, a.inv_tau, a.scale2);
@@ -322,6 +325,8 @@ __global__ __launch_bounds__(BT) void token_fwd_kernel(FwdArgs a) {
           }
           continue;
         }
+        for (int k = threadIdx.x; k < a.teacher.K; k += BT)
+          lds.teacher[0].x[k] = lds.teacher[0].id[k] >= 0 ? to_f32(x[lds.teacher[0].id[k]]) : 0.f;
       }
     } else {
       tok = a.tokens ? load_id(a.tokens, a.token_bytes, row) : 0;
@@ -329,6 +334,7 @@ __global__ __launch_bounds__(BT) void token_fwd_kernel(FwdArgs a) {
         if (a.parts == 1) write_padding<BT>(a, row);
         continue;
       }
+      if (tok < a.V && a.parts == 1) token_logit = to_f32(x[tok]);
     }
     const RowCut<T, VN> cut(x, a.V);
     const int v0 = part * a.part_vecs;
@@ -338,24 +344,21 @@ __global__ __launch_bounds__(BT) void token_fwd_kernel(FwdArgs a) {
     if (ei >= 0 && (ei < cut.head ? part != 0 : part != a.parts - 1)) ei = -1;  // the head goes with the first piece
     const float edge = ei >= 0 ? to_f32(x[ei]) : -INFINITY;
     float m, s, t = 0.f, mine;
-    int tile;
-    row_stats<T, BT, ENT>(x, cut, v0, v1, edge, ei >= 0, a.scale2, m, s, t, mine, tile);
+    row_stats<T, BT, ENT, !TOP>(x, cut, v0, v1, edge, ei >= 0, a.scale2, m, s, t, mine);
+    if constexpr (TOP) {
+      char* to = a.scratch + item * part_bytes(a.top_k) + 16;
+      row_top<T, BT>(lds.top[0], x, cut, v0, v1, edge, ei, mine, a.top_k, [&](int rank, uint64_t key) {
+        if (a.parts == 1) emit_top(a, row, rank, key, m, s);
+        else reinterpret_cast<uint64_t*>(to)[rank] = key;
+      });
+    }
     if (a.parts == 1) {
-      if constexpr (TOP)
-        row_top<T, BT>(lds.top[0], x, cut, v0, v1, edge, ei, mine, tile, a.top_k,
-                       [&](int rank, uint64_t key) { emit_top(a, row, rank, key, m, s); });
-      write_row<T, BT, ENT, DIST>(a, row, x, tok, m, s, t, lds.teacher);
-    } else {
-      char* to = a.scratch + item * part_bytes(a.top_k);
-      if (threadIdx.x == 0) {
-        float* f = reinterpret_cast<float*>(to);
-        f[0] = m;
-        f[1] = s;
-        f[2] = t;
-      }
-      if constexpr (TOP)
-        row_top<T, BT>(lds.top[0], x, cut, v0, v1, edge, ei, mine, tile, a.top_k,
-                       [&](int rank, uint64_t key) { reinterpret_cast<uint64_t*>(to + 16)[rank] = key; });
+      write_row<BT, ENT, DIST>(a, row, tok, token_logit, m, s, t, lds.teacher);
+    } else if (threadIdx.x == 0) {
+      float* f = reinterpret_cast<float*>(a.scratch + item * part_bytes(a.top_k));
+      f[0] = m;
+      f[1] = s;
+      f[2] = t;
     }
   }
 }
@@ -367,9 +370,33 @@ __global__ __launch_bounds__(BT) void token_join_kernel(FwdArgs a) {
     TopLds<TOP ? BT : 64> top[TOP ? 1 : 0];
     TeacherRow<BT> teacher[DIST ? 1 : 0];
   } lds;
+  constexpr int R = kCand / BT;     // keys a thread holds; more of them are read where they are
   for (int64_t row = blockIdx.x; row < a.N; row += gridDim.x) {
     const T* x = (const T*)a.logits + row * a.row_stride;
-    int64_t tok = 0;
+    // everything that does not depend on anything else is on its way first
+    const char* from = a.scratch + row * a.parts * part_bytes(a.top_k);
+    const int n = a.parts * a.top_k;
+    auto key_at = [&](int i) {
+      const int p = i / a.top_k;
+      return reinterpret_cast<const uint64_t*>(from + p * part_bytes(a.top_k) + 16)[i - p * a.top_k];
+    };
+    const int64_t tok = !DIST && a.tokens ? load_id(a.tokens, a.token_bytes, row) : 0;
+    float mp = -INFINITY, sp = 0.f, tp = 0.f;
+    if ((int)threadIdx.x < a.parts) {   // parts <= BT
+      const float* f = reinterpret_cast<const float*>(from + threadIdx.x * part_bytes(a.top_k));
+      mp = f[0];
+      sp = f[1];
+      tp = f[2];
+    }
+    uint64_t keys[TOP ? R : 1], below = 0;
+    if constexpr (TOP) {
+#pragma unroll
+      for (int r = 0; r < R; ++r) keys[r] = (int)threadIdx.x + r * BT < n ? key_at(threadIdx.x + r * BT) : 0;
+      // a piece's keys are in order: the ceil(k / parts)-th of every piece has k keys at or above the least of them
+      const int at = (a.top_k + a.parts - 1) / a.parts - 1;
+      if ((int)threadIdx.x < a.parts) below = ~key_at(threadIdx.x * a.top_k + at);
+    }
+    float token_logit = 0.f;
     if constexpr (DIST) {
       const int state = lds.teacher[0].load(a.teacher, row, a.V, a.inv_tau, a.scale2);
       if (state != kRowFine) {
@@ -379,20 +406,14 @@ __global__ __launch_bounds__(BT) void token_join_kernel(FwdArgs a) {
         }
         continue;
       }
+      for (int k = threadIdx.x; k < a.teacher.K; k += BT)
+        lds.teacher[0].x[k] = lds.teacher[0].id[k] >= 0 ? to_f32(x[lds.teacher[0].id[k]]) : 0.f;
     } else {
-      tok = a.tokens ? load_id(a.tokens, a.token_bytes, row) : 0;
       if (tok < 0) {
         write_padding<BT>(a, row);
         continue;
       }
-    }
-    const char* from = a.scratch + row * a.parts * part_bytes(a.top_k);
-    float mp = -INFINITY, sp = 0.f, tp = 0.f;
-    if ((int)threadIdx.x < a.parts) {   // parts <= BT
-      const float* f = reinterpret_cast<const float*>(from + threadIdx.x * part_bytes(a.top_k));
-      mp = f[0];
-      sp = f[1];
-      tp = f[2];
+      if (tok < a.V) token_logit = to_f32(x[tok]);
     }
     const float m = block_max<BT>(mp);
     const float d = sp == 0.f ? 0.f : (mp - m) * a.scale2;
@@ -401,33 +422,28 @@ __global__ __launch_bounds__(BT) void token_join_kernel(FwdArgs a) {
     float t = 0.f;
     if constexpr (ENT) t = block_sum<BT>(w * __builtin_fmaf(max_raw(d, -300.f), sp, tp));
     if constexpr (TOP) {
-      const int n = a.parts * a.top_k;
-      auto key_at = [&](int i) {
-        const int p = i / a.top_k;
-        return reinterpret_cast<const uint64_t*>(from + p * part_bytes(a.top_k) + 16)[i - p * a.top_k];
-      };
       auto emit = [&](int rank, uint64_t key) { emit_top(a, row, rank, key, m, s); };
-      uint64_t mine = 0;
-      for (int i = threadIdx.x; i < n; i += BT) {
-        const uint64_t key = key_at(i);
-        mine = key > mine ? key : mine;
-      }
-      const uint64_t bound = kth_key(lds.top[0], mine, a.top_k);
-      for (int i = threadIdx.x; i < n; i += BT) push_key(lds.top[0], key_at(i), bound);
+      auto for_keys = [&](auto f) {
+#pragma unroll
+        for (int r = 0; r < R; ++r) f(keys[r]);
+        for (int i = kCand + threadIdx.x; i < n; i += BT) f(key_at(i));
+      };
+      const uint64_t bound = ~block_max_key<BT>(below);
+      lds_barrier();                 // the row before this one has been ranked
+      if (threadIdx.x == 0) lds.top[0].ncand = 0;
+      lds_barrier();
+      for_keys([&](uint64_t key) { push_key(lds.top[0], key, bound); });
       if (!emit_ranked(lds.top[0], a.top_k, emit)) {
         uint64_t last = ~0ull;
         for (int r = 0; r < a.top_k; ++r) {
           uint64_t best = 0;
-          for (int i = threadIdx.x; i < n; i += BT) {
-            const uint64_t key = key_at(i);
-            if (key < last && key > best) best = key;
-          }
+          for_keys([&](uint64_t key) { best = key < last && key > best ? key : best; });
           last = block_max_key<BT>(best);
           if (threadIdx.x == 0) emit(r, last);
         }
       }
     }
-    write_row<T, BT, ENT, DIST>(a, row, x, tok, m, s, t, lds.teacher);
+    write_row<BT, ENT, DIST>(a, row, tok, token_logit, m, s, t, lds.teacher);
   }
 }
 

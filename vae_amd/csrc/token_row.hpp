@@ -148,8 +148,9 @@ struct Packet {
   typedef uint32_t Raw __attribute__((ext_vector_type(4)));
   static constexpr int kBytes = 16;
   Raw raw;
+  template <bool NT = true>   // NT: not read again
   __device__ __forceinline__ void load(const Buffer& b, int lane_byte, int byte) {
-    raw = __builtin_amdgcn_raw_buffer_load_b128(b.rsrc, lane_byte, byte, kNonTemporal);
+    raw = __builtin_amdgcn_raw_buffer_load_b128(b.rsrc, lane_byte, byte, NT ? kNonTemporal : 0);
   }
   __device__ __forceinline__ void set_masked() {   // every element -inf
     const uint32_t inf = sizeof(T) == 4 ? 0xff800000u : (DTypeCode<T>::value == 2 ? 0xfc00fc00u : 0xff80ff80u);
@@ -187,6 +188,7 @@ template <typename T>
 struct Packet<T, 1> {
   static constexpr int kBytes = sizeof(T);
   T raw;
+  template <bool NT = true>
   __device__ __forceinline__ void load(const Buffer& b, int lane_byte, int byte) {
     if constexpr (sizeof(T) == 4) raw = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(b.rsrc, lane_byte, byte, 0));
     else raw.bits = __builtin_amdgcn_raw_buffer_load_b16(b.rsrc, lane_byte, byte, 0);
