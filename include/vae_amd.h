@@ -513,21 +513,25 @@ int vae_token_elbo_bwd(const void* gnll, const void* gloss, const void* gelbo, c
 int vae_row_sums(const float* rows, float scale, void* out, int64_t B, int64_t T, int dtype, vae_stream_t stream);
 /* buf[n] *= *factor (a device float); returns without touching buf when it is 1.                                   */
 int vae_grad_scale(void* buf, const float* factor, int64_t n, int dtype, vae_stream_t stream);
-/* Distillation from a teacher's K <= VAE_MAX_TEACHER largest logits per row (t_logits in t_dtype, t_ids; rows t_stride /
- * id_stride apart), both sides at `temperature` > 0:  q = softmax(t_logits / temperature) over the entries that are
- * there (id >= 0 and logit > -inf), p = softmax(logits / temperature) over V,
- * kl[r] = sum_k q_k (ln q_k - ln p[id_k]).  An id may come more than once.  No entry there: kl 0, gradient 0, whatever the
- * row's logits hold.  An id >= V: NaN, nothing is read out of range.  stats [N, 2] for the backward (may be NULL
- * without glogits); glogits != NULL: also grad_scale * d kl / d logits.  scratch: as above with top_k = 0.          */
+/* Distillation from a teacher's K <= VAE_MAX_TEACHER largest logits per row, both sides at `temperature` > 0:
+ * q = softmax(t_logits / temperature) over the entries that are there (id >= 0 and logit > -inf), p = softmax(logits /
+ * temperature) over V,  kl[r] = sum_k q_k (ln q_k - ln p[id_k]).  An id may come more than once.  No entry there: kl 0,
+ * gradient 0, the row's logits are not read.  An id >= V: NaN, nothing is read out of range.
+ * vae_distill_teacher prepares the teacher's side, vae_distill_teacher_floats(N, K) floats that the calls below read
+ * (one preparation serves forward and backward): t_logits [N, K] in t_dtype, t_ids, rows t_stride / id_stride apart.  */
 #define VAE_MAX_TEACHER 256
-int vae_distill_fwd(const void* logits, int64_t row_stride, const void* t_logits, int64_t t_stride, int t_dtype,
-                    const void* t_ids, int64_t id_stride, int id_bytes, int64_t K, float temperature, float* kl,
-                    float* stats, void* glogits, float grad_scale, void* scratch, int64_t N, int64_t V, int dtype,
-                    vae_stream_t stream);
+size_t vae_distill_teacher_floats(int64_t N, int64_t K);
+int vae_distill_teacher(const void* t_logits, int64_t t_stride, int t_dtype, const void* t_ids, int64_t id_stride,
+                        int id_bytes, int64_t K, float temperature, float* teacher, int64_t N, int64_t V,
+                        vae_stream_t stream);
+/* kl [N] and stats [N, 2] for the backward (may be NULL without glogits); glogits != NULL: also grad_scale * d kl /
+ * d logits.  scratch: vae_token_scratch_bytes(N, V, 0, dtype).                                                     */
+int vae_distill_fwd(const void* logits, int64_t row_stride, const float* teacher, int64_t K, float temperature,
+                    float* kl, float* stats, void* glogits, float grad_scale, void* scratch, int64_t N, int64_t V,
+                    int dtype, vae_stream_t stream);
 /* glogits[r] = (gkl[r] + *gmean * mean_scale) * d kl[r] / d logits[r]; gkl [N], gmean (one float): each may be NULL
  * (both NULL: mean_scale on every row).                                                                          */
-int vae_distill_bwd(const void* logits, int64_t row_stride, const void* t_logits, int64_t t_stride, int t_dtype,
-                    const void* t_ids, int64_t id_stride, int id_bytes, int64_t K, float temperature,
+int vae_distill_bwd(const void* logits, int64_t row_stride, const float* teacher, int64_t K, float temperature,
                     const float* stats, const float* gkl, const float* gmean, float mean_scale, void* glogits,
                     int64_t N, int64_t V, int dtype, vae_stream_t stream);
 

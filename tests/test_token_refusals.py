@@ -89,20 +89,24 @@ def fused(**kw):
 
 
 def dfwd(**kw):
-    a = dict(logits=P, stride=10, y=P, ys=2, yt=0, ids=P, ids_s=2, ib=8, K=2, tau=1.0, kl=P, stats=P, out=P, scale=1.0,
-             scratch=P, N=2, V=10, dtype=0)
+    a = dict(logits=P, stride=10, t=P, K=2, tau=1.0, kl=P, stats=P, out=P, scale=1.0, scratch=P, N=2, V=10, dtype=0)
     a.update(kw)
-    return _call('vae_distill_fwd', [a[n] for n in ('logits', 'stride', 'y', 'ys', 'yt', 'ids', 'ids_s', 'ib', 'K', 'tau',
-                                                    'kl', 'stats', 'out', 'scale', 'scratch', 'N', 'V', 'dtype')]
-                 + [None])
+    return _call('vae_distill_fwd', [a[n] for n in ('logits', 'stride', 't', 'K', 'tau', 'kl', 'stats', 'out', 'scale',
+                                                    'scratch', 'N', 'V', 'dtype')] + [None])
 
 
 def dbwd(**kw):
-    a = dict(logits=P, stride=10, y=P, ys=2, yt=0, ids=P, ids_s=2, ib=8, K=2, tau=1.0, stats=P, gkl=P, gm=P, scale=1.0,
-             out=P, N=2, V=10, dtype=0)
+    a = dict(logits=P, stride=10, t=P, K=2, tau=1.0, stats=P, gkl=P, gm=P, scale=1.0, out=P, N=2, V=10, dtype=0)
     a.update(kw)
-    return _call('vae_distill_bwd', [a[n] for n in ('logits', 'stride', 'y', 'ys', 'yt', 'ids', 'ids_s', 'ib', 'K', 'tau',
-                                                    'stats', 'gkl', 'gm', 'scale', 'out', 'N', 'V', 'dtype')] + [None])
+    return _call('vae_distill_bwd', [a[n] for n in ('logits', 'stride', 't', 'K', 'tau', 'stats', 'gkl', 'gm', 'scale',
+                                                    'out', 'N', 'V', 'dtype')] + [None])
+
+
+def teach(**kw):
+    a = dict(y=P, ys=2, yt=0, ids=P, ids_s=2, ib=8, K=2, tau=1.0, t=P, N=2, V=10)
+    a.update(kw)
+    return _call('vae_distill_teacher', [a[n] for n in ('y', 'ys', 'yt', 'ids', 'ids_s', 'ib', 'K', 'tau', 't', 'N', 'V')]
+                 + [None])
 
 
 BAD = [dict(N=-1), dict(V=0), dict(V=(1 << 24) + 1, stride=1 << 25), dict(stride=9), dict(dtype=3), dict(logits=None)]
@@ -122,19 +126,31 @@ def test_c_entry_points_refuse_bad_shapes(f, bad):
     (bwd, dict(tb=1)), (bwd, dict(ent=None)), (bwd, dict(gtop=None)), (bwd, dict(ids=None)), (bwd, dict(tokens=None)),
     (fused, dict(tokens=None)), (fused, dict(logp=None)), (fused, dict(stats=None)), (fused, dict(out=None)),
     (fused, dict(tb=0)),
-    (dfwd, dict(K=0)), (dfwd, dict(K=257, ys=300, ids_s=300)), (dfwd, dict(ys=1)), (dfwd, dict(ids_s=1)),
-    (dfwd, dict(ib=2)), (dfwd, dict(yt=9)), (dfwd, dict(tau=0.0)), (dfwd, dict(tau=float('nan'))),
-    (dfwd, dict(tau=float('inf'))), (dfwd, dict(y=None)), (dfwd, dict(ids=None)), (dfwd, dict(kl=None)),
-    (dfwd, dict(stats=None)),
-    (dbwd, dict(K=0)), (dbwd, dict(tau=-1.0)), (dbwd, dict(stats=None)), (dbwd, dict(out=None)), (dbwd, dict(y=None)),
+    (dfwd, dict(K=0)), (dfwd, dict(K=257)), (dfwd, dict(tau=0.0)), (dfwd, dict(tau=float('nan'))),
+    (dfwd, dict(tau=float('inf'))), (dfwd, dict(t=None)), (dfwd, dict(kl=None)), (dfwd, dict(stats=None)),
+    (dbwd, dict(K=0)), (dbwd, dict(tau=-1.0)), (dbwd, dict(stats=None)), (dbwd, dict(out=None)), (dbwd, dict(t=None)),
+    (teach, dict(K=0)), (teach, dict(K=257, ys=300, ids_s=300)), (teach, dict(ys=1)), (teach, dict(ids_s=1)),
+    (teach, dict(ib=2)), (teach, dict(yt=9)), (teach, dict(tau=0.0)), (teach, dict(tau=float('nan'))),
+    (teach, dict(tau=float('inf'))), (teach, dict(y=None)), (teach, dict(ids=None)), (teach, dict(t=None)),
+    (teach, dict(N=-1)), (teach, dict(V=0)),
 ])
 def test_c_entry_points_refuse_bad_arguments(f, bad):
     assert f(**bad) == _lib.VAE_ERR_ARG
 
 
-@pytest.mark.parametrize('f', [fwd, bwd, fused, dfwd, dbwd])
+@pytest.mark.parametrize('f', [fwd, bwd, fused, dfwd, dbwd, teach])
 def test_no_rows_is_fine(f):
     assert f(N=0) == _lib.VAE_OK
+
+
+def test_scratch_sizes():
+    lib = _lib.load()
+    assert lib.vae_token_scratch_bytes(4096, 131072, 20, 1) == 0          # rows enough: no pieces
+    assert lib.vae_token_scratch_bytes(1, 131072, 20, 1) > 0
+    for bad in ((0, 100, 0, 0), (1, 0, 0, 0), (1, 100, 65, 0), (1, 100, -1, 0), (1, (1 << 24) + 1, 0, 0)):
+        assert lib.vae_token_scratch_bytes(*bad) == 0
+    assert lib.vae_distill_teacher_floats(10, 7) == 10 * 22
+    assert lib.vae_distill_teacher_floats(10, 0) == lib.vae_distill_teacher_floats(10, 257) == 0
 
 
 def test_sums_and_scale_refusals():

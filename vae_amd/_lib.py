@@ -100,12 +100,15 @@ SIGNATURES = {
     'vae_token_elbo_bwd': [_p, _p, _p, _pp, _i, _f, _f, _p, _p, _i64, _p, _p, _p, _i64, _i, _p],
     'vae_row_sums': [_p, _f, _p, _i64, _i64, _i, _p],
     'vae_grad_scale': [_p, _p, _i64, _i, _p],
-    'vae_distill_fwd': [_p, _i64, _p, _i64, _i, _p, _i64, _i, _i64, _f, _p, _p, _p, _f, _p, _i64, _i64, _i, _p],
-    'vae_distill_bwd': [_p, _i64, _p, _i64, _i, _p, _i64, _i, _i64, _f, _p, _p, _p, _f, _p, _i64, _i64, _i, _p],
+    'vae_distill_teacher_floats': [_i64, _i64],
+    'vae_distill_teacher': [_p, _i64, _i, _p, _i64, _i, _i64, _f, _p, _i64, _i64, _p],
+    'vae_distill_fwd': [_p, _i64, _p, _i64, _f, _p, _p, _p, _f, _p, _i64, _i64, _i, _p],
+    'vae_distill_bwd': [_p, _i64, _p, _i64, _f, _p, _p, _p, _f, _p, _i64, _i64, _i, _p],
 }
 
 # entry points that return a size_t
-SIZES = ('vae_workspace_bytes', 'vae_bnflow_stats_floats', 'vae_token_scratch_bytes')
+SIZES = ('vae_workspace_bytes', 'vae_bnflow_stats_floats', 'vae_token_scratch_bytes',
+         'vae_distill_teacher_floats')
 
 _lib = None
 

@@ -27,7 +27,7 @@ struct FwdArgs {
   int parts, part_vecs;              // pieces of a row, vectors per piece
   char* scratch;                     // per (row, piece): m, s, t, -, then top_k keys
   float scale2, inv_tau;
-  TeacherArgs teacher;
+  Teacher teacher;
 };
 __device__ __forceinline__ int64_t part_bytes(int top_k) { return 16 + 8 * (int64_t)top_k; }
 
@@ -269,6 +269,16 @@ __device__ __forceinline__ void emit_top(const FwdArgs& a, int64_t row, int rank
   a.top_logp[row * a.top_k + rank] = key ? row_log_prob(key_value(key), m, s, 1.0f) : nan_f();
   a.top_ids[row * a.top_k + rank] = key ? key_index(key) : -1;
 }
+// true: the row is done, one without entries or with an id beyond the vocabulary
+__device__ __forceinline__ bool write_no_teacher(const FwdArgs& a, int64_t row, bool write) {
+  const int state = a.teacher.state[row];
+  if (state != kRowFine && write && threadIdx.x == 0) {
+    const float v = state == kRowEmpty ? 0.f : nan_f();
+    a.logp[row] = v;
+    if (a.stats) a.stats[2 * row] = 0.f, a.stats[2 * row + 1] = v;   // a sum of 0 or NaN: what the backward goes by
+  }
+  return state != kRowFine;
+}
 template <int BT>
 __device__ __forceinline__ void write_padding(const FwdArgs& a, int64_t row) {
   if (threadIdx.x == 0) {
@@ -284,13 +294,9 @@ __device__ __forceinline__ void write_padding(const FwdArgs& a, int64_t row) {
 // what a row's statistics give, once they are whole
 template <int BT, bool ENT, bool DIST>
 __device__ __forceinline__ void write_row(const FwdArgs& a, int64_t row, int64_t tok, float token_logit, float m, float s,
-                                          float t, const TeacherRow<BT>* tr) {
+                                          float t, const TeacherTerms<BT>& terms) {
   float kl = 0.f;
-  if constexpr (DIST) {
-    for (int k = threadIdx.x; k < a.teacher.K; k += BT)
-      if (tr->id[k] >= 0) kl += tr->q[k] * (tr->logq[k] - row_log_prob(tr->x[k], m, s, a.inv_tau));
-    kl = block_sum<BT>(kl);
-  }
+  if constexpr (DIST) kl = terms.kl(m, s, a.inv_tau);
   if (threadIdx.x == 0) {
     if constexpr (DIST) a.logp[row] = kl;
     else if (a.logp) a.logp[row] = tok < a.V ? row_log_prob(token_logit, m, s, 1.0f) : nan_f();
@@ -307,7 +313,6 @@ __global__ __launch_bounds__(BT) void token_fwd_kernel(FwdArgs a) {
   constexpr int VN = VecOf<T>::n;
   __shared__ struct {
     TopLds<TOP ? BT : 64> top[TOP ? 1 : 0];
-    TeacherRow<BT> teacher[DIST ? 1 : 0];
   } lds;
   for (int64_t item = blockIdx.x; item < a.N * a.parts; item += gridDim.x) {
     const int64_t row = a.parts == 1 ? item : item / a.parts;
@@ -315,18 +320,12 @@ __global__ __launch_bounds__(BT) void token_fwd_kernel(FwdArgs a) {
     const T* x = (const T*)a.logits + row * a.row_stride;
     int64_t tok = 0;
     float token_logit = 0.f;       // asked for in front of the row: it is there when the row's sum is
+    TeacherTerms<BT> terms;
     if constexpr (DIST) {
+      if (write_no_teacher(a, row, a.parts == 1)) continue;
       if (a.parts == 1) {
-        const int state = lds.teacher[0].load(a.teacher, row, a.V, a.inv_tau, a.scale2);
-        if (state != kRowFine) {
-          if (threadIdx.x == 0) {
-            a.logp[row] = state == kRowEmpty ? 0.f : nan_f();
-            if (a.stats) a.stats[2 * row] = 0.f, a.stats[2 * row + 1] = a.logp[row];  // the backward's sign of either
-          }
-          continue;
-        }
-        for (int k = threadIdx.x; k < a.teacher.K; k += BT)
-          lds.teacher[0].x[k] = lds.teacher[0].id[k] >= 0 ? to_f32(x[lds.teacher[0].id[k]]) : 0.f;
+        terms.fetch(a.teacher, row);
+        terms.fetch_logits(x);
       }
     } else {
       tok = a.tokens ? load_id(a.tokens, a.token_bytes, row) : 0;
@@ -353,7 +352,7 @@ __global__ __launch_bounds__(BT) void token_fwd_kernel(FwdArgs a) {
       });
     }
     if (a.parts == 1) {
-      write_row<BT, ENT, DIST>(a, row, tok, token_logit, m, s, t, lds.teacher);
+      write_row<BT, ENT, DIST>(a, row, tok, token_logit, m, s, t, terms);
     } else if (threadIdx.x == 0) {
       float* f = reinterpret_cast<float*>(a.scratch + item * part_bytes(a.top_k));
       f[0] = m;
@@ -368,7 +367,6 @@ template <typename T, int BT, bool ENT, bool TOP, bool DIST>
 __global__ __launch_bounds__(BT) void token_join_kernel(FwdArgs a) {
   __shared__ struct {
     TopLds<TOP ? BT : 64> top[TOP ? 1 : 0];
-    TeacherRow<BT> teacher[DIST ? 1 : 0];
   } lds;
   constexpr int R = kCand / BT;     // keys a thread holds; more of them are read where they are
   for (int64_t row = blockIdx.x; row < a.N; row += gridDim.x) {
@@ -397,17 +395,11 @@ __global__ __launch_bounds__(BT) void token_join_kernel(FwdArgs a) {
       if ((int)threadIdx.x < a.parts) below = ~key_at(threadIdx.x * a.top_k + at);
     }
     float token_logit = 0.f;
+    TeacherTerms<BT> terms;
     if constexpr (DIST) {
-      const int state = lds.teacher[0].load(a.teacher, row, a.V, a.inv_tau, a.scale2);
-      if (state != kRowFine) {
-        if (threadIdx.x == 0) {
-          a.logp[row] = state == kRowEmpty ? 0.f : nan_f();
-          if (a.stats) a.stats[2 * row] = 0.f, a.stats[2 * row + 1] = a.logp[row];
-        }
-        continue;
-      }
-      for (int k = threadIdx.x; k < a.teacher.K; k += BT)
-        lds.teacher[0].x[k] = lds.teacher[0].id[k] >= 0 ? to_f32(x[lds.teacher[0].id[k]]) : 0.f;
+      if (write_no_teacher(a, row, true)) continue;
+      terms.fetch(a.teacher, row);
+      terms.fetch_logits(x);
     } else {
       if (tok < 0) {
         write_padding<BT>(a, row);
@@ -443,7 +435,7 @@ __global__ __launch_bounds__(BT) void token_join_kernel(FwdArgs a) {
         }
       }
     }
-    write_row<BT, ENT, DIST>(a, row, tok, token_logit, m, s, t, lds.teacher);
+    write_row<BT, ENT, DIST>(a, row, tok, token_logit, m, s, t, terms);
   }
 }
 
@@ -495,7 +487,7 @@ static int fwd_type(const FwdArgs& a, hipStream_t st) {
 }
 
 // kl and stats; vae_distill_fwd (token_grad.hip) has checked the arguments
-int distill_stats(const void* logits, int64_t row_stride, const TeacherArgs& teacher, float temperature, float* kl,
+int distill_stats(const void* logits, int64_t row_stride, const Teacher& teacher, float temperature, float* kl,
                   float* stats, void* scratch, int64_t N, int64_t V, int dtype, hipStream_t stream) {
   const Cut cut = cut_rows(N, V, dtype);
   if (cut.parts > 1 && !scratch) return VAE_ERR_ARG;

@@ -11,52 +11,31 @@
 
 namespace vae {
 
-// A piece's entries in LDS: each thread's own in a list.  Entries of one id are merged first, in entry order, so what
-// a gradient element receives does not depend on the order of the list.
+// A piece's entries in LDS, each thread's own in a list.  No id comes twice, so the order of a list does not matter.
 constexpr int kMaxEntries = VAE_MAX_TEACHER;
 template <int BT>
 struct Entries {
-  static constexpr int R = (kMaxEntries + BT - 1) / BT;
   int head[BT];
   int next[kMaxEntries], id[kMaxEntries];
   float g[kMaxEntries];
 
-  // id[0..n), g[0..n) have been written by the workgroup (id < 0: none)
-  template <typename T, int VN>
-  __device__ __forceinline__ void link(int n, const RowCut<T, VN>& cut, int v0, int v1) {
-    int own[R];
-    float sum[R];
+  __device__ __forceinline__ void clear() {
+    lds_barrier();   // the row before this one has been read
     head[threadIdx.x] = -1;
     lds_barrier();
-#pragma unroll
-    for (int r = 0; r < R; ++r) {
-      const int k = threadIdx.x + r * BT;
-      own[r] = k < n ? id[k] : -1;
-      sum[r] = 0.f;
-      if (own[r] >= 0) {
-        bool first = true;
-        for (int q = 0; q < n; ++q)
-          if (id[q] == own[r]) {
-            first &= q >= k;
-            sum[r] += g[q];
-          }
-        if (!first) own[r] = -1;
-      }
-    }
-    lds_barrier();
-#pragma unroll
-    for (int r = 0; r < R; ++r) {
-      const int k = threadIdx.x + r * BT;
-      if (own[r] < 0) continue;
-      g[k] = sum[r];
-      const int off = own[r] - cut.head;
-      int owner = -1;
-      if (off < 0) owner = own[r];                                      // RowCut::edge
-      else if (off >= cut.nvec * VN) owner = 16 + off - cut.nvec * VN;
-      else if (off / VN >= v0 && off / VN < v1) owner = (off / VN - v0) % BT;
-      if (owner >= 0) next[k] = atomicExch(&head[owner], k);
-    }
-    lds_barrier();
+  }
+  template <typename T, int VN>
+  __device__ __forceinline__ void put(int k, int id_k, float g_k, const RowCut<T, VN>& cut, int v0, int v1) {
+    if (id_k < 0) return;
+    const int off = id_k - cut.head;
+    int owner = -1;
+    if (off < 0) owner = id_k;                                      // RowCut::edge
+    else if (off >= cut.nvec * VN) owner = 16 + off - cut.nvec * VN;
+    else if (off / VN >= v0 && off / VN < v1) owner = (off / VN - v0) % BT;
+    if (owner < 0) return;
+    id[k] = id_k;
+    g[k] = g_k;
+    next[k] = atomicExch(&head[owner], k);
   }
 };
 
@@ -114,8 +93,7 @@ struct GradArgs {
   const float *gentropy, *gtop;
   const int64_t* top_ids;
   int top_k;
-  // teacher
-  TeacherArgs teacher;
+  Teacher teacher;
   const float *gkl, *gmean;
   float mean_scale;
   // fused
@@ -165,7 +143,6 @@ template <typename T, int VN, int BT, int U, bool ENT, bool LIST, bool DIST>
 __global__ __launch_bounds__(BT) void token_bwd_kernel(GradArgs a) {
   __shared__ struct {
     Entries<BT> entries[LIST ? 1 : 0];
-    TeacherRow<BT> teacher[DIST ? 1 : 0];
   } lds;
   for (int64_t item = blockIdx.x; item < a.N * a.parts; item += gridDim.x) {
     const int64_t row = a.parts == 1 ? item : item / a.parts;
@@ -186,6 +163,8 @@ __global__ __launch_bounds__(BT) void token_bwd_kernel(GradArgs a) {
       if (ei >= 0) gx[ei] = from_f32<T>(0.f);
       continue;
     }
+    TeacherTerms<BT> terms;
+    if constexpr (DIST) terms.fetch(a.teacher, row);
     piece.load();
     const float edge = ei >= 0 ? to_f32(x[ei]) : 0.f;
     Adds<T, VN, BT, LIST> adds;
@@ -193,14 +172,14 @@ __global__ __launch_bounds__(BT) void token_bwd_kernel(GradArgs a) {
     float A, B = 0.f;
     const float inv = 1.0f / s;
     if constexpr (DIST) {
-      lds.teacher[0].load(a.teacher, row, a.V, a.inv_tau, a.scale2);   // an id beyond the vocabulary: s is NaN
       const float g0 = a.gmean ? a.gmean[0] * a.mean_scale : (a.gkl ? 0.f : a.mean_scale);
       const float w = ((a.gkl ? a.gkl[row] : 0.f) + g0) * a.inv_tau;
-      A = w * inv;
-      for (int k = threadIdx.x; k < a.teacher.K; k += BT) {
-        lds.entries[0].id[k] = lds.teacher[0].id[k];
-        lds.entries[0].g[k] = -w * lds.teacher[0].q[k];
-      }
+      A = w * inv;               // an id beyond the vocabulary: s is NaN
+      lds.entries[0].clear();
+#pragma unroll
+      for (int r = 0; r < TeacherTerms<BT>::R; ++r)
+        lds.entries[0].put((int)threadIdx.x + r * BT, terms.id[r], -w * terms.q[r], cut, v0, v1);
+      lds_barrier();
     } else {
       float gt = a.tokens ? (a.glogp ? a.glogp[row / a.rows_per_g] * a.g_scale : a.g_scale) : 0.f;
       const bool inside = a.tokens && tok < a.V;
@@ -210,11 +189,16 @@ __global__ __launch_bounds__(BT) void token_bwd_kernel(GradArgs a) {
       adds.one_g = gt;
       if constexpr (LIST) {
         for (int k = 0; k < a.top_k; ++k) sum += a.gtop[row * a.top_k + k];
-        lds_barrier();  // the row before this one has been read
+        // the alternatives differ from each other; the token may be one of them
+        lds.entries[0].clear();
+        bool other = true;
+        for (int k = 0; k < a.top_k; ++k) other &= a.top_ids[row * a.top_k + k] != tok;
         for (int k = threadIdx.x; k <= a.top_k; k += BT) {
-          lds.entries[0].id[k] = k == 0 ? adds.one_id : (int)a.top_ids[row * a.top_k + k - 1];
-          lds.entries[0].g[k] = k == 0 ? gt : a.gtop[row * a.top_k + k - 1];
+          const int id = k < a.top_k ? (int)a.top_ids[row * a.top_k + k] : (other ? adds.one_id : -1);
+          const float g = k < a.top_k ? a.gtop[row * a.top_k + k] : 0.f;
+          lds.entries[0].put(k, id, g + (id == adds.one_id ? gt : 0.f), cut, v0, v1);
         }
+        lds_barrier();
       }
       if constexpr (ENT) {
         const float gh = a.gentropy[row];
@@ -223,7 +207,6 @@ __global__ __launch_bounds__(BT) void token_bwd_kernel(GradArgs a) {
       }
       A = -sum * inv;
     }
-    if constexpr (LIST) lds.entries[0].template link<T, VN>(DIST ? a.teacher.K : a.top_k + 1, cut, v0, v1);
     adds.prepare(cut, v0, v1);
     auto grad = [&](float v) {
       const float d = (v - m) * a.scale2;
@@ -249,17 +232,18 @@ __global__ __launch_bounds__(BT) void token_bwd_kernel(GradArgs a) {
 }
 
 // ---------------------------------------------------------------------------------------------------------------
-// loss and gradient in one pass: a workgroup holds its row in registers, U vectors a thread.
-//   KEEP: every element's exponential against the thread's own maximum, in float32: one exponential an element, the
-//         gradient is a product.  8 registers a 16-bit vector, 4 an fp32 one.
-//   else: the packets as they were read, 4 registers a vector whatever the type; the exponentials are formed twice.
+// loss and gradient in one pass: a workgroup holds its row in registers, U vectors a thread, as every element's
+// exponential against the thread's own maximum: one exponential an element, the gradient is a product.
+//   in float32: 8 registers a 16-bit vector, 4 an fp32 one;
+//   HALF (bf16 rows that do not fit so): as 2^15 e in binary16, 4 registers a vector, where the packet was.  Its 11 bits
+//         are rounded once more to the gradient's 8; e < 2^-29, a probability 2^-29 of the thread's largest, begins to
+//         lose bits.  The sum is taken before the rounding.
 // ---------------------------------------------------------------------------------------------------------------
-template <typename T, int BT, int U, bool KEEP, bool DIST>
-__global__ __launch_bounds__(BT) void token_fused_kernel(GradArgs a) {
+template <typename T, int BT, int U, bool HALF, bool DIST>
+__global__ __launch_bounds__(BT, 4) void token_fused_kernel(GradArgs a) {
   constexpr int VN = VecOf<T>::n;
   __shared__ struct {
     Entries<BT> entries[DIST ? 1 : 0];
-    TeacherRow<BT> teacher[DIST ? 1 : 0];
   } lds;
   for (int64_t row = blockIdx.x; row < a.N; row += gridDim.x) {
     const T* x = (const T*)a.logits + row * a.row_stride;
@@ -269,12 +253,13 @@ __global__ __launch_bounds__(BT) void token_fused_kernel(GradArgs a) {
     Piece<T, VN, BT, U> piece(x, gx, cut, 0, cut.nvec);
     int64_t tok = 0;
     int state = kRowFine;
-    typename TeacherRow<BT>::Mine mine;
+    float token_logit = 0.f;
     if constexpr (DIST) {
-      if (!TeacherRow<BT>::fetch(mine, a.teacher, row, a.V)) state = kRowEmpty;
+      state = a.teacher.state[row];
     } else {
       tok = load_id(a.tokens, a.token_bytes, row);
       state = tok < 0 ? kRowEmpty : (tok >= a.V ? kRowBad : kRowFine);
+      if (state == kRowFine) token_logit = to_f32(x[tok]);
     }
     if (state != kRowFine) {
       const float v = state == kRowEmpty ? 0.f : nan_f();
@@ -287,21 +272,21 @@ __global__ __launch_bounds__(BT) void token_fused_kernel(GradArgs a) {
       }
       continue;
     }
+    TeacherTerms<BT> terms;
+    if constexpr (DIST) terms.fetch(a.teacher, row);
     piece.load();
     const float edge = ei >= 0 ? to_f32(x[ei]) : -INFINITY;
     Adds<T, VN, BT, DIST> adds;
     const float w = DIST ? a.mean_scale * a.inv_tau : a.g_scale;   // of p; the entries have the other sign
     if constexpr (DIST) {
       // while the row is on its way
-      state = lds.teacher[0].finish(mine, a.teacher, a.V, a.inv_tau, a.scale2);
-      for (int k = threadIdx.x; k < a.teacher.K; k += BT) {
-        const int id = lds.teacher[0].id[k];
-        lds.teacher[0].x[k] = id >= 0 ? to_f32(x[id]) : 0.f;
-        lds.entries[0].id[k] = id;
-        lds.entries[0].g[k] = -w * lds.teacher[0].q[k];
-      }
       adds.lds = lds.entries;
-      lds.entries[0].template link<T, VN>(a.teacher.K, cut, 0, cut.nvec);
+      lds.entries[0].clear();
+      terms.fetch_logits(x);
+#pragma unroll
+      for (int r = 0; r < TeacherTerms<BT>::R; ++r)
+        lds.entries[0].put((int)threadIdx.x + r * BT, terms.id[r], -w * terms.q[r], cut, 0, cut.nvec);
+      lds_barrier();
     } else {
       adds.one_id = (int)tok;
       adds.one_g = -w;
@@ -316,7 +301,7 @@ __global__ __launch_bounds__(BT) void token_fused_kernel(GradArgs a) {
         piece.p[u].get(v);
         mt = vec_max(v, mt);
       }
-    float e[KEEP ? U : 1][VN];
+    float e[HALF ? 1 : U][VN];
     float s = exp2_raw((edge - mt) * a.scale2);
 #pragma unroll
     for (int u = 0; u < U; ++u)
@@ -326,25 +311,28 @@ __global__ __launch_bounds__(BT) void token_fused_kernel(GradArgs a) {
         piece.p[u].get(v);
 #pragma unroll
         for (int i = 0; i < VN; ++i) {
-          const float ev = exp2_raw((v[i] - mt) * a.scale2);
-          s += ev;
-          if constexpr (KEEP) e[u][i] = ev;
+          v[i] = exp2_raw((v[i] - mt) * a.scale2);
+          s += v[i];
+        }
+        if constexpr (HALF) {
+#pragma unroll
+          for (int i = 0; i < VN; i += 2) piece.p[u].raw[i / 2] = pack2<f16_t>(v[i] * 32768.f, v[i + 1] * 32768.f);
+        } else {
+#pragma unroll
+          for (int i = 0; i < VN; ++i) e[u][i] = v[i];
         }
       }
     const float m = block_max<BT>(mt);
     float f = exp2_raw((mt - m) * a.scale2);       // from the thread's maximum to the row's
     s = block_sum<BT>(s * f);
-    if (DIST && state == kRowBad) s = nan_f();
-    if constexpr (DIST) {
-      float kl = 0.f;
-      for (int k = threadIdx.x; k < a.teacher.K; k += BT)
-        if (lds.teacher[0].id[k] >= 0)
-          kl += lds.teacher[0].q[k] * (lds.teacher[0].logq[k] - row_log_prob(lds.teacher[0].x[k], m, s, a.inv_tau));
-      kl = block_sum<BT>(kl);
-      if (threadIdx.x == 0) a.out[row] = state == kRowBad ? nan_f() : kl;
-    } else if (threadIdx.x == 0) {
-      a.out[row] = row_log_prob(to_f32(x[tok]), m, s, 1.0f);
-    }
+    auto loss = [&]() {             // behind the gradient: it waits for nobody
+      if constexpr (DIST) {
+        const float kl = terms.kl(m, s, a.inv_tau);
+        if (threadIdx.x == 0) a.out[row] = kl;
+      } else if (threadIdx.x == 0) {
+        a.out[row] = row_log_prob(token_logit, m, s, 1.0f);
+      }
+    };
     if (threadIdx.x == 0) {
       a.stats_out[2 * row] = m;
       a.stats_out[2 * row + 1] = s;
@@ -352,6 +340,7 @@ __global__ __launch_bounds__(BT) void token_fused_kernel(GradArgs a) {
     if (s == 0.f) {
       piece.fill(a.nts, 0.f);
       if (ei >= 0) gx[ei] = from_f32<T>(0.f);
+      loss();
       continue;
     }
     const float A = w / s;
@@ -360,14 +349,15 @@ __global__ __launch_bounds__(BT) void token_fused_kernel(GradArgs a) {
     for (int u = 0; u < U; ++u)
       if (piece.any(u)) {
         float v[VN];
-        if constexpr (KEEP) {
+        if constexpr (HALF) {
+          Packet<f16_t, VN> h;
+          h.raw = piece.p[u].raw;
+          h.get(v);
+#pragma unroll
+          for (int i = 0; i < VN; ++i) v[i] *= f * (1.f / 32768.f);
+        } else {
 #pragma unroll
           for (int i = 0; i < VN; ++i) v[i] = f * e[u][i];
-        } else {
-          asm volatile("" : "+v"(piece.p[u].raw));
-          piece.p[u].get(v);
-#pragma unroll
-          for (int i = 0; i < VN; ++i) v[i] = A * exp2_raw((v[i] - m) * a.scale2);
         }
         if (adds.mask >> u & 1u) adds.to(cut.index(u * BT + (int)threadIdx.x), v);
         piece.store(a.nts, u, v);
@@ -377,6 +367,7 @@ __global__ __launch_bounds__(BT) void token_fused_kernel(GradArgs a) {
       adds.to(ei, v);
       gx[ei] = from_f32<T>(v[0]);
     }
+    loss();
   }
 }
 
@@ -427,10 +418,10 @@ static int bwd_type(const GradArgs& a, hipStream_t st) {
   return same_phase<T>(a) ? bwd_kind<T, VecOf<T>::n, DIST>(a, st) : bwd_kind<T, 1, DIST>(a, st);
 }
 
-template <typename T, int BT, int U, bool KEEP, bool DIST>
+template <typename T, int BT, int U, bool HALF, bool DIST>
 static int fused_launch(GradArgs a, hipStream_t st) {
   a.nts = (int64_t)sizeof(T) * a.N * a.V >= kNtStoreMinBytes;
-  hipLaunchKernelGGL((token_fused_kernel<T, BT, U, KEEP, DIST>), dim3(grid_for(a.N)), dim3(BT), 0, st, a);
+  hipLaunchKernelGGL((token_fused_kernel<T, BT, U, HALF, DIST>), dim3(grid_for(a.N)), dim3(BT), 0, st, a);
   return launched();
 }
 // true when the one-pass kernel takes this call: the row fits a workgroup's registers, and there are rows enough
@@ -438,19 +429,20 @@ template <typename T, bool DIST>
 static bool fused_type(const GradArgs& a, hipStream_t st, int* rc) {
   constexpr int E = 64 / VecOf<T>::n;    // vectors a thread: 64 elements
   const int64_t nvec = (int64_t)a.V / VecOf<T>::n;
-  if (!same_phase<T>(a) || nvec > 16384 || (a.N < 256 && nvec > 4096)) return false;
-  if (nvec <= 64 * E) *rc = fused_launch<T, 64, E, true, DIST>(a, st);
-  else if (nvec <= 128 * E) *rc = fused_launch<T, 128, E, true, DIST>(a, st);
-  else if (nvec <= 256 * E) *rc = fused_launch<T, 256, E, true, DIST>(a, st);
-  else if (nvec <= 512 * E) *rc = fused_launch<T, 512, E, true, DIST>(a, st);
-  else if (nvec <= 1024 * E) *rc = fused_launch<T, 1024, E, true, DIST>(a, st);
-  else *rc = fused_launch<T, 1024, 16, false, DIST>(a, st);
+  // bf16 only: the other types' gradients have no bits to spare for HALF's rounding
+  constexpr int most = DTypeCode<T>::value == VAE_BF16 ? 16 : E;
+  if (!same_phase<T>(a) || nvec > 1024 * most || (a.N < 256 && nvec > 4096)) return false;
+  if (nvec <= 64 * E) *rc = fused_launch<T, 64, E, false, DIST>(a, st);
+  else if (nvec <= 128 * E) *rc = fused_launch<T, 128, E, false, DIST>(a, st);
+  else if (nvec <= 256 * E) *rc = fused_launch<T, 256, E, false, DIST>(a, st);
+  else if (nvec <= 512 * E) *rc = fused_launch<T, 512, E, false, DIST>(a, st);
+  else if (nvec <= 1024 * E) *rc = fused_launch<T, 1024, E, false, DIST>(a, st);
+  else if constexpr (most > E) *rc = fused_launch<T, 1024, most, true, DIST>(a, st);
   return true;
 }
 
-static bool bad_teacher(const TeacherArgs& t, int64_t N, float temperature) {
-  return !type_ok(t.dtype) || t.K < 1 || t.K > VAE_MAX_TEACHER || (N > 1 && (t.stride < t.K || t.id_stride < t.K)) ||
-         (t.id_bytes != 4 && t.id_bytes != 8) || !(temperature > 0.f) || !(temperature < INFINITY);
+static bool bad_teacher(int64_t K, float temperature) {
+  return K < 1 || K > VAE_MAX_TEACHER || !(temperature > 0.f) || !(temperature < INFINITY);
 }
 static void set_temperature(GradArgs& a, float temperature) {
   a.scale2 = (float)(1.4426950408889634 / (double)temperature);
@@ -506,16 +498,14 @@ int vae_token_nll_fused(const void* logits, int64_t row_stride, const void* toke
                             nullptr, nullptr, 0, glogits, N, V, dtype, stream);
 }
 
-int vae_distill_bwd(const void* logits, int64_t row_stride, const void* t_logits, int64_t t_stride, int t_dtype,
-                    const void* t_ids, int64_t id_stride, int id_bytes, int64_t K, float temperature,
+int vae_distill_bwd(const void* logits, int64_t row_stride, const float* teacher, int64_t K, float temperature,
                     const float* stats, const float* gkl, const float* gmean, float mean_scale, void* glogits,
                     int64_t N, int64_t V, int dtype, vae_stream_t stream) {
-  if (K > VAE_MAX_TEACHER) return VAE_ERR_ARG;
-  GradArgs a = {};
-  a.teacher = {t_logits, t_ids, t_stride, id_stride, t_dtype, id_bytes, (int)K};
-  if (bad_rows(N, V, row_stride, dtype) || bad_teacher(a.teacher, N, temperature)) return VAE_ERR_ARG;
+  if (bad_rows(N, V, row_stride, dtype) || bad_teacher(K, temperature)) return VAE_ERR_ARG;
   if (N == 0) return VAE_OK;
-  if (!logits || !t_logits || !t_ids || !stats || !glogits) return VAE_ERR_ARG;
+  if (!logits || !teacher || !stats || !glogits) return VAE_ERR_ARG;
+  GradArgs a = {};
+  a.teacher = teacher_of(teacher, N, K);
   a.logits = logits; a.row_stride = row_stride; a.glogits = glogits; a.N = N; a.V = (int)V;
   a.stats_in = stats; a.gkl = gkl; a.gmean = gmean; a.mean_scale = mean_scale;
   set_temperature(a, temperature);
@@ -523,16 +513,14 @@ int vae_distill_bwd(const void* logits, int64_t row_stride, const void* t_logits
   return VAE_ERR_ARG;
 }
 
-int vae_distill_fwd(const void* logits, int64_t row_stride, const void* t_logits, int64_t t_stride, int t_dtype,
-                    const void* t_ids, int64_t id_stride, int id_bytes, int64_t K, float temperature, float* kl,
-                    float* stats, void* glogits, float grad_scale, void* scratch, int64_t N, int64_t V, int dtype,
-                    vae_stream_t stream) {
-  if (K > VAE_MAX_TEACHER) return VAE_ERR_ARG;
-  GradArgs a = {};
-  a.teacher = {t_logits, t_ids, t_stride, id_stride, t_dtype, id_bytes, (int)K};
-  if (bad_rows(N, V, row_stride, dtype) || bad_teacher(a.teacher, N, temperature)) return VAE_ERR_ARG;
+int vae_distill_fwd(const void* logits, int64_t row_stride, const float* teacher, int64_t K, float temperature,
+                    float* kl, float* stats, void* glogits, float grad_scale, void* scratch, int64_t N, int64_t V,
+                    int dtype, vae_stream_t stream) {
+  if (bad_rows(N, V, row_stride, dtype) || bad_teacher(K, temperature)) return VAE_ERR_ARG;
   if (N == 0) return VAE_OK;
-  if (!logits || !t_logits || !t_ids || !kl || (glogits && !stats)) return VAE_ERR_ARG;
+  if (!logits || !teacher || !kl || (glogits && !stats)) return VAE_ERR_ARG;
+  GradArgs a = {};
+  a.teacher = teacher_of(teacher, N, K);
   if (glogits) {
     a.logits = logits; a.row_stride = row_stride; a.glogits = glogits; a.N = N; a.V = (int)V;
     a.mean_scale = grad_scale; a.out = kl; a.stats_out = stats;
@@ -543,8 +531,8 @@ int vae_distill_fwd(const void* logits, int64_t row_stride, const void* t_logits
   const int rc = distill_stats(logits, row_stride, a.teacher, temperature, kl, stats, scratch, N, V, dtype,
                                (hipStream_t)stream);
   if (rc != VAE_OK || !glogits) return rc;
-  return vae_distill_bwd(logits, row_stride, t_logits, t_stride, t_dtype, t_ids, id_stride, id_bytes, K, temperature,
-                         stats, nullptr, nullptr, grad_scale, glogits, N, V, dtype, stream);
+  return vae_distill_bwd(logits, row_stride, teacher, K, temperature, stats, nullptr, nullptr, grad_scale, glogits, N, V,
+                         dtype, stream);
 }
 
 }  // extern "C"

@@ -208,88 +208,55 @@ __device__ __forceinline__ float vec_max(const float (&v)[VN], float m) {
   return m;
 }
 
-// ---------------------------------------------------------------------------------------------------------------
-// The teacher's row of a distillation, in LDS: q = softmax(y / tau) over the entries that are there.  Entries with the
-// same id are merged into the first of them (in index order: the sums do not depend on timing), the others get id -1.
-// ---------------------------------------------------------------------------------------------------------------
-struct TeacherArgs {
-  const void* logits;
-  const void* ids;
-  int64_t stride, id_stride;
-  int dtype, id_bytes, K;
-};
-// kl [N] and stats [N, 2] of a distillation (token.hip); the arguments have been checked
-int distill_stats(const void* logits, int64_t row_stride, const TeacherArgs& teacher, float temperature, float* kl,
-                  float* stats, void* scratch, int64_t N, int64_t V, int dtype, hipStream_t stream);
+// The teacher's entries as vae_distill_teacher (token_teacher.hip) leaves them: per row a state, and K entries of
+// id (-1: none), q and ln q; entries of one id are merged into the first of them.
 enum { kRowFine = 0, kRowEmpty = 1, kRowBad = 2 };  // nothing there | an id beyond the vocabulary
-
+struct Teacher {
+  const int* state;       // [N]
+  const int* id;          // [N, K]
+  const float *q, *logq;  // [N, K]
+  int K;
+};
+inline Teacher teacher_of(const float* buf, int64_t N, int64_t K) {
+  Teacher t;
+  t.state = reinterpret_cast<const int*>(buf);
+  t.id = t.state + N;
+  t.q = buf + N + N * K;
+  t.logq = t.q + N * K;
+  t.K = (int)K;
+  return t;
+}
+// kl [N] and stats [N, 2] of a distillation (token.hip); the arguments have been checked
+int distill_stats(const void* logits, int64_t row_stride, const Teacher& teacher, float temperature, float* kl,
+                  float* stats, void* scratch, int64_t N, int64_t V, int dtype, hipStream_t stream);
+// Each thread's entries of a row, asked for in three steps so that nobody waits: the entries in front of the row's
+// packets, the student's logits there when the ids have come, the KL when the row's statistics are known.
 template <int BT>
-struct TeacherRow {
+struct TeacherTerms {
   static constexpr int R = (VAE_MAX_TEACHER + BT - 1) / BT;
-  int id[VAE_MAX_TEACHER];
-  float q[VAE_MAX_TEACHER], logq[VAE_MAX_TEACHER];
-  float x[VAE_MAX_TEACHER];   // the student's logits there, for who keeps them
-
-  // A thread's own entries between fetch() and finish(): loads of the row's logits fit in between.
-  struct Mine {
-    float y[R];
-    int id[R];
-  };
-
-  // true when the row has an entry, or an id beyond the vocabulary
-  __device__ __forceinline__ static bool fetch(Mine& e, const TeacherArgs& a, int64_t row, int V) {
-    bool any = false;
+  int id[R];
+  float q[R], logq[R], x[R];
+  __device__ __forceinline__ void fetch(const Teacher& t, int64_t row) {
 #pragma unroll
     for (int r = 0; r < R; ++r) {
       const int k = threadIdx.x + r * BT;
-      e.y[r] = -INFINITY;
-      e.id[r] = -1;
-      if (k < a.K) {
-        const int64_t i = load_id(a.ids, a.id_bytes, row * a.id_stride + k);
-        const float y = load_any(a.logits, a.dtype, row * a.stride + k);
-        if (i >= V) e.id[r] = V;
-        else if (i >= 0) {
-          e.id[r] = (int)i;
-          e.y[r] = y;
-        }
-        any |= i >= V || (i >= 0 && y != -INFINITY);
-      }
+      const bool has = k < t.K;
+      id[r] = has ? t.id[row * t.K + k] : -1;
+      q[r] = has ? t.q[row * t.K + k] : 0.f;
+      logq[r] = has ? t.logq[row * t.K + k] : 0.f;
     }
-    return block_sum<BT>(any ? 1.f : 0.f) > 0.f;
   }
-  __device__ __forceinline__ int finish(const Mine& mine, const TeacherArgs& a, int V, float inv_tau, float scale2) {
-    float m = kLowest;
-    bool bad = false;
+  template <typename T>
+  __device__ __forceinline__ void fetch_logits(const T* __restrict__ logits) {
 #pragma unroll
-    for (int r = 0; r < R; ++r) {
-      m = max_raw(m, mine.y[r]);
-      bad |= mine.id[r] == V;
-    }
-    m = block_max<BT>(m);
-    float e[R], s = 0.f;
-#pragma unroll
-    for (int r = 0; r < R; ++r) {
-      e[r] = mine.id[r] >= 0 && mine.id[r] < V ? exp2_raw((mine.y[r] - m) * scale2) : 0.f;
-      s += e[r];
-    }
-    s = block_sum<BT>(s);
-    const float any_bad = block_sum<BT>(bad ? 1.f : 0.f);
-    lds_barrier();  // the row before this one has been read
-#pragma unroll
-    for (int r = 0; r < R; ++r) {
-      const int k = threadIdx.x + r * BT;
-      if (k < a.K) {
-        q[k] = e[r] / s;
-        logq[k] = row_log_prob(mine.y[r], m, s, inv_tau);
-        id[k] = e[r] == 0.f ? -1 : mine.id[r];   // e NaN keeps its id: the row comes out NaN
-      }
-    }
-    lds_barrier();
-    return any_bad > 0.f ? kRowBad : (s == 0.f ? kRowEmpty : kRowFine);
+    for (int r = 0; r < R; ++r) x[r] = id[r] >= 0 ? to_f32(logits[id[r]]) : 0.f;
   }
-  __device__ __forceinline__ int load(const TeacherArgs& a, int64_t row, int V, float inv_tau, float scale2) {
-    Mine e;
-    return fetch(e, a, row, V) ? finish(e, a, V, inv_tau, scale2) : kRowEmpty;
+  __device__ __forceinline__ float kl(float m, float s, float inv_tau) const {
+    float v = 0.f;
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+      if (id[r] >= 0) v += q[r] * (logq[r] - row_log_prob(x[r], m, s, inv_tau));
+    return block_sum<BT>(v);
   }
 };
 

@@ -6,22 +6,28 @@
 
 namespace vae {
 
-template <typename T, int VN, int U, bool ENT>
-__global__ __launch_bounds__(kBlock) void token_short_kernel(ShortArgs a, int G, int64_t tiles) {
-  const int rpb = kBlock / G, sub = threadIdx.x % G, rloc = threadIdx.x / G;
+enum { kEnt = 1, kTop = 2, kGrad = 4 };   // what a kernel forms beside log prob and statistics
+
+template <typename T, int VN, int U, int WHAT>
+__global__ __launch_bounds__(kBlock) void token_short_kernel(ShortArgs a, int log_g, int64_t tiles) {
+  constexpr bool ENT = WHAT & kEnt, TOP = WHAT & kTop, GRAD = WHAT & kGrad;
+  const int G = 1 << log_g;
+  const int sub = threadIdx.x & (G - 1), rloc = threadIdx.x >> log_g;
   const int nvec = a.V / VN;
   const bool nts = nt_stores((int64_t)a.N * a.V * (int64_t)sizeof(T));
   for (int64_t tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
-    const int64_t row = tile * rpb + rloc;
+    const int64_t row = (tile << (8 - log_g)) + rloc;     // kBlock / G rows a tile
     const bool live = row < a.N;
     const int64_t r = live ? row : a.N - 1;
     const T* x = (const T*)a.logits + r * a.row_stride;
-    const int64_t tok = a.tokens ? load_id(a.tokens, a.token_bytes, r) : 0;
-    const bool pad = tok < 0 || !live;
+    const int64_t tok64 = a.tokens ? load_id(a.tokens, a.token_bytes, r) : 0;
+    const bool pad = tok64 < 0 || !live, beyond = tok64 >= a.V;
+    const int tok = pad || beyond ? -1 : (int)tok64;
+    const float token_logit = a.logp && tok >= 0 ? to_f32(x[tok]) : 0.f;
     float v[U][VN];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const int j = sub + u * G;
+      const int j = sub + (u << log_g);
       if (j < nvec && !pad) {
         load_vec<T, VN>(x + j * VN, v[u]);
       } else {
@@ -35,22 +41,27 @@ __global__ __launch_bounds__(kBlock) void token_short_kernel(ShortArgs a, int G,
     m = group_max(m, G);
     float s = 0.f, t = 0.f, e[U][VN];
 #pragma unroll
-    for (int u = 0; u < U; ++u)
+    for (int u = 0; u < U; ++u) {
 #pragma unroll
       for (int i = 0; i < VN; ++i) {
         const float d = (v[u][i] - m) * kLog2e;
-        e[u][i] = exp2_raw(d);
-        s += e[u][i];
-        if constexpr (ENT) t = __builtin_fmaf(max_raw(d, -300.f), e[u][i], t);
+        const float ev = exp2_raw(d);
+        s += ev;
+        if constexpr (ENT) t = __builtin_fmaf(max_raw(d, -300.f), ev, t);
+        if constexpr (GRAD) e[u][i] = ev;
       }
+      __builtin_amdgcn_sched_barrier(0);   // vector by vector: fewer registers
+    }
     s = group_sum(s, G);
+    const float ls = log2f(s);
     float h = 0.f;
     if constexpr (ENT) {
       t = group_sum(t, G);
-      h = s == 0.f ? 0.f : kLn2 * (log2f(s) - t / s);
+      h = s == 0.f ? 0.f : kLn2 * (ls - t / s);
     }
     if (sub == 0 && live) {
-      if (a.logp) a.logp[row] = pad ? 0.f : (tok < a.V ? row_log_prob(to_f32(x[tok]), m, s, 1.0f) : nan_f());
+      if (a.logp)
+        a.logp[row] = pad ? 0.f : (beyond ? nan_f() : (s == 0.f ? -INFINITY : token_logit - m - kLn2 * ls));
       if constexpr (ENT) {
         if (a.entropy) a.entropy[row] = h;
       }
@@ -59,16 +70,16 @@ __global__ __launch_bounds__(kBlock) void token_short_kernel(ShortArgs a, int G,
         a.stats[2 * row + 1] = s;
       }
     }
-    if (a.top_k) {
+    if constexpr (TOP) {
       uint64_t last = ~0ull;
       for (int k = 0; k < a.top_k; ++k) {
         uint64_t best = 0;
 #pragma unroll
         for (int u = 0; u < U; ++u)
-          if (sub + u * G < nvec)
+          if (sub + (u << log_g) < nvec)
 #pragma unroll
             for (int i = 0; i < VN; ++i) {
-              const uint64_t key = order_key(v[u][i], (uint32_t)((sub + u * G) * VN + i));
+              const uint64_t key = order_key(v[u][i], (uint32_t)((sub + (u << log_g)) * VN + i));
               best = key < last && key > best ? key : best;
             }
         for (int o = G >> 1; o >= 1; o >>= 1) {
@@ -82,58 +93,70 @@ __global__ __launch_bounds__(kBlock) void token_short_kernel(ShortArgs a, int G,
         }
       }
     }
-    if (!a.glogits || !live) continue;
-    const bool zero = pad || s == 0.f;
-    float gt = a.tokens ? (a.glogp ? a.glogp[row / a.rows_per_g] * a.g_scale : a.g_scale) : 0.f;
-    if (tok >= a.V && (!a.glogp || a.g_scale != 0.f)) gt = nan_f();
-    float sum = gt;
-    for (int k = 0; k < a.gtop_k; ++k) sum += a.gtop[row * a.gtop_k + k];
-    const float inv = 1.0f / s;
-    float B = 0.f;
-    if constexpr (ENT) {
-      const float gh = a.gentropy ? a.gentropy[row] : 0.f;
-      sum += gh * (h - kLn2 * log2f(s));
-      B = -gh * kLn2 * inv;
-    }
-    const float A = -sum * inv;
-    T* gx = (T*)a.glogits + row * (int64_t)a.V;
-#pragma unroll
-    for (int u = 0; u < U; ++u)
-#pragma unroll
-      for (int i = 0; i < VN; ++i)
-        e[u][i] *= ENT ? __builtin_fmaf(B, max_raw((v[u][i] - m) * kLog2e, -300.f), A) : A;
-    auto add = [&](int64_t id, float g) {
+    if constexpr (GRAD) {
+      if (!live) continue;
+      float gt = 0.f;
+      if (a.tokens) {
+        gt = a.g_scale;
+        if (a.glogp) {
+          int64_t at = row;
+          if (a.rows_per_g != 1)   // a 64-bit division costs as much as the row
+            at = (a.N | a.rows_per_g) >> 32 ? row / a.rows_per_g
+                                            : (int64_t)((uint32_t)row / (uint32_t)a.rows_per_g);
+          gt *= a.glogp[at];
+        }
+        if (beyond && (!a.glogp || a.g_scale != 0.f)) gt = nan_f();
+      }
+      float sum = gt;
+      for (int k = 0; k < a.gtop_k; ++k) sum += a.gtop[row * a.gtop_k + k];
+      const float inv = 1.0f / s;
+      float B = 0.f;
+      if constexpr (ENT) {
+        const float gh = a.gentropy[row];
+        sum += gh * (h - kLn2 * ls);
+        B = -gh * kLn2 * inv;
+      }
+      const float A = -sum * inv;
+      const bool zero = pad || s == 0.f;
+      T* gx = (T*)a.glogits + row * (int64_t)a.V;
 #pragma unroll
       for (int u = 0; u < U; ++u) {
-        const int64_t at = id - (sub + u * G) * VN;
+        const int j = sub + (u << log_g);
+        float o[VN];
 #pragma unroll
-        for (int i = 0; i < VN; ++i) e[u][i] += at == i ? g : 0.f;
-      }
-    };
-    if (a.tokens) add(tok < a.V ? tok : -1, gt);
-    for (int k = 0; k < a.gtop_k; ++k) add(a.gtop_ids[row * a.gtop_k + k], a.gtop[row * a.gtop_k + k]);
+        for (int i = 0; i < VN; ++i)
+          o[i] = e[u][i] * (ENT ? __builtin_fmaf(B, max_raw((v[u][i] - m) * kLog2e, -300.f), A) : A);
+        auto add = [&](int id, float g) {
+          const int at = id - j * VN;
+          if (at >= 0 && at < VN)
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int j = sub + u * G;
-      if (j < nvec) {
-        if (zero)
+            for (int i = 0; i < VN; ++i) o[i] += at == i ? g : 0.f;
+        };
+        add(tok, gt);
+        for (int k = 0; k < a.gtop_k; ++k) add((int)a.gtop_ids[row * a.gtop_k + k], a.gtop[row * a.gtop_k + k]);
+        if (j < nvec) {
+          if (zero)
 #pragma unroll
-          for (int i = 0; i < VN; ++i) e[u][i] = 0.f;
-        store_vec<T, VN>(nts, gx + j * VN, e[u]);
+            for (int i = 0; i < VN; ++i) o[i] = 0.f;
+          store_vec<T, VN>(nts, gx + j * VN, o);
+        }
       }
     }
   }
 }
 
-template <typename T, int VN, bool ENT>
+template <typename T, int VN, int WHAT>
 static int short_launch(const ShortArgs& a, const RowGeom& g, hipStream_t st) {
-  VAE_SWITCH_U(g.U, hipLaunchKernelGGL((token_short_kernel<T, VN, U, ENT>), dim3(g.grid), dim3(kBlock), 0, st, a, g.G,
+  const int log_g = __builtin_ctz(g.G);
+  VAE_SWITCH_U(g.U, hipLaunchKernelGGL((token_short_kernel<T, VN, U, WHAT>), dim3(g.grid), dim3(kBlock), 0, st, a, log_g,
                                        g.tiles));
   return hipGetLastError() == hipSuccess ? VAE_OK : VAE_ERR_LAUNCH;
 }
 template <typename T, int VN>
 static int short_kind(const ShortArgs& a, const RowGeom& g, hipStream_t st) {
-  return a.entropy || a.gentropy ? short_launch<T, VN, true>(a, g, st) : short_launch<T, VN, false>(a, g, st);
+  if (a.glogits) return a.gentropy ? short_launch<T, VN, kGrad | kEnt>(a, g, st) : short_launch<T, VN, kGrad>(a, g, st);
+  if (a.top_k) return a.entropy ? short_launch<T, VN, kTop | kEnt>(a, g, st) : short_launch<T, VN, kTop>(a, g, st);
+  return a.entropy ? short_launch<T, VN, kEnt>(a, g, st) : short_launch<T, VN, 0>(a, g, st);
 }
 
 bool short_rows(const ShortArgs& a, int dtype, hipStream_t st, int* rc) {

@@ -1,0 +1,121 @@
+// The teacher's side of a distillation, once per call: q = softmax(y / tau) over the entries that are there (id >= 0,
+// logit > -inf), ln q, and what comes twice merged, so that the kernels over the vocabulary find each id once.  A wave a
+// row, no barrier: K entries are 2 KB at most.  Prepared here and not in those kernels: there the chain of loads and
+// reductions stood in front of every row (4096 x 131072 bf16 with K = 64: 531 us against 423 us of the loss that has no
+// teacher; 8192 x 32768: 435 against 182).
+#include "token_row.hpp"
+
+namespace vae {
+
+template <int R>   // entries a lane
+__global__ __launch_bounds__(kBlock) void distill_teacher_kernel(const void* __restrict__ logits, int64_t stride, int dtype,
+                                                                 const void* __restrict__ ids, int64_t id_stride,
+                                                                 int id_bytes, int K, float inv_tau, float scale2,
+                                                                 int* __restrict__ state, int* __restrict__ id_out,
+                                                                 float* __restrict__ q_out, float* __restrict__ logq_out,
+                                                                 int64_t N, int V) {
+  const int lane = threadIdx.x & 63;
+  for (int64_t row = (int64_t)blockIdx.x * (kBlock / 64) + (threadIdx.x >> 6); row < N;
+       row += (int64_t)gridDim.x * (kBlock / 64)) {
+    float y[R], q[R], logq[R], m = kLowest;
+    int id[R];
+    bool bad = false;
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      const int k = lane + 64 * r;
+      y[r] = -INFINITY;
+      id[r] = -1;
+      if (k < K) {
+        const int64_t i = load_id(ids, id_bytes, row * id_stride + k);
+        bad |= i >= V;
+        if (i >= 0 && i < V) {
+          id[r] = (int)i;
+          y[r] = load_any(logits, dtype, row * stride + k);
+        }
+      }
+      m = max_raw(m, y[r]);
+    }
+    m = group_max(m, 64);
+    float s = 0.f;
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      q[r] = id[r] >= 0 ? exp2_raw((y[r] - m) * scale2) : 0.f;
+      if (q[r] == 0.f) id[r] = -1;   // NaN keeps its id: the row comes out NaN
+      s += q[r];
+    }
+    s = group_sum(s, 64);
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      q[r] /= s;
+      logq[r] = row_log_prob(y[r], m, s, inv_tau);
+    }
+    // equal ids into the first: the sum of q, and of q ln q, in the entries' order
+    float qs[R], ql[R];
+    bool first[R], twice = false;
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      qs[r] = ql[r] = 0.f;
+      first[r] = true;
+    }
+#pragma unroll
+    for (int r2 = 0; r2 < R; ++r2)
+      for (int l = 0; l < 64 && l + 64 * r2 < K; ++l) {
+        const int other = __builtin_amdgcn_readlane(id[r2], l);
+        const float oq = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, q[r2]), l));
+        const float ol = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, logq[r2]), l));
+#pragma unroll
+        for (int r = 0; r < R; ++r)
+          if (id[r] == other) {
+            const int k = lane + 64 * r, k2 = l + 64 * r2;
+            first[r] &= k2 >= k;
+            twice |= k2 != k;
+            qs[r] += oq;
+            ql[r] = __builtin_fmaf(oq, ol, ql[r]);
+          }
+      }
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      const int k = lane + 64 * r;
+      if (k >= K) continue;
+      const bool merged = twice && id[r] >= 0 && qs[r] != q[r];
+      id_out[row * K + k] = first[r] ? id[r] : -1;
+      q_out[row * K + k] = merged ? qs[r] : q[r];
+      logq_out[row * K + k] = merged ? ql[r] / qs[r] : logq[r];   // weighted: q (ln q - ln p) of the merged entry is their sum
+    }
+    const bool any_bad = __ballot(bad) != 0;
+    if (lane == 0) state[row] = any_bad ? kRowBad : (s == 0.f ? kRowEmpty : kRowFine);
+  }
+}
+
+}  // namespace vae
+
+using namespace vae;
+
+extern "C" {
+
+size_t vae_distill_teacher_floats(int64_t N, int64_t K) {
+  return N < 0 || K < 1 || K > VAE_MAX_TEACHER ? 0 : (size_t)N * (1 + 3 * (size_t)K);
+}
+
+int vae_distill_teacher(const void* t_logits, int64_t t_stride, int t_dtype, const void* t_ids, int64_t id_stride,
+                        int id_bytes, int64_t K, float temperature, float* teacher, int64_t N, int64_t V,
+                        vae_stream_t stream) {
+  if (N < 0 || V < 1 || V > VAE_MAX_ROW || K < 1 || K > VAE_MAX_TEACHER || (id_bytes != 4 && id_bytes != 8) ||
+      (t_dtype != VAE_F32 && t_dtype != VAE_BF16 && t_dtype != VAE_F16) || (N > 1 && (t_stride < K || id_stride < K)) ||
+      !(temperature > 0.f) || !(temperature < INFINITY))
+    return VAE_ERR_ARG;
+  if (N == 0) return VAE_OK;
+  if (!t_logits || !t_ids || !teacher) return VAE_ERR_ARG;
+  const Teacher t = teacher_of(teacher, N, K);
+  const int64_t blocks = (N + kBlock / 64 - 1) / (kBlock / 64);
+  const int grid = (int)(blocks < kMaxGrid ? blocks : kMaxGrid);
+  const float inv_tau = (float)(1.0 / (double)temperature);
+  const float scale2 = (float)(1.4426950408889634 / (double)temperature);
+  const auto kernel = K <= 64 ? distill_teacher_kernel<1> : (K <= 128 ? distill_teacher_kernel<2> : distill_teacher_kernel<4>);
+  hipLaunchKernelGGL(kernel, dim3(grid), dim3(kBlock), 0, (hipStream_t)stream, t_logits, t_stride, t_dtype, t_ids,
+                     id_stride, id_bytes, (int)K, inv_tau, scale2, const_cast<int*>(t.state), const_cast<int*>(t.id),
+                     const_cast<float*>(t.q), const_cast<float*>(t.logq), N, (int)V);
+  return hipGetLastError() == hipSuccess ? VAE_OK : VAE_ERR_LAUNCH;
+}
+
+}  // extern "C"

@@ -747,20 +747,20 @@ class _Distill(torch.autograd.Function):
     backward() when only the mean's gradient arrives (rescaled on the device when that is not 1)."""
 
     @staticmethod
-    def forward(ctx, logits, teacher, ids, temperature, inv_count, fuse):
+    def forward(ctx, logits, t_logits, t_ids, temperature, inv_count, fuse):
         ctx.set_materialize_grads(False)
-        kl, mean, stats, grad = _distill_fwd(logits, teacher, ids, temperature, inv_count, True, fuse)
-        ctx.save_for_backward(logits, teacher, ids, stats)
+        kl, mean, stats, grad, teacher = _distill_fwd(logits, t_logits, t_ids, temperature, inv_count, True, fuse)
+        ctx.save_for_backward(logits, teacher, stats)
         ctx.grad = grad
-        ctx.cfg = (temperature, inv_count)
+        ctx.cfg = (temperature, inv_count, t_ids.shape[-1])
         return kl, mean
 
     @staticmethod
     def backward(ctx, gkl, gmean):
         if gkl is None and gmean is None:
             return (None,) * 6
-        logits, teacher, ids, stats = ctx.saved_tensors
-        temperature, inv_count = ctx.cfg
+        logits, teacher, stats = ctx.saved_tensors
+        temperature, inv_count, K = ctx.cfg
         dev = logits.device
         grad, ctx.grad = ctx.grad, None
         gkl, gmean = _dense(gkl), _dense(gmean)
@@ -770,27 +770,28 @@ class _Distill(torch.autograd.Function):
             else:
                 rows = _rows(logits)
                 grad = torch.empty(logits.shape, dtype=logits.dtype, device=dev)
-                call('vae_distill_bwd', ptr(rows), rows.stride(0), ptr(teacher), teacher.stride(0),
-                     dtype_code(teacher), ptr(ids), ids.stride(0), ids.element_size(), ids.shape[1], temperature,
-                     ptr(stats), ptr(gkl), ptr(gmean), inv_count, ptr(grad), rows.shape[0], rows.shape[1],
-                     dtype_code(rows), stream_ptr(dev))
+                call('vae_distill_bwd', ptr(rows), rows.stride(0), ptr(teacher), K, temperature, ptr(stats), ptr(gkl),
+                     ptr(gmean), inv_count, ptr(grad), rows.shape[0], rows.shape[1], dtype_code(rows), stream_ptr(dev))
         return grad, None, None, None, None, None
 
 
-def _distill_fwd(logits, teacher, ids, temperature, inv_count, want_stats, fuse):
-    dev = check_device(logits, teacher, ids)
-    rows = _rows(logits)
-    N, V = rows.shape
+def _distill_fwd(logits, t_logits, t_ids, temperature, inv_count, want_stats, fuse):
+    dev = check_device(logits, t_logits, t_ids)
+    rows, t_logits, t_ids = _rows(logits), _rows(t_logits), _rows(t_ids)
+    (N, V), K = rows.shape, t_ids.shape[1]
     kl = torch.empty(logits.shape[:-1], dtype=torch.float32, device=dev)
     stats = torch.empty((N, 2), dtype=torch.float32, device=dev) if want_stats else None
     grad = torch.empty(logits.shape, dtype=logits.dtype, device=dev) if fuse else None
+    teacher = torch.empty((N, 1 + 3 * K), dtype=torch.float32, device=dev)   # vae_distill_teacher_floats
     scratch = _token_scratch(rows, 0, dev)
+    st = stream_ptr(dev)
     with _Guard(dev):
-        call('vae_distill_fwd', ptr(rows), rows.stride(0), ptr(teacher), teacher.stride(0), dtype_code(teacher),
-             ptr(ids), ids.stride(0), ids.element_size(), ids.shape[1], temperature, ptr(kl), ptr(stats), ptr(grad),
-             inv_count, ptr(scratch), N, V, dtype_code(rows), stream_ptr(dev))
+        call('vae_distill_teacher', ptr(t_logits), t_logits.stride(0), dtype_code(t_logits), ptr(t_ids), t_ids.stride(0),
+             t_ids.element_size(), K, temperature, ptr(teacher), N, V, st)
+        call('vae_distill_fwd', ptr(rows), rows.stride(0), ptr(teacher), K, temperature, ptr(kl), ptr(stats), ptr(grad),
+             inv_count, ptr(scratch), N, V, dtype_code(rows), st)
         mean = _row_sums(kl, inv_count, (), torch.float32)
-    return kl, mean, stats, grad
+    return kl, mean, stats, grad, teacher
 
 
 def distill_top_logits(logits, teacher_logits, teacher_ids, temperature=1.0, inv_count=None, fuse_backward=True):
@@ -800,8 +801,8 @@ def distill_top_logits(logits, teacher_logits, teacher_ids, temperature=1.0, inv
     mean = inv_count * sum(kl), inv_count = 1 / rows unless given (1 / unpadded rows, times temperature^2 where the
     loss is to be weighted so).  Differentiable with respect to `logits` only.
 
-    A negative id or a teacher logit of -inf is no entry; a row without entries has kl 0 and gradient 0 whatever it
-    holds; an id may come twice; an id beyond the vocabulary gives NaN.  `fuse_backward`: d(mean)/d(logits) is formed by
+    A negative id or a teacher logit of -inf is no entry; a row without entries has kl 0 and gradient 0 and its
+    logits are not read; an id may come twice; an id beyond the vocabulary gives NaN.  `fuse_backward`: d(mean)/d(logits) is formed by
     the forward launch (one read of the logits per step instead of two); a gradient on `kl` takes the general kernel."""
     _check_vocab(logits, 'distill_top_logits')
     _id_bytes(teacher_ids, 'distill_top_logits')
@@ -815,13 +816,12 @@ def distill_top_logits(logits, teacher_logits, teacher_ids, temperature=1.0, inv
         raise ValueError("distill_top_logits: temperature must be positive and finite, got %r" % temperature)
     if teacher_logits.requires_grad and torch.is_grad_enabled():
         raise ValueError("distill_top_logits: no gradient is formed for the teacher; pass teacher_logits.detach()")
-    teacher, ids = _rows(teacher_logits), _rows(teacher_ids)
     inv_count = 1.0 / max(logits.shape[:-1].numel(), 1) if inv_count is None else float(inv_count)
     if logits.requires_grad and torch.is_grad_enabled():
         # fp16: two passes, for the reason given in nll_elbo
         fuse = bool(fuse_backward) and logits.dtype != torch.float16 and logits.numel() > 0
-        return _Distill.apply(logits, teacher, ids, temperature, inv_count, fuse)
-    return _distill_fwd(logits, teacher, ids, temperature, inv_count, False, False)[:2]
+        return _Distill.apply(logits, teacher_logits, teacher_ids, temperature, inv_count, fuse)
+    return _distill_fwd(logits, teacher_logits, teacher_ids, temperature, inv_count, False, False)[:2]
 
 
 class _SampleSums(torch.autograd.Function):
