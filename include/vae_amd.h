@@ -498,7 +498,8 @@ int vae_token_nll_fused(const void* logits, int64_t row_stride, const void* toke
                         float* stats, void* glogits, float grad_scale, void* scratch, int64_t N, int64_t V, int dtype,
                         vae_stream_t stream);
 /* The loss of B samples of T tokens each, from logp [B * T]: nll[b] = -sum_t logp[b T + t] (in double, in a fixed
- * order), loss / elbo / means as vae_elbo_combine_fwd (abstract_vae.py:356-388); loss == elbo == NULL: nll alone.   */
+ * order), loss / elbo / means as vae_elbo_combine_fwd (abstract_vae.py:356-388) but from the unrounded nll, each
+ * rounded once; loss == elbo == NULL: nll alone.                                                                   */
 int vae_token_elbo_fwd(const float* logp, int64_t T, const void* kld, const void* add, const void* mi, float kl_beta,
                        float inv_count, void* nll, void* loss, void* elbo, float* means, float* workspace, int64_t B,
                        int dtype, vae_stream_t stream);

@@ -296,7 +296,7 @@ template <int BT, bool ENT, bool DIST>
 __device__ __forceinline__ void write_row(const FwdArgs& a, int64_t row, int64_t tok, float token_logit, float m, float s,
                                           float t, const TeacherTerms<BT>& terms) {
   float kl = 0.f;
-  if constexpr (DIST) kl = terms.kl(m, s, a.inv_tau);
+  if constexpr (DIST) kl = terms.kl(a.teacher.K, m, s, a.inv_tau);
   if (threadIdx.x == 0) {
     if constexpr (DIST) a.logp[row] = kl;
     else if (a.logp) a.logp[row] = tok < a.V ? row_log_prob(token_logit, m, s, 1.0f) : nan_f();

@@ -20,14 +20,13 @@ __global__ __launch_bounds__(kBlock) void token_elbo_fwd_kernel(
       for (int64_t t = sub; t < len; t += G) v += (double)logp[b * len + t];
     for (int o = G >> 1; o >= 1; o >>= 1) v += __shfl_xor(v, o, 64);
     if (sub != 0 || b >= B) continue;
-    const float n = to_f32(from_f32<T>((float)-v));
+    const float n = (float)-v;          // loss and elbo from the unrounded sum: every output is rounded once
     nll[b] = from_f32<T>(n);
     if (!loss) continue;
     const float k = kld ? to_f32(kld[b]) : 0.f;
     const float ad = add ? to_f32(add[b]) : 0.f;
     const float m = mi ? to_f32(mi[b]) : 0.f;
-    const float e = to_f32(from_f32<T>(n + k));
-    const float l = to_f32(from_f32<T>((n + ad + kl_beta * k) - m));
+    const float e = n + k, l = (n + ad + kl_beta * k) - m;
     loss[b] = from_f32<T>(l);
     elbo[b] = from_f32<T>(e);
     acc[0] += l; acc[1] += e; acc[2] += n; acc[3] += k; acc[4] += ad; acc[5] += m;

@@ -19,10 +19,10 @@ struct Entries {
   int next[kMaxEntries], id[kMaxEntries];
   float g[kMaxEntries];
 
-  __device__ __forceinline__ void clear() {
-    lds_barrier();   // the row before this one has been read
+  // a barrier of the caller's stands between clear() and put(), and between put() and the lists' use
+  __device__ __forceinline__ void clear(bool again) {
+    if (again) lds_barrier();   // the row before this one has been read
     head[threadIdx.x] = -1;
-    lds_barrier();
   }
   template <typename T, int VN>
   __device__ __forceinline__ void put(int k, int id_k, float g_k, const RowCut<T, VN>& cut, int v0, int v1) {
@@ -39,7 +39,7 @@ struct Entries {
   }
 };
 
-// What a thread adds to its elements: one entry known to all (ONE), or the workgroup's lists.
+// What a thread adds to its elements: one entry known to all, or (LIST) the workgroup's lists.
 template <typename T, int VN, int BT, bool LIST>
 struct Adds {
   const Entries<BT>* lds;
@@ -175,7 +175,8 @@ __global__ __launch_bounds__(BT) void token_bwd_kernel(GradArgs a) {
       const float g0 = a.gmean ? a.gmean[0] * a.mean_scale : (a.gkl ? 0.f : a.mean_scale);
       const float w = ((a.gkl ? a.gkl[row] : 0.f) + g0) * a.inv_tau;
       A = w * inv;               // an id beyond the vocabulary: s is NaN
-      lds.entries[0].clear();
+      lds.entries[0].clear(item != blockIdx.x);
+      lds_barrier();
 #pragma unroll
       for (int r = 0; r < TeacherTerms<BT>::R; ++r)
         lds.entries[0].put((int)threadIdx.x + r * BT, terms.id[r], -w * terms.q[r], cut, v0, v1);
@@ -190,7 +191,8 @@ __global__ __launch_bounds__(BT) void token_bwd_kernel(GradArgs a) {
       if constexpr (LIST) {
         for (int k = 0; k < a.top_k; ++k) sum += a.gtop[row * a.top_k + k];
         // the alternatives differ from each other; the token may be one of them
-        lds.entries[0].clear();
+        lds.entries[0].clear(item != blockIdx.x);
+        lds_barrier();
         bool other = true;
         for (int k = 0; k < a.top_k; ++k) other &= a.top_ids[row * a.top_k + k] != tok;
         for (int k = threadIdx.x; k <= a.top_k; k += BT) {
@@ -276,22 +278,10 @@ __global__ __launch_bounds__(BT, 4) void token_fused_kernel(GradArgs a) {
     if constexpr (DIST) terms.fetch(a.teacher, row);
     piece.load();
     const float edge = ei >= 0 ? to_f32(x[ei]) : -INFINITY;
-    Adds<T, VN, BT, DIST> adds;
-    const float w = DIST ? a.mean_scale * a.inv_tau : a.g_scale;   // of p; the entries have the other sign
     if constexpr (DIST) {
-      // while the row is on its way
-      adds.lds = lds.entries;
-      lds.entries[0].clear();
+      lds.entries[0].clear(row != blockIdx.x);
       terms.fetch_logits(x);
-#pragma unroll
-      for (int r = 0; r < TeacherTerms<BT>::R; ++r)
-        lds.entries[0].put((int)threadIdx.x + r * BT, terms.id[r], -w * terms.q[r], cut, 0, cut.nvec);
-      lds_barrier();
-    } else {
-      adds.one_id = (int)tok;
-      adds.one_g = -w;
     }
-    adds.prepare(cut, 0, cut.nvec);
     piece.mask();
     float mt = max_raw(edge, kLowest);
 #pragma unroll
@@ -324,15 +314,30 @@ __global__ __launch_bounds__(BT, 4) void token_fused_kernel(GradArgs a) {
       }
     const float m = block_max<BT>(mt);
     float f = exp2_raw((mt - m) * a.scale2);       // from the thread's maximum to the row's
+    // The entries between the two reductions, whose barriers they need: a wave's exponentials wait for its own packets
+    // alone.
+    Adds<T, VN, BT, DIST> adds;
+    const float w = DIST ? a.mean_scale * a.inv_tau : a.g_scale;   // of p; the entries have the other sign
+    if constexpr (DIST) {
+      adds.lds = lds.entries;
+      if constexpr (BT == 64) lds_barrier();       // block_max has none
+#pragma unroll
+      for (int r = 0; r < TeacherTerms<BT>::R; ++r)
+        lds.entries[0].put((int)threadIdx.x + r * BT, terms.id[r], -w * terms.q[r], cut, 0, cut.nvec);
+      if constexpr (BT == 64) lds_barrier();
+    } else {
+      adds.one_id = (int)tok;
+      adds.one_g = -w;
+    }
     s = block_sum<BT>(s * f);
-    auto loss = [&]() {             // behind the gradient: it waits for nobody
-      if constexpr (DIST) {
-        const float kl = terms.kl(m, s, a.inv_tau);
-        if (threadIdx.x == 0) a.out[row] = kl;
-      } else if (threadIdx.x == 0) {
-        a.out[row] = row_log_prob(token_logit, m, s, 1.0f);
-      }
-    };
+    adds.prepare(cut, 0, cut.nvec);
+    // in front of the gradient: behind it this would wait for the stores, loads and stores share a counter
+    if constexpr (DIST) {
+      const float kl = terms.kl(a.teacher.K, m, s, a.inv_tau);
+      if (threadIdx.x == 0) a.out[row] = kl;
+    } else if (threadIdx.x == 0) {
+      a.out[row] = row_log_prob(token_logit, m, s, 1.0f);
+    }
     if (threadIdx.x == 0) {
       a.stats_out[2 * row] = m;
       a.stats_out[2 * row + 1] = s;
@@ -340,7 +345,6 @@ __global__ __launch_bounds__(BT, 4) void token_fused_kernel(GradArgs a) {
     if (s == 0.f) {
       piece.fill(a.nts, 0.f);
       if (ei >= 0) gx[ei] = from_f32<T>(0.f);
-      loss();
       continue;
     }
     const float A = w / s;
@@ -367,7 +371,6 @@ __global__ __launch_bounds__(BT, 4) void token_fused_kernel(GradArgs a) {
       adds.to(ei, v);
       gx[ei] = from_f32<T>(v[0]);
     }
-    loss();
   }
 }
 

@@ -251,12 +251,13 @@ struct TeacherTerms {
 #pragma unroll
     for (int r = 0; r < R; ++r) x[r] = id[r] >= 0 ? to_f32(logits[id[r]]) : 0.f;
   }
-  __device__ __forceinline__ float kl(float m, float s, float inv_tau) const {
+  // the row's KL, in thread 0
+  __device__ __forceinline__ float kl(int K, float m, float s, float inv_tau) const {
     float v = 0.f;
 #pragma unroll
     for (int r = 0; r < R; ++r)
       if (id[r] >= 0) v += q[r] * (logq[r] - row_log_prob(x[r], m, s, inv_tau));
-    return block_sum<BT>(v);
+    return K <= 64 ? group_sum(v, 64) : block_sum<BT>(v);   // up to 64 entries are the first wave's: no barrier
   }
 };
 
