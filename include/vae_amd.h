@@ -499,10 +499,13 @@ int vae_token_nll_fused(const void* logits, int64_t row_stride, const void* toke
                         vae_stream_t stream);
 /* The loss of B samples of T tokens each, from logp [B * T]: nll[b] = -sum_t logp[b T + t] (in double, in a fixed
  * order), loss / elbo / means as vae_elbo_combine_fwd (abstract_vae.py:356-388) but from the unrounded nll, each
- * rounded once; loss == elbo == NULL: nll alone.                                                                   */
+ * rounded once; loss == elbo == NULL: nll alone.  means: VAE_TOKEN_MEANS_FLOATS floats, the six means in front, the rest
+ * scratch; loss_mean (mean_dtype; may be NULL): the first of them once more, in a place of its own.  workspace (may be
+ * NULL): its saw-a-NaN word alone is used.                                                                         */
+#define VAE_TOKEN_MEANS_FLOATS (6 + 6 * 256)
 int vae_token_elbo_fwd(const float* logp, int64_t T, const void* kld, const void* add, const void* mi, float kl_beta,
-                       float inv_count, void* nll, void* loss, void* elbo, float* means, float* workspace, int64_t B,
-                       int dtype, vae_stream_t stream);
+                       float inv_count, void* nll, void* loss, void* elbo, float* means, void* loss_mean,
+                       int mean_dtype, float* workspace, int64_t B, int dtype, vae_stream_t stream);
 /* Its backward.  gnll / gloss / gelbo [B] (dtype) and gmeans, a HOST array of 6 device pointers to one value each
  * (gmeans_dtype): every one may be NULL.  grow [B] (float32) = d / d nll[b], what vae_token_logp_bwd takes with
  * rows_per_g = T and g_scale = -1; or grad [n] = a stored d(loss_mean) / d logits (vae_token_nll_fused), multiplied by

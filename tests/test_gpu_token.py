@@ -668,3 +668,142 @@ def test_many_short_rows_and_offsets_beyond_32_bits():
         p[0, tok[r].cpu()] -= 1.0
         check_grad(g[r], p[0] / N, 1.0 / N)
     assert bool((g[1] == 0).all()) and bool((g[N - 2] == 0).all())
+
+
+@pytest.mark.parametrize('V,dt', [(257, 'bf16'), (300, 'f32')])
+def test_more_rows_than_a_launch_has_blocks(V, dt):
+    """2^20 rows and some: the workgroups go round again, with the same shared memory."""
+    from vae_amd import functional as F_
+    N = (1 << 20) + 37
+    x = torch.empty(N, V, dtype=TYPES[dt], device=DEV)
+    x.normal_(generator=torch.Generator(device=DEV).manual_seed(1))
+    if dt == 'f32':
+        x = x[:, :V - 1]                       # rows 1200 bytes apart of 299 elements: no short-row form
+    V = x.shape[1]
+    x = x.detach().requires_grad_(True)
+    tok = torch.randint(0, V, (N,), generator=torch.Generator(device=DEV).manual_seed(2), device=DEV)
+    lp, h, top, ids = F_.token_log_probs(x, tok, top_k=3)
+    g, = torch.autograd.grad([lp, h, top], [x], [torch.ones_like(lp), torch.ones_like(h), torch.ones_like(top)])
+    kl, mean = F_.distill_top_logits(x, top.detach(), ids, inv_count=1.0)
+    gd, = torch.autograd.grad(mean, x)
+    _, _, _, means = F_.nll_elbo(tok[:, None], x[:, None], 'categorical', inv_count=1.0, fuse_backward=True)
+    gn, = torch.autograd.grad(means[0], x)
+    rows = torch.tensor([0, 1, 5, 36, 37, (1 << 20) - 1, 1 << 20, (1 << 20) + 1, (1 << 20) + 36])
+    z = x.detach()[rows.to(DEV)].double().cpu()
+    t = tok[rows.to(DEV)].cpu()
+    logp, p, hr = ref_rows(z)
+    want = ref_top(z, 3)
+    at = lambda v: v.detach()[rows.to(DEV)].cpu()
+    close(at(lp), logp.gather(1, t[:, None])[:, 0], 1e-6, 4e-6)
+    close(at(h), hr, 1e-6, 2e-5)
+    assert torch.equal(at(ids), want)
+    ref = -4.0 * p - p * (logp + hr[:, None])
+    ref[torch.arange(len(rows)), t] += 1.0
+    ref.scatter_add_(1, want, torch.ones(len(rows), 3).double())
+    check_grad(at(g), ref, 8.0)
+    klr, gr = ref_distill(z, logp.gather(1, want), want, 1.0)
+    close(at(kl), klr, 1e-6, 2e-5)
+    check_grad(at(gd), gr, 2.0)
+    q = p.clone()
+    q[torch.arange(len(rows)), t] -= 1.0
+    check_grad(at(gn), q, 1.0)
+    close(means[0], -torch.log_softmax(x.detach().double(), 1).gather(1, tok[:, None]).sum().cpu(), 1e-5, 0.0)
+
+
+@pytest.mark.parametrize('dt', ['bf16', 'f32'])
+@pytest.mark.parametrize('k', [1, 20, 64])
+def test_alternatives_of_whole_rows(k, dt):
+    """Rows enough that none is split: equal values, masks that leave little, sorted rows, and large values that all sit in
+    one thread's share of a long row (more of them than the candidates' list holds)."""
+    from vae_amd import functional as F_
+    vec = 4 if dt == 'f32' else 8
+    N, V = 520, 300000 if dt == 'bf16' else 310000
+    x = torch.empty(N, V, dtype=TYPES[dt], device=DEV)
+    x.normal_(generator=torch.Generator(device=DEV).manual_seed(k))
+    low = float('-inf')
+    x[0] = 1.0
+    x[1] = low
+    x[2] = low
+    x[2, [7, 100000, V - 1]] = torch.tensor([1.0, 3.0, 1.0], dtype=x.dtype, device=DEV)
+    x[3] = torch.sort(x[3].float())[0].to(x.dtype)
+    x[4] = torch.sort(x[4].float(), descending=True)[0].to(x.dtype)
+    col = (3 * vec + torch.arange(0, V - 4 * vec, 256 * vec, device=DEV)[:, None]
+           + torch.arange(vec, device=DEV)[None]).reshape(-1)
+    x[5, col] = (20.0 + torch.arange(col.numel(), device=DEV) * 0.01).to(x.dtype)
+    x[6] = torch.randint(-2, 3, (V,), device=DEV).to(x.dtype)
+    x[7] = torch.finfo(TYPES[dt]).min
+    _, _, top, ids = F_.token_log_probs(x, top_k=k, want_entropy=False)
+    for r in list(range(8)) + [100, N - 1]:
+        z = x[r].double().cpu()[None]
+        want = ref_top(z, k)
+        assert torch.equal(ids[r].cpu(), want[0]), r
+        close(top[r], ref_rows(z)[0].gather(1, want)[0], 1e-6, 4e-6)
+
+
+def test_loss_mean_may_be_scaled_in_place():
+    """An accumulation loop's loss /= n, as with the other likelihoods."""
+    import vae_amd
+    z = torch.randn(3, 2, 30, generator=gen(1))
+    x = torch.randint(0, 30, (3, 2), generator=gen(2))
+    for dt in ('f32', 'bf16'):
+        xr = z.to(TYPES[dt]).to(DEV).requires_grad_(True)
+        loss = vae_amd.loss_function(xr, x.to(DEV), torch.zeros(3, device=DEV), 'categorical')['loss_mean']
+        loss /= 4
+        g, = torch.autograd.grad(loss, xr)
+        ref = ref_elbo(z.to(TYPES[dt]).double(), x, torch.zeros(3).double(), 1.0)
+        close(loss, ref[0].mean() / 4, 2 * HALF[TYPES[dt]] + 1e-6, 1e-5)
+        # stored as d(loss_mean), rounded, then scaled by 1/4: exact
+        check_grad(g, ref[3] / 12, 0.1)
+
+
+def test_means_over_many_samples():
+    """More samples than one block takes: the means of 10000 x 3 tokens, with KL, additional and mutual-information terms."""
+    from vae_amd import functional as F_
+    B, T, V = 10000, 3, 20
+    z = torch.randn(B, T, V, generator=gen(1))
+    x = torch.randint(-1, V, (B, T), generator=gen(2))
+    terms = [torch.rand(B, generator=gen(3 + i)) for i in range(3)]
+    nll, loss, elbo, means = F_.nll_elbo(x.to(DEV), z.to(DEV), 'categorical', *[t.to(DEV) for t in terms], kl_beta=0.25)
+    n = ref_elbo(z.double(), x, torch.zeros(B).double(), 1.0)[0]
+    kld, add, mi = [t.double() for t in terms]
+    want = torch.stack([(n + add + 0.25 * kld - mi).mean(), (n + kld).mean(), n.mean(), kld.mean(), add.mean(), mi.mean()])
+    close(means, want, 2e-6, 1e-6)
+    close(loss, n + add + 0.25 * kld - mi, 1e-6, 1e-5)
+
+
+def test_nan_in_the_loss_raises_the_flag():
+    import vae_amd
+    vae_amd.nan_flags()
+    x = torch.zeros(5, dtype=torch.int64, device=DEV)
+    z = torch.randn(5, 12, generator=gen(1)).to(DEV)
+    vae_amd.loss_function(z, x, torch.zeros(5, device=DEV), 'categorical')
+    assert vae_amd.nan_flags() == 0
+    z[3, 4] = float('nan')
+    vae_amd.loss_function(z, x, torch.zeros(5, device=DEV), 'categorical')
+    assert vae_amd.nan_flags() & 1
+
+
+def test_second_derivatives_are_refused():
+    from vae_amd import functional as F_
+    x = torch.randn(3, 9, device=DEV, requires_grad=True)
+    tok = torch.tensor([1, 2, 3], device=DEV)
+    y = (x * 2).requires_grad_(True)
+    lp, _, _, _ = F_.token_log_probs(y, tok)
+    g, = torch.autograd.grad(lp.sum(), x, create_graph=True)
+    with pytest.raises(RuntimeError):
+        g.sum().backward()
+
+
+def test_expanded_logits():
+    """One row shared by several tokens (a broadcast input): its gradient is the sum."""
+    from vae_amd import functional as F_
+    x = torch.randn(1, 40, generator=gen(1)).to(DEV).requires_grad_(True)
+    tok = torch.tensor([3, 5, 5, -1], device=DEV)
+    lp, h, _, _ = F_.token_log_probs(x.expand(4, 40), tok)
+    g, = torch.autograd.grad(lp.sum(), x)
+    p = torch.softmax(x.detach().double().cpu(), 1)
+    ref = -3.0 * p
+    ref[0, 3] += 1.0
+    ref[0, 5] += 2.0
+    check_grad(g, ref, 4.0)
+    assert bool((h[:3] == h[0]).all()) and float(h[3]) == 0.0

@@ -169,12 +169,12 @@ def test_sums_and_scale_refusals():
 
 def test_loss_closing_refusals():
     f, b = 'vae_token_elbo_fwd', 'vae_token_elbo_bwd'
-    ok = [P, 3, None, None, None, 1.0, 1.0, P, P, P, P, P, 0, 0, None]          # no samples: nothing is launched
+    ok = [P, 3, None, None, None, 1.0, 1.0, P, P, P, P, P, 0, P, 0, 0, None]     # no samples: nothing is launched
     assert _call(f, ok) == _lib.VAE_OK
-    for i, v in ((12, -1), (1, -1), (13, 5)):
+    for i, v in ((14, -1), (1, -1), (15, 5), (12, 4)):
         assert _call(f, ok[:i] + [v] + ok[i + 1:]) == _lib.VAE_ERR_ARG
-    some = ok[:12] + [2] + ok[13:]
-    for i in (0, 7, 8, 9, 10, 11):
+    some = ok[:14] + [2] + ok[15:]
+    for i in (0, 7, 8, 9, 10):
         assert _call(f, some[:i] + [None] + some[i + 1:]) == _lib.VAE_ERR_ARG
     ok = [None, None, None, None, 0, 1.0, 1.0, P, None, 0, None, None, None, 0, 0, None]
     assert _call(b, ok) == _lib.VAE_OK

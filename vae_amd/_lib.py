@@ -96,7 +96,7 @@ SIGNATURES = {
     'vae_token_logp_fwd': [_p, _i64, _p, _i, _p, _p, _p, _p, _p, _i64, _p, _i64, _i64, _i, _p],
     'vae_token_logp_bwd': [_p, _i64, _p, _i, _p, _p, _p, _i64, _f, _p, _p, _p, _i64, _p, _i64, _i64, _i, _p],
     'vae_token_nll_fused': [_p, _i64, _p, _i, _p, _p, _p, _f, _p, _i64, _i64, _i, _p],
-    'vae_token_elbo_fwd': [_p, _i64, _p, _p, _p, _f, _f, _p, _p, _p, _p, _p, _i64, _i, _p],
+    'vae_token_elbo_fwd': [_p, _i64, _p, _p, _p, _f, _f, _p, _p, _p, _p, _p, _i, _p, _i64, _i, _p],
     'vae_token_elbo_bwd': [_p, _p, _p, _pp, _i, _f, _f, _p, _p, _i64, _p, _p, _p, _i64, _i, _p],
     'vae_row_sums': [_p, _f, _p, _i64, _i64, _i, _p],
     'vae_grad_scale': [_p, _p, _i64, _i, _p],
@@ -191,6 +191,20 @@ def stream_ptr(device):
     return _stream_handle(device)
 
 
+_current_device = torch._C._cuda_getDevice if hasattr(torch._C, '_cuda_getDevice') else torch.cuda.current_device
+
+
+def launch(device, name, *args):
+    """call(name, *args, stream) on `device`'s current stream, with the device made current when it is not."""
+    index = device.index
+    if index != _current_device():
+        with torch.cuda.device(device):
+            return call(name, *args, _stream_handle(device))
+    rc = getattr(_lib or load(), name)(*args, _stream_handle(device))
+    if rc != VAE_OK:
+        _fail(name, rc)
+
+
 _workspaces = {}
 
 
@@ -239,5 +253,9 @@ def describe_nan_flags(flags):
 def call(name, *args):
     rc = getattr(load(), name)(*args)
     if rc != VAE_OK:
-        what = {VAE_ERR_ARG: 'invalid argument', VAE_ERR_LAUNCH: 'kernel launch failed'}.get(rc, 'error %d' % rc)
-        raise RuntimeError("vae_amd: %s: %s" % (name, what))
+        _fail(name, rc)
+
+
+def _fail(name, rc):
+    what = {VAE_ERR_ARG: 'invalid argument', VAE_ERR_LAUNCH: 'kernel launch failed'}.get(rc, 'error %d' % rc)
+    raise RuntimeError("vae_amd: %s: %s" % (name, what))

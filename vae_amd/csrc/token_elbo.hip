@@ -5,12 +5,34 @@
 
 namespace vae {
 
-// G lanes a sample (a power of two, up to a wave); samples in order, so a result does not depend on the grid
+// The six means leave the first launch as block partials in the caller's `means` buffer and a second one adds them, in
+// block order and in double; a single block writes them itself.  No counters, so calls and captured graphs share nothing
+// (the saw-a-NaN word of the workspace is a bit that several may set).
+constexpr int kElboBlocks = 256;
+static_assert(VAE_TOKEN_MEANS_FLOATS == 6 + 6 * kElboBlocks, "the header says how long `means` is");
+
+__device__ __forceinline__ void store_any(void* p, int dtype, float v) {
+  if (dtype == VAE_F32) *reinterpret_cast<float*>(p) = v;
+  else if (dtype == VAE_BF16) *reinterpret_cast<bf16_t*>(p) = from_f32<bf16_t>(v);
+  else *reinterpret_cast<f16_t*>(p) = from_f32<f16_t>(v);
+}
+// thread k < 6: total k -> mean k; thread 0 leaves the loss mean in its own place too
+__device__ __forceinline__ void write_mean(int k, double total, float inv_count, float* means, void* loss_mean,
+                                           int mean_dtype, float* ws) {
+  const float v = (float)(total * (double)inv_count);
+  means[k] = v;
+  if (k == 0 && loss_mean) store_any(loss_mean, mean_dtype, v);
+  if (ws) note_nan(ws, v, kNanElbo6, k);
+}
+
+// G lanes a sample (a power of two, up to a wave); samples in order, so a result does not depend on timing
 template <typename T>
 __global__ __launch_bounds__(kBlock) void token_elbo_fwd_kernel(
     const float* __restrict__ logp, int64_t len, const T* __restrict__ kld, const T* __restrict__ add,
     const T* __restrict__ mi, float kl_beta, float inv_count, T* __restrict__ nll, T* __restrict__ loss,
-    T* __restrict__ elbo, float* __restrict__ means, float* __restrict__ ws, int64_t B, int G) {
+    T* __restrict__ elbo, float* __restrict__ means, void* __restrict__ loss_mean, int mean_dtype,
+    float* __restrict__ ws, int64_t B, int G) {
+  __shared__ float part[kBlock / 64][6];
   const int rpb = kBlock / G, sub = threadIdx.x % G, rloc = threadIdx.x / G;
   float acc[6] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
   for (int64_t b0 = (int64_t)blockIdx.x * rpb; b0 < B; b0 += (int64_t)gridDim.x * rpb) {
@@ -31,7 +53,30 @@ __global__ __launch_bounds__(kBlock) void token_elbo_fwd_kernel(
     elbo[b] = from_f32<T>(e);
     acc[0] += l; acc[1] += e; acc[2] += n; acc[3] += k; acc[4] += ad; acc[5] += m;
   }
-  if (loss) grid_reduce<6>(acc, ws, inv_count, means, kNanElbo6);
+  if (!loss) return;
+#pragma unroll
+  for (int k = 0; k < 6; ++k) {
+    const float s = wave_total(acc[k]);
+    if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6][k] = s;
+  }
+  lds_barrier();
+  if (threadIdx.x < 6) {
+    const int k = threadIdx.x;
+    float s = 0.f;
+    for (int w = 0; w < kBlock / 64; ++w) s += part[w][k];
+    if (gridDim.x == 1) write_mean(k, s, inv_count, means, loss_mean, mean_dtype, ws);
+    else means[6 + 6 * blockIdx.x + k] = s;
+  }
+}
+__global__ __launch_bounds__(64) void token_elbo_means_kernel(float* __restrict__ means, int blocks, float inv_count,
+                                                              void* __restrict__ loss_mean, int mean_dtype,
+                                                              float* __restrict__ ws) {
+  for (int k = 0; k < 6; ++k) {
+    double v = 0.0;
+    for (int b = threadIdx.x; b < blocks; b += 64) v += (double)means[6 + 6 * b + k];
+    v = wave_sum_d(v);
+    if ((int)threadIdx.x == k) write_mean(k, v, inv_count, means, loss_mean, mean_dtype, ws);
+  }
 }
 
 struct Scalars6 {
@@ -108,19 +153,22 @@ using namespace vae;
 extern "C" {
 
 int vae_token_elbo_fwd(const float* logp, int64_t len, const void* kld, const void* add, const void* mi, float kl_beta,
-                       float inv_count, void* nll, void* loss, void* elbo, float* means, float* workspace, int64_t B,
-                       int dtype, vae_stream_t stream) {
-  if (B < 0 || len < 0 || !type_ok(dtype)) return VAE_ERR_ARG;
+                       float inv_count, void* nll, void* loss, void* elbo, float* means, void* loss_mean,
+                       int mean_dtype, float* workspace, int64_t B, int dtype, vae_stream_t stream) {
+  if (B < 0 || len < 0 || !type_ok(dtype) || (loss_mean && !type_ok(mean_dtype))) return VAE_ERR_ARG;
   if (B == 0) return VAE_OK;
-  if (!nll || (len > 0 && !logp) || (loss == nullptr) != (elbo == nullptr) || (loss && (!means || !workspace)))
-    return VAE_ERR_ARG;
+  if (!nll || (len > 0 && !logp) || (loss == nullptr) != (elbo == nullptr) || (loss && !means)) return VAE_ERR_ARG;
   int G = 1;
   while (G < 64 && G < len) G <<= 1;
   const int64_t blocks = (B + kBlock / G - 1) / (kBlock / G);
-  const int grid = (int)(blocks < kGridReduce ? blocks : kGridReduce);
+  // without the means nothing is left to add up: as many blocks as there are samples for
+  const int grid = (int)(blocks < (loss ? kElboBlocks : kMaxGrid) ? blocks : (loss ? kElboBlocks : kMaxGrid));
   VAE_BY_TYPE(dtype, hipLaunchKernelGGL((token_elbo_fwd_kernel<T>), dim3(grid), dim3(kBlock), 0, (hipStream_t)stream,
                                         logp, len, (const T*)kld, (const T*)add, (const T*)mi, kl_beta, inv_count,
-                                        (T*)nll, (T*)loss, (T*)elbo, means, workspace, B, G));
+                                        (T*)nll, (T*)loss, (T*)elbo, means, loss_mean, mean_dtype, workspace, B, G));
+  if (loss && grid > 1)
+    hipLaunchKernelGGL(token_elbo_means_kernel, dim3(1), dim3(64), 0, (hipStream_t)stream, means, grid, inv_count,
+                       loss_mean, mean_dtype, workspace);
   return launched();
 }
 

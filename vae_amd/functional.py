@@ -8,9 +8,10 @@ reference's shapes.
 import ctypes
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import _lib
-from ._lib import call, check_device, dtype_code, ptr, stream_ptr, workspace
+from ._lib import call, check_device, dtype_code, launch, ptr, stream_ptr, workspace
 
 _MASK64 = (1 << 64) - 1
 
@@ -515,6 +516,7 @@ def categorical_kl(log_q, log_p):
 # --------------------------------------------------------------------------------------
 MAX_TOP = 64        # VAE_MAX_TOP in include/vae_amd.h
 MAX_TEACHER = 256   # VAE_MAX_TEACHER
+MEANS = 6 + 6 * 256  # VAE_TOKEN_MEANS_FLOATS
 
 
 def _is_categorical(nll_type):
@@ -548,10 +550,10 @@ def _token_scratch(rows, top_k, dev):
 
 def _row_sums(rows, scale, shape, dtype):
     """scale * sum over equal runs of `rows` (fp32, summed in double), one run for each entry of `shape`."""
-    out = torch.empty(shape, dtype=dtype, device=rows.device)
+    dev = rows.device
+    out = torch.empty(shape, dtype=dtype, device=dev)
     B = out.numel()
-    call('vae_row_sums', ptr(rows), scale, ptr(out), B, rows.numel() // max(B, 1), dtype_code(out),
-         stream_ptr(rows.device))
+    launch(dev, 'vae_row_sums', ptr(rows), scale, ptr(out), B, rows.numel() // max(B, 1), dtype_code(out))
     return out
 
 
@@ -568,10 +570,9 @@ def _token_fwd(logits, tokens, top_k, want_entropy, want_stats):
     top = new(shape + (top_k,)) if top_k else None
     ids = torch.empty(shape + (top_k,), dtype=torch.int64, device=dev) if top_k else None
     scratch = _token_scratch(rows, top_k, dev)
-    with _Guard(dev):
-        call('vae_token_logp_fwd', ptr(rows), rows.stride(0), ptr(tokens),
-             0 if tokens is None else tokens.element_size(), ptr(logp), ptr(entropy), ptr(stats), ptr(top), ptr(ids),
-             top_k, ptr(scratch), N, V, dtype_code(rows), stream_ptr(dev))
+    launch(dev, 'vae_token_logp_fwd', ptr(rows), rows.stride(0), ptr(tokens),
+           0 if tokens is None else tokens.element_size(), ptr(logp), ptr(entropy), ptr(stats), ptr(top), ptr(ids),
+           top_k, ptr(scratch), N, V, dtype_code(rows))
     return logp, entropy, top, ids, stats
 
 
@@ -583,11 +584,10 @@ def _token_bwd(logits, tokens, entropy, ids, stats, glogp, rows_per_g, g_scale, 
     grad = torch.empty(logits.shape, dtype=logits.dtype, device=dev)
     if glogp is None and tokens is not None:
         glogp, rows_per_g, g_scale = torch.zeros((1,), dtype=torch.float32, device=dev), N, 0.0
-    with _Guard(dev):
-        call('vae_token_logp_bwd', ptr(rows), rows.stride(0), ptr(tokens),
-             0 if tokens is None else tokens.element_size(), ptr(stats), ptr(entropy), ptr(glogp), max(rows_per_g, 1),
-             g_scale, ptr(gentropy), ptr(gtop), ptr(ids) if gtop is not None else None,
-             ids.shape[-1] if gtop is not None else 0, ptr(grad), N, V, dtype_code(rows), stream_ptr(dev))
+    launch(dev, 'vae_token_logp_bwd', ptr(rows), rows.stride(0), ptr(tokens),
+           0 if tokens is None else tokens.element_size(), ptr(stats), ptr(entropy), ptr(glogp), max(rows_per_g, 1),
+           g_scale, ptr(gentropy), ptr(gtop), ptr(ids) if gtop is not None else None,
+           ids.shape[-1] if gtop is not None else 0, ptr(grad), N, V, dtype_code(rows))
     return grad
 
 
@@ -602,6 +602,7 @@ class _TokenLogProbs(torch.autograd.Function):
         return logp, entropy, top, ids
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, glogp, gentropy, gtop, gids):
         if glogp is None and gentropy is None and gtop is None:
             return None, None, None, None
@@ -654,32 +655,34 @@ class _TokenNllElbo(torch.autograd.Function):
         dev = check_device(logits, tokens, kld, add, mi)
         rows, B = _rows(logits), tokens.shape[0]
         N, V = rows.shape
-        code, st = dtype_code(rows), stream_ptr(dev)
+        code = dtype_code(rows)
         logp = torch.empty((N,), dtype=torch.float32, device=dev)
         stats = torch.empty((N, 2), dtype=torch.float32, device=dev)
         grad = torch.empty(logits.shape, dtype=logits.dtype, device=dev) if fuse else None
         scratch = _token_scratch(rows, 0, dev)
         nll = torch.empty((B,), dtype=logits.dtype, device=dev)
-        loss = elbo = means = ws = None
+        loss = elbo = means = first = ws = None
         if with_elbo:
-            loss, elbo, means, ws = torch.empty_like(nll), torch.empty_like(nll), _scalars(6, dev, B), workspace(dev)
-        with _Guard(dev):
-            if fuse:
-                call('vae_token_nll_fused', ptr(rows), rows.stride(0), ptr(tokens), tokens.element_size(), ptr(logp),
-                     ptr(stats), ptr(grad), inv_count, ptr(scratch), N, V, code, st)
-            else:
-                call('vae_token_logp_fwd', ptr(rows), rows.stride(0), ptr(tokens), tokens.element_size(), ptr(logp),
-                     None, ptr(stats), None, None, 0, ptr(scratch), N, V, code, st)
-            call('vae_token_elbo_fwd', ptr(logp), N // max(B, 1), ptr(kld), ptr(add), ptr(mi), kl_beta, inv_count,
-                 ptr(nll), ptr(loss), ptr(elbo), ptr(means), ptr(ws), B, code, st)
+            loss, elbo, means, ws = torch.empty_like(nll), torch.empty_like(nll), _scalars(MEANS, dev, B), workspace(dev)
+            first = torch.empty((), dtype=mean_dtype, device=dev) if B else torch.zeros((), dtype=mean_dtype, device=dev)
+        if fuse:
+            launch(dev, 'vae_token_nll_fused', ptr(rows), rows.stride(0), ptr(tokens), tokens.element_size(), ptr(logp),
+                   ptr(stats), ptr(grad), inv_count, ptr(scratch), N, V, code)
+        else:
+            launch(dev, 'vae_token_logp_fwd', ptr(rows), rows.stride(0), ptr(tokens), tokens.element_size(), ptr(logp),
+                   None, ptr(stats), None, None, 0, ptr(scratch), N, V, code)
+        launch(dev, 'vae_token_elbo_fwd', ptr(logp), N // max(B, 1), ptr(kld), ptr(add), ptr(mi), kl_beta, inv_count,
+               ptr(nll), ptr(loss), ptr(elbo), ptr(means), ptr(first), _lib.DTYPE_CODES[mean_dtype], ptr(ws), B, code)
         ctx.save_for_backward(logits, tokens, stats)
         ctx.grad = grad
         ctx.cfg = (kl_beta, inv_count, kld is not None, add is not None, mi is not None, mean_dtype)
         if not with_elbo:
             return (nll,) + (None,) * 8
-        return (nll, loss, elbo) + means.to(mean_dtype).unbind(0)
+        # the loss mean is a tensor of its own (a caller may scale it in place), the other five are views of one
+        return (nll, loss, elbo, first) + means[1:6].to(mean_dtype).unbind(0)
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, gnll, gloss, gelbo, *gmeans):
         logits, tokens, stats = ctx.saved_tensors
         kl_beta, inv_count, has_kld, has_add, has_mi, mean_dtype = ctx.cfg
@@ -693,10 +696,9 @@ class _TokenNllElbo(torch.autograd.Function):
         grow = None if stored else torch.empty((B,), dtype=torch.float32, device=dev)
         gnll, gloss, gelbo = _dense(gnll), _dense(gloss), _dense(gelbo)
         at = (ctypes.c_void_p * 6)(*[None if g is None else g.data_ptr() for g in gmeans])
-        with _Guard(dev):
-            call('vae_token_elbo_bwd', ptr(gnll), ptr(gloss), ptr(gelbo), at, _lib.DTYPE_CODES[mean_dtype], kl_beta,
-                 inv_count, ptr(grow), ptr(grad) if stored else None, grad.numel() if stored else 0, ptr(terms[0]),
-                 ptr(terms[1]), ptr(terms[2]), B, dtype_code(logits), stream_ptr(dev))
+        launch(dev, 'vae_token_elbo_bwd', ptr(gnll), ptr(gloss), ptr(gelbo), at, _lib.DTYPE_CODES[mean_dtype], kl_beta,
+               inv_count, ptr(grow), ptr(grad) if stored else None, grad.numel() if stored else 0, ptr(terms[0]),
+               ptr(terms[1]), ptr(terms[2]), B, dtype_code(logits))
         if not stored:
             grad = None
             if need[0]:
@@ -756,6 +758,7 @@ class _Distill(torch.autograd.Function):
         return kl, mean
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, gkl, gmean):
         if gkl is None and gmean is None:
             return (None,) * 6
@@ -764,14 +767,13 @@ class _Distill(torch.autograd.Function):
         dev = logits.device
         grad, ctx.grad = ctx.grad, None
         gkl, gmean = _dense(gkl), _dense(gmean)
-        with _Guard(dev):
-            if gkl is None and grad is not None:
-                call('vae_grad_scale', ptr(grad), ptr(gmean), grad.numel(), dtype_code(grad), stream_ptr(dev))
-            else:
-                rows = _rows(logits)
-                grad = torch.empty(logits.shape, dtype=logits.dtype, device=dev)
-                call('vae_distill_bwd', ptr(rows), rows.stride(0), ptr(teacher), K, temperature, ptr(stats), ptr(gkl),
-                     ptr(gmean), inv_count, ptr(grad), rows.shape[0], rows.shape[1], dtype_code(rows), stream_ptr(dev))
+        if gkl is None and grad is not None:
+            launch(dev, 'vae_grad_scale', ptr(grad), ptr(gmean), grad.numel(), dtype_code(grad))
+        else:
+            rows = _rows(logits)
+            grad = torch.empty(logits.shape, dtype=logits.dtype, device=dev)
+            launch(dev, 'vae_distill_bwd', ptr(rows), rows.stride(0), ptr(teacher), K, temperature, ptr(stats), ptr(gkl),
+                   ptr(gmean), inv_count, ptr(grad), rows.shape[0], rows.shape[1], dtype_code(rows))
         return grad, None, None, None, None, None
 
 
@@ -784,13 +786,11 @@ def _distill_fwd(logits, t_logits, t_ids, temperature, inv_count, want_stats, fu
     grad = torch.empty(logits.shape, dtype=logits.dtype, device=dev) if fuse else None
     teacher = torch.empty((N, 1 + 3 * K), dtype=torch.float32, device=dev)   # vae_distill_teacher_floats
     scratch = _token_scratch(rows, 0, dev)
-    st = stream_ptr(dev)
-    with _Guard(dev):
-        call('vae_distill_teacher', ptr(t_logits), t_logits.stride(0), dtype_code(t_logits), ptr(t_ids), t_ids.stride(0),
-             t_ids.element_size(), K, temperature, ptr(teacher), N, V, st)
-        call('vae_distill_fwd', ptr(rows), rows.stride(0), ptr(teacher), K, temperature, ptr(kl), ptr(stats), ptr(grad),
-             inv_count, ptr(scratch), N, V, dtype_code(rows), st)
-        mean = _row_sums(kl, inv_count, (), torch.float32)
+    launch(dev, 'vae_distill_teacher', ptr(t_logits), t_logits.stride(0), dtype_code(t_logits), ptr(t_ids),
+           t_ids.stride(0), t_ids.element_size(), K, temperature, ptr(teacher), N, V)
+    launch(dev, 'vae_distill_fwd', ptr(rows), rows.stride(0), ptr(teacher), K, temperature, ptr(kl), ptr(stats),
+           ptr(grad), inv_count, ptr(scratch), N, V, dtype_code(rows))
+    mean = _row_sums(kl, inv_count, (), torch.float32)
     return kl, mean, stats, grad, teacher
 
 
@@ -801,9 +801,10 @@ def distill_top_logits(logits, teacher_logits, teacher_ids, temperature=1.0, inv
     mean = inv_count * sum(kl), inv_count = 1 / rows unless given (1 / unpadded rows, times temperature^2 where the
     loss is to be weighted so).  Differentiable with respect to `logits` only.
 
-    A negative id or a teacher logit of -inf is no entry; a row without entries has kl 0 and gradient 0 and its
-    logits are not read; an id may come twice; an id beyond the vocabulary gives NaN.  `fuse_backward`: d(mean)/d(logits) is formed by
-    the forward launch (one read of the logits per step instead of two); a gradient on `kl` takes the general kernel."""
+    A negative id or a teacher logit of -inf is no entry; a row without entries has kl 0 and gradient 0 and its logits
+    are not read; an id may come twice; an id beyond the vocabulary gives NaN.  `fuse_backward`: d(mean)/d(logits) is
+    formed by the forward launch (one read of the logits per step instead of two); a gradient on `kl` takes the general
+    kernel."""
     _check_vocab(logits, 'distill_top_logits')
     _id_bytes(teacher_ids, 'distill_top_logits')
     if teacher_logits.shape != teacher_ids.shape or teacher_ids.dim() < 1 or teacher_ids.shape[:-1] != logits.shape[:-1]:
@@ -831,10 +832,10 @@ class _SampleSums(torch.autograd.Function):
     def forward(ctx, rows, B, dtype):
         dev = check_device(rows)
         ctx.n = rows.numel()
-        with _Guard(dev):
-            return _row_sums(rows, 1.0, (B,), dtype)
+        return _row_sums(rows, 1.0, (B,), dtype)
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, g):
         B = g.shape[0]
         return g.float()[:, None].expand(B, ctx.n // max(B, 1)).reshape(-1), None, None
