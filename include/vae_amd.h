@@ -493,26 +493,26 @@ int vae_token_logp_bwd(const void* logits, int64_t row_stride, const void* token
                        const float* entropy, const float* glogp, int64_t rows_per_g, float g_scale,
                        const float* gentropy, const float* gtop, const int64_t* top_ids, int64_t top_k, void* glogits,
                        int64_t N, int64_t V, int dtype, vae_stream_t stream);
-/* logp and stats as above together with glogits = grad_scale * d(-logp) / d logits, the training step's form.      */
-int vae_token_nll_fused(const void* logits, int64_t row_stride, const void* tokens, int token_bytes, float* logp,
-                        float* stats, void* glogits, float grad_scale, void* scratch, int64_t N, int64_t V, int dtype,
-                        vae_stream_t stream);
-/* The loss of B samples of T tokens each, from logp [B * T]: nll[b] = -sum_t logp[b T + t] (in double, in a fixed
- * order), loss / elbo / means as vae_elbo_combine_fwd (abstract_vae.py:356-388) but from the unrounded nll, each
- * rounded once; loss == elbo == NULL: nll alone.  means: VAE_TOKEN_MEANS_FLOATS floats, the six means in front, the rest
- * scratch; loss_mean (mean_dtype; may be NULL): the first of them once more, in a place of its own.  workspace (may be
- * NULL): its saw-a-NaN word alone is used.                                                                         */
+/* The categorical likelihood of B samples of T tokens each (logits [B T, V], tokens [B T]) with the ELBO combine:
+ * logp [B T] and stats [B T, 2] as above, nll[b] = -sum_t logp[b T + t] (in double, in a fixed order), loss / elbo / means
+ * as vae_elbo_combine_fwd (abstract_vae.py:356-388) but from the unrounded nll, each rounded once.  loss == elbo == NULL:
+ * nll alone; nll may be NULL otherwise.  glogits [B T, V] != NULL: also d(loss mean) / d logits, inv_count its 1/B: the
+ * training step's one read of the logits.  means: VAE_TOKEN_MEANS_FLOATS floats, the six means in front, the rest scratch;
+ * loss_mean (mean_dtype; may be NULL): the first of them once more, in a place of its own.  workspace (may be NULL): its
+ * saw-a-NaN word alone is used.                                                                                     */
 #define VAE_TOKEN_MEANS_FLOATS (6 + 6 * 256)
-int vae_token_elbo_fwd(const float* logp, int64_t T, const void* kld, const void* add, const void* mi, float kl_beta,
-                       float inv_count, void* nll, void* loss, void* elbo, float* means, void* loss_mean,
-                       int mean_dtype, float* workspace, int64_t B, int dtype, vae_stream_t stream);
+int vae_token_nll_elbo_fwd(const void* logits, int64_t row_stride, const void* tokens, int token_bytes, int64_t T,
+                           const void* kld, const void* add, const void* mi, float kl_beta, float inv_count, float* logp,
+                           float* stats, void* glogits, void* nll, void* loss, void* elbo, float* means, void* loss_mean,
+                           int mean_dtype, float* workspace, void* scratch, int64_t B, int64_t V, int dtype,
+                           vae_stream_t stream);
 /* Its backward.  gnll / gloss / gelbo [B] (dtype) and gmeans, a HOST array of 6 device pointers to one value each
  * (gmeans_dtype): every one may be NULL.  grow [B] (float32) = d / d nll[b], what vae_token_logp_bwd takes with
- * rows_per_g = T and g_scale = -1; or grad [n] = a stored d(loss_mean) / d logits (vae_token_nll_fused), multiplied by
+ * rows_per_g = T and g_scale = -1; or grad [n] = the forward's glogits, multiplied by
  * the mean gradients' sum where that is not 1 (gnll, gloss and gelbo NULL).  gkld / gadd / gmi [B] (dtype) or NULL.  */
-int vae_token_elbo_bwd(const void* gnll, const void* gloss, const void* gelbo, const void* const* gmeans,
-                       int gmeans_dtype, float kl_beta, float inv_count, float* grow, void* grad, int64_t n, void* gkld,
-                       void* gadd, void* gmi, int64_t B, int dtype, vae_stream_t stream);
+int vae_token_nll_elbo_bwd(const void* gnll, const void* gloss, const void* gelbo, const void* const* gmeans,
+                           int gmeans_dtype, float kl_beta, float inv_count, float* grow, void* grad, int64_t n,
+                           void* gkld, void* gadd, void* gmi, int64_t B, int dtype, vae_stream_t stream);
 /* out[b] (dtype) = scale * sum of rows[b T .. b T + T), summed in double in a fixed order.                         */
 int vae_row_sums(const float* rows, float scale, void* out, int64_t B, int64_t T, int dtype, vae_stream_t stream);
 /* buf[n] *= *factor (a device float); returns without touching buf when it is 1.                                   */
@@ -521,18 +521,17 @@ int vae_grad_scale(void* buf, const float* factor, int64_t n, int dtype, vae_str
  * q = softmax(t_logits / temperature) over the entries that are there (id >= 0 and logit > -inf), p = softmax(logits /
  * temperature) over V,  kl[r] = sum_k q_k (ln q_k - ln p[id_k]).  An id may come more than once.  No entry there: kl 0,
  * gradient 0, the row's logits are not read.  An id >= V: NaN, nothing is read out of range.
- * vae_distill_teacher prepares the teacher's side, vae_distill_teacher_floats(N, K) floats that the calls below read
- * (one preparation serves forward and backward): t_logits [N, K] in t_dtype, t_ids, rows t_stride / id_stride apart.  */
+ * t_logits [N, K] in t_dtype and t_ids [N, K], rows t_stride / id_stride apart.  teacher: vae_distill_teacher_floats(N, K)
+ * floats that the call fills (the teacher's softmax, each id once) and the backward reads.  mean (may be NULL):
+ * mean_scale * sum of kl.  stats [N, 2] for the backward (may be NULL without glogits); glogits [N, V] != NULL: also
+ * mean_scale * d kl / d logits, the training step's one read of the logits.  scratch: vae_token_scratch_bytes(N, V, 0,
+ * dtype).                                                                                                          */
 #define VAE_MAX_TEACHER 256
 size_t vae_distill_teacher_floats(int64_t N, int64_t K);
-int vae_distill_teacher(const void* t_logits, int64_t t_stride, int t_dtype, const void* t_ids, int64_t id_stride,
-                        int id_bytes, int64_t K, float temperature, float* teacher, int64_t N, int64_t V,
-                        vae_stream_t stream);
-/* kl [N] and stats [N, 2] for the backward (may be NULL without glogits); glogits != NULL: also grad_scale * d kl /
- * d logits.  scratch: vae_token_scratch_bytes(N, V, 0, dtype).                                                     */
-int vae_distill_fwd(const void* logits, int64_t row_stride, const float* teacher, int64_t K, float temperature,
-                    float* kl, float* stats, void* glogits, float grad_scale, void* scratch, int64_t N, int64_t V,
-                    int dtype, vae_stream_t stream);
+int vae_distill_fwd(const void* logits, int64_t row_stride, const void* t_logits, int64_t t_stride, int t_dtype,
+                    const void* t_ids, int64_t id_stride, int id_bytes, int64_t K, float temperature, float* teacher,
+                    float* kl, float* mean, float mean_scale, float* stats, void* glogits, void* scratch, int64_t N,
+                    int64_t V, int dtype, vae_stream_t stream);
 /* glogits[r] = (gkl[r] + *gmean * mean_scale) * d kl[r] / d logits[r]; gkl [N], gmean (one float): each may be NULL
  * (both NULL: mean_scale on every row).                                                                          */
 int vae_distill_bwd(const void* logits, int64_t row_stride, const float* teacher, int64_t K, float temperature,

@@ -81,18 +81,22 @@ def bwd(**kw):
 
 
 def fused(**kw):
-    a = dict(logits=P, stride=10, tokens=P, tb=8, logp=P, stats=P, out=P, scale=1.0, scratch=P, N=2, V=10,
-             dtype=0)
+    a = dict(logits=P, stride=10, tokens=P, tb=8, T=1, kld=None, add=None, mi=None, beta=1.0, inv=1.0, logp=P, stats=P,
+             out=P, nll=P, loss=P, elbo=P, means=P, first=P, md=0, ws=P, scratch=P, N=2, V=10, dtype=0)
     a.update(kw)
-    return _call('vae_token_nll_fused', [a[n] for n in ('logits', 'stride', 'tokens', 'tb', 'logp', 'stats', 'out',
-                                                        'scale', 'scratch', 'N', 'V', 'dtype')] + [None])
+    return _call('vae_token_nll_elbo_fwd',
+                 [a[n] for n in ('logits', 'stride', 'tokens', 'tb', 'T', 'kld', 'add', 'mi', 'beta', 'inv', 'logp', 'stats',
+                                 'out', 'nll', 'loss', 'elbo', 'means', 'first', 'md', 'ws', 'scratch', 'N', 'V', 'dtype')]
+                 + [None])
 
 
 def dfwd(**kw):
-    a = dict(logits=P, stride=10, t=P, K=2, tau=1.0, kl=P, stats=P, out=P, scale=1.0, scratch=P, N=2, V=10, dtype=0)
+    a = dict(logits=P, stride=10, y=P, ys=2, yt=0, ids=P, ids_s=2, ib=8, K=2, tau=1.0, t=P, kl=P, mean=None, scale=1.0,
+             stats=P, out=P, scratch=P, N=2, V=10, dtype=0)
     a.update(kw)
-    return _call('vae_distill_fwd', [a[n] for n in ('logits', 'stride', 't', 'K', 'tau', 'kl', 'stats', 'out', 'scale',
-                                                    'scratch', 'N', 'V', 'dtype')] + [None])
+    return _call('vae_distill_fwd', [a[n] for n in ('logits', 'stride', 'y', 'ys', 'yt', 'ids', 'ids_s', 'ib', 'K', 'tau',
+                                                    't', 'kl', 'mean', 'scale', 'stats', 'out', 'scratch', 'N', 'V',
+                                                    'dtype')] + [None])
 
 
 def dbwd(**kw):
@@ -100,13 +104,6 @@ def dbwd(**kw):
     a.update(kw)
     return _call('vae_distill_bwd', [a[n] for n in ('logits', 'stride', 't', 'K', 'tau', 'stats', 'gkl', 'gm', 'scale',
                                                     'out', 'N', 'V', 'dtype')] + [None])
-
-
-def teach(**kw):
-    a = dict(y=P, ys=2, yt=0, ids=P, ids_s=2, ib=8, K=2, tau=1.0, t=P, N=2, V=10)
-    a.update(kw)
-    return _call('vae_distill_teacher', [a[n] for n in ('y', 'ys', 'yt', 'ids', 'ids_s', 'ib', 'K', 'tau', 't', 'N', 'V')]
-                 + [None])
 
 
 BAD = [dict(N=-1), dict(V=0), dict(V=(1 << 24) + 1, stride=1 << 25), dict(stride=9), dict(dtype=3), dict(logits=None)]
@@ -120,25 +117,25 @@ def test_c_entry_points_refuse_bad_shapes(f, bad):
 
 @pytest.mark.parametrize('f,bad', [
     (fwd, dict(k=-1)), (fwd, dict(k=65, V=100, stride=100)), (fwd, dict(k=11)), (fwd, dict(tb=2)),
-    (fwd, dict(scratch=None, V=65536, stride=65536)), (dfwd, dict(out=None, scratch=None, V=65536, stride=65536)),
+    (fwd, dict(scratch=None, V=65536, stride=65536)), (dfwd, dict(scratch=None, V=65536, stride=65536)),
     (fused, dict(scratch=None, V=65536, stride=65536)), (fwd, dict(tokens=None)), (fwd, dict(top=None)), (fwd, dict(ids=None)),
     (bwd, dict(k=65)), (bwd, dict(k=-1)), (bwd, dict(per=0)), (bwd, dict(stats=None)), (bwd, dict(out=None)),
     (bwd, dict(tb=1)), (bwd, dict(ent=None)), (bwd, dict(gtop=None)), (bwd, dict(ids=None)), (bwd, dict(tokens=None)),
-    (fused, dict(tokens=None)), (fused, dict(logp=None)), (fused, dict(stats=None)), (fused, dict(out=None)),
+    (fused, dict(tokens=None)), (fused, dict(logp=None)), (fused, dict(stats=None)),
     (fused, dict(tb=0)),
     (dfwd, dict(K=0)), (dfwd, dict(K=257)), (dfwd, dict(tau=0.0)), (dfwd, dict(tau=float('nan'))),
     (dfwd, dict(tau=float('inf'))), (dfwd, dict(t=None)), (dfwd, dict(kl=None)), (dfwd, dict(stats=None)),
     (dbwd, dict(K=0)), (dbwd, dict(tau=-1.0)), (dbwd, dict(stats=None)), (dbwd, dict(out=None)), (dbwd, dict(t=None)),
-    (teach, dict(K=0)), (teach, dict(K=257, ys=300, ids_s=300)), (teach, dict(ys=1)), (teach, dict(ids_s=1)),
-    (teach, dict(ib=2)), (teach, dict(yt=9)), (teach, dict(tau=0.0)), (teach, dict(tau=float('nan'))),
-    (teach, dict(tau=float('inf'))), (teach, dict(y=None)), (teach, dict(ids=None)), (teach, dict(t=None)),
-    (teach, dict(N=-1)), (teach, dict(V=0)),
+    (dfwd, dict(K=257, ys=300, ids_s=300)), (dfwd, dict(ys=1)), (dfwd, dict(ids_s=1)), (dfwd, dict(ib=2)),
+    (dfwd, dict(yt=9)), (dfwd, dict(y=None)), (dfwd, dict(ids=None)),
+    (fused, dict(T=-1)), (fused, dict(md=4)), (fused, dict(loss=None)), (fused, dict(elbo=None)),
+    (fused, dict(means=None)), (fused, dict(loss=None, elbo=None, nll=None)),
 ])
 def test_c_entry_points_refuse_bad_arguments(f, bad):
     assert f(**bad) == _lib.VAE_ERR_ARG
 
 
-@pytest.mark.parametrize('f', [fwd, bwd, fused, dfwd, dbwd, teach])
+@pytest.mark.parametrize('f', [fwd, bwd, fused, dfwd, dbwd])
 def test_no_rows_is_fine(f):
     assert f(N=0) == _lib.VAE_OK
 
@@ -167,15 +164,8 @@ def test_sums_and_scale_refusals():
     assert _call('vae_grad_scale', [None, None, 0, 0, None]) == _lib.VAE_OK
 
 
-def test_loss_closing_refusals():
-    f, b = 'vae_token_elbo_fwd', 'vae_token_elbo_bwd'
-    ok = [P, 3, None, None, None, 1.0, 1.0, P, P, P, P, P, 0, P, 0, 0, None]     # no samples: nothing is launched
-    assert _call(f, ok) == _lib.VAE_OK
-    for i, v in ((14, -1), (1, -1), (15, 5), (12, 4)):
-        assert _call(f, ok[:i] + [v] + ok[i + 1:]) == _lib.VAE_ERR_ARG
-    some = ok[:14] + [2] + ok[15:]
-    for i in (0, 7, 8, 9, 10):
-        assert _call(f, some[:i] + [None] + some[i + 1:]) == _lib.VAE_ERR_ARG
+def test_loss_backward_refusals():
+    b = 'vae_token_nll_elbo_bwd'
     ok = [None, None, None, None, 0, 1.0, 1.0, P, None, 0, None, None, None, 0, 0, None]
     assert _call(b, ok) == _lib.VAE_OK
     for i, v in ((13, -1), (9, -1), (14, 3), (4, 3)):

@@ -43,7 +43,7 @@ __global__ __launch_bounds__(kBlock) void token_elbo_fwd_kernel(
     for (int o = G >> 1; o >= 1; o >>= 1) v += __shfl_xor(v, o, 64);
     if (sub != 0 || b >= B) continue;
     const float n = (float)-v;          // loss and elbo from the unrounded sum: every output is rounded once
-    nll[b] = from_f32<T>(n);
+    if (nll) nll[b] = from_f32<T>(n);
     if (!loss) continue;
     const float k = kld ? to_f32(kld[b]) : 0.f;
     const float ad = add ? to_f32(add[b]) : 0.f;
@@ -152,17 +152,33 @@ using namespace vae;
 
 extern "C" {
 
-int vae_token_elbo_fwd(const float* logp, int64_t len, const void* kld, const void* add, const void* mi, float kl_beta,
-                       float inv_count, void* nll, void* loss, void* elbo, float* means, void* loss_mean,
-                       int mean_dtype, float* workspace, int64_t B, int dtype, vae_stream_t stream) {
-  if (B < 0 || len < 0 || !type_ok(dtype) || (loss_mean && !type_ok(mean_dtype))) return VAE_ERR_ARG;
+int vae_token_nll_elbo_fwd(const void* logits, int64_t row_stride, const void* tokens, int token_bytes, int64_t len,
+                           const void* kld, const void* add, const void* mi, float kl_beta, float inv_count, float* logp,
+                           float* stats, void* glogits, void* nll, void* loss, void* elbo, float* means, void* loss_mean,
+                           int mean_dtype, float* workspace, void* scratch, int64_t B, int64_t V, int dtype,
+                           vae_stream_t stream) {
+  if (B < 0 || len < 0 || V < 1 || V > VAE_MAX_ROW || (B * len > 1 && row_stride < V) || !type_ok(dtype) ||
+      (loss_mean && !type_ok(mean_dtype)))
+    return VAE_ERR_ARG;
   if (B == 0) return VAE_OK;
-  if (!nll || (len > 0 && !logp) || (loss == nullptr) != (elbo == nullptr) || (loss && !means)) return VAE_ERR_ARG;
+  const int64_t N = B * len;
+  if ((loss == nullptr) != (elbo == nullptr) || (!nll && !loss) || (loss && !means)) return VAE_ERR_ARG;
+  if (N > 0 && (!logits || !tokens || (token_bytes != 4 && token_bytes != 8) || !logp || !stats ||
+                (vae_token_scratch_bytes(N, V, 0, dtype) && !scratch)))
+    return VAE_ERR_ARG;
+  int rc = VAE_OK;
+  if (N > 0)
+    rc = glogits ? token_nll_grad(logits, row_stride, tokens, token_bytes, logp, stats, glogits, inv_count, scratch, N, V,
+                                  dtype, (hipStream_t)stream)
+                 : vae_token_logp_fwd(logits, row_stride, tokens, token_bytes, logp, nullptr, stats, nullptr, nullptr, 0,
+                                      scratch, N, V, dtype, stream);
+  if (rc != VAE_OK) return rc;
   int G = 1;
   while (G < 64 && G < len) G <<= 1;
   const int64_t blocks = (B + kBlock / G - 1) / (kBlock / G);
   // without the means nothing is left to add up: as many blocks as there are samples for
-  const int grid = (int)(blocks < (loss ? kElboBlocks : kMaxGrid) ? blocks : (loss ? kElboBlocks : kMaxGrid));
+  const int64_t most = loss ? kElboBlocks : kMaxGrid;
+  const int grid = (int)(blocks < most ? blocks : most);
   VAE_BY_TYPE(dtype, hipLaunchKernelGGL((token_elbo_fwd_kernel<T>), dim3(grid), dim3(kBlock), 0, (hipStream_t)stream,
                                         logp, len, (const T*)kld, (const T*)add, (const T*)mi, kl_beta, inv_count,
                                         (T*)nll, (T*)loss, (T*)elbo, means, loss_mean, mean_dtype, workspace, B, G));
@@ -172,9 +188,9 @@ int vae_token_elbo_fwd(const float* logp, int64_t len, const void* kld, const vo
   return launched();
 }
 
-int vae_token_elbo_bwd(const void* gnll, const void* gloss, const void* gelbo, const void* const* gmeans,
-                       int gmeans_dtype, float kl_beta, float inv_count, float* grow, void* grad, int64_t n, void* gkld,
-                       void* gadd, void* gmi, int64_t B, int dtype, vae_stream_t stream) {
+int vae_token_nll_elbo_bwd(const void* gnll, const void* gloss, const void* gelbo, const void* const* gmeans,
+                           int gmeans_dtype, float kl_beta, float inv_count, float* grow, void* grad, int64_t n,
+                           void* gkld, void* gadd, void* gmi, int64_t B, int dtype, vae_stream_t stream) {
   if (B < 0 || n < 0 || !type_ok(dtype) || !type_ok(gmeans_dtype)) return VAE_ERR_ARG;
   if (grad && (gnll || gloss || gelbo)) return VAE_ERR_ARG;
   if (B == 0 && (n == 0 || !grad)) return VAE_OK;
@@ -195,8 +211,8 @@ int vae_grad_scale(void* buf, const float* factor, int64_t n, int dtype, vae_str
   if (n == 0) return type_ok(dtype) ? VAE_OK : VAE_ERR_ARG;
   if (!buf || !factor) return VAE_ERR_ARG;
   const void* g[6] = {factor, nullptr, nullptr, nullptr, nullptr, nullptr};
-  return vae_token_elbo_bwd(nullptr, nullptr, nullptr, g, VAE_F32, 0.f, 0.f, nullptr, buf, n, nullptr, nullptr, nullptr, 0,
-                            dtype, stream);
+  return vae_token_nll_elbo_bwd(nullptr, nullptr, nullptr, g, VAE_F32, 0.f, 0.f, nullptr, buf, n, nullptr, nullptr,
+                                nullptr, 0, dtype, stream);
 }
 
 int vae_row_sums(const float* rows, float scale, void* out, int64_t B, int64_t len, int dtype, vae_stream_t stream) {

@@ -1,6 +1,5 @@
 // Gradients with respect to rows of logits [N, V]: of log probs, entropy and alternatives (token_logp_bwd), of the
-// distillation KL (distill_bwd), and both losses together with their gradient in one pass (token_nll_fused,
-// distill_fwd with glogits).  Formulas and the conventions for masks: token_row.hpp.
+// distillation KL (distill_bwd), and both losses together with their gradient in one pass (token_fused_kernel).  Formulas and the conventions for masks: token_row.hpp.
 //
 // Every one of them is   g_j = e_j (A + B d_j) + sum over a few entries (id, g) with id = j,   d = (x - m) c, e = 2^d:
 //   tokens:   A = -(sum_i g_i + g_H (H - ln s)) / s,  B = -g_H ln2 / s,  entries: the token and the alternatives
@@ -452,6 +451,25 @@ static void set_temperature(GradArgs& a, float temperature) {
   a.inv_tau = (float)(1.0 / (double)temperature);
 }
 
+int token_nll_grad(const void* logits, int64_t row_stride, const void* tokens, int token_bytes, float* logp, float* stats,
+                   void* glogits, float grad_scale, void* scratch, int64_t N, int64_t V, int dtype,
+                   hipStream_t stream) {
+  int rc = VAE_ERR_ARG;
+  ShortArgs sa = {logits, row_stride, tokens, token_bytes, N, (int)V, logp, nullptr, stats, nullptr, nullptr, 0,
+                  glogits, nullptr, 1, -grad_scale, nullptr, nullptr, nullptr, 0};
+  if (short_rows(sa, dtype, stream, &rc)) return rc;
+  GradArgs a = {};
+  a.logits = logits; a.row_stride = row_stride; a.glogits = glogits; a.N = N; a.V = (int)V;
+  a.scale2 = kLog2e; a.inv_tau = 1.0f;
+  a.tokens = tokens; a.token_bytes = token_bytes; a.g_scale = grad_scale; a.out = logp; a.stats_out = stats;
+  VAE_BY_TYPE(dtype, if (fused_type<T, false>(a, stream, &rc)) return rc);
+  rc = vae_token_logp_fwd(logits, row_stride, tokens, token_bytes, logp, nullptr, stats, nullptr, nullptr, 0, scratch, N,
+                          V, dtype, stream);
+  if (rc != VAE_OK) return rc;
+  return vae_token_logp_bwd(logits, row_stride, tokens, token_bytes, stats, nullptr, nullptr, 1, -grad_scale, nullptr,
+                            nullptr, nullptr, 0, glogits, N, V, dtype, stream);
+}
+
 }  // namespace vae
 
 using namespace vae;
@@ -479,28 +497,6 @@ int vae_token_logp_bwd(const void* logits, int64_t row_stride, const void* token
   return VAE_ERR_ARG;
 }
 
-int vae_token_nll_fused(const void* logits, int64_t row_stride, const void* tokens, int token_bytes, float* logp,
-                        float* stats, void* glogits, float grad_scale, void* scratch, int64_t N, int64_t V, int dtype,
-                        vae_stream_t stream) {
-  if (bad_rows(N, V, row_stride, dtype)) return VAE_ERR_ARG;
-  if (N == 0) return VAE_OK;
-  if (!logits || !tokens || !logp || !stats || !glogits || (token_bytes != 4 && token_bytes != 8)) return VAE_ERR_ARG;
-  int rc = VAE_ERR_ARG;
-  ShortArgs sa = {logits, row_stride, tokens, token_bytes, N, (int)V, logp, nullptr, stats, nullptr, nullptr, 0,
-                  glogits, nullptr, 1, -grad_scale, nullptr, nullptr, nullptr, 0};
-  if (short_rows(sa, dtype, (hipStream_t)stream, &rc)) return rc;
-  GradArgs a = {};
-  a.logits = logits; a.row_stride = row_stride; a.glogits = glogits; a.N = N; a.V = (int)V;
-  a.scale2 = kLog2e; a.inv_tau = 1.0f;
-  a.tokens = tokens; a.token_bytes = token_bytes; a.g_scale = grad_scale; a.out = logp; a.stats_out = stats;
-  VAE_BY_TYPE(dtype, if (fused_type<T, false>(a, (hipStream_t)stream, &rc)) return rc);
-  rc = vae_token_logp_fwd(logits, row_stride, tokens, token_bytes, logp, nullptr, stats, nullptr, nullptr, 0, scratch, N,
-                          V, dtype, stream);
-  if (rc != VAE_OK) return rc;
-  return vae_token_logp_bwd(logits, row_stride, tokens, token_bytes, stats, nullptr, nullptr, 1, -grad_scale, nullptr,
-                            nullptr, nullptr, 0, glogits, N, V, dtype, stream);
-}
-
 int vae_distill_bwd(const void* logits, int64_t row_stride, const float* teacher, int64_t K, float temperature,
                     const float* stats, const float* gkl, const float* gmean, float mean_scale, void* glogits,
                     int64_t N, int64_t V, int dtype, vae_stream_t stream) {
@@ -516,26 +512,36 @@ int vae_distill_bwd(const void* logits, int64_t row_stride, const float* teacher
   return VAE_ERR_ARG;
 }
 
-int vae_distill_fwd(const void* logits, int64_t row_stride, const float* teacher, int64_t K, float temperature,
-                    float* kl, float* stats, void* glogits, float grad_scale, void* scratch, int64_t N, int64_t V,
-                    int dtype, vae_stream_t stream) {
-  if (bad_rows(N, V, row_stride, dtype) || bad_teacher(K, temperature)) return VAE_ERR_ARG;
-  if (N == 0) return VAE_OK;
-  if (!logits || !teacher || !kl || (glogits && !stats)) return VAE_ERR_ARG;
+int vae_distill_fwd(const void* logits, int64_t row_stride, const void* t_logits, int64_t t_stride, int t_dtype,
+                    const void* t_ids, int64_t id_stride, int id_bytes, int64_t K, float temperature, float* teacher,
+                    float* kl, float* mean, float mean_scale, float* stats, void* glogits, void* scratch, int64_t N,
+                    int64_t V, int dtype, vae_stream_t stream) {
+  if (bad_rows(N, V, row_stride, dtype) || bad_teacher(K, temperature) || !type_ok(t_dtype) ||
+      (id_bytes != 4 && id_bytes != 8) || (N > 1 && (t_stride < K || id_stride < K)))
+    return VAE_ERR_ARG;
+  if (N == 0) return mean ? vae_row_sums(nullptr, mean_scale, mean, 1, 0, VAE_F32, stream) : VAE_OK;
+  if (!logits || !t_logits || !t_ids || !teacher || !kl || (glogits && !stats)) return VAE_ERR_ARG;
+  hipStream_t st = (hipStream_t)stream;
+  if (vae_token_scratch_bytes(N, V, 0, dtype) && !scratch) return VAE_ERR_ARG;
+  int rc = prepare_teacher(t_logits, t_stride, t_dtype, t_ids, id_stride, id_bytes, K, temperature, teacher, N, V, st);
+  if (rc != VAE_OK) return rc;
   GradArgs a = {};
   a.teacher = teacher_of(teacher, N, K);
+  bool done = false;
   if (glogits) {
     a.logits = logits; a.row_stride = row_stride; a.glogits = glogits; a.N = N; a.V = (int)V;
-    a.mean_scale = grad_scale; a.out = kl; a.stats_out = stats;
+    a.mean_scale = mean_scale; a.out = kl; a.stats_out = stats;
     set_temperature(a, temperature);
-    int rc = VAE_ERR_ARG;
-    VAE_BY_TYPE(dtype, if (fused_type<T, true>(a, (hipStream_t)stream, &rc)) return rc);
+    VAE_BY_TYPE(dtype, done = fused_type<T, true>(a, st, &rc));
   }
-  const int rc = distill_stats(logits, row_stride, a.teacher, temperature, kl, stats, scratch, N, V, dtype,
-                               (hipStream_t)stream);
-  if (rc != VAE_OK || !glogits) return rc;
-  return vae_distill_bwd(logits, row_stride, teacher, K, temperature, stats, nullptr, nullptr, grad_scale, glogits, N, V,
-                         dtype, stream);
+  if (!done) {
+    rc = distill_stats(logits, row_stride, a.teacher, temperature, kl, stats, scratch, N, V, dtype, st);
+    if (rc == VAE_OK && glogits)
+      rc = vae_distill_bwd(logits, row_stride, teacher, K, temperature, stats, nullptr, nullptr, mean_scale, glogits, N,
+                           V, dtype, stream);
+  }
+  if (rc != VAE_OK || !mean) return rc;
+  return vae_row_sums(kl, mean_scale, mean, 1, N, VAE_F32, stream);
 }
 
 }  // extern "C"

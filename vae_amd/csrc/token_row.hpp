@@ -208,7 +208,7 @@ __device__ __forceinline__ float vec_max(const float (&v)[VN], float m) {
   return m;
 }
 
-// The teacher's entries as vae_distill_teacher (token_teacher.hip) leaves them: per row a state, and K entries of
+// The teacher's entries as prepare_teacher (token_teacher.hip) leaves them: per row a state, and K entries of
 // id (-1: none), q and ln q; entries of one id are merged into the first of them.
 enum { kRowFine = 0, kRowEmpty = 1, kRowBad = 2 };  // nothing there | an id beyond the vocabulary
 struct Teacher {
@@ -226,9 +226,14 @@ inline Teacher teacher_of(const float* buf, int64_t N, int64_t K) {
   t.K = (int)K;
   return t;
 }
+int prepare_teacher(const void* t_logits, int64_t t_stride, int t_dtype, const void* t_ids, int64_t id_stride,
+                    int id_bytes, int64_t K, float temperature, float* teacher, int64_t N, int64_t V, hipStream_t stream);
 // kl [N] and stats [N, 2] of a distillation (token.hip); the arguments have been checked
 int distill_stats(const void* logits, int64_t row_stride, const Teacher& teacher, float temperature, float* kl,
                   float* stats, void* scratch, int64_t N, int64_t V, int dtype, hipStream_t stream);
+// logp and stats together with glogits = grad_scale * d(-logp) / d logits (token_grad.hip); checked
+int token_nll_grad(const void* logits, int64_t row_stride, const void* tokens, int token_bytes, float* logp, float* stats,
+                   void* glogits, float grad_scale, void* scratch, int64_t N, int64_t V, int dtype, hipStream_t stream);
 // Each thread's entries of a row, asked for in three steps so that nobody waits: the entries in front of the row's
 // packets, the student's logits there when the ids have come, the KL when the row's statistics are known.
 template <int BT>

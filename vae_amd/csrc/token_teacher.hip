@@ -87,35 +87,29 @@ __global__ __launch_bounds__(kBlock) void distill_teacher_kernel(const void* __r
   }
 }
 
-}  // namespace vae
-
-using namespace vae;
-
-extern "C" {
-
-size_t vae_distill_teacher_floats(int64_t N, int64_t K) {
-  return N < 0 || K < 1 || K > VAE_MAX_TEACHER ? 0 : (size_t)N * (1 + 3 * (size_t)K);
-}
-
-int vae_distill_teacher(const void* t_logits, int64_t t_stride, int t_dtype, const void* t_ids, int64_t id_stride,
-                        int id_bytes, int64_t K, float temperature, float* teacher, int64_t N, int64_t V,
-                        vae_stream_t stream) {
-  if (N < 0 || V < 1 || V > VAE_MAX_ROW || K < 1 || K > VAE_MAX_TEACHER || (id_bytes != 4 && id_bytes != 8) ||
-      (t_dtype != VAE_F32 && t_dtype != VAE_BF16 && t_dtype != VAE_F16) || (N > 1 && (t_stride < K || id_stride < K)) ||
-      !(temperature > 0.f) || !(temperature < INFINITY))
-    return VAE_ERR_ARG;
-  if (N == 0) return VAE_OK;
-  if (!t_logits || !t_ids || !teacher) return VAE_ERR_ARG;
+int prepare_teacher(const void* t_logits, int64_t t_stride, int t_dtype, const void* t_ids, int64_t id_stride,
+                    int id_bytes, int64_t K, float temperature, float* teacher, int64_t N, int64_t V,
+                    hipStream_t stream) {
   const Teacher t = teacher_of(teacher, N, K);
   const int64_t blocks = (N + kBlock / 64 - 1) / (kBlock / 64);
   const int grid = (int)(blocks < kMaxGrid ? blocks : kMaxGrid);
   const float inv_tau = (float)(1.0 / (double)temperature);
   const float scale2 = (float)(1.4426950408889634 / (double)temperature);
-  const auto kernel = K <= 64 ? distill_teacher_kernel<1> : (K <= 128 ? distill_teacher_kernel<2> : distill_teacher_kernel<4>);
-  hipLaunchKernelGGL(kernel, dim3(grid), dim3(kBlock), 0, (hipStream_t)stream, t_logits, t_stride, t_dtype, t_ids,
-                     id_stride, id_bytes, (int)K, inv_tau, scale2, const_cast<int*>(t.state), const_cast<int*>(t.id),
+  const auto kernel = K <= 64    ? distill_teacher_kernel<1>
+                      : K <= 128 ? distill_teacher_kernel<2>
+                                 : distill_teacher_kernel<4>;
+  hipLaunchKernelGGL(kernel, dim3(grid), dim3(kBlock), 0, stream, t_logits, t_stride, t_dtype, t_ids, id_stride,
+                     id_bytes, (int)K, inv_tau, scale2, const_cast<int*>(t.state), const_cast<int*>(t.id),
                      const_cast<float*>(t.q), const_cast<float*>(t.logq), N, (int)V);
   return hipGetLastError() == hipSuccess ? VAE_OK : VAE_ERR_LAUNCH;
+}
+
+}  // namespace vae
+
+extern "C" {
+
+size_t vae_distill_teacher_floats(int64_t N, int64_t K) {
+  return N < 0 || K < 1 || K > VAE_MAX_TEACHER ? 0 : (size_t)N * (1 + 3 * (size_t)K);
 }
 
 }  // extern "C"

@@ -71,7 +71,7 @@ def loss_function(recon_x, x, kld, nll_type, kl_beta=1.0, mut_info=None, extra_l
                                                  kl_beta=kl_beta, inv_count=inv_count)
     elif nll_given is None and F_._is_categorical(nll_type):
         _, loss, elbo, means = F_.token_nll_elbo(x, recon_x, kld, add, mut_info, kl_beta, inv_count, fuse_backward,
-                                                 mean_dtype=recon_x.dtype)
+                                                 mean_dtype=recon_x.dtype, want_nll=False)
     elif nll_given is None:
         _, loss, elbo, means = F_.nll_elbo(x, recon_x, nll_type, kld=kld, add=add, mi=mut_info, kl_beta=kl_beta,
                                            inv_count=inv_count, fuse_backward=fuse_backward)

@@ -11,7 +11,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from . import _lib
-from ._lib import call, check_device, dtype_code, launch, ptr, stream_ptr, workspace
+from ._lib import DTYPE_CODES, call, check_device, dtype_code, launch, ptr, stream_ptr, workspace
 
 _MASK64 = (1 << 64) - 1
 
@@ -341,7 +341,8 @@ def nll(x, recon_x, nll_type):
     nll_type 'categorical': x holds integer tokens [B, ...] (negative: padding), recon_x their logits [B, ..., V]."""
     if _is_categorical(nll_type):
         _check_tokens(x, recon_x)
-        return _TokenNllElbo.apply(recon_x, x.contiguous(), None, None, None, 0.0, 0.0, False, False, torch.float32)[0]
+        return _TokenNllElbo.apply(recon_x, x.contiguous(), None, None, None, 0.0, 0.0, False, False, torch.float32,
+                                   True)[0]
     code, xf, rf = _flat_pixels(x, recon_x, nll_type)
     return _NllElbo.apply(xf, rf, None, None, None, code, 0.0, 0.0, False)[0]
 
@@ -523,12 +524,9 @@ def _is_categorical(nll_type):
     return nll_type.strip().lower() == 'categorical'
 
 
-def _id_bytes(t, what):
-    if t.dtype == torch.int64:
-        return 8
-    if t.dtype == torch.int32:
-        return 4
-    raise TypeError("%s: ids must be int32 or int64, got %s" % (what, t.dtype))
+def _check_ids(t, what):
+    if t.dtype != torch.int64 and t.dtype != torch.int32:
+        raise TypeError("%s: ids must be int32 or int64, got %s" % (what, t.dtype))
 
 
 def _check_vocab(logits, what):
@@ -536,13 +534,10 @@ def _check_vocab(logits, what):
         raise ValueError("%s: logits need a last dimension over the vocabulary, got %s" % (what, tuple(logits.shape)))
 
 
-_SPLIT_ROWS = 512   # with fewer rows the library may cut a row into pieces (csrc/token.hip: kFillRows)
-
-
 def _token_scratch(rows, top_k, dev):
-    """The pieces of split rows (few rows): the caller's own memory each call, so that calls on several streams and
-    captured graphs share nothing."""
-    if rows.shape[0] >= _SPLIT_ROWS:
+    """The pieces of split rows (fewer than 512, of at least 1024 16-byte vectors: csrc/token.hip): the caller's own
+    memory each call, so that calls on several streams and captured graphs share nothing."""
+    if rows.shape[0] >= 512 or rows.shape[1] < 4096:
         return None
     n = _lib.load().vae_token_scratch_bytes(rows.shape[0], rows.shape[1], top_k, dtype_code(rows))
     return torch.empty((n,), dtype=torch.uint8, device=dev) if n else None
@@ -626,7 +621,7 @@ def token_log_probs(logits, tokens=None, top_k=0, want_entropy=True):
         raise ValueError("token_log_probs: top_k must be in 0..min(%d, V = %d), got %d"
                          % (MAX_TOP, logits.shape[-1], top_k))
     if tokens is not None:
-        _id_bytes(tokens, 'token_log_probs')
+        _check_ids(tokens, 'token_log_probs')
         if tokens.shape != logits.shape[:-1]:
             raise ValueError("token_log_probs: tokens %s do not fit logits %s"
                              % (tuple(tokens.shape), tuple(logits.shape)))
@@ -638,7 +633,7 @@ def token_log_probs(logits, tokens=None, top_k=0, want_entropy=True):
 
 def _check_tokens(x, recon):
     """Tokens x [B, ...] and their logits recon [B, ..., V]."""
-    _id_bytes(x, "nll 'categorical'")
+    _check_ids(x, "nll 'categorical'")
     if x.dim() < 1 or recon.dim() < 2 or recon.shape[0] != x.shape[0] or recon.shape[:-1].numel() != x.numel():
         raise ValueError("nll 'categorical': logits %s do not fit tokens %s (a last dimension over the vocabulary)"
                          % (tuple(recon.shape), tuple(x.shape)))
@@ -650,41 +645,42 @@ class _TokenNllElbo(torch.autograd.Function):
     their own, in `mean_dtype`) and d(loss_mean)/d(logits) out of the same launch (fuse), as in _NllElboFused."""
 
     @staticmethod
-    def forward(ctx, logits, tokens, kld, add, mi, kl_beta, inv_count, with_elbo, fuse, mean_dtype):
+    def forward(ctx, logits, tokens, kld, add, mi, kl_beta, inv_count, with_elbo, fuse, mean_dtype, want_nll):
         ctx.set_materialize_grads(False)
         dev = check_device(logits, tokens, kld, add, mi)
         rows, B = _rows(logits), tokens.shape[0]
         N, V = rows.shape
-        code = dtype_code(rows)
-        logp = torch.empty((N,), dtype=torch.float32, device=dev)
-        stats = torch.empty((N, 2), dtype=torch.float32, device=dev)
+        # logp [N], stats [N, 2], means: one allocation
+        buf = torch.empty((3 * N + MEANS,), dtype=torch.float32, device=dev)
+        at = buf.data_ptr()
         grad = torch.empty(logits.shape, dtype=logits.dtype, device=dev) if fuse else None
+        nll = torch.empty((B,), dtype=logits.dtype, device=dev) if want_nll else None
+        loss = elbo = first = means = ws = None
         scratch = _token_scratch(rows, 0, dev)
-        nll = torch.empty((B,), dtype=logits.dtype, device=dev)
-        loss = elbo = means = first = ws = None
         if with_elbo:
-            loss, elbo, means, ws = torch.empty_like(nll), torch.empty_like(nll), _scalars(MEANS, dev, B), workspace(dev)
-            first = torch.empty((), dtype=mean_dtype, device=dev) if B else torch.zeros((), dtype=mean_dtype, device=dev)
-        if fuse:
-            launch(dev, 'vae_token_nll_fused', ptr(rows), rows.stride(0), ptr(tokens), tokens.element_size(), ptr(logp),
-                   ptr(stats), ptr(grad), inv_count, ptr(scratch), N, V, code)
-        else:
-            launch(dev, 'vae_token_logp_fwd', ptr(rows), rows.stride(0), ptr(tokens), tokens.element_size(), ptr(logp),
-                   None, ptr(stats), None, None, 0, ptr(scratch), N, V, code)
-        launch(dev, 'vae_token_elbo_fwd', ptr(logp), N // max(B, 1), ptr(kld), ptr(add), ptr(mi), kl_beta, inv_count,
-               ptr(nll), ptr(loss), ptr(elbo), ptr(means), ptr(first), _lib.DTYPE_CODES[mean_dtype], ptr(ws), B, code)
-        ctx.save_for_backward(logits, tokens, stats)
+            loss = torch.empty((B,), dtype=logits.dtype, device=dev)
+            elbo = torch.empty_like(loss)
+            means, ws = at + 12 * N, workspace(dev)
+            first = torch.empty((), dtype=mean_dtype, device=dev)
+        launch(dev, 'vae_token_nll_elbo_fwd', ptr(rows), rows.stride(0), ptr(tokens), tokens.element_size(),
+               N // max(B, 1), ptr(kld), ptr(add), ptr(mi), kl_beta, inv_count, at, at + 4 * N, ptr(grad), ptr(nll),
+               ptr(loss), ptr(elbo), means, ptr(first), DTYPE_CODES[mean_dtype], ptr(ws), ptr(scratch), B, V,
+               dtype_code(rows))
+        ctx.save_for_backward(logits, tokens, buf)
         ctx.grad = grad
         ctx.cfg = (kl_beta, inv_count, kld is not None, add is not None, mi is not None, mean_dtype)
         if not with_elbo:
             return (nll,) + (None,) * 8
+        if B == 0:
+            first.zero_()
+            buf.zero_()
         # the loss mean is a tensor of its own (a caller may scale it in place), the other five are views of one
-        return (nll, loss, elbo, first) + means[1:6].to(mean_dtype).unbind(0)
+        return (nll, loss, elbo, first) + buf[3 * N + 1:3 * N + 6].to(mean_dtype).unbind(0)
 
     @staticmethod
     @once_differentiable
     def backward(ctx, gnll, gloss, gelbo, *gmeans):
-        logits, tokens, stats = ctx.saved_tensors
+        logits, tokens, buf = ctx.saved_tensors
         kl_beta, inv_count, has_kld, has_add, has_mi, mean_dtype = ctx.cfg
         dev, B = logits.device, tokens.shape[0]
         need = ctx.needs_input_grad
@@ -696,19 +692,20 @@ class _TokenNllElbo(torch.autograd.Function):
         grow = None if stored else torch.empty((B,), dtype=torch.float32, device=dev)
         gnll, gloss, gelbo = _dense(gnll), _dense(gloss), _dense(gelbo)
         at = (ctypes.c_void_p * 6)(*[None if g is None else g.data_ptr() for g in gmeans])
-        launch(dev, 'vae_token_elbo_bwd', ptr(gnll), ptr(gloss), ptr(gelbo), at, _lib.DTYPE_CODES[mean_dtype], kl_beta,
+        launch(dev, 'vae_token_nll_elbo_bwd', ptr(gnll), ptr(gloss), ptr(gelbo), at, DTYPE_CODES[mean_dtype], kl_beta,
                inv_count, ptr(grow), ptr(grad) if stored else None, grad.numel() if stored else 0, ptr(terms[0]),
                ptr(terms[1]), ptr(terms[2]), B, dtype_code(logits))
         if not stored:
             grad = None
             if need[0]:
-                grad = _token_bwd(logits, tokens, None, None, stats, grow, tokens.numel() // max(B, 1), -1.0, None, None)
-        return (grad, None) + tuple(terms) + (None, None, None, None, None)
+                N = tokens.numel()
+                grad = _token_bwd(logits, tokens, None, None, buf[N:3 * N], grow, N // max(B, 1), -1.0, None, None)
+        return (grad, None) + tuple(terms) + (None,) * 6
 
 
 def token_nll_elbo(x, recon_x, kld=None, add=None, mi=None, kl_beta=1.0, inv_count=None, fuse_backward=False,
-                   mean_dtype=torch.float32):
-    """nll_elbo for nll_type 'categorical' with the six means as scalars: (nll, loss, elbo [B], 6 scalars in
+                   mean_dtype=torch.float32, want_nll=True):
+    """nll_elbo for nll_type 'categorical' with the six means as scalars: (nll [B] or None, loss, elbo [B], 6 scalars in
     `mean_dtype`)."""
     _check_tokens(x, recon_x)
     if inv_count is None:
@@ -718,7 +715,7 @@ def token_nll_elbo(x, recon_x, kld=None, add=None, mi=None, kl_beta=1.0, inv_cou
     fuse = bool(fuse_backward and recon_x.dtype != torch.float16 and recon_x.requires_grad and torch.is_grad_enabled()
                 and recon_x.numel() > 0)
     out = _TokenNllElbo.apply(recon_x, x.contiguous(), kld, add, mi, float(kl_beta), float(inv_count), True, fuse,
-                              mean_dtype)
+                              mean_dtype, want_nll)
     return out[0], out[1], out[2], out[3:]
 
 
@@ -751,8 +748,8 @@ class _Distill(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, t_logits, t_ids, temperature, inv_count, fuse):
         ctx.set_materialize_grads(False)
-        kl, mean, stats, grad, teacher = _distill_fwd(logits, t_logits, t_ids, temperature, inv_count, True, fuse)
-        ctx.save_for_backward(logits, teacher, stats)
+        kl, mean, grad, buf = _distill_fwd(logits, t_logits, t_ids, temperature, inv_count, fuse)
+        ctx.save_for_backward(logits, buf)
         ctx.grad = grad
         ctx.cfg = (temperature, inv_count, t_ids.shape[-1])
         return kl, mean
@@ -762,7 +759,7 @@ class _Distill(torch.autograd.Function):
     def backward(ctx, gkl, gmean):
         if gkl is None and gmean is None:
             return (None,) * 6
-        logits, teacher, stats = ctx.saved_tensors
+        logits, buf = ctx.saved_tensors
         temperature, inv_count, K = ctx.cfg
         dev = logits.device
         grad, ctx.grad = ctx.grad, None
@@ -771,27 +768,29 @@ class _Distill(torch.autograd.Function):
             launch(dev, 'vae_grad_scale', ptr(grad), ptr(gmean), grad.numel(), dtype_code(grad))
         else:
             rows = _rows(logits)
+            N, V = rows.shape
             grad = torch.empty(logits.shape, dtype=logits.dtype, device=dev)
-            launch(dev, 'vae_distill_bwd', ptr(rows), rows.stride(0), ptr(teacher), K, temperature, ptr(stats), ptr(gkl),
-                   ptr(gmean), inv_count, ptr(grad), rows.shape[0], rows.shape[1], dtype_code(rows))
+            at = buf.data_ptr()
+            launch(dev, 'vae_distill_bwd', ptr(rows), rows.stride(0), at, K, temperature, at + 4 * N * (1 + 3 * K),
+                   ptr(gkl), ptr(gmean), inv_count, ptr(grad), N, V, dtype_code(rows))
         return grad, None, None, None, None, None
 
 
-def _distill_fwd(logits, t_logits, t_ids, temperature, inv_count, want_stats, fuse):
+def _distill_fwd(logits, t_logits, t_ids, temperature, inv_count, fuse):
     dev = check_device(logits, t_logits, t_ids)
     rows, t_logits, t_ids = _rows(logits), _rows(t_logits), _rows(t_ids)
     (N, V), K = rows.shape, t_ids.shape[1]
     kl = torch.empty(logits.shape[:-1], dtype=torch.float32, device=dev)
-    stats = torch.empty((N, 2), dtype=torch.float32, device=dev) if want_stats else None
+    mean = torch.empty((), dtype=torch.float32, device=dev)
+    # the teacher's side (vae_distill_teacher_floats) and behind it the statistics [N, 2]: the backward's
+    buf = torch.empty((N * (3 + 3 * K),), dtype=torch.float32, device=dev)
+    at = buf.data_ptr()
     grad = torch.empty(logits.shape, dtype=logits.dtype, device=dev) if fuse else None
-    teacher = torch.empty((N, 1 + 3 * K), dtype=torch.float32, device=dev)   # vae_distill_teacher_floats
     scratch = _token_scratch(rows, 0, dev)
-    launch(dev, 'vae_distill_teacher', ptr(t_logits), t_logits.stride(0), dtype_code(t_logits), ptr(t_ids),
-           t_ids.stride(0), t_ids.element_size(), K, temperature, ptr(teacher), N, V)
-    launch(dev, 'vae_distill_fwd', ptr(rows), rows.stride(0), ptr(teacher), K, temperature, ptr(kl), ptr(stats),
-           ptr(grad), inv_count, ptr(scratch), N, V, dtype_code(rows))
-    mean = _row_sums(kl, inv_count, (), torch.float32)
-    return kl, mean, stats, grad, teacher
+    launch(dev, 'vae_distill_fwd', ptr(rows), rows.stride(0), ptr(t_logits), t_logits.stride(0), dtype_code(t_logits),
+           ptr(t_ids), t_ids.stride(0), t_ids.element_size(), K, temperature, at, ptr(kl), ptr(mean), inv_count,
+           at + 4 * N * (1 + 3 * K), ptr(grad), ptr(scratch), N, V, dtype_code(rows))
+    return kl, mean, grad, buf
 
 
 def distill_top_logits(logits, teacher_logits, teacher_ids, temperature=1.0, inv_count=None, fuse_backward=True):
@@ -806,7 +805,7 @@ def distill_top_logits(logits, teacher_logits, teacher_ids, temperature=1.0, inv
     formed by the forward launch (one read of the logits per step instead of two); a gradient on `kl` takes the general
     kernel."""
     _check_vocab(logits, 'distill_top_logits')
-    _id_bytes(teacher_ids, 'distill_top_logits')
+    _check_ids(teacher_ids, 'distill_top_logits')
     if teacher_logits.shape != teacher_ids.shape or teacher_ids.dim() < 1 or teacher_ids.shape[:-1] != logits.shape[:-1]:
         raise ValueError("distill_top_logits: teacher logits %s / ids %s do not fit logits %s"
                          % (tuple(teacher_logits.shape), tuple(teacher_ids.shape), tuple(logits.shape)))
@@ -822,7 +821,7 @@ def distill_top_logits(logits, teacher_logits, teacher_ids, temperature=1.0, inv
         # fp16: two passes, for the reason given in nll_elbo
         fuse = bool(fuse_backward) and logits.dtype != torch.float16 and logits.numel() > 0
         return _Distill.apply(logits, teacher_logits, teacher_ids, temperature, inv_count, fuse)
-    return _distill_fwd(logits, teacher_logits, teacher_ids, temperature, inv_count, False, False)[:2]
+    return _distill_fwd(logits, teacher_logits, teacher_ids, temperature, inv_count, False)[:2]
 
 
 class _SampleSums(torch.autograd.Function):
