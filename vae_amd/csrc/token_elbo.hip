@@ -25,6 +25,21 @@ __device__ __forceinline__ void write_mean(int k, double total, float inv_count,
   if (ws) note_nan(ws, v, kNanElbo6, k);
 }
 
+// `len` values p[first], p[first + step], ... in double; eight loads on their way at a time
+__device__ __forceinline__ double strided_sum(const float* __restrict__ p, int64_t first, int64_t step, int64_t len) {
+  double v = 0.0;
+  int64_t t = first;
+  for (; t + 7 * step < len; t += 8 * step) {
+    float x[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = p[t + i * step];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v += (double)x[i];
+  }
+  for (; t < len; t += step) v += (double)p[t];
+  return v;
+}
+
 // G lanes a sample (a power of two, up to a wave); samples in order, so a result does not depend on timing
 template <typename T>
 __global__ __launch_bounds__(kBlock) void token_elbo_fwd_kernel(
@@ -37,12 +52,10 @@ __global__ __launch_bounds__(kBlock) void token_elbo_fwd_kernel(
   float acc[6] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
   for (int64_t b0 = (int64_t)blockIdx.x * rpb; b0 < B; b0 += (int64_t)gridDim.x * rpb) {
     const int64_t b = b0 + rloc;
-    double v = 0.0;
-    if (b < B)
-      for (int64_t t = sub; t < len; t += G) v += (double)logp[b * len + t];
+    double v = b < B ? strided_sum(logp + b * len, sub, G, len) : 0.0;
     for (int o = G >> 1; o >= 1; o >>= 1) v += __shfl_xor(v, o, 64);
     if (sub != 0 || b >= B) continue;
-    const float n = (float)-v;          // loss and elbo from the unrounded sum: every output is rounded once
+    const float n = (float)(0.0 - v);   // loss and elbo from the unrounded sum: every output is rounded once
     if (nll) nll[b] = from_f32<T>(n);
     if (!loss) continue;
     const float k = kld ? to_f32(kld[b]) : 0.f;
@@ -109,21 +122,21 @@ __global__ __launch_bounds__(kBlock) void token_elbo_bwd_kernel(
   }
 }
 
-// out[b] = scale * sum of `len` consecutive row values, in a fixed order, summed in double: a workgroup a sum
-template <typename O>
-__global__ __launch_bounds__(kBlock) void row_sums_kernel(const float* __restrict__ rows, float scale,
+// out[b] = scale * sum of `len` consecutive row values, in a fixed order, summed in double: a workgroup a sum.  One sum
+// over everything (a mean over all rows) is bound by its loads' latency: 1024 threads, eight loads each on their way
+// (65536 values: 60 us with 256 threads and a load at a time).
+template <typename O, int BT>
+__global__ __launch_bounds__(BT) void row_sums_kernel(const float* __restrict__ rows, float scale,
                                                           O* __restrict__ out, int64_t B, int64_t len) {
-  __shared__ double part[kBlock / 64];
+  __shared__ double part[BT / 64];
   for (int64_t b = blockIdx.x; b < B; b += gridDim.x) {
-    double v = 0.0;
-    for (int64_t t = threadIdx.x; t < len; t += kBlock) v += (double)rows[b * len + t];
-    v = wave_sum_d(v);
+    const double v = wave_sum_d(strided_sum(rows + b * len, threadIdx.x, BT, len));
     lds_barrier();
     if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = v;
     lds_barrier();
     if (threadIdx.x == 0) {
       double r = 0.0;
-      for (int w = 0; w < kBlock / 64; ++w) r += part[w];
+      for (int w = 0; w < BT / 64; ++w) r += part[w];
       out[b] = from_f32<O>((float)(r * (double)scale));
     }
   }
@@ -219,8 +232,11 @@ int vae_row_sums(const float* rows, float scale, void* out, int64_t B, int64_t l
   if (B < 0 || len < 0 || !type_ok(dtype)) return VAE_ERR_ARG;
   if (B == 0) return VAE_OK;
   if (!out || (len > 0 && !rows)) return VAE_ERR_ARG;
-  VAE_BY_TYPE(dtype, hipLaunchKernelGGL((row_sums_kernel<T>), dim3((int)(B < kMaxGrid ? B : kMaxGrid)), dim3(kBlock), 0,
-                                        (hipStream_t)stream, rows, scale, (T*)out, B, len));
+  const int grid = (int)(B < kMaxGrid ? B : kMaxGrid);
+  VAE_BY_TYPE(dtype, if (len > 4096) hipLaunchKernelGGL((row_sums_kernel<T, 1024>), dim3(grid), dim3(1024), 0,
+                                                        (hipStream_t)stream, rows, scale, (T*)out, B, len);
+              else hipLaunchKernelGGL((row_sums_kernel<T, kBlock>), dim3(grid), dim3(kBlock), 0, (hipStream_t)stream, rows,
+                                      scale, (T*)out, B, len));
   return launched();
 }
 

@@ -2,10 +2,15 @@
 // logit > -inf), ln q, and what comes twice merged, so that the kernels over the vocabulary find each id once.  A wave a
 // row, no barrier: K entries are 2 KB at most.  Prepared here and not in those kernels: there the chain of loads and
 // reductions stood in front of every row (4096 x 131072 bf16 with K = 64: 531 us against 423 us of the loss that has no
-// teacher; 8192 x 32768: 435 against 182).
+// teacher; 8192 x 32768: 435 against 182).  65536 rows of 64 entries: 27 us.  1, 2 or 4 entries a lane as
+// K asks (the whole call for 65536 x 1024 with 64 entries: 117 us, 131 with 4 for all).
 #include "token_row.hpp"
 
 namespace vae {
+
+constexpr int kSlots = 1024;   // 64 ids leave about 2 pairs in one slot, 256 about 32
+static_assert(VAE_MAX_ROW <= 1 << 24 && VAE_MAX_TEACHER <= 256, "an id and its place share 32 bits");
+__device__ __forceinline__ uint32_t slot_of(int id) { return (uint32_t)id * 2654435761u >> 22; }
 
 template <int R>   // entries a lane
 __global__ __launch_bounds__(kBlock) void distill_teacher_kernel(const void* __restrict__ logits, int64_t stride, int dtype,
@@ -14,6 +19,7 @@ __global__ __launch_bounds__(kBlock) void distill_teacher_kernel(const void* __r
                                                                  int* __restrict__ state, int* __restrict__ id_out,
                                                                  float* __restrict__ q_out, float* __restrict__ logq_out,
                                                                  int64_t N, int V) {
+  __shared__ uint32_t slots[kBlock / 64][kSlots];
   const int lane = threadIdx.x & 63;
   for (int64_t row = (int64_t)blockIdx.x * (kBlock / 64) + (threadIdx.x >> 6); row < N;
        row += (int64_t)gridDim.x * (kBlock / 64)) {
@@ -49,38 +55,69 @@ __global__ __launch_bounds__(kBlock) void distill_teacher_kernel(const void* __r
       q[r] /= s;
       logq[r] = row_log_prob(y[r], m, s, inv_tau);
     }
-    // equal ids into the first: the sum of q, and of q ln q, in the entries' order
-    float qs[R], ql[R];
-    bool first[R], twice = false;
+    // Which ids come twice: every entry writes (id, its place) into the slot of its id's hash and reads the slot back.  Its
+    // own: it is the first to stand for its id.  The same id at another place: it is a second one.  Another id: once more,
+    // without those that are settled.  Every round settles each slot's writer, so it ends.  (An entry compared with every
+    // other one: 194 us for 65536 rows of 64 entries.)
+    volatile uint32_t* slot = slots[threadIdx.x >> 6];   // a wave's LDS accesses are in order
+    bool todo[R], again[R];
 #pragma unroll
     for (int r = 0; r < R; ++r) {
-      qs[r] = ql[r] = 0.f;
-      first[r] = true;
+      todo[r] = id[r] >= 0;
+      again[r] = false;
     }
+    for (;;) {
+      bool any = false;
 #pragma unroll
-    for (int r2 = 0; r2 < R; ++r2)
-      for (int l = 0; l < 64 && l + 64 * r2 < K; ++l) {
-        const int other = __builtin_amdgcn_readlane(id[r2], l);
-        const float oq = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, q[r2]), l));
-        const float ol = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, logq[r2]), l));
+      for (int r = 0; r < R; ++r) any |= todo[r];
+      if (__ballot(any) == 0) break;
+#pragma unroll
+      for (int r = 0; r < R; ++r)
+        if (todo[r]) slot[slot_of(id[r])] = (uint32_t)id[r] | (uint32_t)(lane + 64 * r) << 24;
+#pragma unroll
+      for (int r = 0; r < R; ++r)
+        if (todo[r]) {
+          const uint32_t w = slot[slot_of(id[r])];
+          todo[r] = (w & 0xffffffu) != (uint32_t)id[r];
+          again[r] = !todo[r] && (int)(w >> 24) != lane + 64 * r;
+        }
+    }
+    // one id's entries into the first of them: the sum of q, and of q ln q, in the entries' order
+#pragma unroll
+    for (int r0 = 0; r0 < R; ++r0)
+      for (uint64_t left = __ballot(again[r0]); left != 0; left = __ballot(again[r0])) {
+        const int common = __builtin_amdgcn_readlane(id[r0], __ffsll((unsigned long long)left) - 1);
+        float qs = 0.f, ql = 0.f;
+        int first = -1;
 #pragma unroll
         for (int r = 0; r < R; ++r)
-          if (id[r] == other) {
-            const int k = lane + 64 * r, k2 = l + 64 * r2;
-            first[r] &= k2 >= k;
-            twice |= k2 != k;
-            qs[r] += oq;
-            ql[r] = __builtin_fmaf(oq, ol, ql[r]);
+          for (uint64_t all = __ballot(id[r] == common); all != 0; all &= all - 1) {
+            const int l = __ffsll((unsigned long long)all) - 1;
+            const float oq = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, q[r]), l));
+            const float ol = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, logq[r]), l));
+            qs += oq;
+            ql = __builtin_fmaf(oq, ol, ql);
+            first = first < 0 ? l + 64 * r : first;
+          }
+#pragma unroll
+        for (int r = 0; r < R; ++r)
+          if (id[r] == common) {
+            again[r] = false;
+            if (lane + 64 * r == first) {
+              q[r] = qs;
+              logq[r] = ql / qs;   // weighted: q (ln q - ln p) of the merged entry is their sum
+            } else {
+              id[r] = -1;
+            }
           }
       }
 #pragma unroll
     for (int r = 0; r < R; ++r) {
       const int k = lane + 64 * r;
       if (k >= K) continue;
-      const bool merged = twice && id[r] >= 0 && qs[r] != q[r];
-      id_out[row * K + k] = first[r] ? id[r] : -1;
-      q_out[row * K + k] = merged ? qs[r] : q[r];
-      logq_out[row * K + k] = merged ? ql[r] / qs[r] : logq[r];   // weighted: q (ln q - ln p) of the merged entry is their sum
+      id_out[row * K + k] = id[r];
+      q_out[row * K + k] = q[r];
+      logq_out[row * K + k] = logq[r];
     }
     const bool any_bad = __ballot(bad) != 0;
     if (lane == 0) state[row] = any_bad ? kRowBad : (s == 0.f ? kRowEmpty : kRowFine);
