@@ -602,6 +602,65 @@ def test_repeats_streams_and_graphs_give_the_same_bits(N, V, dt):
             assert torch.equal(a, b)
 
 
+@pytest.mark.parametrize('kind', ['nll', 'distill'])
+def test_backward_captured_apart_from_its_forward(kind):
+    """A stored gradient is multiplied in place: replays of a backward pass whose forward pass was eager must not
+    multiply it again and again."""
+    from vae_amd import functional as F_
+    N, V = 12, 3000
+    x = torch.randn(N, V, generator=gen(3)).to(DEV)
+    tok = torch.randint(0, V, (N, 1), generator=gen(4)).to(DEV)
+    y, ids = torch.randn(N, 5, generator=gen(5)).to(DEV), torch.randint(0, V, (N, 5), generator=gen(6)).to(DEV)
+
+    def loss(x):
+        if kind == 'nll':
+            return F_.token_nll_elbo(tok, x[:, None], fuse_backward=True)[3][0]
+        return F_.distill_top_logits(x, y, ids)[1]
+
+    two = torch.full((), 2.0, device=DEV)
+    xr = x.clone().requires_grad_(True)
+    want, = torch.autograd.grad(loss(xr), xr, two)
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        leaf = x.clone().requires_grad_(True)
+        value = loss(leaf)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=s):
+        g, = torch.autograd.grad(value, leaf, two)
+    for _ in range(3):
+        g.zero_()
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        # the two forms round d, e = 2^d, the sum, 1 / s and the products apart.  p |d| < 0.6 (e^-y y at most 1/e) and p < 1
+        # bound what each rounding moves: under 16 steps of 2^-24 of a gradient of 2 / N
+        assert (g - want).abs().max() <= 16 * 2.0 ** -24 * 2.0 / N
+
+
+@pytest.mark.parametrize('V', [40, 3000, 70000])
+def test_an_id_beyond_the_vocabulary_in_a_masked_row(V):
+    """Both at once: the id decides, in every form of the gradient."""
+    from vae_amd import functional as F_
+    x = torch.randn(3, V, generator=gen(1)).to(torch.bfloat16)
+    x[1] = float('-inf')
+    tok = torch.tensor([1, V, -1]).to(DEV)
+    x = x.to(DEV)
+    for fuse in (False, True):
+        xr = x.clone().requires_grad_(True)
+        out = F_.token_nll_elbo(tok[:, None], xr[:, None], fuse_backward=fuse)
+        g, = torch.autograd.grad(out[3][0], xr)
+        assert g[1].isnan().all() and (g[2] == 0).all() and not g[0].isnan().any()
+        assert out[0][1].isnan() and out[0][2] == 0 and not torch.signbit(out[0][2])
+    xr = x.clone().requires_grad_(True)
+    lp, h, _, _ = F_.token_log_probs(xr, tok)
+    g, = torch.autograd.grad(lp.sum() + h.sum(), xr)
+    assert g[1].isnan().all() and (g[2] == 0).all() and not g[0].isnan().any()
+    g, = torch.autograd.grad(F_.token_log_probs(xr, tok)[1].sum(), xr)     # the entropy alone knows no token
+    assert not g.isnan().any() and (g[1:] == 0).all()
+
+
 def test_two_captured_graphs_do_not_share_scratch():
     """Two graphs of the split-row form on different inputs, replayed on two streams at once."""
     from vae_amd import functional as F_
@@ -807,3 +866,92 @@ def test_expanded_logits():
     ref[0, 5] += 2.0
     check_grad(g, ref, 4.0)
     assert bool((h[:3] == h[0]).all()) and float(h[3]) == 0.0
+
+
+def _slot(i):
+    return (i * 2654435761 & 0xffffffff) >> 22
+
+
+@pytest.mark.parametrize('V,dt', [(5000, 'f32'), (70000, 'bf16')])
+@pytest.mark.parametrize('K', [60, 128, 256])
+def test_distillation_of_ids_that_come_often(V, K, dt):
+    """Many ids many times, many of them in one slot of the table that looks for them, and one id alone."""
+    from vae_amd import functional as F_
+    one_slot = [i for i in range(V) if _slot(i) == _slot(4321)]
+    assert len(one_slot) >= 4
+    g = gen(K)
+    ids = torch.stack([torch.tensor(one_slot)[torch.randint(0, len(one_slot), (K,), generator=g)],
+                       torch.tensor((one_slot * K)[:K]), torch.full((K,), 77), torch.randint(0, V, (K,), generator=g)])
+    ids[2, K // 2:] = -1
+    z = torch.randn(4, V, generator=g).to(TYPES[dt])
+    y = torch.randn(4, K, generator=g)
+    kl_ref, grad_ref = ref_distill(z.double(), y.double(), ids, 1.0)
+    for fuse in (True, False):
+        x = z.to(DEV).requires_grad_(True)
+        kl, mean = F_.distill_top_logits(x, y.to(DEV), ids.to(DEV), fuse_backward=fuse)
+        close(kl, kl_ref, 1e-6, 2e-5)
+        grad, = torch.autograd.grad(mean, x)
+        check_grad(grad, grad_ref / 4, 0.25)
+
+
+@pytest.mark.parametrize('V,dt', [(1050001, 'f32'), (1050001, 'bf16'), (140000, 'bf16')])
+@pytest.mark.parametrize('k', [1, 5, 64])
+def test_alternatives_over_many_pieces(V, dt, k):
+    """More pieces than alternatives, and fewer; equal values, the large ones in one piece."""
+    from vae_amd import functional as F_
+    z = torch.randn(4, V, generator=gen(k)).to(TYPES[dt])
+    z[1] = 0.25
+    z[2, V // 2:V // 2 + 90] = 9.0
+    z[3] = torch.sort(z[3])[0]
+    _, _, top, ids = F_.token_log_probs(z.to(DEV), top_k=k)
+    assert torch.equal(ids.cpu(), ref_top(z.double(), k))
+    _, _, _, alone = F_.token_log_probs(z[:1].to(DEV), top_k=k)
+    assert torch.equal(alone.cpu(), ids[:1].cpu())
+
+
+@pytest.mark.parametrize('dt', ['f32', 'bf16'])
+@pytest.mark.parametrize('V,k', [(200, 64), (512, 7), (512, 8), (512, 48), (512, 49), (513, 49), (1024, 3), (1024, 4),
+                                 (1024, 64), (1025, 3), (900, 64), (1790, 49), (1800, 49), (2000, 64), (8192, 48),
+                                 (8193, 49)])
+def test_alternatives_where_the_kernels_change(V, k, dt):
+    from vae_amd import functional as F_
+    z = torch.randn(5, V, generator=gen(V + k)).to(TYPES[dt])
+    z[1] = -2.0
+    z[2, :V - 3] = float('-inf')
+    tok = torch.tensor([0, V - 1, V - 2, -1, 5])
+    lp, h, top, ids = F_.token_log_probs(z.to(DEV), tok.to(DEV), top_k=k)
+    logp, _, hr = ref_rows(z.double())
+    live = [0, 1, 2, 4]
+    assert torch.equal(ids.cpu()[live], ref_top(z.double(), k)[live])
+    assert (ids[3] == -1).all()
+    close(lp[live], logp[live, tok[live]], 1e-6, 4e-6)
+    close(h[live], hr[live], 1e-6, 2e-5)
+
+
+def test_many_rows_of_a_wave_each():
+    from vae_amd import functional as F_
+    N, V = 2100, 8192
+    x = torch.randn(N, V, device=DEV, generator=torch.Generator(DEV).manual_seed(1)).to(torch.bfloat16)
+    tok = torch.randint(0, V, (N,), generator=gen(2)).to(DEV)
+    lp, h, top, ids = F_.token_log_probs(x, tok, top_k=3)
+    few = torch.arange(0, N, 37)
+    z = x[few.to(DEV)].double().cpu()
+    logp, _, hr = ref_rows(z)
+    close(lp[few.to(DEV)], logp.gather(1, tok.cpu()[few][:, None])[:, 0], 1e-6, 4e-6)
+    close(h[few.to(DEV)], hr, 1e-6, 2e-5)
+    assert torch.equal(ids.cpu()[few], ref_top(z, 3))
+
+
+@pytest.mark.parametrize('B,T', [(1, 70001), (3, 5003), (2, 4096), (700, 9), (1, 1)])
+def test_long_sums(B, T):
+    """Sums of many rows: in double, rounded once (half a step of fp32), the double sum itself 2^-40 off at most."""
+    from vae_amd import functional as F_
+    rows = torch.rand(B, T, generator=gen(T)) + 0.5
+    got = F_.sample_sums(rows.to(DEV))
+    close(got, rows.double().sum(1), 2.0 ** -24 + 2.0 ** -40, 0.0)
+    z, x = torch.randn(B, T, 5, generator=gen(B)), torch.randint(0, 5, (B, T), generator=gen(3))
+    lp = F_.token_log_probs(z.to(DEV), x.to(DEV), want_entropy=False)[0]
+    close(F_.nll(x.to(DEV), z.to(DEV), 'categorical'), -lp.double().cpu().sum(1), 2.0 ** -24 + 2.0 ** -40, 0.0)
+    kl, mean = F_.distill_top_logits(z.to(DEV), torch.randn(B, T, 2, generator=gen(4)).to(DEV),
+                                     torch.randint(0, 5, (B, T, 2), generator=gen(5)).to(DEV), inv_count=0.25)
+    close(mean, 0.25 * kl.double().cpu().sum(), 2.0 ** -24 + 2.0 ** -40, 0.0)

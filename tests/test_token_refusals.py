@@ -125,6 +125,7 @@ def test_c_entry_points_refuse_bad_shapes(f, bad):
     (fused, dict(tb=0)),
     (dfwd, dict(K=0)), (dfwd, dict(K=257)), (dfwd, dict(tau=0.0)), (dfwd, dict(tau=float('nan'))),
     (dfwd, dict(tau=float('inf'))), (dfwd, dict(t=None)), (dfwd, dict(kl=None)), (dfwd, dict(stats=None)),
+    (dfwd, dict(tau=1e-39)), (dbwd, dict(tau=1e-39)),
     (dbwd, dict(K=0)), (dbwd, dict(tau=-1.0)), (dbwd, dict(stats=None)), (dbwd, dict(out=None)), (dbwd, dict(t=None)),
     (dfwd, dict(K=257, ys=300, ids_s=300)), (dfwd, dict(ys=1)), (dfwd, dict(ids_s=1)), (dfwd, dict(ib=2)),
     (dfwd, dict(yt=9)), (dfwd, dict(y=None)), (dfwd, dict(ids=None)),

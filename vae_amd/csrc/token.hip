@@ -6,7 +6,9 @@
 //
 // One pass over the logits: every thread keeps a running (max, sum, weighted sum) of its vectors, merged across the
 // workgroup at the end, so a row is read once whatever its length.  Few rows are cut into `parts` pieces of one
-// workgroup each, whose partial results a second launch joins.
+// workgroup each, whose partial results a second launch joins.  Bound by the read: 4096 x 32768 bf16 with entropy 44 us
+// (6.1 TB/s), 2048 x 50021 fp16 (rows at every alignment) 39 us (5.3 TB/s); the arithmetic is an fma, an exponential and
+// an addition an element, two more with the entropy.
 #include "token_row.hpp"
 
 namespace vae {
@@ -136,8 +138,8 @@ __device__ __forceinline__ void row_stats(const T* __restrict__ x, const RowCut<
 // The k largest keys (order_key: value, then the lower index) of what a workgroup has read.  A bound from below comes
 // from the threads' own maxima: every wave takes the ceil(k / waves)-th largest of its lanes', the least of those has k
 // elements at or above it.  Only the few threads whose maximum reaches the bound can hold any of the k; their vectors
-// are read once more (out of the caches), all lanes side by side.  Measured beside a list kept while reading: the list
-// costs every element a comparison (4096 x 32768, k = 20: 145 us with it, see fwd_type for this one).
+// are read once more (out of the caches), all lanes side by side.  4096 x 32768 bf16, k = 20: 67 us, 57 for k = 4, 44
+// without alternatives; a list kept while reading costs every element a comparison (145 us).
 // ---------------------------------------------------------------------------------------------------------------
 constexpr int kCand = 1024;      // candidates that LDS holds
 constexpr int kMostShares = 96;  // threads at the bound beyond which equal values are told apart by their index first
@@ -150,31 +152,25 @@ struct TopLds {
   int nshare, ncand;
 };
 
-// the n-th largest of a wave's 64 keys, or a number below it that no more than the n-th largest share down to bit
-// `last`; 0 where there are fewer than n
+// the n-th largest of a wave's 64 keys, its bits below `last` cleared; 0 where there are fewer than n
 __device__ __forceinline__ uint64_t wave_nth(uint64_t key, int n, int last) {
   uint64_t b = 0;
   for (int bit = 63; bit >= last; --bit) {
     const uint64_t want = b | (1ull << bit);
-    const int c = __popcll(__ballot(key >= want));
-    if (c >= n) {
-      b = want;
-      if (c == n) break;
-    }
+    b = __popcll(__ballot(key >= want)) >= n ? want : b;
   }
   return b;
 }
+// the least of the first `waves` waves' `each`-th largest keys: waves * each keys are at or above it
 template <int BT>
-__device__ __forceinline__ uint64_t block_bound(TopLds<BT>& lds, uint64_t key, int k, int last) {
-  constexpr int NW = BT / 64;
-  const uint64_t mine = wave_nth(key, (k + NW - 1) / NW, last);
+__device__ __forceinline__ uint64_t block_bound(TopLds<BT>& lds, uint64_t key, int each, int waves, int last) {
+  const uint64_t mine = wave_nth(key, each, last);
   lds_barrier();   // what the last one left has been read
   if ((threadIdx.x & 63) == 0) lds.wave_bound[threadIdx.x >> 6] = mine;
   if (threadIdx.x == 0) lds.nshare = lds.ncand = 0;
   lds_barrier();
   uint64_t b = lds.wave_bound[0];
-#pragma unroll
-  for (int w = 1; w < NW; ++w) b = lds.wave_bound[w] < b ? lds.wave_bound[w] : b;
+  for (int w = 1; w < waves; ++w) b = lds.wave_bound[w] < b ? lds.wave_bound[w] : b;
   return b;
 }
 template <int BT>
@@ -221,7 +217,8 @@ __device__ __forceinline__ void row_top(TopLds<BT>& lds, const T* __restrict__ x
   uint64_t key = v0 + tid < v1 ? (uint64_t)order_bits(mine) << 32 : 0;
   const uint64_t edge_top = edge_key >> 32 << 32;
   key = edge_top > key ? edge_top : key;
-  uint64_t bound = block_bound(lds, key, k, kLastBit);
+  constexpr int NW = BT / 64;
+  uint64_t bound = block_bound(lds, key, (k + NW - 1) / NW, NW, kLastBit);
   auto take_share = [&]() {
     if (key != 0 && key >= bound) lds.share[atomicAdd(&lds.nshare, 1)] = tid;
     lds_barrier();
@@ -235,7 +232,7 @@ __device__ __forceinline__ void row_top(TopLds<BT>& lds, const T* __restrict__ x
     for (int j = v0 + tid; j < v1 && best == 0; j += BT)
       each(j, [&](float v, uint32_t at) { best = v == mine && best == 0 ? order_key(v, at) : best; });
     key = best > key ? best : key;
-    bound = block_bound(lds, key, k, 0);
+    bound = block_bound(lds, key, (k + NW - 1) / NW, NW, 0);
     n = take_share();
   }
   push_key(lds, edge_key, bound);
@@ -374,6 +371,7 @@ __global__ __launch_bounds__(BT) void token_join_kernel(FwdArgs a) {
     // everything that does not depend on anything else is on its way first
     const char* from = a.scratch + row * a.parts * part_bytes(a.top_k);
     const int n = a.parts * a.top_k;
+    const int at = (a.top_k + a.parts - 1) / a.parts - 1;   // a piece's keys are in order
     auto key_at = [&](int i) {
       const int p = i / a.top_k;
       return reinterpret_cast<const uint64_t*>(from + p * part_bytes(a.top_k) + 16)[i - p * a.top_k];
@@ -386,13 +384,11 @@ __global__ __launch_bounds__(BT) void token_join_kernel(FwdArgs a) {
       sp = f[1];
       tp = f[2];
     }
-    uint64_t keys[TOP ? R : 1], below = 0;
+    uint64_t keys[TOP ? R : 1], lead = 0;
     if constexpr (TOP) {
 #pragma unroll
       for (int r = 0; r < R; ++r) keys[r] = (int)threadIdx.x + r * BT < n ? key_at(threadIdx.x + r * BT) : 0;
-      // a piece's keys are in order: the ceil(k / parts)-th of every piece has k keys at or above the least of them
-      const int at = (a.top_k + a.parts - 1) / a.parts - 1;
-      if ((int)threadIdx.x < a.parts) below = ~key_at(threadIdx.x * a.top_k + at);
+      if ((int)threadIdx.x < a.parts) lead = key_at(threadIdx.x * a.top_k + at);
     }
     float token_logit = 0.f;
     TeacherTerms<BT> terms;
@@ -420,10 +416,9 @@ __global__ __launch_bounds__(BT) void token_join_kernel(FwdArgs a) {
         for (int r = 0; r < R; ++r) f(keys[r]);
         for (int i = kCand + threadIdx.x; i < n; i += BT) f(key_at(i));
       };
-      const uint64_t bound = ~block_max_key<BT>(below);
-      lds_barrier();                 // the row before this one has been ranked
-      if (threadIdx.x == 0) lds.top[0].ncand = 0;
-      lds_barrier();
+      // at + 1 keys of a piece are at or above its at-th one: the `need` largest of those have k between them
+      const int need = (a.top_k + at) / (at + 1), full = a.parts < 64 ? 1 : a.parts / 64;
+      const uint64_t bound = block_bound(lds.top[0], lead, (need + full - 1) / full, full, 32);
       for_keys([&](uint64_t key) { push_key(lds.top[0], key, bound); });
       if (!emit_ranked(lds.top[0], a.top_k, emit)) {
         uint64_t last = ~0ull;
@@ -445,18 +440,22 @@ static bool bad_shape(int64_t N, int64_t V, int64_t row_stride, int dtype) {
 }
 static int grid_for(int64_t items) { return (int)(items < kMaxGrid ? items : kMaxGrid); }
 
-// Pieces of a row: with fewer than kFillRows rows a workgroup a row leaves compute units idle; a piece keeps at least
-// kPieceVecs vectors, so that the join's cost stays below what the split saves.
-constexpr int64_t kFillRows = 512, kPieceVecs = 512;
+// Pieces of a row: with up to kFillRows rows a workgroup a row leaves compute units idle.  Four workgroups a compute unit
+// are aimed at, of kPieceVecs vectors or more (1 x 131072 bf16: 5.2 us with 512 or 128, 6.1 with 2048).  The second launch
+// has its price, about 3 us, 5 with alternatives, so short rows stay whole:
+//   bf16, split against whole:  64 x 131072 7.9 / 14.9 us,  256 x 131072 15.8 / 19.6,  400 x 131072 24.1 / 21.5,
+//     1 x 65536 5.4 / 6.0,  256 x 65536 10.8 / 10.8,  1 x 32768 5.3 / 4.3,  128 x 32768 7.5 / 6.3;
+//   with 5 alternatives:  1 x 131072 10.0 / 13.6,  64 x 131072 13.9 / 19.3,  1 x 65536 10.2 / 8.9,  256 x 65536 16.5 / 14.4.
+constexpr int64_t kFillRows = 256, kPieceVecs = 512, kSplitVecs = 8192, kSplitVecsTop = 16384;
 struct Cut {
   int parts, part_vecs;
 };
-static Cut cut_rows(int64_t N, int64_t V, int dtype) {
+static Cut cut_rows(int64_t N, int64_t V, int64_t top_k, int dtype) {
   const int64_t vn = dtype == VAE_F32 ? 4 : 8;
   const int64_t nvec = (V + vn - 1) / vn;
   int64_t parts = 1;
-  if (N < kFillRows) {
-    parts = 2 * kFillRows / (N > 0 ? N : 1);
+  if (N <= kFillRows && V / vn >= (top_k ? kSplitVecsTop : kSplitVecs)) {
+    parts = 4 * kFillRows / (N > 0 ? N : 1);
     const int64_t most = nvec / kPieceVecs;
     parts = parts < most ? parts : most;
     parts = parts < 1 ? 1 : (parts > kBlock ? kBlock : parts);
@@ -464,8 +463,6 @@ static Cut cut_rows(int64_t N, int64_t V, int dtype) {
   const int64_t per = (nvec + parts - 1) / parts;
   return {(int)((nvec + per - 1) / per), (int)per};
 }
-// rows of up to this many vectors take one wave each
-constexpr int64_t kWaveVecs = 512;
 
 template <typename T, int BT, bool ENT, bool TOP, bool DIST>
 static int fwd_launch(const FwdArgs& a, hipStream_t st) {
@@ -474,9 +471,15 @@ static int fwd_launch(const FwdArgs& a, hipStream_t st) {
     hipLaunchKernelGGL((token_join_kernel<T, kBlock, ENT, TOP, DIST>), dim3(grid_for(a.N)), dim3(kBlock), 0, st, a);
   return hipGetLastError() == hipSuccess ? VAE_OK : VAE_ERR_LAUNCH;
 }
+// A wave a row for rows of up to 512 vectors, and of up to 1024 where there are many: no barriers, and four or more rows a
+// compute unit's worth of loads.  65536 x 4096 bf16: 82 us (6.5 TB/s) against 142 with a workgroup a row; 8192 x 8192:
+// 24.4 against 25.2, but 512 x 8192: 5.9 against 4.7; 8192 x 16384: 48.7 against 45.2.  Beyond 48 alternatives the bound
+// would take nearly every lane's maximum, the least of 64, and a quarter of the row with it (16384 x 2000 bf16, 64 of
+// them: 320 us against 84 with a workgroup, which asks each wave for its 16 largest; 48 of them: 61 against 73).
 template <typename T, bool DIST>
 static int fwd_type(const FwdArgs& a, hipStream_t st) {
-  const bool wave = a.parts == 1 && (a.V + VecOf<T>::n - 1) / VecOf<T>::n <= kWaveVecs;
+  const int64_t nvec = (a.V + VecOf<T>::n - 1) / VecOf<T>::n;
+  const bool wave = a.parts == 1 && (nvec <= 512 || (nvec <= 1024 && a.N >= 2048)) && !(a.top_k > 48 && nvec >= 224);
 #define VAE_FWD(E, K) (wave ? fwd_launch<T, 64, E, K, DIST>(a, st) : fwd_launch<T, kBlock, E, K, DIST>(a, st))
   if constexpr (DIST) return VAE_FWD(false, false);
   else {
@@ -489,7 +492,7 @@ static int fwd_type(const FwdArgs& a, hipStream_t st) {
 // kl and stats; vae_distill_fwd (token_grad.hip) has checked the arguments
 int distill_stats(const void* logits, int64_t row_stride, const Teacher& teacher, float temperature, float* kl,
                   float* stats, void* scratch, int64_t N, int64_t V, int dtype, hipStream_t stream) {
-  const Cut cut = cut_rows(N, V, dtype);
+  const Cut cut = cut_rows(N, V, 0, dtype);
   if (cut.parts > 1 && !scratch) return VAE_ERR_ARG;
   const FwdArgs a = {logits, row_stride, nullptr, 0, kl, nullptr, stats, nullptr, nullptr, 0, N, (int)V, cut.parts,
                      cut.part_vecs, (char*)scratch, (float)(1.4426950408889634 / (double)temperature),
@@ -506,7 +509,7 @@ extern "C" {
 
 size_t vae_token_scratch_bytes(int64_t N, int64_t V, int64_t top_k, int dtype) {
   if (N < 1 || V < 1 || V > VAE_MAX_ROW || top_k < 0 || top_k > VAE_MAX_TOP) return 0;
-  const Cut c = cut_rows(N, V, dtype);
+  const Cut c = cut_rows(N, V, top_k, dtype);
   return c.parts == 1 ? 0 : (size_t)N * c.parts * (16 + 8 * (size_t)top_k);
 }
 
@@ -520,7 +523,7 @@ int vae_token_logp_fwd(const void* logits, int64_t row_stride, const void* token
   int rc = VAE_OK;
   ShortArgs sa = {logits, row_stride, tokens, token_bytes, N, (int)V, logp, entropy, stats, top_logp, top_ids, (int)top_k};
   if (short_rows(sa, dtype, (hipStream_t)stream, &rc)) return rc;
-  const Cut cut = cut_rows(N, V, dtype);
+  const Cut cut = cut_rows(N, V, top_k, dtype);
   if (cut.parts > 1 && !scratch) return VAE_ERR_ARG;
   const FwdArgs a = {logits, row_stride, tokens, token_bytes, logp, entropy, stats, top_logp, top_ids, (int)top_k, N,
                      (int)V, cut.parts, cut.part_vecs, (char*)scratch, kLog2e, 1.0f, {}};

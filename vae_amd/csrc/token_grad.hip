@@ -1,5 +1,6 @@
 // Gradients with respect to rows of logits [N, V]: of log probs, entropy and alternatives (token_logp_bwd), of the
-// distillation KL (distill_bwd), and both losses together with their gradient in one pass (token_fused_kernel).  Formulas and the conventions for masks: token_row.hpp.
+// distillation KL (distill_bwd), and both losses together with their gradient in one pass (token_fused_kernel).  Formulas
+// and the conventions for masks: token_row.hpp.
 //
 // Every one of them is   g_j = e_j (A + B d_j) + sum over a few entries (id, g) with id = j,   d = (x - m) c, e = 2^d:
 //   tokens:   A = -(sum_i g_i + g_H (H - ln s)) / s,  B = -g_H ln2 / s,  entries: the token and the alternatives
@@ -134,9 +135,9 @@ struct Piece {
 };
 
 // ---------------------------------------------------------------------------------------------------------------
-// from given statistics: one read, one write.  A workgroup takes one piece of U vectors a thread, all loads in front of
-// all stores: in a loop the loads of a turn wait for the stores of the turn before it (4096 x 32768 bf16: 153 us with
-// a loop over U = 4, see bwd_launch for what one piece takes).
+// from given statistics: one read, one write, and bound by them.  A workgroup takes one piece of U vectors a thread, all
+// loads in front of all stores: in a loop the loads of a turn wait for the stores of the turn before it.  4096 x 32768
+// bf16: 87 us (6.1 TB/s read + written), with entropy too; 153 us with a loop over U = 4.  Distillation, 64 entries: 85.
 // ---------------------------------------------------------------------------------------------------------------
 template <typename T, int VN, int BT, int U, bool ENT, bool LIST, bool DIST>
 __global__ __launch_bounds__(BT) void token_bwd_kernel(GradArgs a) {
@@ -157,9 +158,11 @@ __global__ __launch_bounds__(BT) void token_bwd_kernel(GradArgs a) {
     Piece<T, VN, BT, U> piece(x, gx, cut, v0, v1 - v0);
     const float m = a.stats_in[2 * row], s = a.stats_in[2 * row + 1];
     const int64_t tok = !DIST && a.tokens ? load_id(a.tokens, a.token_bytes, row) : 0;
-    if (tok < 0 || s == 0.f) {
-      piece.fill(a.nts, 0.f);
-      if (ei >= 0) gx[ei] = from_f32<T>(0.f);
+    const bool bad = !DIST && tok >= a.V && (!a.glogp || a.g_scale != 0.f);   // the gradient of its NaN
+    if (tok < 0 || s == 0.f || bad) {
+      const float v = bad ? nan_f() : 0.f;
+      piece.fill(a.nts, v);
+      if (ei >= 0) gx[ei] = from_f32<T>(v);
       continue;
     }
     TeacherTerms<BT> terms;
@@ -181,9 +184,8 @@ __global__ __launch_bounds__(BT) void token_bwd_kernel(GradArgs a) {
         lds.entries[0].put((int)threadIdx.x + r * BT, terms.id[r], -w * terms.q[r], cut, v0, v1);
       lds_barrier();
     } else {
-      float gt = a.tokens ? (a.glogp ? a.glogp[row / a.rows_per_g] * a.g_scale : a.g_scale) : 0.f;
+      const float gt = a.tokens ? (a.glogp ? a.glogp[row / a.rows_per_g] * a.g_scale : a.g_scale) : 0.f;
       const bool inside = a.tokens && tok < a.V;
-      if (tok >= a.V && (!a.glogp || a.g_scale != 0.f)) gt = nan_f();
       float sum = gt;
       adds.one_id = inside ? (int)tok : -1;
       adds.one_g = gt;
@@ -235,6 +237,8 @@ __global__ __launch_bounds__(BT) void token_bwd_kernel(GradArgs a) {
 // ---------------------------------------------------------------------------------------------------------------
 // loss and gradient in one pass: a workgroup holds its row in registers, U vectors a thread, as every element's
 // exponential against the thread's own maximum: one exponential an element, the gradient is a product.
+// Bound by memory: 4096 x 131072 bf16 400 us (5.4 TB/s read + written), 430 as a distillation; 8144 x 65536 381 us (5.6);
+// 16384 x 16384 181 us (5.9); two passes over the logits instead 525, 584, 553 and 268.
 //   in float32: 8 registers a 16-bit vector, 4 an fp32 one;
 //   HALF (bf16 rows that do not fit so): as 2^15 e in binary16, 4 registers a vector, where the packet was.  Its 11 bits
 //         are rounded once more to the gradient's 8; e < 2^-29, a probability 2^-29 of the thread's largest, begins to
@@ -402,9 +406,11 @@ static int bwd_launch(GradArgs a, hipStream_t st) {
 template <typename T, int VN, bool ENT, bool LIST, bool DIST>
 static int bwd_block(const GradArgs& a, hipStream_t st) {
   const int64_t nvec = ((int64_t)a.V + VN - 1) / VN;
+  // a wave a row where it fits (distillation of 65536 x 2048 bf16: 92 us, 146 with 256 threads; 1024: 58, 135)
   if (nvec <= 256) return bwd_launch<T, VN, 64, 4, ENT, LIST, DIST>(a, st);
-  // the entries are prepared once a piece: longer pieces where there are many
-  return bwd_launch<T, VN, kBlock, LIST ? 8 : 4, ENT, LIST, DIST>(a, st);
+  // U = 4 (65536 x 4096 bf16: 179 us; U = 8 192, U = 16 242).  Alternatives are looked through once a piece: twice as
+  // long a piece for them (4096 x 32768, 8 of them: U = 4 114 us, U = 8 102; the teacher's come prepared: 87 and 91).
+  return bwd_launch<T, VN, kBlock, LIST && !DIST ? 8 : 4, ENT, LIST, DIST>(a, st);
 }
 template <typename T, int VN, bool DIST>
 static int bwd_kind(const GradArgs& a, hipStream_t st) {
@@ -426,25 +432,36 @@ static int fused_launch(GradArgs a, hipStream_t st) {
   hipLaunchKernelGGL((token_fused_kernel<T, BT, U, HALF, DIST>), dim3(grid_for(a.N)), dim3(BT), 0, st, a);
   return launched();
 }
-// true when the one-pass kernel takes this call: the row fits a workgroup's registers, and there are rows enough
+// true when the one-pass kernel takes this call: the row fits a workgroup's registers, and there are rows enough.
+// fp16 never: a stored gradient is of a mean, whose 1 / N is a subnormal of fp16.
 template <typename T, bool DIST>
 static bool fused_type(const GradArgs& a, hipStream_t st, int* rc) {
-  constexpr int E = 64 / VecOf<T>::n;    // vectors a thread: 64 elements
-  const int64_t nvec = (int64_t)a.V / VecOf<T>::n;
-  // bf16 only: the other types' gradients have no bits to spare for HALF's rounding
-  constexpr int most = DTypeCode<T>::value == VAE_BF16 ? 16 : E;
-  if (!same_phase<T>(a) || nvec > 1024 * most || (a.N < 256 && nvec > 4096)) return false;
-  if (nvec <= 64 * E) *rc = fused_launch<T, 64, E, false, DIST>(a, st);
-  else if (nvec <= 128 * E) *rc = fused_launch<T, 128, E, false, DIST>(a, st);
-  else if (nvec <= 256 * E) *rc = fused_launch<T, 256, E, false, DIST>(a, st);
-  else if (nvec <= 512 * E) *rc = fused_launch<T, 512, E, false, DIST>(a, st);
-  else if (nvec <= 1024 * E) *rc = fused_launch<T, 1024, E, false, DIST>(a, st);
-  else if constexpr (most > E) *rc = fused_launch<T, 1024, most, true, DIST>(a, st);
-  return true;
+  if constexpr (DTypeCode<T>::value != VAE_F16) {
+    constexpr int E = 64 / VecOf<T>::n, H = E / 2;   // vectors a thread: 64 or 32 elements
+    const int64_t nvec = (int64_t)a.V / VecOf<T>::n;
+    // bf16 only: fp32's gradient has no bits to spare for HALF's rounding
+    constexpr int most = DTypeCode<T>::value == VAE_BF16 ? 16 : E;
+    // HALF with few rows: two launches that cut the rows (64 x 131072 bf16: 19.1 us, 20.8 in one; 1 x 98000 11.1, 14.0;
+    // but 100 x 131072: 25.9, 21.7; without HALF 16 x 65536 12.2, 10.7)
+    if (!same_phase<T>(a) || nvec > 1024 * most || (a.N <= 64 && nvec > 1024 * E && most > E)) return false;
+    // 32 elements a thread while 512 threads hold the row so: more waves in flight (32768 x 8192 bf16 179 us, 189 with
+    // 64; 8192 x 16384 fp32 186, 213); 64 beyond, where 1024 threads of 32 wait for each other longer (8192 x 32768 bf16:
+    // 193 us, 235 with 32)
+    if (nvec <= 64 * H) *rc = fused_launch<T, 64, H, false, DIST>(a, st);
+    else if (nvec <= 128 * H) *rc = fused_launch<T, 128, H, false, DIST>(a, st);
+    else if (nvec <= 256 * H) *rc = fused_launch<T, 256, H, false, DIST>(a, st);
+    else if (nvec <= 512 * H) *rc = fused_launch<T, 512, H, false, DIST>(a, st);
+    else if (nvec <= 512 * E) *rc = fused_launch<T, 512, E, false, DIST>(a, st);
+    else if (nvec <= 1024 * E) *rc = fused_launch<T, 1024, E, false, DIST>(a, st);
+    else if constexpr (most > E) *rc = fused_launch<T, 1024, most, true, DIST>(a, st);
+    return true;
+  }
+  return false;
 }
 
 static bool bad_teacher(int64_t K, float temperature) {
-  return K < 1 || K > VAE_MAX_TEACHER || !(temperature > 0.f) || !(temperature < INFINITY);
+  // below 4.3e-39 its reciprocal leaves fp32's range
+  return K < 1 || K > VAE_MAX_TEACHER || !(temperature > 4.3e-39f) || !(temperature < INFINITY);
 }
 static void set_temperature(GradArgs& a, float temperature) {
   a.scale2 = (float)(1.4426950408889634 / (double)temperature);

@@ -1,7 +1,8 @@
-// Short rows of logits (at most 256 vectors: 2048 16-bit or 1024 fp32 entries, 256 of either where a row is not aligned):
-// a row is held by a group of G lanes, several rows to a wave, and everything that is asked of it -- log prob,
-// entropy, alternatives, gradient -- comes from those registers.  The backward pass recomputes the row's statistics: they
-// cost less than reading them.  Formulas and the conventions for masks: token_row.hpp.
+// Short rows of logits (up to 1024 entries, 256 where rows are not aligned; see `takes`): a row is held by a group of G
+// lanes, several rows to a wave, and everything that is asked of it -- log prob, entropy, alternatives, gradient -- comes
+// from those registers.  The backward pass recomputes the row's statistics: they cost less than reading them.  Bound by
+// memory: loss and gradient of 200704 x 256 bf16 43 us (4.8 TB/s read + written), 65536 x 1024 fp32 87 us (6.2 TB/s).
+// Formulas and the conventions for masks: token_row.hpp.
 #include "token_row.hpp"
 
 namespace vae {
@@ -105,7 +106,6 @@ __global__ __launch_bounds__(kBlock) void token_short_kernel(ShortArgs a, int lo
                                             : (int64_t)((uint32_t)row / (uint32_t)a.rows_per_g);
           gt *= a.glogp[at];
         }
-        if (beyond && (!a.glogp || a.g_scale != 0.f)) gt = nan_f();
       }
       float sum = gt;
       for (int k = 0; k < a.gtop_k; ++k) sum += a.gtop[row * a.gtop_k + k];
@@ -117,7 +117,8 @@ __global__ __launch_bounds__(kBlock) void token_short_kernel(ShortArgs a, int lo
         B = -gh * kLn2 * inv;
       }
       const float A = -sum * inv;
-      const bool zero = pad || s == 0.f;
+      const bool bad = beyond && (!a.glogp || a.g_scale != 0.f);   // the gradient of its NaN
+      const bool fixed = pad || s == 0.f || bad;
       T* gx = (T*)a.glogits + row * (int64_t)a.V;
 #pragma unroll
       for (int u = 0; u < U; ++u) {
@@ -135,9 +136,9 @@ __global__ __launch_bounds__(kBlock) void token_short_kernel(ShortArgs a, int lo
         add(tok, gt);
         for (int k = 0; k < a.gtop_k; ++k) add((int)a.gtop_ids[row * a.gtop_k + k], a.gtop[row * a.gtop_k + k]);
         if (j < nvec) {
-          if (zero)
+          if (fixed)
 #pragma unroll
-            for (int i = 0; i < VN; ++i) o[i] = 0.f;
+            for (int i = 0; i < VN; ++i) o[i] = bad ? nan_f() : 0.f;
           store_vec<T, VN>(nts, gx + j * VN, o);
         }
       }
@@ -159,13 +160,25 @@ static int short_kind(const ShortArgs& a, const RowGeom& g, hipStream_t st) {
   return a.entropy ? short_launch<T, VN, kEnt>(a, g, st) : short_launch<T, VN, 0>(a, g, st);
 }
 
+// Which rows these kernels take, against the long ones (token.hip, token_grad.hip) for 65536 rows, in us:
+//   log prob of 256 bf16 9.3 / 27, 1024 bf16 29 / 38, 1024 fp32 41 / 42, but 2000 bf16 55 / 62 and 2048 bf16 54 / 49;
+//   loss and gradient 256 bf16 17 / 56, 1024 bf16 58 / 78, 1024 fp32 93 / 107, 2048 bf16 104 / 96: up to 1024 entries.
+//   Entropy's gradient holds value and exponential: 512 bf16 36 / 40, but 1024 bf16 65 / 54 (8 registers a vector each).
+//   Alternatives cost a turn over the registers each: 256 bf16 k = 8 44 / 73, k = 20 79 / 84; 512 bf16 k = 4 57 / 68,
+//   k = 8 80 / 75; 1024 bf16 k = 4 111 / 83: while k V < 4096; beyond 48 of them the long kernel's bound gives way (k = 64:
+//   256 bf16 213 / 486, 512 bf16 425 / 470, 1024 bf16 860 / 650).
+static bool takes(const ShortArgs& a, bool wide) {
+  if (a.V > 1024 || (a.glogits && a.gentropy && !wide && a.V > 512)) return false;
+  return (int64_t)a.top_k * a.V < 4096 || (a.top_k > 48 && a.V <= 512);
+}
+
 bool short_rows(const ShortArgs& a, int dtype, hipStream_t st, int* rc) {
   const int64_t vn = dtype == VAE_F32 ? 4 : 8;
   const bool vec = a.V % vn == 0 && (a.N <= 1 || a.row_stride % vn == 0) && aligned16(a.logits) &&
                    (!a.glogits || aligned16(a.glogits));
   const int64_t nvec = vec ? a.V / vn : a.V;
   RowGeom g;
-  if (nvec > 4 * 64 || !row_geom_resident(a.N, nvec, kGridStream, &g)) return false;
+  if (nvec > 4 * 64 || !takes(a, dtype == VAE_F32) || !row_geom_resident(a.N, nvec, kGridStream, &g)) return false;
   VAE_BY_TYPE(dtype, *rc = vec ? short_kind<T, VecOf<T>::n>(a, g, st) : short_kind<T, 1>(a, g, st));
   return true;
 }

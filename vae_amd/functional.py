@@ -535,9 +535,9 @@ def _check_vocab(logits, what):
 
 
 def _token_scratch(rows, top_k, dev):
-    """The pieces of split rows (fewer than 512, of at least 1024 16-byte vectors: csrc/token.hip): the caller's own
+    """The pieces of split rows (256 at most, of at least 8192 16-byte vectors: csrc/token.hip): the caller's own
     memory each call, so that calls on several streams and captured graphs share nothing."""
-    if rows.shape[0] >= 512 or rows.shape[1] < 4096:
+    if rows.shape[0] > 256 or rows.shape[1] < 32768:
         return None
     n = _lib.load().vae_token_scratch_bytes(rows.shape[0], rows.shape[1], top_k, dtype_code(rows))
     return torch.empty((n,), dtype=torch.uint8, device=dev) if n else None
@@ -640,6 +640,21 @@ def _check_tokens(x, recon):
     _check_vocab(recon, "nll 'categorical'")
 
 
+class _Stored:
+    """A gradient that the forward launch has formed, for one backward pass, which multiplies it in place: not for a pass
+    captured into a graph when the forward pass was not, since every replay would multiply it once more."""
+
+    def __init__(self, grad):
+        self.grad = grad
+        self.captured = grad is not None and torch.cuda.is_current_stream_capturing()
+
+    def take(self):
+        grad, self.grad = self.grad, None
+        if grad is not None and not self.captured and torch.cuda.is_current_stream_capturing():
+            return None
+        return grad
+
+
 class _TokenNllElbo(torch.autograd.Function):
     """Categorical nll [B] of B samples with T tokens each, with the ELBO combine (with_elbo; the six means as scalars of
     their own, in `mean_dtype`) and d(loss_mean)/d(logits) out of the same launch (fuse), as in _NllElboFused."""
@@ -648,7 +663,7 @@ class _TokenNllElbo(torch.autograd.Function):
     def forward(ctx, logits, tokens, kld, add, mi, kl_beta, inv_count, with_elbo, fuse, mean_dtype, want_nll):
         ctx.set_materialize_grads(False)
         dev = check_device(logits, tokens, kld, add, mi)
-        rows, B = _rows(logits), tokens.shape[0]
+        rows, B, code = _rows(logits), tokens.shape[0], dtype_code(logits)
         N, V = rows.shape
         # logp [N], stats [N, 2], means: one allocation
         buf = torch.empty((3 * N + MEANS,), dtype=torch.float32, device=dev)
@@ -664,10 +679,9 @@ class _TokenNllElbo(torch.autograd.Function):
             first = torch.empty((), dtype=mean_dtype, device=dev)
         launch(dev, 'vae_token_nll_elbo_fwd', ptr(rows), rows.stride(0), ptr(tokens), tokens.element_size(),
                N // max(B, 1), ptr(kld), ptr(add), ptr(mi), kl_beta, inv_count, at, at + 4 * N, ptr(grad), ptr(nll),
-               ptr(loss), ptr(elbo), means, ptr(first), DTYPE_CODES[mean_dtype], ptr(ws), ptr(scratch), B, V,
-               dtype_code(rows))
+               ptr(loss), ptr(elbo), means, ptr(first), DTYPE_CODES[mean_dtype], ptr(ws), ptr(scratch), B, V, code)
         ctx.save_for_backward(logits, tokens, buf)
-        ctx.grad = grad
+        ctx.grad = _Stored(grad)
         ctx.cfg = (kl_beta, inv_count, kld is not None, add is not None, mi is not None, mean_dtype)
         if not with_elbo:
             return (nll,) + (None,) * 8
@@ -686,7 +700,7 @@ class _TokenNllElbo(torch.autograd.Function):
         need = ctx.needs_input_grad
         terms = [torch.empty((B,), dtype=logits.dtype, device=dev) if has and need[i] else None
                  for i, has in ((2, has_kld), (3, has_add), (4, has_mi))]
-        grad, ctx.grad = ctx.grad, None
+        grad = ctx.grad.take()
         stored = gnll is None and gloss is None and gelbo is None and grad is not None
         # otherwise: the per-sample upstream gradient, in fp32 (1/B of a mean is a subnormal of fp16)
         grow = None if stored else torch.empty((B,), dtype=torch.float32, device=dev)
@@ -750,7 +764,7 @@ class _Distill(torch.autograd.Function):
         ctx.set_materialize_grads(False)
         kl, mean, grad, buf = _distill_fwd(logits, t_logits, t_ids, temperature, inv_count, fuse)
         ctx.save_for_backward(logits, buf)
-        ctx.grad = grad
+        ctx.grad = _Stored(grad)
         ctx.cfg = (temperature, inv_count, t_ids.shape[-1])
         return kl, mean
 
@@ -762,7 +776,7 @@ class _Distill(torch.autograd.Function):
         logits, buf = ctx.saved_tensors
         temperature, inv_count, K = ctx.cfg
         dev = logits.device
-        grad, ctx.grad = ctx.grad, None
+        grad = ctx.grad.take()
         gkl, gmean = _dense(gkl), _dense(gmean)
         if gkl is None and grad is not None:
             launch(dev, 'vae_grad_scale', ptr(grad), ptr(gmean), grad.numel(), dtype_code(grad))
