@@ -12,6 +12,13 @@ constexpr int kSlots = 1024;   // 64 ids leave about 2 pairs in one slot, 256 ab
 static_assert(VAE_MAX_ROW <= 1 << 24 && VAE_MAX_TEACHER <= 256, "an id and its place share 32 bits");
 __device__ __forceinline__ uint32_t slot_of(int id) { return (uint32_t)id * 2654435761u >> 22; }
 
+// LDS that only one wave uses: its lanes' writes in front of its lanes' reads, without a barrier of the workgroup (the
+// waves of one take different numbers of rounds)
+__device__ __forceinline__ void wave_fence() {
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+}
+
 template <int R>   // entries a lane
 __global__ __launch_bounds__(kBlock) void distill_teacher_kernel(const void* __restrict__ logits, int64_t stride, int dtype,
                                                                  const void* __restrict__ ids, int64_t id_stride,
@@ -20,7 +27,7 @@ __global__ __launch_bounds__(kBlock) void distill_teacher_kernel(const void* __r
                                                                  float* __restrict__ q_out, float* __restrict__ logq_out,
                                                                  int64_t N, int V) {
   __shared__ uint32_t slots[kBlock / 64][kSlots];
-  const int lane = threadIdx.x & 63;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   for (int64_t row = (int64_t)blockIdx.x * (kBlock / 64) + (threadIdx.x >> 6); row < N;
        row += (int64_t)gridDim.x * (kBlock / 64)) {
     float y[R], q[R], logq[R], m = kLowest;
@@ -59,7 +66,6 @@ __global__ __launch_bounds__(kBlock) void distill_teacher_kernel(const void* __r
     // own: it is the first to stand for its id.  The same id at another place: it is a second one.  Another id: once more,
     // without those that are settled.  Every round settles each slot's writer, so it ends.  (An entry compared with every
     // other one: 194 us for 65536 rows of 64 entries.)
-    volatile uint32_t* slot = slots[threadIdx.x >> 6];   // a wave's LDS accesses are in order
     bool todo[R], again[R];
 #pragma unroll
     for (int r = 0; r < R; ++r) {
@@ -73,14 +79,19 @@ __global__ __launch_bounds__(kBlock) void distill_teacher_kernel(const void* __r
       if (__ballot(any) == 0) break;
 #pragma unroll
       for (int r = 0; r < R; ++r)
-        if (todo[r]) slot[slot_of(id[r])] = (uint32_t)id[r] | (uint32_t)(lane + 64 * r) << 24;
+        if (todo[r])
+          __hip_atomic_store(&slots[wave][slot_of(id[r])], (uint32_t)id[r] | (uint32_t)(lane + 64 * r) << 24,
+                             __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WAVEFRONT);
+      wave_fence();
 #pragma unroll
       for (int r = 0; r < R; ++r)
         if (todo[r]) {
-          const uint32_t w = slot[slot_of(id[r])];
+          const uint32_t w = __hip_atomic_load(&slots[wave][slot_of(id[r])], __ATOMIC_RELAXED,
+                                               __HIP_MEMORY_SCOPE_WAVEFRONT);
           todo[r] = (w & 0xffffffu) != (uint32_t)id[r];
           again[r] = !todo[r] && (int)(w >> 24) != lane + 64 * r;
         }
+      wave_fence();
     }
     // one id's entries into the first of them: the sum of q, and of q ln q, in the entries' order
 #pragma unroll
