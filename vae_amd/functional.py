@@ -518,6 +518,7 @@ def categorical_kl(log_q, log_p):
 MAX_TOP = 64        # VAE_MAX_TOP in include/vae_amd.h
 MAX_TEACHER = 256   # VAE_MAX_TEACHER
 MEANS = 6 + 6 * 256  # VAE_TOKEN_MEANS_FLOATS
+_Pointers6 = ctypes.c_void_p * 6
 
 
 def _is_categorical(nll_type):
@@ -705,7 +706,7 @@ class _TokenNllElbo(torch.autograd.Function):
         # otherwise: the per-sample upstream gradient, in fp32 (1/B of a mean is a subnormal of fp16)
         grow = None if stored else torch.empty((B,), dtype=torch.float32, device=dev)
         gnll, gloss, gelbo = _dense(gnll), _dense(gloss), _dense(gelbo)
-        at = (ctypes.c_void_p * 6)(*[None if g is None else g.data_ptr() for g in gmeans])
+        at = _Pointers6(*[None if g is None else g.data_ptr() for g in gmeans])
         launch(dev, 'vae_token_nll_elbo_bwd', ptr(gnll), ptr(gloss), ptr(gelbo), at, DTYPE_CODES[mean_dtype], kl_beta,
                inv_count, ptr(grow), ptr(grad) if stored else None, grad.numel() if stored else 0, ptr(terms[0]),
                ptr(terms[1]), ptr(terms[2]), B, dtype_code(logits))
