@@ -498,14 +498,14 @@ int vae_token_logp_bwd(const void* logits, int64_t row_stride, const void* token
  * as vae_elbo_combine_fwd (abstract_vae.py:356-388) but from the unrounded nll, each rounded once.  loss == elbo == NULL:
  * nll alone; nll may be NULL otherwise.  glogits [B T, V] != NULL: also d(loss mean) / d logits, inv_count its 1/B: the
  * training step's one read of the logits.  means: VAE_TOKEN_MEANS_FLOATS floats, the six means in front, the rest scratch;
- * loss_mean (mean_dtype; may be NULL): the first of them once more, in a place of its own.  workspace (may be NULL): its
+ * loss_mean [1] and other_means [5] (mean_dtype; each may be NULL): the means once more, in places of their own.  workspace (may be NULL): its
  * saw-a-NaN word alone is used.                                                                                     */
 #define VAE_TOKEN_MEANS_FLOATS (6 + 6 * 256)
 int vae_token_nll_elbo_fwd(const void* logits, int64_t row_stride, const void* tokens, int token_bytes, int64_t T,
                            const void* kld, const void* add, const void* mi, float kl_beta, float inv_count, float* logp,
                            float* stats, void* glogits, void* nll, void* loss, void* elbo, float* means, void* loss_mean,
-                           int mean_dtype, float* workspace, void* scratch, int64_t B, int64_t V, int dtype,
-                           vae_stream_t stream);
+                           void* other_means, int mean_dtype, float* workspace, void* scratch, int64_t B, int64_t V,
+                           int dtype, vae_stream_t stream);
 /* Its backward.  gnll / gloss / gelbo [B] (dtype) and gmeans, a HOST array of 6 device pointers to one value each
  * (gmeans_dtype): every one may be NULL.  grow [B] (float32) = d / d nll[b], what vae_token_logp_bwd takes with
  * rows_per_g = T and g_scale = -1; or grad [n] = the forward's glogits, multiplied by

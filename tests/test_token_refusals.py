@@ -82,11 +82,12 @@ def bwd(**kw):
 
 def fused(**kw):
     a = dict(logits=P, stride=10, tokens=P, tb=8, T=1, kld=None, add=None, mi=None, beta=1.0, inv=1.0, logp=P, stats=P,
-             out=P, nll=P, loss=P, elbo=P, means=P, first=P, md=0, ws=P, scratch=P, N=2, V=10, dtype=0)
+             out=P, nll=P, loss=P, elbo=P, means=P, first=P, others=P, md=0, ws=P, scratch=P, N=2, V=10, dtype=0)
     a.update(kw)
     return _call('vae_token_nll_elbo_fwd',
                  [a[n] for n in ('logits', 'stride', 'tokens', 'tb', 'T', 'kld', 'add', 'mi', 'beta', 'inv', 'logp', 'stats',
-                                 'out', 'nll', 'loss', 'elbo', 'means', 'first', 'md', 'ws', 'scratch', 'N', 'V', 'dtype')]
+                                 'out', 'nll', 'loss', 'elbo', 'means', 'first', 'others', 'md', 'ws', 'scratch', 'N', 'V',
+                                 'dtype')]
                  + [None])
 
 

@@ -95,7 +95,7 @@ SIGNATURES = {
     'vae_token_scratch_bytes': [_i64, _i64, _i64, _i],
     'vae_token_logp_fwd': [_p, _i64, _p, _i, _p, _p, _p, _p, _p, _i64, _p, _i64, _i64, _i, _p],
     'vae_token_logp_bwd': [_p, _i64, _p, _i, _p, _p, _p, _i64, _f, _p, _p, _p, _i64, _p, _i64, _i64, _i, _p],
-    'vae_token_nll_elbo_fwd': [_p, _i64, _p, _i, _i64, _p, _p, _p, _f, _f, _p, _p, _p, _p, _p, _p, _p, _p, _i, _p, _p,
+    'vae_token_nll_elbo_fwd': [_p, _i64, _p, _i, _i64, _p, _p, _p, _f, _f, _p, _p, _p, _p, _p, _p, _p, _p, _p, _i, _p, _p,
                                _i64, _i64, _i, _p],
     'vae_token_nll_elbo_bwd': [_p, _p, _p, _pp, _i, _f, _f, _p, _p, _i64, _p, _p, _p, _i64, _i, _p],
     'vae_row_sums': [_p, _f, _p, _i64, _i64, _i, _p],

@@ -12,17 +12,23 @@ constexpr int kElboBlocks = 256;
 constexpr int kOneBlock = 1024;
 static_assert(VAE_TOKEN_MEANS_FLOATS == 6 + 6 * kElboBlocks, "the header says how long `means` is");
 
-__device__ __forceinline__ void store_any(void* p, int dtype, float v) {
-  if (dtype == VAE_F32) *reinterpret_cast<float*>(p) = v;
-  else if (dtype == VAE_BF16) *reinterpret_cast<bf16_t*>(p) = from_f32<bf16_t>(v);
-  else *reinterpret_cast<f16_t*>(p) = from_f32<f16_t>(v);
+__device__ __forceinline__ void store_any(void* p, int dtype, int i, float v) {
+  if (dtype == VAE_F32) reinterpret_cast<float*>(p)[i] = v;
+  else if (dtype == VAE_BF16) reinterpret_cast<bf16_t*>(p)[i] = from_f32<bf16_t>(v);
+  else reinterpret_cast<f16_t*>(p)[i] = from_f32<f16_t>(v);
 }
-// thread k < 6: total k -> mean k; thread 0 leaves the loss mean in its own place too
-__device__ __forceinline__ void write_mean(int k, double total, float inv_count, float* means, void* loss_mean,
-                                           int mean_dtype, float* ws) {
+// where the caller wants the means, in its own type; each may be NULL
+struct MeansTo {
+  void *loss, *others;
+  int dtype;
+};
+// thread k < 6: total k -> mean k
+__device__ __forceinline__ void write_mean(int k, double total, float inv_count, float* means, const MeansTo& to,
+                                           float* ws) {
   const float v = (float)(total * (double)inv_count);
   means[k] = v;
-  if (k == 0 && loss_mean) store_any(loss_mean, mean_dtype, v);
+  if (k == 0 && to.loss) store_any(to.loss, to.dtype, 0, v);
+  if (k > 0 && to.others) store_any(to.others, to.dtype, k - 1, v);
   if (ws) note_nan(ws, v, kNanElbo6, k);
 }
 
@@ -46,8 +52,7 @@ template <typename T, int BT>
 __global__ __launch_bounds__(BT) void token_elbo_fwd_kernel(
     const float* __restrict__ logp, int64_t len, const T* __restrict__ kld, const T* __restrict__ add,
     const T* __restrict__ mi, float kl_beta, float inv_count, T* __restrict__ nll, T* __restrict__ loss,
-    T* __restrict__ elbo, float* __restrict__ means, void* __restrict__ loss_mean, int mean_dtype,
-    float* __restrict__ ws, int64_t B, int G) {
+    T* __restrict__ elbo, float* __restrict__ means, MeansTo to, float* __restrict__ ws, int64_t B, int G) {
   __shared__ float part[BT / 64][6];
   const int rpb = BT / G, sub = threadIdx.x % G, rloc = threadIdx.x / G;
   float acc[6] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
@@ -78,18 +83,17 @@ __global__ __launch_bounds__(BT) void token_elbo_fwd_kernel(
     const int k = threadIdx.x;
     float s = 0.f;
     for (int w = 0; w < BT / 64; ++w) s += part[w][k];
-    if (gridDim.x == 1) write_mean(k, s, inv_count, means, loss_mean, mean_dtype, ws);
+    if (gridDim.x == 1) write_mean(k, s, inv_count, means, to, ws);
     else means[6 + 6 * blockIdx.x + k] = s;
   }
 }
 __global__ __launch_bounds__(64) void token_elbo_means_kernel(float* __restrict__ means, int blocks, float inv_count,
-                                                              void* __restrict__ loss_mean, int mean_dtype,
-                                                              float* __restrict__ ws) {
+                                                              MeansTo to, float* __restrict__ ws) {
   for (int k = 0; k < 6; ++k) {
     double v = 0.0;
     for (int b = threadIdx.x; b < blocks; b += 64) v += (double)means[6 + 6 * b + k];
     v = wave_sum_d(v);
-    if ((int)threadIdx.x == k) write_mean(k, v, inv_count, means, loss_mean, mean_dtype, ws);
+    if ((int)threadIdx.x == k) write_mean(k, v, inv_count, means, to, ws);
   }
 }
 
@@ -169,10 +173,10 @@ extern "C" {
 int vae_token_nll_elbo_fwd(const void* logits, int64_t row_stride, const void* tokens, int token_bytes, int64_t len,
                            const void* kld, const void* add, const void* mi, float kl_beta, float inv_count, float* logp,
                            float* stats, void* glogits, void* nll, void* loss, void* elbo, float* means, void* loss_mean,
-                           int mean_dtype, float* workspace, void* scratch, int64_t B, int64_t V, int dtype,
-                           vae_stream_t stream) {
+                           void* other_means, int mean_dtype, float* workspace, void* scratch, int64_t B, int64_t V,
+                           int dtype, vae_stream_t stream) {
   if (B < 0 || len < 0 || V < 1 || V > VAE_MAX_ROW || (B * len > 1 && row_stride < V) || !type_ok(dtype) ||
-      (loss_mean && !type_ok(mean_dtype)))
+      ((loss_mean || other_means) && !type_ok(mean_dtype)))
     return VAE_ERR_ARG;
   if (B == 0) return VAE_OK;
   const int64_t N = B * len;
@@ -187,6 +191,7 @@ int vae_token_nll_elbo_fwd(const void* logits, int64_t row_stride, const void* t
                  : vae_token_logp_fwd(logits, row_stride, tokens, token_bytes, logp, nullptr, stats, nullptr, nullptr, 0,
                                       scratch, N, V, dtype, stream);
   if (rc != VAE_OK) return rc;
+  const MeansTo to = {loss_mean, other_means, mean_dtype};
   int G = 1;
   while (G < 64 && G < len) G <<= 1;
   const int64_t blocks = (B + kBlock / G - 1) / (kBlock / G);
@@ -199,12 +204,12 @@ int vae_token_nll_elbo_fwd(const void* logits, int64_t row_stride, const void* t
 #define VAE_ELBO_FWD(BT)                                                                                                \
   hipLaunchKernelGGL((token_elbo_fwd_kernel<T, BT>), dim3(grid), dim3(BT), 0, (hipStream_t)stream, logp, len,            \
                      (const T*)kld, (const T*)add, (const T*)mi, kl_beta, inv_count, (T*)nll, (T*)loss, (T*)elbo, means, \
-                     loss_mean, mean_dtype, workspace, B, G)
+                     to, workspace, B, G)
   VAE_BY_TYPE(dtype, if (one) VAE_ELBO_FWD(kOneBlock); else VAE_ELBO_FWD(kBlock));
 #undef VAE_ELBO_FWD
   if (loss && grid > 1)
     hipLaunchKernelGGL(token_elbo_means_kernel, dim3(1), dim3(64), 0, (hipStream_t)stream, means, grid, inv_count,
-                       loss_mean, mean_dtype, workspace);
+                       to, workspace);
   return launched();
 }
 

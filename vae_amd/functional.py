@@ -671,16 +671,17 @@ class _TokenNllElbo(torch.autograd.Function):
         at = buf.data_ptr()
         grad = torch.empty(logits.shape, dtype=logits.dtype, device=dev) if fuse else None
         nll = torch.empty((B,), dtype=logits.dtype, device=dev) if want_nll else None
-        loss = elbo = first = means = ws = None
+        loss = elbo = first = others = means = ws = None
         scratch = _token_scratch(rows, 0, dev)
         if with_elbo:
             loss = torch.empty((B,), dtype=logits.dtype, device=dev)
             elbo = torch.empty_like(loss)
             means, ws = at + 12 * N, workspace(dev)
-            first = torch.empty((), dtype=mean_dtype, device=dev)
+            first, others = torch.empty((), dtype=mean_dtype, device=dev), torch.empty((5,), dtype=mean_dtype, device=dev)
         launch(dev, 'vae_token_nll_elbo_fwd', ptr(rows), rows.stride(0), ptr(tokens), tokens.element_size(),
                N // max(B, 1), ptr(kld), ptr(add), ptr(mi), kl_beta, inv_count, at, at + 4 * N, ptr(grad), ptr(nll),
-               ptr(loss), ptr(elbo), means, ptr(first), DTYPE_CODES[mean_dtype], ptr(ws), ptr(scratch), B, V, code)
+               ptr(loss), ptr(elbo), means, ptr(first), ptr(others), DTYPE_CODES[mean_dtype], ptr(ws), ptr(scratch), B, V,
+               code)
         ctx.save_for_backward(logits, tokens, buf)
         ctx.grad = _Stored(grad)
         ctx.cfg = (kl_beta, inv_count, kld is not None, add is not None, mi is not None, mean_dtype)
@@ -688,9 +689,9 @@ class _TokenNllElbo(torch.autograd.Function):
             return (nll,) + (None,) * 8
         if B == 0:
             first.zero_()
-            buf.zero_()
+            others.zero_()
         # the loss mean is a tensor of its own (a caller may scale it in place), the other five are views of one
-        return (nll, loss, elbo, first) + buf[3 * N + 1:3 * N + 6].to(mean_dtype).unbind(0)
+        return (nll, loss, elbo, first) + others.unbind(0)
 
     @staticmethod
     @once_differentiable
