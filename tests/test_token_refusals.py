@@ -53,6 +53,9 @@ def test_python_refusals():
         F_.distill_top_logits(x, torch.zeros(4, 2, requires_grad=True), ids)
     with pytest.raises(TypeError):
         F_.sample_sums(torch.zeros(4, 2, dtype=torch.float64))
+    for term in ('kld', 'add', 'mi'):       # the kernel reads one of each for every sample
+        with pytest.raises(ValueError, match=term):
+            F_.nll_elbo(tok, x, 'categorical', **{term: torch.zeros(3)})
 
 
 def _call(name, args):

@@ -726,6 +726,10 @@ def token_nll_elbo(x, recon_x, kld=None, add=None, mi=None, kl_beta=1.0, inv_cou
     _check_tokens(x, recon_x)
     if inv_count is None:
         inv_count = 1.0 / max(x.shape[0], 1)
+    for name, t in (('kld', kld), ('add', add), ('mi', mi)):
+        if t is not None and t.numel() != x.shape[0]:
+            raise ValueError("nll_elbo: %s must hold a value for each of the %d samples, got %s"
+                             % (name, x.shape[0], tuple(t.shape)))
     kld, add, mi = (None if t is None else t.to(recon_x.dtype).contiguous() for t in (kld, add, mi))
     # fp16: two passes, for the reason given in nll_elbo
     fuse = bool(fuse_backward and recon_x.dtype != torch.float16 and recon_x.requires_grad and torch.is_grad_enabled()
