@@ -403,6 +403,40 @@ def test_nll_forms_agree():
     check_grad(g, ref_elbo(zs[0].double(), xs[0], torch.zeros(B).double(), 1.0)[3] / B, 1.0 / B)
 
 
+@pytest.mark.parametrize('dt', ['bf16', 'f16'])
+def test_forms_that_add_up_round_once(dt):
+    """The multi-sample and the per-step form on 16-bit logits, with fp32 terms of the host's: every output is one rounding
+    of the fp32 value (half a step), the gradients are whole."""
+    from vae_amd import functional as F_
+    B, T, V, S = 5, 4, 300, 3
+    zs = [torch.randn(B, T, V, generator=gen(i)).to(TYPES[dt]) for i in range(S)]
+    x = torch.randint(-1, V, (B, T), generator=gen(9))
+    kld, add = torch.rand(B, generator=gen(1)) * 30, torch.rand(B, generator=gen(2))
+    refs = [ref_elbo(z.double(), x, torch.zeros(B).double(), 1.0) for z in zs]
+    half = HALF[TYPES[dt]]
+    nll = sum(r[0] for r in refs) / S
+    leaves = [z.to(DEV).requires_grad_(True) for z in zs]
+    k = kld.to(DEV).requires_grad_(True)
+    out = F_.nll_multi_elbo(x.to(DEV), leaves, 'categorical', kld=k, add=add.to(DEV), kl_beta=0.5)
+    assert all(t.dtype == TYPES[dt] for t in out[:3])
+    for got, want in zip(out, (nll, nll + add.double() + 0.5 * kld.double(), nll + kld.double())):
+        close(got, want, half + 1e-6, 1e-5)
+    close(out[3][:4], torch.stack([(nll + add.double() + 0.5 * kld.double()).mean(), (nll + kld.double()).mean(),
+                                   nll.mean(), kld.double().mean()]), 1e-6, 1e-5)
+    gs = torch.autograd.grad(out[3][0], leaves + [k])
+    for g, r in zip(gs, refs):
+        check_grad(g, r[3] / (B * S), 1.0 / (B * S))
+    close(gs[-1], torch.full((B,), 0.5 / B).double(), 2.0 ** -22, 0.0)
+    steps = F_.nll_steps_elbo([x.to(DEV)] * S, [z.to(DEV) for z in zs], 'categorical', kld=kld.repeat(S).to(DEV))
+    per = torch.stack([r[0] + kld.double() for r in refs])
+    close(steps[1], per.reshape(-1), half + 1e-6, 1e-5)
+    close(steps[4], per.mean(0), half + 1e-6, 1e-5)
+    with pytest.raises(ValueError):
+        F_.nll_multi_elbo(x.to(DEV), leaves, 'categorical', kld=k[:2])
+    with pytest.raises(ValueError):
+        F_.nll_steps_elbo([x.to(DEV)] * S, [z.to(DEV) for z in zs], 'categorical', kld=k)
+
+
 def test_vrnn_loss_over_categorical_steps():
     """VRNNMixin scores categorical steps one by one; a stateful annealer weighs every step by its own value."""
     from vae_amd.vrnn import VRNNMixin

@@ -719,6 +719,27 @@ class _TokenNllElbo(torch.autograd.Function):
         return (grad, None) + tuple(terms) + (None,) * 6
 
 
+def _check_terms(B, kld, add, mi):
+    for name, t in (('kld', kld), ('add', add), ('mi', mi)):
+        if t is not None and t.numel() != B:
+            raise ValueError("nll_elbo: %s must hold a value for each of the %d samples, got %s"
+                             % (name, B, tuple(t.shape)))
+
+
+def _token_nll(x, recon):
+    """Categorical nll [B] in float32, for what is still to be added up."""
+    _check_tokens(x, recon)
+    return -sample_sums(token_log_probs(recon, x.reshape(recon.shape[:-1]), want_entropy=False)[0])
+
+
+def _token_combine(nll_, kld, add, mi, kl_beta, inv_count, dtype):
+    """elbo_combine of float32 nll [B]; (nll, loss, elbo) rounded once, to `dtype`, and means[6]."""
+    _check_terms(nll_.shape[0], kld, add, mi)
+    kld, add, mi = (None if t is None else t.float().reshape(-1) for t in (kld, add, mi))
+    loss, elbo, means = elbo_combine(nll_, kld=kld, add=add, mi=mi, kl_beta=float(kl_beta), inv_count=inv_count)
+    return nll_.to(dtype), loss.to(dtype), elbo.to(dtype), means
+
+
 def token_nll_elbo(x, recon_x, kld=None, add=None, mi=None, kl_beta=1.0, inv_count=None, fuse_backward=False,
                    mean_dtype=torch.float32, want_nll=True):
     """nll_elbo for nll_type 'categorical' with the six means as scalars: (nll [B] or None, loss, elbo [B], 6 scalars in
@@ -726,10 +747,8 @@ def token_nll_elbo(x, recon_x, kld=None, add=None, mi=None, kl_beta=1.0, inv_cou
     _check_tokens(x, recon_x)
     if inv_count is None:
         inv_count = 1.0 / max(x.shape[0], 1)
-    for name, t in (('kld', kld), ('add', add), ('mi', mi)):
-        if t is not None and t.numel() != x.shape[0]:
-            raise ValueError("nll_elbo: %s must hold a value for each of the %d samples, got %s"
-                             % (name, x.shape[0], tuple(t.shape)))
+    _check_terms(x.shape[0], kld, add, mi)
+    # the terms in the logits' type, as loss and elbo come out: half a step of each term beside half a step of the sum
     kld, add, mi = (None if t is None else t.to(recon_x.dtype).contiguous() for t in (kld, add, mi))
     # fp16: two passes, for the reason given in nll_elbo
     fuse = bool(fuse_backward and recon_x.dtype != torch.float16 and recon_x.requires_grad and torch.is_grad_enabled()
@@ -749,16 +768,14 @@ def _token_steps_elbo(xs, recons, kld, add, mi, kl_beta, inv_count, with_lse):
             raise NotImplementedError("nll_steps_elbo: 'categorical' takes one KL weight for all steps (a host model "
                                       "with an annealer scores its steps one by one: vae_amd.vrnn.loss_function)")
         kl_beta = kl_beta[0]
-    for name, v in (('kld', kld), ('add', add), ('mi', mi)):
-        if v is not None and v.numel() != T * B:
-            raise ValueError("nll_steps_elbo: %s must hold T*B = %d values, got %d" % (name, T * B, v.numel()))
-    nll_ = torch.cat([nll(x, r, 'categorical') for x, r in zip(xs, recons)], 0)
+    nll_ = torch.cat([_token_nll(x, r) for x, r in zip(xs, recons)], 0)
     if nll_.numel() != T * B:
         raise ValueError("nll_steps_elbo: every step must have the same shapes and dtype")
-    loss, elbo, means = elbo_combine(nll_, kld=kld, add=add, mi=mi, kl_beta=float(kl_beta),
-                                     inv_count=1.0 / max(T * B, 1) if inv_count is None else inv_count)
-    out = (nll_, loss, elbo, means, loss.view(T, B).mean(0), elbo.view(T, B).mean(0))
-    return out + (torch.logsumexp(elbo.detach().view(T, B), 0),) if with_lse else out
+    dtype = recons[0].dtype
+    nll_, loss, elbo, means = _token_combine(nll_, kld, add, mi, kl_beta, inv_count, torch.float32)
+    out = tuple(t.to(dtype) for t in (nll_, loss, elbo)) + (means,)
+    out += (loss.view(T, B).mean(0).to(dtype), elbo.view(T, B).mean(0).to(dtype))
+    return out + (torch.logsumexp(elbo.detach().view(T, B), 0).to(dtype),) if with_lse else out
 
 
 class _Distill(torch.autograd.Function):
@@ -1479,14 +1496,10 @@ def nll_multi_elbo(x, recons, nll_type, kld=None, add=None, mi=None, kl_beta=1.0
     nll_type 'categorical': one launch per output, then the same."""
     S = len(recons)
     if _is_categorical(nll_type):
-        total = None
-        for r in recons:
-            part = nll(x, r, nll_type) / S
-            total = part if total is None else total + part
+        total = sum(_token_nll(x, r) for r in recons) / S
         if not with_elbo:
-            return total, None, None, None
-        loss, elbo, means = elbo_combine(total, kld=kld, add=add, mi=mi, kl_beta=kl_beta, inv_count=inv_count)
-        return total, loss, elbo, means
+            return total.to(recons[0].dtype), None, None, None
+        return _token_combine(total, kld, add, mi, kl_beta, inv_count, recons[0].dtype)
     flat = [_flat_pixels(x, r, nll_type) for r in recons]
     code, xf = flat[0][0], flat[0][1]
     rfs = [f[2] for f in flat]
