@@ -6,6 +6,7 @@ current HIP stream through `_lib.call` and never synchronises.  Shapes are flatt
 reference's shapes.
 """
 import ctypes
+import functools
 
 import torch
 from torch.autograd.function import once_differentiable
@@ -535,12 +536,17 @@ def _check_vocab(logits, what):
         raise ValueError("%s: logits need a last dimension over the vocabulary, got %s" % (what, tuple(logits.shape)))
 
 
+@functools.lru_cache(maxsize=256)
+def _scratch_bytes(N, V, top_k, code):
+    return _lib.load().vae_token_scratch_bytes(N, V, top_k, code)
+
+
 def _token_scratch(rows, top_k, dev):
     """The pieces of split rows (256 at most, of at least 8192 16-byte vectors: csrc/token.hip): the caller's own
     memory each call, so that calls on several streams and captured graphs share nothing."""
     if rows.shape[0] > 256 or rows.shape[1] < 32768:
         return None
-    n = _lib.load().vae_token_scratch_bytes(rows.shape[0], rows.shape[1], top_k, dtype_code(rows))
+    n = _scratch_bytes(rows.shape[0], rows.shape[1], top_k, dtype_code(rows))
     return torch.empty((n,), dtype=torch.uint8, device=dev) if n else None
 
 
