@@ -1,0 +1,111 @@
+"""Categorical observations where they can go wrong: gradients inside a larger buffer, small temperatures, logits far apart,
+terms of another type or shape.  Against float64 on the CPU.
+
+Gradients are checked element by element.  p_j = 2^d / s: d = (x - m) c takes two roundings, at most |d| 2^-23 off in the
+exponent, 64 2^-23 ln2 = 5.3e-6 of p where |d| <= 64; v_exp_f32 and the sum add less than 2.5e-6 (V <= 2^18 terms in 256 or
+more partial sums).  So p is within 8e-6 of itself and the result is rounded once: eps / 2.  Only where an entry is added to
+it (the token's, the teacher's) do two terms cancel: there 8e-6 of the upstream factor, absolutely."""
+import pytest
+import torch
+
+from vae_amd import _lib
+
+pytestmark = pytest.mark.gpu
+DEV = 'cuda:0'
+TYPES = {'f32': torch.float32, 'bf16': torch.bfloat16, 'f16': torch.float16}
+
+
+def gen(seed):
+    return torch.Generator().manual_seed(seed)
+
+
+def check_elements(g, ref, entries, scale, more=0.0):
+    """`entries`: truth values, where a second term was added; `scale`: the upstream factor; `more`: another rounding."""
+    tol = (torch.finfo(g.dtype).eps / 2 + 8e-6 + more) * ref.abs() + 8e-6 * scale * entries
+    if g.dtype == torch.float16:
+        tol = tol + 2.0 ** -25                     # half a step of its subnormals
+    off = (g.detach().double().cpu() - ref).abs()
+    worst = (off / tol.clamp(min=1e-300)).max()
+    assert bool((off <= tol).all()), 'up to %g times the tolerance' % worst
+
+
+# ---------------------------------------------------------------------------------------------------------------------
+# memory around a gradient
+# ---------------------------------------------------------------------------------------------------------------------
+GUARD = 150000          # elements: more than the longest piece a workgroup stores
+
+
+class Guarded:
+    """[N, V] inside a buffer of sevens, `off` elements behind a 16-byte boundary."""
+
+    def __init__(self, N, V, dtype, off):
+        self.all = torch.full((N * V + 2 * GUARD + 8,), 7.0, dtype=dtype, device=DEV)
+        self.lo, self.hi = GUARD + off, GUARD + off + N * V
+        self.rows = self.all[self.lo:self.hi].view(N, V)
+
+    def check(self):
+        assert bool((self.all[:self.lo] == 7).all()) and bool((self.all[self.hi:] == 7).all())
+
+
+@pytest.mark.parametrize('dt', ['f32', 'bf16', 'f16'])
+@pytest.mark.parametrize('V', [3, 8, 9, 300, 1500, 5000, 20000, 50021, 70001, 140001])
+@pytest.mark.parametrize('off', [0, 1])
+def test_nothing_is_written_beside_a_gradient(V, dt, off):
+    """Padded rows, the last one among them, in every gradient kernel: the fill of a row or a piece that is shorter than its
+    workgroup stays inside it, and the rows in front of it keep their values."""
+    N, dtype = 4, TYPES[dt]
+    code = _lib.DTYPE_CODES[dtype]
+    dev = torch.device(DEV)
+    x = (torch.randn(N, V, generator=gen(V)) * 2).to(dtype)
+    z = x.double()
+    xd = x.to(DEV)
+    new = lambda *s: torch.empty(s, dtype=torch.float32, device=DEV)
+    p_ = _lib.ptr
+    tok = torch.tensor([V // 2, -1, V - 1, -1])
+    td = tok.to(DEV)
+    live = tok >= 0
+    logp = torch.log_softmax(z, -1)
+    p = logp.exp() * live[:, None]
+    at = torch.zeros(N, V, dtype=torch.bool)
+    at[torch.arange(N), tok.clamp(min=0)] = live
+    scratch = torch.empty(_lib.load().vae_token_scratch_bytes(N, V, 0, code) + 8, dtype=torch.uint8, device=DEV)
+
+    lp, stats = new(N), new(N, 2)
+    _lib.launch(dev, 'vae_token_logp_fwd', p_(xd), V, p_(td), 8, p_(lp), None, p_(stats), None, None, 0, p_(scratch), N, V,
+                code)
+    g = Guarded(N, V, dtype, off)
+    w = torch.tensor([0.5, 3.0, -2.0, 4.0])
+    wd = w.to(DEV)
+    _lib.launch(dev, 'vae_token_logp_bwd', p_(xd), V, p_(td), 8, p_(stats), None, p_(wd), 1, 1.0, None, None, None, 0,
+                p_(g.rows), N, V, code)
+    g.check()
+    check_elements(g.rows, w.double()[:, None] * (at.double() - p), at, 2.0)
+
+    nll, buf = torch.empty(N, dtype=dtype, device=DEV), new(3 * N)
+    g = Guarded(N, V, dtype, off)
+    _lib.launch(dev, 'vae_token_nll_elbo_fwd', p_(xd), V, p_(td), 8, 1, None, None, None, 0.0, 0.25, buf.data_ptr(),
+                buf.data_ptr() + 4 * N, p_(g.rows), p_(nll), None, None, None, None, None, 0, None, p_(scratch), N, V, code)
+    g.check()
+    # bf16 rows that are kept as binary16 exponentials: 2^-12 more
+    check_elements(g.rows, 0.25 * (p - at.double()), at, 0.25, 2.0 ** -12 if dt == 'bf16' and V > 65536 else 0.0)
+
+    K, tau = 3, 1.5
+    y = torch.randn(N, K, generator=gen(1))
+    ids = torch.randint(0, V, (N, K), generator=gen(2))
+    ids[1] = ids[3] = -1
+    yd, idd = y.to(DEV), ids.to(DEV)
+    teacher, kl = new(_lib.load().vae_distill_teacher_floats(N, K)), new(N)
+    q = torch.softmax(y.double() / tau, -1) * live[:, None]
+    ref = torch.softmax(z / tau, -1) * live[:, None]
+    ref.scatter_add_(1, ids.clamp(min=0), -q)
+    at = torch.zeros(N, V, dtype=torch.bool)
+    at.scatter_(1, ids.clamp(min=0), True)
+    g = Guarded(N, V, dtype, off)
+    _lib.launch(dev, 'vae_distill_fwd', p_(xd), V, p_(yd), K, 0, p_(idd), K, 8, K, tau, p_(teacher), p_(kl), None, 0.5,
+                p_(stats), p_(g.rows), p_(scratch), N, V, code)
+    g.check()
+    check_elements(g.rows, 0.5 / tau * ref, at, 0.5 / tau, 2.0 ** -12 if dt == 'bf16' and V > 65536 else 0.0)
+    g = Guarded(N, V, dtype, off)
+    _lib.launch(dev, 'vae_distill_bwd', p_(xd), V, p_(teacher), K, tau, p_(stats), p_(wd), None, 0.0, p_(g.rows), N, V, code)
+    g.check()
+    check_elements(g.rows, w.double()[:, None] / tau * ref, at, 2.0 / tau)

@@ -93,7 +93,7 @@ __device__ __forceinline__ void row_stats(const T* __restrict__ x, const RowCut<
   }
   for (; j < v1; j += BT) {
     Packet<T, VN> p[1];
-    p[0].template load<NT>(body, j * kVecBytes, 0);
+    p[0].template load<NT>(body, j * kVecBytes);
     group(p);
   }
   mine = st.m;
@@ -123,7 +123,7 @@ __device__ __forceinline__ void row_stats(const T* __restrict__ x, const RowCut<
   };
   for (j = v0 + (int)threadIdx.x; j < v1; j += BT) {
     Packet<T, VN> p;
-    p.template load<NT>(body, j * kVecBytes, 0);
+    p.template load<NT>(body, j * kVecBytes);
     float v[VN];
     p.get(v);
 #pragma unroll
@@ -207,7 +207,7 @@ __device__ __forceinline__ void row_top(TopLds<BT>& lds, const T* __restrict__ x
   const int tid = threadIdx.x;
   auto each = [&](int j, auto f) {   // the elements of vector j
     Packet<T, VN> p;
-    p.template load<false>(body, j * kVecBytes, 0);
+    p.template load<false>(body, j * kVecBytes);
     float v[VN];
     p.get(v);
 #pragma unroll

@@ -115,7 +115,7 @@ struct Piece {
   __device__ __forceinline__ bool any(int u) const { return u * BT < nvec; }   // the same for all threads
   __device__ __forceinline__ void load() {
 #pragma unroll
-    for (int u = 0; u < U; ++u) p[u].load(in, byte, u * BT * P::kBytes);
+    for (int u = 0; u < U; ++u) p[u].load(in, byte + u * BT * P::kBytes);
   }
   __device__ __forceinline__ void mask() {       // what is not there counts as masked out
 #pragma unroll
@@ -123,14 +123,17 @@ struct Piece {
       if ((u + 1) * BT > nvec && (int)threadIdx.x + u * BT >= nvec) p[u].set_masked();
   }
   __device__ __forceinline__ void store(bool nts, int u, const float (&v)[VN]) const {
-    P::store(out, nts, byte, u * BT * P::kBytes, v);
+    int at = byte;
+    asm volatile("" : "+v"(at));   // added up again: the loads' offsets are not kept in registers for it
+    P::store(out, nts, at + u * BT * P::kBytes, v);
   }
   __device__ __forceinline__ void fill(bool nts, float value) const {
     float v[VN];
 #pragma unroll
     for (int i = 0; i < VN; ++i) v[i] = value;
 #pragma unroll
-    for (int u = 0; u < U; ++u) store(nts, u, v);
+    for (int u = 0; u < U; ++u)
+      if (any(u)) store(nts, u, v);
   }
 };
 

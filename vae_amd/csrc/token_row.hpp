@@ -132,9 +132,10 @@ struct RowCut {
   __device__ __forceinline__ int index(int vec) const { return head + vec * VN; }
 };
 
-// A run of memory behind a buffer descriptor: the base and the length sit in scalar registers, a lane brings one 32-bit
-// byte offset for all its accesses, and the hardware checks every access against the length: a load beyond it returns
-// zeros and a store beyond it is dropped, without a branch or a predicate.
+// A run of memory behind a buffer descriptor: the base and the length sit in scalar registers, a lane brings a 32-bit byte
+// offset, and the hardware checks that offset against the length: a load beyond it returns zeros and a store beyond it is
+// dropped, without a branch or a predicate.  The check covers the LANE's offset alone, not the instruction's scalar one, so
+// whatever may lie beyond the run is addressed by the lane's offset.
 struct Buffer {
   __amdgpu_buffer_rsrc_t rsrc;
   __device__ __forceinline__ Buffer(const void* base, int bytes)
@@ -148,9 +149,10 @@ struct Packet {
   typedef uint32_t Raw __attribute__((ext_vector_type(4)));
   static constexpr int kBytes = 16;
   Raw raw;
-  template <bool NT = true>   // NT: not read again
-  __device__ __forceinline__ void load(const Buffer& b, int lane_byte, int byte) {
-    raw = __builtin_amdgcn_raw_buffer_load_b128(b.rsrc, lane_byte, byte, NT ? kNonTemporal : 0);
+  // `inside` is a scalar offset: lane_byte + inside is known to be within the run.  NT: not read again
+  template <bool NT = true>
+  __device__ __forceinline__ void load(const Buffer& b, int lane_byte, int inside = 0) {
+    raw = __builtin_amdgcn_raw_buffer_load_b128(b.rsrc, lane_byte, inside, NT ? kNonTemporal : 0);
   }
   __device__ __forceinline__ void set_masked() {   // every element -inf
     const uint32_t inf = sizeof(T) == 4 ? 0xff800000u : (DTypeCode<T>::value == 2 ? 0xfc00fc00u : 0xff80ff80u);
@@ -171,16 +173,15 @@ struct Packet {
       }
     }
   }
-  __device__ __forceinline__ static void store(const Buffer& b, bool nts, int lane_byte, int byte,
-                                               const float (&v)[VN]) {
+  __device__ __forceinline__ static void store(const Buffer& b, bool nts, int lane_byte, const float (&v)[VN]) {
     Raw r;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       if constexpr (sizeof(T) == 4) r[i] = __float_as_uint(v[i]);
       else r[i] = pack2<T>(v[2 * i], v[2 * i + 1]);
     }
-    if (nts) __builtin_amdgcn_raw_buffer_store_b128(r, b.rsrc, lane_byte, byte, kNonTemporal);
-    else __builtin_amdgcn_raw_buffer_store_b128(r, b.rsrc, lane_byte, byte, 0);
+    if (nts) __builtin_amdgcn_raw_buffer_store_b128(r, b.rsrc, lane_byte, 0, kNonTemporal);
+    else __builtin_amdgcn_raw_buffer_store_b128(r, b.rsrc, lane_byte, 0, 0);
   }
 };
 // rows whose gradient is not aligned as they are: element by element
@@ -189,15 +190,15 @@ struct Packet<T, 1> {
   static constexpr int kBytes = sizeof(T);
   T raw;
   template <bool NT = true>
-  __device__ __forceinline__ void load(const Buffer& b, int lane_byte, int byte) {
-    if constexpr (sizeof(T) == 4) raw = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(b.rsrc, lane_byte, byte, 0));
-    else raw.bits = __builtin_amdgcn_raw_buffer_load_b16(b.rsrc, lane_byte, byte, 0);
+  __device__ __forceinline__ void load(const Buffer& b, int lane_byte) {
+    if constexpr (sizeof(T) == 4) raw = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(b.rsrc, lane_byte, 0, 0));
+    else raw.bits = __builtin_amdgcn_raw_buffer_load_b16(b.rsrc, lane_byte, 0, 0);
   }
   __device__ __forceinline__ void set_masked() { raw = from_f32<T>(-INFINITY); }
   __device__ __forceinline__ void get(float (&v)[1]) const { v[0] = to_f32(raw); }
-  __device__ __forceinline__ static void store(const Buffer& b, bool, int lane_byte, int byte, const float (&v)[1]) {
-    if constexpr (sizeof(T) == 4) __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(v[0]), b.rsrc, lane_byte, byte, 0);
-    else __builtin_amdgcn_raw_buffer_store_b16(from_f32<T>(v[0]).bits, b.rsrc, lane_byte, byte, 0);
+  __device__ __forceinline__ static void store(const Buffer& b, bool, int lane_byte, const float (&v)[1]) {
+    if constexpr (sizeof(T) == 4) __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(v[0]), b.rsrc, lane_byte, 0, 0);
+    else __builtin_amdgcn_raw_buffer_store_b16(from_f32<T>(v[0]).bits, b.rsrc, lane_byte, 0, 0);
   }
 };
 template <int VN>
