@@ -19,9 +19,10 @@ def gen(seed):
     return torch.Generator().manual_seed(seed)
 
 
-def check_elements(g, ref, entries, scale, more=0.0):
-    """`entries`: truth values, where a second term was added; `scale`: the upstream factor; `more`: another rounding."""
-    tol = (torch.finfo(g.dtype).eps / 2 + 8e-6 + more) * ref.abs() + 8e-6 * scale * entries
+def check_elements(g, ref, entries, scale, more=0.0, floor=0.0):
+    """`entries`: truth values, where a second term was added; `scale`: the upstream factor; `more`: another rounding;
+    `floor`: what need not be there."""
+    tol = (torch.finfo(g.dtype).eps / 2 + 8e-6 + more) * ref.abs() + scale * (8e-6 * entries + floor)
     if g.dtype == torch.float16:
         tol = tol + 2.0 ** -25                     # half a step of its subnormals
     off = (g.detach().double().cpu() - ref).abs()
@@ -109,3 +110,51 @@ def test_nothing_is_written_beside_a_gradient(V, dt, off):
     _lib.launch(dev, 'vae_distill_bwd', p_(xd), V, p_(teacher), K, tau, p_(stats), p_(wd), None, 0.0, p_(g.rows), N, V, code)
     g.check()
     check_elements(g.rows, w.double()[:, None] / tau * ref, at, 2.0 / tau)
+
+
+# ---------------------------------------------------------------------------------------------------------------------
+# small temperatures
+# ---------------------------------------------------------------------------------------------------------------------
+def ref_distill(z, y, ids, tau):
+    """kl [N], d kl / d z and where the teacher's entries are; float64, every id there"""
+    logp, q = torch.log_softmax(z / tau, -1), torch.softmax(y / tau, -1)
+    logq = torch.log_softmax(y / tau, -1)
+    kl = torch.where(q > 0, q * (logq - logp.gather(1, ids)), torch.zeros_like(q)).sum(1)
+    grad = logp.exp() / tau
+    grad.scatter_add_(1, ids, -q / tau)
+    at = torch.zeros(z.shape, dtype=torch.bool)
+    at.scatter_(1, ids, True)
+    return kl, grad, at
+
+
+@pytest.mark.parametrize('dt', ['f32', 'bf16', 'f16'])
+@pytest.mark.parametrize('N,V', [(3, 90), (3, 9000), (2, 70001), (300, 2500)])
+@pytest.mark.parametrize('tau,shift', [(1e-4, 0.0), (1e-9, 0.0), (1e-30, 0.0), (1e-4, 6e5), (1e-9, -6e4), (3e-7, 11.3)])
+def test_small_temperatures(N, V, dt, tau, shift):
+    """x / tau beyond what float32 holds to a unit: one pass, two passes and evaluation agree with float64.  c = log2(e) / tau
+    is rounded too, a third step of the exponent: 60 2^-24 ln2 = 2.5e-6 of p more where |d| <= 60; a probability below 2^-60
+    of the row's largest need not be there.  The KL's largest term is one such q times a number of five roundings."""
+    from vae_amd import functional as F_
+    shift = max(min(shift, 6e4), -6e4) if dt == 'f16' else shift
+    z = (torch.randn(N, V, generator=gen(V)) * 3 + shift).to(TYPES[dt])
+    K = 4
+    ids = torch.stack([torch.randperm(V, generator=gen(i))[:K] for i in range(N)])
+    y = torch.randn(N, K, generator=gen(2)) * 3 + shift
+    kl_r, grad_r, at = ref_distill(z.double(), y.double(), ids, tau)
+    w = torch.rand(N, generator=gen(8)) + 0.5
+
+    def near(kl):
+        torch.testing.assert_close(kl.detach().double().cpu(), kl_r, rtol=1.2e-5, atol=2e-5)
+
+    with torch.no_grad():
+        near(F_.distill_top_logits(z.to(DEV), y.to(DEV), ids.to(DEV), temperature=tau)[0])
+    for fuse in (True, False):
+        x = z.to(DEV).requires_grad_(True)
+        kl, mean = F_.distill_top_logits(x, y.to(DEV), ids.to(DEV), temperature=tau, fuse_backward=fuse)
+        near(kl)
+        # upstream factors of tau: gradients around 1.  The stored one is rounded, multiplied and rounded again
+        g, = torch.autograd.grad(mean, x, torch.tensor(tau, device=DEV), retain_graph=True)
+        more = 3e-6 + (torch.finfo(g.dtype).eps / 2 if fuse else 0.0) + (2.0 ** -12 if dt == 'bf16' and V > 65536 else 0.0)
+        check_elements(g, grad_r * tau / N, at, 1.5 / N, more, 2.0 ** -60)
+        g, = torch.autograd.grad(kl, x, (w * tau).to(DEV))
+        check_elements(g, grad_r * (w.double() * tau)[:, None], at, 1.5, 3e-6, 2.0 ** -60)

@@ -14,7 +14,7 @@
 namespace vae {
 
 constexpr int kVecBytes = 16;
-constexpr float kHuge = 1.0e6f;      // |max| beyond which the shifted exponent is formed as (x - m) c, see row_stats
+constexpr float kHuge = 1.0e6f;      // |max c| beyond which the shifted exponent is formed as (x - m) c, see row_stats
 
 struct FwdArgs {
   const void* logits;
@@ -33,16 +33,17 @@ struct FwdArgs {
 };
 __device__ __forceinline__ int64_t part_bytes(int top_k) { return 16 + 8 * (int64_t)top_k; }
 
-// One thread's running statistics.  With the reference r = max(m, -kHuge) and S = r c rounded once, e_j = 2^(x_j c - S)
-// takes one fma and one exponential an element; S is the same for the whole sum, so its rounding drops out (finish()).
+// One thread's running statistics.  With the reference S = max(m c, -kHuge) rounded once, e_j = 2^(x_j c - S) takes one
+// fma and one exponential an element; S is the same for the whole sum, so its rounding drops out at the end of row_stats,
+// which takes these sums where |max c| <= kHuge: S is at most 2^-5 off there.  Beyond it (large logits, a small temperature)
+// the rounding of S alone could carry a sum out of the type's range.
 template <bool ENT>
 struct RunStats {
-  float m = -INFINITY, S, s = 0.f, t = 0.f;
-  __device__ __forceinline__ explicit RunStats(float c) : S(mul_rn(-kHuge, c)) {}
+  float m = -INFINITY, S = -kHuge, s = 0.f, t = 0.f;
   // make room for a maximum of mt
   __device__ __forceinline__ void raise(float mt, float c) {
     m = max_raw(m, mt);
-    const float Sn = mul_rn(max_raw(m, -kHuge), c);   // rounded here, not fused into the difference below
+    const float Sn = max_raw(mul_rn(m, c), -kHuge);   // rounded here, not fused into the difference below
     const float w = exp2_raw(S - Sn);
     if constexpr (ENT) t = w * __builtin_fmaf(S - Sn, s, t);
     s *= w;
@@ -65,7 +66,7 @@ __device__ __forceinline__ void row_stats(const T* __restrict__ x, const RowCut<
                                           float& mine) {
   constexpr int VN = VecOf<T>::n, U = 4;
   const Buffer body(x + cut.head, cut.nvec * kVecBytes);
-  RunStats<ENT> st(c);
+  RunStats<ENT> st;
   // W vectors of a lane; a running maximum for all of them
   auto group = [&](auto& p) {
     constexpr int W = sizeof(p) / sizeof(p[0]);
@@ -102,7 +103,7 @@ __device__ __forceinline__ void row_stats(const T* __restrict__ x, const RowCut<
     st.add(edge, c);
   }
   m = block_max<BT>(st.m);
-  if (!(fabsf(m) > kHuge) || m == -INFINITY) {
+  if (!(fabsf(m) * c > kHuge) || m == -INFINITY) {
     st.raise(m, c);
     s = block_sum<BT>(st.s);
     if constexpr (ENT) t = block_sum<BT>(st.t);
@@ -113,7 +114,7 @@ __device__ __forceinline__ void row_stats(const T* __restrict__ x, const RowCut<
     s *= w;
     return;
   }
-  // a maximum so large that x c - S loses it: once more, the difference first
+  // a maximum so large that x c - S loses the difference: once more, the difference first
   s = t = 0.f;
   auto add = [&](float v) {
     const float d = (v - m) * c;
