@@ -158,3 +158,27 @@ def test_small_temperatures(N, V, dt, tau, shift):
         check_elements(g, grad_r * tau / N, at, 1.5 / N, more, 2.0 ** -60)
         g, = torch.autograd.grad(kl, x, (w * tau).to(DEV))
         check_elements(g, grad_r * (w.double() * tau)[:, None], at, 1.5, 3e-6, 2.0 ** -60)
+
+
+# ---------------------------------------------------------------------------------------------------------------------
+# the ELBO's terms
+# ---------------------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize('fuse', [True, False])
+@pytest.mark.parametrize('B,shape', [(4, (4, 1)), (1, ()), (6, (2, 3))])
+def test_terms_of_another_shape(B, shape, fuse):
+    """A value for each sample, in whatever shape: forward, and each gradient in its term's shape."""
+    import vae_amd
+    z, x = torch.randn(B, 3, 40, generator=gen(1)), torch.randint(0, 40, (B, 3), generator=gen(2))
+    leaves = [torch.rand(shape, generator=gen(3 + i)).to(DEV).requires_grad_(True) for i in range(3)]
+    xr = z.to(DEV).requires_grad_(True)
+    out = vae_amd.loss_function(xr, x.to(DEV), leaves[0], 'categorical', kl_beta=0.5, mut_info=leaves[2],
+                                extra_loss_terms={'more': leaves[1]}, fuse_backward=fuse)
+    nll = -torch.log_softmax(z.double(), -1).gather(2, x[..., None])[..., 0].sum(1)
+    k, a, m = (t.detach().double().cpu().reshape(-1) for t in leaves)
+    torch.testing.assert_close(out['loss'].double().cpu(), nll + a + 0.5 * k - m, rtol=1e-6, atol=1e-5)
+    gs = torch.autograd.grad(out['loss_mean'], [xr] + leaves)
+    for g, want, t in zip(gs[1:], (0.5 / B, 1.0 / B, -1.0 / B), leaves):
+        assert g.shape == t.shape
+        torch.testing.assert_close(g, torch.full_like(g, want), rtol=2.0 ** -22, atol=0.0)
+    at = torch.zeros(z.shape, dtype=torch.bool).scatter_(2, x[..., None], True)
+    check_elements(gs[0], (torch.softmax(z.double(), -1) - at.double()) / B, at, 1.0 / B)

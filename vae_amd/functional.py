@@ -755,7 +755,8 @@ def token_nll_elbo(x, recon_x, kld=None, add=None, mi=None, kl_beta=1.0, inv_cou
         inv_count = 1.0 / max(x.shape[0], 1)
     _check_terms(x.shape[0], kld, add, mi)
     # the terms in the logits' type, as loss and elbo come out: half a step of each term beside half a step of the sum
-    kld, add, mi = (None if t is None else t.to(recon_x.dtype).contiguous() for t in (kld, add, mi))
+    kld, add, mi = (None if t is None else (t if t.dim() == 1 else t.reshape(-1)).to(recon_x.dtype).contiguous()
+                    for t in (kld, add, mi))
     # fp16: two passes, for the reason given in nll_elbo
     fuse = bool(fuse_backward and recon_x.dtype != torch.float16 and recon_x.requires_grad and torch.is_grad_enabled()
                 and recon_x.numel() > 0)
