@@ -1,0 +1,30 @@
+"""Which steps the categorical per-step loss refuses, before any launch: no GPU needed."""
+import pytest
+import torch
+
+from vae_amd import functional as F_
+
+
+@pytest.mark.parametrize('sizes', [(3, 2, 4), (3, 4, 2), (2, 3)])
+def test_steps_of_different_batches_are_refused(sizes):
+    """Also where they hold T B entries together: the averages over the steps would mix samples."""
+    xs = [torch.zeros(b, 2, dtype=torch.int64) for b in sizes]
+    recons = [torch.zeros(b, 2, 10) for b in sizes]
+    with pytest.raises(ValueError, match='same shapes'):
+        F_.nll_steps_elbo(xs, recons, 'categorical')
+
+
+def test_steps_of_different_types_or_vocabularies_are_refused():
+    x = torch.zeros(3, dtype=torch.int64)
+    for other in (torch.zeros(3, 10, dtype=torch.bfloat16), torch.zeros(3, 11), torch.zeros(3, 2, 10)):
+        with pytest.raises(ValueError, match='same shapes'):
+            F_.nll_steps_elbo([x, x], [torch.zeros(3, 10), other], 'categorical')
+    with pytest.raises(ValueError, match='same shapes'):
+        F_.nll_steps_elbo([x, x.repeat(2)], [torch.zeros(3, 10)] * 2, 'categorical')
+
+
+def test_steps_of_one_size_in_another_shape_pass():
+    """[B] and [B, 1] tokens are the same: they get as far as the device check."""
+    x, r = torch.zeros(3, dtype=torch.int32), torch.zeros(3, 10)
+    with pytest.raises(RuntimeError, match='no CPU fallback'):
+        F_.nll_steps_elbo([x, x[:, None], x.long()], [r, r[:, None], r], 'categorical')

@@ -775,10 +775,11 @@ def _token_steps_elbo(xs, recons, kld, add, mi, kl_beta, inv_count, with_lse):
             raise NotImplementedError("nll_steps_elbo: 'categorical' takes one KL weight for all steps (a host model "
                                       "with an annealer scores its steps one by one: vae_amd.vrnn.loss_function)")
         kl_beta = kl_beta[0]
-    nll_ = torch.cat([_token_nll(x, r) for x, r in zip(xs, recons)], 0)
-    if nll_.numel() != T * B:
-        raise ValueError("nll_steps_elbo: every step must have the same shapes and dtype")
     dtype = recons[0].dtype
+    sizes = [(x.shape[:1], x.numel(), r.shape[:1], r.shape[-1:], r.numel(), r.dtype) for x, r in zip(xs, recons)]
+    if any(size != sizes[0] for size in sizes):
+        raise ValueError("nll_steps_elbo: every step must have the same shapes and dtype")
+    nll_ = torch.cat([_token_nll(x, r) for x, r in zip(xs, recons)], 0)
     nll_, loss, elbo, means = _token_combine(nll_, kld, add, mi, kl_beta, inv_count, torch.float32)
     out = tuple(t.to(dtype) for t in (nll_, loss, elbo)) + (means,)
     out += (loss.view(T, B).mean(0).to(dtype), elbo.view(T, B).mean(0).to(dtype))
