@@ -28,3 +28,22 @@ def test_steps_of_one_size_in_another_shape_pass():
     x, r = torch.zeros(3, dtype=torch.int32), torch.zeros(3, 10)
     with pytest.raises(RuntimeError, match='no CPU fallback'):
         F_.nll_steps_elbo([x, x[:, None], x.long()], [r, r[:, None], r], 'categorical')
+
+
+def test_many_steps_of_different_batches_are_refused():
+    """Beyond the steps of one launch, without a host model."""
+    from vae_amd import vrnn
+
+    class Latent:
+        def kl(self, dist_a, prior=None):
+            return dist_a
+
+    sizes = [3, 2, 4] * 50
+    xs, recons = [torch.zeros(b, dtype=torch.int64) for b in sizes], [torch.zeros(b, 10) for b in sizes]
+    params = [{'posterior': torch.zeros(b), 'prior': None} for b in sizes]
+    config = {'nll_type': 'categorical', 'kl_beta': 1.0, 'use_prior_kl': False}
+    with pytest.raises(ValueError, match='same shapes'):
+        vrnn.loss_function(Latent(), config, recons, xs, params)
+    same = [torch.zeros(3, dtype=torch.int64)] * 150, [torch.zeros(3, 10)] * 150, params[:1] * 150
+    with pytest.raises(RuntimeError, match='no CPU fallback'):
+        vrnn.loss_function(Latent(), config, same[1], same[0], same[2])

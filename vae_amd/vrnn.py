@@ -179,6 +179,8 @@ def loss_function(reparameterizer, config, recon_x, x, params, K=1, kl_beta=None
             raise NotImplementedError("vae_amd.vrnn.loss_function: more than %d steps with a per-step KL weight needs "
                                       "a host model (model=...) for the per-step loop" % F_.MAX_STEPS)
         if F_._is_categorical(config['nll_type']):
+            if any(r.shape != recon_x[0].shape or xi.shape != x[0].shape for r, xi in zip(recon_x, x)):
+                raise ValueError("vae_amd.vrnn.loss_function: every step must have the same shapes")
             recon_all, x_all = torch.cat(list(recon_x), 0), torch.cat(list(x), 0)      # [T*B, ..., V], [T*B, ...]
         else:
             recon_all = torch.cat([r.reshape(B, -1) for r in recon_x], 0)              # [T*B, D or 2D]
