@@ -506,6 +506,12 @@ int vae_token_nll_elbo_fwd(const void* logits, int64_t row_stride, const void* t
                            float* stats, void* glogits, void* nll, void* loss, void* elbo, float* means, void* loss_mean,
                            void* other_means, int mean_dtype, float* workspace, void* scratch, int64_t B, int64_t V,
                            int dtype, vae_stream_t stream);
+/* The same, kld / add / mi in a type of their own (terms_dtype; above: dtype): read as they are, added in float32.      */
+int vae_token_nll_elbo_terms_fwd(const void* logits, int64_t row_stride, const void* tokens, int token_bytes, int64_t T,
+                                 const void* kld, const void* add, const void* mi, int terms_dtype, float kl_beta,
+                                 float inv_count, float* logp, float* stats, void* glogits, void* nll, void* loss,
+                                 void* elbo, float* means, void* loss_mean, void* other_means, int mean_dtype,
+                                 float* workspace, void* scratch, int64_t B, int64_t V, int dtype, vae_stream_t stream);
 /* Its backward.  gnll / gloss / gelbo [B] (dtype) and gmeans, a HOST array of 6 device pointers to one value each
  * (gmeans_dtype): every one may be NULL.  grow [B] (float32) = d / d nll[b], what vae_token_logp_bwd takes with
  * rows_per_g = T and g_scale = -1; or grad [n] = the forward's glogits, multiplied by
@@ -513,6 +519,11 @@ int vae_token_nll_elbo_fwd(const void* logits, int64_t row_stride, const void* t
 int vae_token_nll_elbo_bwd(const void* gnll, const void* gloss, const void* gelbo, const void* const* gmeans,
                            int gmeans_dtype, float kl_beta, float inv_count, float* grow, void* grad, int64_t n,
                            void* gkld, void* gadd, void* gmi, int64_t B, int dtype, vae_stream_t stream);
+/* The same, gkld / gadd / gmi in terms_dtype.                                                                          */
+int vae_token_nll_elbo_terms_bwd(const void* gnll, const void* gloss, const void* gelbo, const void* const* gmeans,
+                                 int gmeans_dtype, float kl_beta, float inv_count, float* grow, void* grad, int64_t n,
+                                 void* gkld, void* gadd, void* gmi, int terms_dtype, int64_t B, int dtype,
+                                 vae_stream_t stream);
 /* out[b] (dtype) = scale * sum of rows[b T .. b T + T), summed in double in a fixed order.                         */
 int vae_row_sums(const float* rows, float scale, void* out, int64_t B, int64_t T, int dtype, vae_stream_t stream);
 /* buf[n] *= *factor (a device float); returns without touching buf when it is 1.                                   */

@@ -182,3 +182,36 @@ def test_terms_of_another_shape(B, shape, fuse):
         torch.testing.assert_close(g, torch.full_like(g, want), rtol=2.0 ** -22, atol=0.0)
     at = torch.zeros(z.shape, dtype=torch.bool).scatter_(2, x[..., None], True)
     check_elements(gs[0], (torch.softmax(z.double(), -1) - at.double()) / B, at, 1.0 / B)
+
+
+@pytest.mark.parametrize('dt', ['bf16', 'f16'])
+@pytest.mark.parametrize('types', [('float32', 'float32', 'float32'), ('float32', 'float64', 'bfloat16'),
+                                   ('float16', 'bfloat16', 'float32'), ('bfloat16', 'bfloat16', 'bfloat16')])
+@pytest.mark.parametrize('fuse', [True, False])
+def test_terms_of_another_type(dt, types, fuse):
+    """16-bit logits beside terms of other types: the terms are added as they are, every output is rounded once (half a step
+    beside a few of float32), as in the multi-sample form of the same loss; gradients in the terms' own types."""
+    from vae_amd import functional as F_
+    B, T, V = 7, 5, 300
+    z = torch.randn(B, T, V, generator=gen(1)).to(TYPES[dt])
+    x = torch.randint(0, V, (B, T), generator=gen(2))
+    terms = [(torch.rand(B, generator=gen(3 + i)) * 30).to(getattr(torch, t)) for i, t in enumerate(types)]
+    kld, add, mi = (t.double() for t in terms)
+    leaves = [t.to(DEV).requires_grad_(True) for t in terms]
+    xr = z.to(DEV).requires_grad_(True)
+    out = F_.nll_elbo(x.to(DEV), xr, 'categorical', *leaves, kl_beta=0.5, fuse_backward=fuse)
+    multi = F_.nll_multi_elbo(x.to(DEV), [z.to(DEV)], 'categorical', *[t.detach() for t in leaves], kl_beta=0.5)
+    nll = -torch.log_softmax(z.double(), -1).gather(2, x[..., None])[..., 0].sum(1)
+    half = torch.finfo(TYPES[dt]).eps / 2
+    loss = nll + add + 0.5 * kld - mi
+    means = torch.stack([loss.mean(), (nll + kld).mean(), nll.mean(), kld.mean(), add.mean(), mi.mean()])
+    for o in (out, multi):
+        for got, want in zip(o, (nll, loss, nll + kld)):
+            assert got.dtype == TYPES[dt]
+            torch.testing.assert_close(got.double().cpu(), want, rtol=half + 1e-6, atol=1e-5)
+        torch.testing.assert_close(o[3].double().cpu(), means, rtol=1e-6, atol=1e-5)
+    gs = torch.autograd.grad(out[3][0], leaves)
+    for g, want, t in zip(gs, (0.5 / B, 1.0 / B, -1.0 / B), terms):
+        assert g.dtype == t.dtype
+        torch.testing.assert_close(g.double().cpu(), torch.full((B,), want, dtype=torch.float64),
+                                   rtol=torch.finfo(t.dtype).eps / 2 + 2.0 ** -22, atol=0.0)

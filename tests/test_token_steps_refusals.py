@@ -47,3 +47,23 @@ def test_many_steps_of_different_batches_are_refused():
     same = [torch.zeros(3, dtype=torch.int64)] * 150, [torch.zeros(3, 10)] * 150, params[:1] * 150
     with pytest.raises(RuntimeError, match='no CPU fallback'):
         vrnn.loss_function(Latent(), config, same[1], same[0], same[2])
+
+
+def test_types_of_the_terms():
+    """The C entry points refuse a type that they do not know, where there are terms; without any it is not looked at."""
+    import ctypes
+    from vae_amd import _lib
+    lib, P = _lib.load(), ctypes.c_void_p(4096)   # never read: every call is refused, or has no samples
+
+    def fwd(kld, terms_dtype, B):
+        return lib.vae_token_nll_elbo_terms_fwd(P, 10, P, 8, 1, kld, None, None, terms_dtype, 1.0, 1.0, P, P, P, P, P, P, P, P,
+                                                P, 0, P, P, B, 10, 0, None)
+
+    def bwd(gkld, terms_dtype, B):
+        return lib.vae_token_nll_elbo_terms_bwd(None, None, None, None, 0, 1.0, 1.0, P, None, 0, gkld, None, None, terms_dtype,
+                                                B, 0, None)
+
+    for f in (fwd, bwd):
+        assert f(P, 3, 2) == f(P, -1, 2) == _lib.VAE_ERR_ARG
+        assert f(P, 3, 0) == _lib.VAE_ERR_ARG
+        assert f(None, 3, 0) == f(P, 2, 0) == _lib.VAE_OK

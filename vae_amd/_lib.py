@@ -14,7 +14,7 @@ import torch  # noqa: F401  (must be imported before the CDLL below, see module 
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.environ.get('VAE_AMD_LIB') or os.path.join(_HERE, 'libvae_amd.so')  # env override: tuning builds only
-ABI_VERSION = 12
+ABI_VERSION = 13
 
 VAE_OK, VAE_ERR_ARG, VAE_ERR_LAUNCH = 0, 1, 2
 VAE_F32, VAE_BF16, VAE_F16 = 0, 1, 2
@@ -98,6 +98,9 @@ SIGNATURES = {
     'vae_token_nll_elbo_fwd': [_p, _i64, _p, _i, _i64, _p, _p, _p, _f, _f, _p, _p, _p, _p, _p, _p, _p, _p, _p, _i, _p, _p,
                                _i64, _i64, _i, _p],
     'vae_token_nll_elbo_bwd': [_p, _p, _p, _pp, _i, _f, _f, _p, _p, _i64, _p, _p, _p, _i64, _i, _p],
+    'vae_token_nll_elbo_terms_fwd': [_p, _i64, _p, _i, _i64, _p, _p, _p, _i, _f, _f, _p, _p, _p, _p, _p, _p, _p, _p, _p, _i,
+                                     _p, _p, _i64, _i64, _i, _p],
+    'vae_token_nll_elbo_terms_bwd': [_p, _p, _p, _pp, _i, _f, _f, _p, _p, _i64, _p, _p, _p, _i, _i64, _i, _p],
     'vae_row_sums': [_p, _f, _p, _i64, _i64, _i, _p],
     'vae_grad_scale': [_p, _p, _i64, _i, _p],
     'vae_distill_teacher_floats': [_i64, _i64],

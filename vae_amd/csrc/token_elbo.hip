@@ -12,7 +12,7 @@ constexpr int kElboBlocks = 256;
 constexpr int kOneBlock = 1024;
 static_assert(VAE_TOKEN_MEANS_FLOATS == 6 + 6 * kElboBlocks, "the header says how long `means` is");
 
-__device__ __forceinline__ void store_any(void* p, int dtype, int i, float v) {
+__device__ __forceinline__ void store_any(void* p, int dtype, int64_t i, float v) {
   if (dtype == VAE_F32) reinterpret_cast<float*>(p)[i] = v;
   else if (dtype == VAE_BF16) reinterpret_cast<bf16_t*>(p)[i] = from_f32<bf16_t>(v);
   else reinterpret_cast<f16_t*>(p)[i] = from_f32<f16_t>(v);
@@ -47,12 +47,17 @@ __device__ __forceinline__ double strided_sum(const float* __restrict__ p, int64
   return v;
 }
 
+// the ELBO's terms [B] beside the nll, in the type that they come in; each may be NULL
+struct Terms {
+  const void *kld, *add, *mi;
+  int dtype;
+};
+
 // G lanes a sample (a power of two, up to a wave); samples in order, so a result does not depend on timing
 template <typename T, int BT>
 __global__ __launch_bounds__(BT) void token_elbo_fwd_kernel(
-    const float* __restrict__ logp, int64_t len, const T* __restrict__ kld, const T* __restrict__ add,
-    const T* __restrict__ mi, float kl_beta, float inv_count, T* __restrict__ nll, T* __restrict__ loss,
-    T* __restrict__ elbo, float* __restrict__ means, MeansTo to, float* __restrict__ ws, int64_t B, int G) {
+    const float* __restrict__ logp, int64_t len, Terms terms, float kl_beta, float inv_count, T* __restrict__ nll,
+    T* __restrict__ loss, T* __restrict__ elbo, float* __restrict__ means, MeansTo to, float* __restrict__ ws, int64_t B, int G) {
   __shared__ float part[BT / 64][6];
   const int rpb = BT / G, sub = threadIdx.x % G, rloc = threadIdx.x / G;
   float acc[6] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
@@ -64,9 +69,9 @@ __global__ __launch_bounds__(BT) void token_elbo_fwd_kernel(
     const float n = (float)(0.0 - v);   // loss and elbo from the unrounded sum: every output is rounded once
     if (nll) nll[b] = from_f32<T>(n);
     if (!loss) continue;
-    const float k = kld ? to_f32(kld[b]) : 0.f;
-    const float ad = add ? to_f32(add[b]) : 0.f;
-    const float m = mi ? to_f32(mi[b]) : 0.f;
+    const float k = terms.kld ? load_any(terms.kld, terms.dtype, b) : 0.f;
+    const float ad = terms.add ? load_any(terms.add, terms.dtype, b) : 0.f;
+    const float m = terms.mi ? load_any(terms.mi, terms.dtype, b) : 0.f;
     const float e = n + k, l = (n + ad + kl_beta * k) - m;
     loss[b] = from_f32<T>(l);
     elbo[b] = from_f32<T>(e);
@@ -100,11 +105,16 @@ __global__ __launch_bounds__(64) void token_elbo_means_kernel(float* __restrict_
 struct Scalars6 {
   const void* p[6];
 };
+// where the terms' gradients go, in the terms' type; each may be NULL
+struct GradTerms {
+  void *kld, *add, *mi;
+  int dtype;
+};
 template <typename T, int V>
 __global__ __launch_bounds__(kBlock) void token_elbo_bwd_kernel(
     const T* __restrict__ gnll, const T* __restrict__ gloss, const T* __restrict__ gelbo, Scalars6 gmeans,
     int gmeans_dtype, float kl_beta, float inv_count, float* __restrict__ grow, T* __restrict__ grad, int64_t items,
-    T* __restrict__ gkld, T* __restrict__ gadd, T* __restrict__ gmi, int64_t B) {
+    GradTerms gterms, int64_t B) {
   float gm[6];
 #pragma unroll
   for (int k = 0; k < 6; ++k) gm[k] = gmeans.p[k] ? load_any(gmeans.p[k], gmeans_dtype, 0) : 0.f;
@@ -113,9 +123,9 @@ __global__ __launch_bounds__(kBlock) void token_elbo_bwd_kernel(
     const float gl = (gloss ? to_f32(gloss[b]) : 0.f) + gm[0] * inv_count;
     const float ge = (gelbo ? to_f32(gelbo[b]) : 0.f) + gm[1] * inv_count;
     if (grow) grow[b] = gl + ge + gm[2] * inv_count + (gnll ? to_f32(gnll[b]) : 0.f);
-    if (gkld) gkld[b] = from_f32<T>(kl_beta * gl + ge + gm[3] * inv_count);
-    if (gadd) gadd[b] = from_f32<T>(gl + gm[4] * inv_count);
-    if (gmi) gmi[b] = from_f32<T>(gm[5] * inv_count - gl);
+    if (gterms.kld) store_any(gterms.kld, gterms.dtype, b, kl_beta * gl + ge + gm[3] * inv_count);
+    if (gterms.add) store_any(gterms.add, gterms.dtype, b, gl + gm[4] * inv_count);
+    if (gterms.mi) store_any(gterms.mi, gterms.dtype, b, gm[5] * inv_count - gl);
   }
   if (!grad || c == 1.0f) return;
   for (int64_t j = (int64_t)blockIdx.x * kBlock + threadIdx.x; j < items; j += (int64_t)gridDim.x * kBlock) {
@@ -152,16 +162,15 @@ static bool type_ok(int d) { return d == VAE_F32 || d == VAE_BF16 || d == VAE_F1
 
 template <typename T, int V>
 static void elbo_bwd_launch(const void* gnll, const void* gloss, const void* gelbo, const Scalars6& gm, int gmeans_dtype,
-                            float kl_beta, float inv_count, float* grow, void* grad, int64_t items, void* gkld,
-                            void* gadd, void* gmi, int64_t B, hipStream_t st) {
+                            float kl_beta, float inv_count, float* grow, void* grad, int64_t items,
+                            const GradTerms& gterms, int64_t B, hipStream_t st) {
   // sized for the [B] part; the (rare) rescale walks the gradient with at least 1024 blocks
   int64_t blocks = (B + kBlock - 1) / kBlock;
   const int64_t wide = (items + kBlock - 1) / kBlock;
   if (grad && blocks < 1024) blocks = wide < 1024 ? (wide > blocks ? wide : blocks) : 1024;
   const int grid = (int)(blocks < 1 ? 1 : (blocks < 4096 ? blocks : 4096));
   hipLaunchKernelGGL((token_elbo_bwd_kernel<T, V>), dim3(grid), dim3(kBlock), 0, st, (const T*)gnll, (const T*)gloss,
-                     (const T*)gelbo, gm, gmeans_dtype, kl_beta, inv_count, grow, (T*)grad, items, (T*)gkld, (T*)gadd,
-                     (T*)gmi, B);
+                     (const T*)gelbo, gm, gmeans_dtype, kl_beta, inv_count, grow, (T*)grad, items, gterms, B);
 }
 
 }  // namespace vae
@@ -170,13 +179,13 @@ using namespace vae;
 
 extern "C" {
 
-int vae_token_nll_elbo_fwd(const void* logits, int64_t row_stride, const void* tokens, int token_bytes, int64_t len,
-                           const void* kld, const void* add, const void* mi, float kl_beta, float inv_count, float* logp,
-                           float* stats, void* glogits, void* nll, void* loss, void* elbo, float* means, void* loss_mean,
-                           void* other_means, int mean_dtype, float* workspace, void* scratch, int64_t B, int64_t V,
-                           int dtype, vae_stream_t stream) {
+int vae_token_nll_elbo_terms_fwd(const void* logits, int64_t row_stride, const void* tokens, int token_bytes, int64_t len,
+                                 const void* kld, const void* add, const void* mi, int terms_dtype, float kl_beta,
+                                 float inv_count, float* logp, float* stats, void* glogits, void* nll, void* loss,
+                                 void* elbo, float* means, void* loss_mean, void* other_means, int mean_dtype,
+                                 float* workspace, void* scratch, int64_t B, int64_t V, int dtype, vae_stream_t stream) {
   if (B < 0 || len < 0 || V < 1 || V > VAE_MAX_ROW || (B * len > 1 && row_stride < V) || !type_ok(dtype) ||
-      ((loss_mean || other_means) && !type_ok(mean_dtype)))
+      ((kld || add || mi) && !type_ok(terms_dtype)) || ((loss_mean || other_means) && !type_ok(mean_dtype)))
     return VAE_ERR_ARG;
   if (B == 0) return VAE_OK;
   const int64_t N = B * len;
@@ -192,6 +201,7 @@ int vae_token_nll_elbo_fwd(const void* logits, int64_t row_stride, const void* t
                                       scratch, N, V, dtype, stream);
   if (rc != VAE_OK) return rc;
   const MeansTo to = {loss_mean, other_means, mean_dtype};
+  const Terms terms = {kld, add, mi, terms_dtype};
   int G = 1;
   while (G < 64 && G < len) G <<= 1;
   const int64_t blocks = (B + kBlock / G - 1) / (kBlock / G);
@@ -203,8 +213,7 @@ int vae_token_nll_elbo_fwd(const void* logits, int64_t row_stride, const void* t
   const int grid = one ? 1 : (int)(blocks < most ? blocks : most);
 #define VAE_ELBO_FWD(BT)                                                                                                \
   hipLaunchKernelGGL((token_elbo_fwd_kernel<T, BT>), dim3(grid), dim3(BT), 0, (hipStream_t)stream, logp, len,            \
-                     (const T*)kld, (const T*)add, (const T*)mi, kl_beta, inv_count, (T*)nll, (T*)loss, (T*)elbo, means, \
-                     to, workspace, B, G)
+                     terms, kl_beta, inv_count, (T*)nll, (T*)loss, (T*)elbo, means, to, workspace, B, G)
   VAE_BY_TYPE(dtype, if (one) VAE_ELBO_FWD(kOneBlock); else VAE_ELBO_FWD(kBlock));
 #undef VAE_ELBO_FWD
   if (loss && grid > 1)
@@ -213,22 +222,42 @@ int vae_token_nll_elbo_fwd(const void* logits, int64_t row_stride, const void* t
   return launched();
 }
 
-int vae_token_nll_elbo_bwd(const void* gnll, const void* gloss, const void* gelbo, const void* const* gmeans,
-                           int gmeans_dtype, float kl_beta, float inv_count, float* grow, void* grad, int64_t n,
-                           void* gkld, void* gadd, void* gmi, int64_t B, int dtype, vae_stream_t stream) {
-  if (B < 0 || n < 0 || !type_ok(dtype) || !type_ok(gmeans_dtype)) return VAE_ERR_ARG;
+int vae_token_nll_elbo_fwd(const void* logits, int64_t row_stride, const void* tokens, int token_bytes, int64_t len,
+                           const void* kld, const void* add, const void* mi, float kl_beta, float inv_count, float* logp,
+                           float* stats, void* glogits, void* nll, void* loss, void* elbo, float* means, void* loss_mean,
+                           void* other_means, int mean_dtype, float* workspace, void* scratch, int64_t B, int64_t V,
+                           int dtype, vae_stream_t stream) {
+  return vae_token_nll_elbo_terms_fwd(logits, row_stride, tokens, token_bytes, len, kld, add, mi, dtype, kl_beta, inv_count,
+                                      logp, stats, glogits, nll, loss, elbo, means, loss_mean, other_means, mean_dtype,
+                                      workspace, scratch, B, V, dtype, stream);
+}
+
+int vae_token_nll_elbo_terms_bwd(const void* gnll, const void* gloss, const void* gelbo, const void* const* gmeans,
+                                 int gmeans_dtype, float kl_beta, float inv_count, float* grow, void* grad, int64_t n,
+                                 void* gkld, void* gadd, void* gmi, int terms_dtype, int64_t B, int dtype,
+                                 vae_stream_t stream) {
+  if (B < 0 || n < 0 || !type_ok(dtype) || !type_ok(gmeans_dtype) || ((gkld || gadd || gmi) && !type_ok(terms_dtype)))
+    return VAE_ERR_ARG;
   if (grad && (gnll || gloss || gelbo)) return VAE_ERR_ARG;
   if (B == 0 && (n == 0 || !grad)) return VAE_OK;
   Scalars6 gm = {};
   if (gmeans)
     for (int k = 0; k < 6; ++k) gm.p[k] = gmeans[k];
+  const GradTerms gterms = {gkld, gadd, gmi, terms_dtype};
   VAE_BY_TYPE(dtype, constexpr int VN = VecOf<T>::n;
               if (n % VN == 0 && aligned16(grad))
-                elbo_bwd_launch<T, VN>(gnll, gloss, gelbo, gm, gmeans_dtype, kl_beta, inv_count, grow, grad, n / VN,
-                                       gkld, gadd, gmi, B, (hipStream_t)stream);
-              else elbo_bwd_launch<T, 1>(gnll, gloss, gelbo, gm, gmeans_dtype, kl_beta, inv_count, grow, grad, n, gkld,
-                                         gadd, gmi, B, (hipStream_t)stream));
+                elbo_bwd_launch<T, VN>(gnll, gloss, gelbo, gm, gmeans_dtype, kl_beta, inv_count, grow, grad, n / VN, gterms,
+                                       B, (hipStream_t)stream);
+              else elbo_bwd_launch<T, 1>(gnll, gloss, gelbo, gm, gmeans_dtype, kl_beta, inv_count, grow, grad, n, gterms, B,
+                                         (hipStream_t)stream));
   return launched();
+}
+
+int vae_token_nll_elbo_bwd(const void* gnll, const void* gloss, const void* gelbo, const void* const* gmeans,
+                           int gmeans_dtype, float kl_beta, float inv_count, float* grow, void* grad, int64_t n,
+                           void* gkld, void* gadd, void* gmi, int64_t B, int dtype, vae_stream_t stream) {
+  return vae_token_nll_elbo_terms_bwd(gnll, gloss, gelbo, gmeans, gmeans_dtype, kl_beta, inv_count, grow, grad, n, gkld,
+                                      gadd, gmi, dtype, B, dtype, stream);
 }
 
 int vae_grad_scale(void* buf, const float* factor, int64_t n, int dtype, vae_stream_t stream) {

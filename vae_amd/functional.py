@@ -678,19 +678,20 @@ class _TokenNllElbo(torch.autograd.Function):
         grad = torch.empty(logits.shape, dtype=logits.dtype, device=dev) if fuse else None
         nll = torch.empty((B,), dtype=logits.dtype, device=dev) if want_nll else None
         loss = elbo = first = others = means = ws = None
+        terms_dtype = next((t.dtype for t in (kld, add, mi) if t is not None), logits.dtype)
         scratch = _token_scratch(rows, 0, dev)
         if with_elbo:
             loss = torch.empty((B,), dtype=logits.dtype, device=dev)
             elbo = torch.empty_like(loss)
             means, ws = at + 12 * N, workspace(dev)
             first, others = torch.empty((), dtype=mean_dtype, device=dev), torch.empty((5,), dtype=mean_dtype, device=dev)
-        launch(dev, 'vae_token_nll_elbo_fwd', ptr(rows), rows.stride(0), ptr(tokens), tokens.element_size(),
-               N // max(B, 1), ptr(kld), ptr(add), ptr(mi), kl_beta, inv_count, at, at + 4 * N, ptr(grad), ptr(nll),
-               ptr(loss), ptr(elbo), means, ptr(first), ptr(others), DTYPE_CODES[mean_dtype], ptr(ws), ptr(scratch), B, V,
-               code)
+        launch(dev, 'vae_token_nll_elbo_terms_fwd', ptr(rows), rows.stride(0), ptr(tokens), tokens.element_size(),
+               N // max(B, 1), ptr(kld), ptr(add), ptr(mi), DTYPE_CODES[terms_dtype], kl_beta, inv_count, at, at + 4 * N,
+               ptr(grad), ptr(nll), ptr(loss), ptr(elbo), means, ptr(first), ptr(others), DTYPE_CODES[mean_dtype], ptr(ws),
+               ptr(scratch), B, V, code)
         ctx.save_for_backward(logits, tokens, buf)
         ctx.grad = _Stored(grad)
-        ctx.cfg = (kl_beta, inv_count, kld is not None, add is not None, mi is not None, mean_dtype)
+        ctx.cfg = (kl_beta, inv_count, kld is not None, add is not None, mi is not None, mean_dtype, terms_dtype)
         if not with_elbo:
             return (nll,) + (None,) * 8
         if B == 0:
@@ -703,10 +704,10 @@ class _TokenNllElbo(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, gnll, gloss, gelbo, *gmeans):
         logits, tokens, buf = ctx.saved_tensors
-        kl_beta, inv_count, has_kld, has_add, has_mi, mean_dtype = ctx.cfg
+        kl_beta, inv_count, has_kld, has_add, has_mi, mean_dtype, terms_dtype = ctx.cfg
         dev, B = logits.device, tokens.shape[0]
         need = ctx.needs_input_grad
-        terms = [torch.empty((B,), dtype=logits.dtype, device=dev) if has and need[i] else None
+        terms = [torch.empty((B,), dtype=terms_dtype, device=dev) if has and need[i] else None
                  for i, has in ((2, has_kld), (3, has_add), (4, has_mi))]
         grad = ctx.grad.take()
         stored = gnll is None and gloss is None and gelbo is None and grad is not None
@@ -714,9 +715,9 @@ class _TokenNllElbo(torch.autograd.Function):
         grow = None if stored else torch.empty((B,), dtype=torch.float32, device=dev)
         gnll, gloss, gelbo = _dense(gnll), _dense(gloss), _dense(gelbo)
         at = _Pointers6(*[None if g is None else g.data_ptr() for g in gmeans])
-        launch(dev, 'vae_token_nll_elbo_bwd', ptr(gnll), ptr(gloss), ptr(gelbo), at, DTYPE_CODES[mean_dtype], kl_beta,
+        launch(dev, 'vae_token_nll_elbo_terms_bwd', ptr(gnll), ptr(gloss), ptr(gelbo), at, DTYPE_CODES[mean_dtype], kl_beta,
                inv_count, ptr(grow), ptr(grad) if stored else None, grad.numel() if stored else 0, ptr(terms[0]),
-               ptr(terms[1]), ptr(terms[2]), B, dtype_code(logits))
+               ptr(terms[1]), ptr(terms[2]), DTYPE_CODES[terms_dtype], B, dtype_code(logits))
         if not stored:
             grad = None
             if need[0]:
@@ -754,8 +755,10 @@ def token_nll_elbo(x, recon_x, kld=None, add=None, mi=None, kl_beta=1.0, inv_cou
     if inv_count is None:
         inv_count = 1.0 / max(x.shape[0], 1)
     _check_terms(x.shape[0], kld, add, mi)
-    # the terms in the logits' type, as loss and elbo come out: half a step of each term beside half a step of the sum
-    kld, add, mi = (None if t is None else (t if t.dim() == 1 else t.reshape(-1)).to(recon_x.dtype).contiguous()
+    # the terms in the type that they have; in float32 where they have several, or one that the kernels do not read
+    types = {t.dtype for t in (kld, add, mi) if t is not None}
+    terms_dtype = next(iter(types)) if len(types) == 1 and types <= DTYPE_CODES.keys() else torch.float32
+    kld, add, mi = (None if t is None else (t if t.dim() == 1 else t.reshape(-1)).to(terms_dtype).contiguous()
                     for t in (kld, add, mi))
     # fp16: two passes, for the reason given in nll_elbo
     fuse = bool(fuse_backward and recon_x.dtype != torch.float16 and recon_x.requires_grad and torch.is_grad_enabled()
