@@ -87,8 +87,7 @@ def test_nothing_is_written_beside_a_gradient(V, dt, off):
     _lib.launch(dev, 'vae_token_nll_elbo_fwd', p_(xd), V, p_(td), 8, 1, None, None, None, 0.0, 0.25, buf.data_ptr(),
                 buf.data_ptr() + 4 * N, p_(g.rows), p_(nll), None, None, None, None, None, 0, None, p_(scratch), N, V, code)
     g.check()
-    # bf16 rows that are kept as binary16 exponentials: 2^-12 more
-    check_elements(g.rows, 0.25 * (p - at.double()), at, 0.25, 2.0 ** -12 if dt == 'bf16' and V > 65536 else 0.0)
+    check_elements(g.rows, 0.25 * (p - at.double()), at, 0.25)
 
     K, tau = 3, 1.5
     y = torch.randn(N, K, generator=gen(1))
@@ -105,7 +104,7 @@ def test_nothing_is_written_beside_a_gradient(V, dt, off):
     _lib.launch(dev, 'vae_distill_fwd', p_(xd), V, p_(yd), K, 0, p_(idd), K, 8, K, tau, p_(teacher), p_(kl), None, 0.5,
                 p_(stats), p_(g.rows), p_(scratch), N, V, code)
     g.check()
-    check_elements(g.rows, 0.5 / tau * ref, at, 0.5 / tau, 2.0 ** -12 if dt == 'bf16' and V > 65536 else 0.0)
+    check_elements(g.rows, 0.5 / tau * ref, at, 0.5 / tau)
     g = Guarded(N, V, dtype, off)
     _lib.launch(dev, 'vae_distill_bwd', p_(xd), V, p_(teacher), K, tau, p_(stats), p_(wd), None, 0.0, p_(g.rows), N, V, code)
     g.check()
@@ -154,7 +153,7 @@ def test_small_temperatures(N, V, dt, tau, shift):
         near(kl)
         # upstream factors of tau: gradients around 1.  The stored one is rounded, multiplied and rounded again
         g, = torch.autograd.grad(mean, x, torch.tensor(tau, device=DEV), retain_graph=True)
-        more = 3e-6 + (torch.finfo(g.dtype).eps / 2 if fuse else 0.0) + (2.0 ** -12 if dt == 'bf16' and V > 65536 else 0.0)
+        more = 3e-6 + (torch.finfo(g.dtype).eps / 2 if fuse else 0.0)
         check_elements(g, grad_r * tau / N, at, 1.5 / N, more, 2.0 ** -60)
         g, = torch.autograd.grad(kl, x, (w * tau).to(DEV))
         check_elements(g, grad_r * (w.double() * tau)[:, None], at, 1.5, 3e-6, 2.0 ** -60)
@@ -215,3 +214,60 @@ def test_terms_of_another_type(dt, types, fuse):
         assert g.dtype == t.dtype
         torch.testing.assert_close(g.double().cpu(), torch.full((B,), want, dtype=torch.float64),
                                    rtol=torch.finfo(t.dtype).eps / 2 + 2.0 ** -22, atol=0.0)
+
+
+# ---------------------------------------------------------------------------------------------------------------------
+# gradients, element by element
+# ---------------------------------------------------------------------------------------------------------------------
+ROWS = [(5, 250), (7, 1024), (6, 5000), (3, 40000), (3, 65536), (2, 70001), (80, 98304), (66, 131072), (2, 131072), (1, 140001)]
+
+
+@pytest.mark.parametrize('dt', ['f32', 'bf16', 'f16'])
+@pytest.mark.parametrize('N,V', ROWS)
+@pytest.mark.parametrize('fuse', [True, False])
+def test_probabilities_far_below_the_largest(N, V, dt, fuse):
+    """Logits evenly spread over 70 units: probabilities down to 2^-101 of the largest, each of which has its bits in the
+    likelihood's and the distillation's gradient (d up to 101: 4e-6 more than where it ends at 64)."""
+    from vae_amd import functional as F_
+    z = (-70.0 * torch.rand(N, V, generator=gen(V))).to(TYPES[dt])
+    tok = torch.randint(0, V, (N, 1), generator=gen(1))
+    x = z.to(DEV).requires_grad_(True)
+    g, = torch.autograd.grad(F_.nll_elbo(tok.to(DEV), x[:, None], 'categorical', fuse_backward=fuse)[3][0], x)
+    p = torch.softmax(z.double(), -1)
+    at = torch.zeros(N, V, dtype=torch.bool).scatter_(1, tok, True)
+    check_elements(g, (p - at.double()) / N, at, 1.0 / N, 4e-6)
+    ids = torch.randint(0, V, (N, 3), generator=gen(2))
+    y = torch.randn(N, 3, generator=gen(3))
+    _, grad, at = ref_distill(z.double(), y.double(), ids, 1.0)
+    g, = torch.autograd.grad(F_.distill_top_logits(x, y.to(DEV), ids.to(DEV), fuse_backward=fuse)[1], x)
+    check_elements(g, grad / N, at, 1.0 / N, 4e-6)
+
+
+@pytest.mark.parametrize('dt', ['f32', 'bf16', 'f16'])
+@pytest.mark.parametrize('N,V', [(5, 250), (7, 1024), (6, 5001), (3, 40000), (2, 131072)])
+@pytest.mark.parametrize('spread', [9.0, 60.0])
+def test_log_prob_entropy_and_alternatives_gradients(N, V, dt, spread):
+    """g_j = -p_j (a + b (ln p_j + H)) and the entries.  Its error is p_j times that of the bracket: 1.2e-5 of each product in
+    it (p's own error included), and b times the entropy's 2e-5."""
+    from vae_amd import functional as F_
+    z = (-spread * torch.rand(N, V, generator=gen(V))).to(TYPES[dt])
+    tok = torch.randint(0, V, (N,), generator=gen(1))
+    a, b, c = (torch.randn(s, generator=gen(2 + i)) for i, s in enumerate([(N,), (N,), (N, 5)]))
+    x = z.to(DEV).requires_grad_(True)
+    lp, h, top, ids = F_.token_log_probs(x, tok.to(DEV), top_k=5)
+    g, = torch.autograd.grad([lp, h, top], x, [t.to(DEV) for t in (a, b, c)])
+    logp = torch.log_softmax(z.double(), -1)
+    p = logp.exp()
+    H = -(p * logp).sum(-1, keepdim=True)
+    A, b = (a.double() + c.double().sum(1))[:, None], b.double()[:, None]
+    ref = -p * (A + b * (logp + H))
+    ref[torch.arange(N), tok] += a.double()
+    ref.scatter_add_(1, ids.cpu(), c.double())
+    at = torch.zeros(N, V, dtype=torch.bool).scatter_(1, ids.cpu(), True).scatter_(1, tok[:, None], True)
+    entries = a.abs().double()[:, None] + c.abs().double().sum(1, keepdim=True)
+    tol = torch.finfo(g.dtype).eps / 2 * ref.abs() + 8e-6 * at * entries
+    tol = tol + p * (1.2e-5 * (entries + b.abs() * (logp.abs() + H)) + 2e-5 * b.abs())
+    if dt == 'f16':
+        tol = tol + 2.0 ** -25
+    off = (g.double().cpu() - ref).abs()
+    assert bool((off <= tol).all()), 'up to %g times the tolerance' % (off / tol.clamp(min=1e-300)).max()

@@ -239,15 +239,14 @@ __global__ __launch_bounds__(BT) void token_bwd_kernel(GradArgs a) {
 
 // ---------------------------------------------------------------------------------------------------------------
 // loss and gradient in one pass: a workgroup holds its row in registers, U vectors a thread, as every element's
-// exponential against the thread's own maximum: one exponential an element, the gradient is a product.
-// Bound by memory: 4096 x 131072 bf16 400 us (5.4 TB/s read + written), 430 as a distillation; 8144 x 65536 381 us (5.6);
+// exponential against the thread's own maximum: one exponential an element (AGAIN: two), the gradient is a product.
+// Bound by memory: 4096 x 131072 bf16 412 us (5.2 TB/s read + written), as a distillation too; 8144 x 65536 375 us (5.7);
 // 16384 x 16384 181 us (5.9); two passes over the logits instead 525, 584, 553 and 268.
-//   in float32: 8 registers a 16-bit vector, 4 an fp32 one;
-//   HALF (bf16 rows that do not fit so): as 2^15 e in binary16, 4 registers a vector, where the packet was.  Its 11 bits
-//         are rounded once more to the gradient's 8; e < 2^-29, a probability 2^-29 of the thread's largest, begins to
-//         lose bits.  The sum is taken before the rounding.
+// An exponential takes a register, 8 a 16-bit vector.  AGAIN: bf16 rows that do not fit so stay as their packets, 4
+// registers a vector, and the gradient forms its exponentials again: 4096 x 131072 412 us, 401 with them kept in binary16,
+// which lost bits of probabilities below 2^-29 of a thread's largest and left nothing of those below 2^-40.
 // ---------------------------------------------------------------------------------------------------------------
-template <typename T, int BT, int U, bool HALF, bool DIST>
+template <typename T, int BT, int U, bool AGAIN, bool DIST>
 __global__ __launch_bounds__(BT, 4) void token_fused_kernel(GradArgs a) {
   constexpr int VN = VecOf<T>::n;
   __shared__ struct {
@@ -297,7 +296,7 @@ __global__ __launch_bounds__(BT, 4) void token_fused_kernel(GradArgs a) {
         piece.p[u].get(v);
         mt = vec_max(v, mt);
       }
-    float e[HALF ? 1 : U][VN];
+    float e[AGAIN ? 1 : U][VN];
     float s = exp2_raw((edge - mt) * a.scale2);
 #pragma unroll
     for (int u = 0; u < U; ++u)
@@ -310,10 +309,7 @@ __global__ __launch_bounds__(BT, 4) void token_fused_kernel(GradArgs a) {
           v[i] = exp2_raw((v[i] - mt) * a.scale2);
           s += v[i];
         }
-        if constexpr (HALF) {
-#pragma unroll
-          for (int i = 0; i < VN; i += 2) piece.p[u].raw[i / 2] = pack2<f16_t>(v[i] * 32768.f, v[i + 1] * 32768.f);
-        } else {
+        if constexpr (!AGAIN) {
 #pragma unroll
           for (int i = 0; i < VN; ++i) e[u][i] = v[i];
         }
@@ -359,12 +355,11 @@ __global__ __launch_bounds__(BT, 4) void token_fused_kernel(GradArgs a) {
     for (int u = 0; u < U; ++u)
       if (piece.any(u)) {
         float v[VN];
-        if constexpr (HALF) {
-          Packet<f16_t, VN> h;
-          h.raw = piece.p[u].raw;
-          h.get(v);
+        if constexpr (AGAIN) {
+          asm volatile("" : "+v"(piece.p[u].raw));
+          piece.p[u].get(v);
 #pragma unroll
-          for (int i = 0; i < VN; ++i) v[i] *= f * (1.f / 32768.f);
+          for (int i = 0; i < VN; ++i) v[i] = A * exp2_raw((v[i] - m) * a.scale2);
         } else {
 #pragma unroll
           for (int i = 0; i < VN; ++i) v[i] = f * e[u][i];
@@ -429,10 +424,10 @@ static int bwd_type(const GradArgs& a, hipStream_t st) {
   return same_phase<T>(a) ? bwd_kind<T, VecOf<T>::n, DIST>(a, st) : bwd_kind<T, 1, DIST>(a, st);
 }
 
-template <typename T, int BT, int U, bool HALF, bool DIST>
+template <typename T, int BT, int U, bool AGAIN, bool DIST>
 static int fused_launch(GradArgs a, hipStream_t st) {
   a.nts = (int64_t)sizeof(T) * a.N * a.V >= kNtStoreMinBytes;
-  hipLaunchKernelGGL((token_fused_kernel<T, BT, U, HALF, DIST>), dim3(grid_for(a.N)), dim3(BT), 0, st, a);
+  hipLaunchKernelGGL((token_fused_kernel<T, BT, U, AGAIN, DIST>), dim3(grid_for(a.N)), dim3(BT), 0, st, a);
   return launched();
 }
 // true when the one-pass kernel takes this call: the row fits a workgroup's registers, and there are rows enough.
@@ -442,10 +437,10 @@ static bool fused_type(const GradArgs& a, hipStream_t st, int* rc) {
   if constexpr (DTypeCode<T>::value != VAE_F16) {
     constexpr int E = 64 / VecOf<T>::n, H = E / 2;   // vectors a thread: 64 or 32 elements
     const int64_t nvec = (int64_t)a.V / VecOf<T>::n;
-    // bf16 only: fp32's gradient has no bits to spare for HALF's rounding
+    // AGAIN for bf16 only: an fp32 packet is as large as its exponentials
     constexpr int most = DTypeCode<T>::value == VAE_BF16 ? 16 : E;
-    // HALF with few rows: two launches that cut the rows (64 x 131072 bf16: 19.1 us, 20.8 in one; 1 x 98000 11.1, 14.0;
-    // but 100 x 131072: 25.9, 21.7; without HALF 16 x 65536 12.2, 10.7)
+    // AGAIN with few rows: two launches that cut the rows (64 x 131072 bf16: 19.1 us, 21.4 in one; 16 x 131072 17.9, 19.3;
+    // but 100 x 131072: 25.4, 23.1; without AGAIN 16 x 65536 12.2, 10.7)
     if (!same_phase<T>(a) || nvec > 1024 * most || (a.N <= 64 && nvec > 1024 * E && most > E)) return false;
     // 32 elements a thread while 512 threads hold the row so: more waves in flight (32768 x 8192 bf16 179 us, 189 with
     // 64; 8192 x 16384 fp32 186, 213); 64 beyond, where 1024 threads of 32 wait for each other longer (8192 x 32768 bf16:
