@@ -78,6 +78,10 @@ int vae_tuning_set(const char* name, int64_t value);
 int vae_rng_next(uint64_t* cell, int64_t n, vae_stream_t stream);
 int vae_rng_reset(vae_stream_t stream);
 
+/* *id (host memory) = 0 while `stream` is not being captured, otherwise a number that its capture has alone: what one
+ * capture has prepared for a later part of itself is not to be used up by another one, whose replays are its own.  */
+int vae_capture_id(uint64_t* id, vae_stream_t stream);
+
 /* "Saw a NaN" word (replaces the per-step host check nan_check_and_break of abstract_vae.py:366-369,
  * isotropic_gaussian.py:89-90, vrnn.py:427-428, which synchronises the stream on every step).  The closing wave of
  * every kernel that finishes batch means ORs VAE_NAN_* bits into one word of `workspace` when a mean comes out NaN

@@ -271,3 +271,78 @@ def test_log_prob_entropy_and_alternatives_gradients(N, V, dt, spread):
         tol = tol + 2.0 ** -25
     off = (g.double().cpu() - ref).abs()
     assert bool((off <= tol).all()), 'up to %g times the tolerance' % (off / tol.clamp(min=1e-300)).max()
+
+
+@pytest.mark.parametrize('kind', ['nll', 'distill'])
+@pytest.mark.parametrize('dt', ['f32', 'bf16'])
+def test_forward_and_backward_in_graphs_of_their_own(kind, dt):
+    """A backward graph replayed more often than its forward graph, upstream gradient 2: the same each time, also after the
+    logits have changed and the forward graph has been replayed."""
+    from vae_amd import functional as F_
+    N, V = 12, 3000
+    x = (torch.randn(N, V, generator=gen(3)) * 2).to(TYPES[dt])
+    tok = torch.randint(0, V, (N, 1), generator=gen(4))
+    y, ids = torch.randn(N, 5, generator=gen(5)), torch.stack([torch.randperm(V, generator=gen(i))[:5] for i in range(N)])
+    td, yd, idd = tok.to(DEV), y.to(DEV), ids.to(DEV)
+
+    def loss(x):
+        if kind == 'nll':
+            return F_.token_nll_elbo(td, x[:, None], fuse_backward=True)[3][0]
+        return F_.distill_top_logits(x, yd, idd)[1]
+
+    def check(g, z):
+        if kind == 'nll':
+            at = torch.zeros(N, V, dtype=torch.bool).scatter_(1, tok, True)
+            check_elements(g, (torch.softmax(z, -1) - at.double()) * 2.0 / N, at, 2.0 / N)
+        else:
+            _, ref, at = ref_distill(z, y.double(), ids, 1.0)
+            check_elements(g, ref * 2.0 / N, at, 2.0 / N)
+
+    two = torch.full((), 2.0, device=DEV)
+    static = x.to(DEV)
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        for _ in range(2):
+            leaf = static.detach().requires_grad_(True)
+            torch.autograd.grad(loss(leaf), leaf, two)
+    torch.cuda.synchronize()
+    leaf = static.detach().requires_grad_(True)
+    forward, backward = torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(forward, stream=s):
+        value = loss(leaf)
+    with torch.cuda.graph(backward, stream=s):
+        g, = torch.autograd.grad(value, leaf, two)
+    for turn in range(3):
+        z = x.flip(1) if turn == 1 else x
+        static.copy_(z)
+        forward.replay()
+        for _ in range(3):
+            backward.replay()
+            torch.cuda.synchronize()
+            check(g, z.double())
+            g.zero_()
+            torch.cuda.synchronize()
+
+
+def test_forward_and_backward_in_one_graph_keep_the_stored_gradient():
+    """... and replays of one graph that holds both are right with an upstream gradient of 2, too."""
+    import vae_amd
+    from vae_amd import functional as F_
+    N, V = 9, 2000
+    x = torch.randn(N, V, generator=gen(3))
+    tok = torch.randint(0, V, (N, 1), generator=gen(4))
+    static, td, two = x.to(DEV), tok.to(DEV), torch.full((), 2.0, device=DEV)
+
+    def step():
+        leaf = static.detach().requires_grad_(True)
+        return torch.autograd.grad(F_.token_nll_elbo(td, leaf[:, None], fuse_backward=True)[3][0], leaf, two)[0]
+
+    replay = vae_amd.graph.capture(step)
+    at = torch.zeros(N, V, dtype=torch.bool).scatter_(1, tok, True)
+    for turn in range(4):
+        z = x.flip(1) if turn % 2 else x
+        static.copy_(z)
+        g = replay()
+        torch.cuda.synchronize()
+        check_elements(g, (torch.softmax(z.double(), -1) - at.double()) * 2.0 / N, at, 2.0 / N, 2.0 ** -24)

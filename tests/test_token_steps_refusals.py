@@ -67,3 +67,8 @@ def test_types_of_the_terms():
         assert f(P, 3, 2) == f(P, -1, 2) == _lib.VAE_ERR_ARG
         assert f(P, 3, 0) == _lib.VAE_ERR_ARG
         assert f(None, 3, 0) == f(P, 2, 0) == _lib.VAE_OK
+
+
+def test_capture_number_needs_a_place():
+    from vae_amd import _lib
+    assert _lib.load().vae_capture_id(None, None) == _lib.VAE_ERR_ARG

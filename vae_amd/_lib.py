@@ -28,6 +28,7 @@ _fp = ctypes.POINTER(ctypes.c_float)    # host array of floats
 SIGNATURES = {
     'vae_abi_version': [],
     'vae_workspace_bytes': [],
+    'vae_capture_id': [ctypes.POINTER(ctypes.c_uint64), _p],
     'vae_rng_next': [_p, _i64, _p],
     'vae_rng_reset': [_p],
     'vae_nan_flag': [_p, _i, ctypes.POINTER(ctypes.c_uint32), _p],
@@ -205,6 +206,15 @@ def launch(device, name, *args):
     rc = getattr(_lib or load(), name)(*args, _stream_handle(device))
     if rc != VAE_OK:
         _fail(name, rc)
+
+
+def capture_id(device):
+    """0, or the number of the capture that records `device`'s current stream."""
+    if device.index == _current_device() and not torch.cuda.is_current_stream_capturing():
+        return 0
+    out = ctypes.c_uint64(0)
+    launch(device, 'vae_capture_id', ctypes.byref(out))
+    return out.value
 
 
 _workspaces = {}

@@ -31,6 +31,14 @@ int vae_rng_reset(vae_stream_t stream) {
   hipLaunchKernelGGL(rng_reset_kernel, dim3(1), dim3(1), 0, (hipStream_t)stream);
   return hipGetLastError() == hipSuccess ? VAE_OK : VAE_ERR_LAUNCH;
 }
+int vae_capture_id(uint64_t* id, vae_stream_t stream) {
+  if (!id) return VAE_ERR_ARG;
+  hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+  unsigned long long number = 0;
+  if (hipStreamGetCaptureInfo((hipStream_t)stream, &status, &number) != hipSuccess) return VAE_ERR_LAUNCH;
+  *id = status == hipStreamCaptureStatusNone ? 0 : number;
+  return VAE_OK;
+}
 // counters + group partials + one partial per block x up to 8 scalars (common.hpp, grid_reduce)
 size_t vae_workspace_bytes(void) { return vae::kWorkspaceFloatsFull * sizeof(float); }
 

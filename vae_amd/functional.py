@@ -12,7 +12,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from . import _lib
-from ._lib import DTYPE_CODES, call, check_device, dtype_code, launch, ptr, stream_ptr, workspace
+from ._lib import DTYPE_CODES, call, capture_id, check_device, dtype_code, launch, ptr, stream_ptr, workspace
 
 _MASK64 = (1 << 64) - 1
 
@@ -648,18 +648,17 @@ def _check_tokens(x, recon):
 
 
 class _Stored:
-    """A gradient that the forward launch has formed, for one backward pass, which multiplies it in place: not for a pass
-    captured into a graph when the forward pass was not, since every replay would multiply it once more."""
+    """A gradient that the forward launch has formed, for one backward pass, which multiplies it in place.  Only for a pass
+    that runs as often as the forward pass does: both eager, or both in one capture.  A graph of the backward pass alone
+    would multiply it once more with every replay."""
 
     def __init__(self, grad):
         self.grad = grad
-        self.captured = grad is not None and torch.cuda.is_current_stream_capturing()
+        self.capture = 0 if grad is None else capture_id(grad.device)
 
     def take(self):
         grad, self.grad = self.grad, None
-        if grad is not None and not self.captured and torch.cuda.is_current_stream_capturing():
-            return None
-        return grad
+        return grad if grad is not None and capture_id(grad.device) == self.capture else None
 
 
 class _TokenNllElbo(torch.autograd.Function):
