@@ -72,3 +72,20 @@ def test_types_of_the_terms():
 def test_capture_number_needs_a_place():
     from vae_amd import _lib
     assert _lib.load().vae_capture_id(None, None) == _lib.VAE_ERR_ARG
+
+
+def test_scratch_is_what_the_library_asks_for():
+    """The binding knows no limits of its own: rows that the kernels would cut get the bytes that they ask for."""
+    from vae_amd import _lib
+    lib = _lib.load()
+    cut = 0
+    for dtype in (torch.float32, torch.bfloat16, torch.float16):
+        for N in (1, 2, 64, 255, 256, 257, 4096):
+            for V in (1, 1000, 32767, 32768, 65535, 65536, 65543, 131071, 131072, 1 << 20):
+                for k in (0, 5, 64):
+                    want = lib.vae_token_scratch_bytes(N, V, min(k, V), _lib.DTYPE_CODES[dtype])
+                    got = F_._token_scratch(torch.empty((N, V), dtype=dtype, device='meta'), min(k, V), 'meta')
+                    assert (0 if got is None else got.numel()) == want
+                    cut += want > 0
+    assert cut > 50
+    assert F_._teacher_floats(10, 7) == lib.vae_distill_teacher_floats(10, 7)

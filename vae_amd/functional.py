@@ -541,11 +541,14 @@ def _scratch_bytes(N, V, top_k, code):
     return _lib.load().vae_token_scratch_bytes(N, V, top_k, code)
 
 
+@functools.lru_cache(maxsize=256)
+def _teacher_floats(N, K):
+    return _lib.load().vae_distill_teacher_floats(N, K)
+
+
 def _token_scratch(rows, top_k, dev):
-    """The pieces of split rows (256 at most, of at least 8192 16-byte vectors: csrc/token.hip): the caller's own
-    memory each call, so that calls on several streams and captured graphs share nothing."""
-    if rows.shape[0] > 256 or rows.shape[1] < 32768:
-        return None
+    """The pieces of split rows (csrc/token.hip says which are): the caller's own memory each call, so that calls on several
+    streams and captured graphs share nothing."""
     n = _scratch_bytes(rows.shape[0], rows.shape[1], top_k, dtype_code(rows))
     return torch.empty((n,), dtype=torch.uint8, device=dev) if n else None
 
@@ -818,7 +821,7 @@ class _Distill(torch.autograd.Function):
             N, V = rows.shape
             grad = torch.empty(logits.shape, dtype=logits.dtype, device=dev)
             at = buf.data_ptr()
-            launch(dev, 'vae_distill_bwd', ptr(rows), rows.stride(0), at, K, temperature, at + 4 * N * (1 + 3 * K),
+            launch(dev, 'vae_distill_bwd', ptr(rows), rows.stride(0), at, K, temperature, at + 4 * _teacher_floats(N, K),
                    ptr(gkl), ptr(gmean), inv_count, ptr(grad), N, V, dtype_code(rows))
         return grad, None, None, None, None, None
 
@@ -829,14 +832,15 @@ def _distill_fwd(logits, t_logits, t_ids, temperature, inv_count, fuse):
     (N, V), K = rows.shape, t_ids.shape[1]
     kl = torch.empty(logits.shape[:-1], dtype=torch.float32, device=dev)
     mean = torch.empty((), dtype=torch.float32, device=dev)
-    # the teacher's side (vae_distill_teacher_floats) and behind it the statistics [N, 2]: the backward's
-    buf = torch.empty((N * (3 + 3 * K),), dtype=torch.float32, device=dev)
+    # the teacher's side and behind it the statistics [N, 2]: the backward's
+    floats = _teacher_floats(N, K)
+    buf = torch.empty((floats + 2 * N,), dtype=torch.float32, device=dev)
     at = buf.data_ptr()
     grad = torch.empty(logits.shape, dtype=logits.dtype, device=dev) if fuse else None
     scratch = _token_scratch(rows, 0, dev)
     launch(dev, 'vae_distill_fwd', ptr(rows), rows.stride(0), ptr(t_logits), t_logits.stride(0), dtype_code(t_logits),
            ptr(t_ids), t_ids.stride(0), t_ids.element_size(), K, temperature, at, ptr(kl), ptr(mean), inv_count,
-           at + 4 * N * (1 + 3 * K), ptr(grad), ptr(scratch), N, V, dtype_code(rows))
+           at + 4 * floats, ptr(grad), ptr(scratch), N, V, dtype_code(rows))
     return kl, mean, grad, buf
 
 
