@@ -202,7 +202,8 @@ template <typename T, int BT, typename Emit>
 __device__ __forceinline__ void row_top(TopLds<BT>& lds, const T* __restrict__ x, const RowCut<T, VecOf<T>::n>& cut,
                                         int v0, int v1, float edge, int edge_index, float mine, int k, Emit emit) {
   constexpr int VN = VecOf<T>::n;
-  // value bits that tell two numbers of the type apart (fp32: enough of them)
+  // How far the bound is worked out: sign, exponent and 7 bits of the fraction tell two bf16 numbers apart; fp16 (10 bits)
+  // and fp32 may find a bound a little lower and with it a few more candidates
   constexpr int kLastBit = sizeof(T) == 2 ? 48 : 40;
   const Buffer body(x + cut.head, cut.nvec * kVecBytes);
   const int tid = threadIdx.x;
