@@ -145,34 +145,34 @@ constexpr long long kNtStoreMinBytes = VAE_NT_STORE_MIN_BYTES;
 __device__ __forceinline__ bool nt_stores(int64_t tensor_bytes) { return tensor_bytes >= kNtStoreMinBytes; }
 
 template <typename T, int V, bool NT = (VAE_NT_LOAD != 0)>
-__device__ __forceinline__ void load_vec(const T* __restrict__ p, float (&out)[V]) {
-  if constexpr (V == 1) {
-    out[0] = to_f32(p[0]);
-  } else {
-    typedef typename PackOf<T, V>::type P;
-    P raw;
-    if constexpr (NT) {
-      raw = __builtin_nontemporal_load(reinterpret_cast<const P*>(p));
-    } else {
-      raw = *reinterpret_cast<const P*>(p);
+__device__ __forceinline__ typename PackOf<T, V>::type load_pack(const T* __restrict__ p) {
+  typedef typename PackOf<T, V>::type P;
+  if constexpr (NT) return __builtin_nontemporal_load(reinterpret_cast<const P*>(p));
+  else return *reinterpret_cast<const P*>(p);
+}
+template <typename T, int V>
+__device__ __forceinline__ void unpack(typename PackOf<T, V>::type raw, float (&out)[V]) {
+  if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) out[i] = raw[i];
+  } else if constexpr (DTypeCode<T>::value == 2) {
+#pragma unroll
+    for (int i = 0; i < V / 2; ++i) {
+      out[2 * i] = (float)__builtin_bit_cast(_Float16, (uint16_t)(raw[i] & 0xffffu));
+      out[2 * i + 1] = (float)__builtin_bit_cast(_Float16, (uint16_t)(raw[i] >> 16));
     }
-    if constexpr (sizeof(T) == 4) {
+  } else {
 #pragma unroll
-      for (int i = 0; i < V; ++i) out[i] = raw[i];
-    } else if constexpr (DTypeCode<T>::value == 2) {
-#pragma unroll
-      for (int i = 0; i < V / 2; ++i) {
-        out[2 * i] = (float)__builtin_bit_cast(_Float16, (uint16_t)(raw[i] & 0xffffu));
-        out[2 * i + 1] = (float)__builtin_bit_cast(_Float16, (uint16_t)(raw[i] >> 16));
-      }
-    } else {
-#pragma unroll
-      for (int i = 0; i < V / 2; ++i) {
-        out[2 * i] = __uint_as_float(raw[i] << 16);
-        out[2 * i + 1] = __uint_as_float(raw[i] & 0xffff0000u);
-      }
+    for (int i = 0; i < V / 2; ++i) {
+      out[2 * i] = __uint_as_float(raw[i] << 16);
+      out[2 * i + 1] = __uint_as_float(raw[i] & 0xffff0000u);
     }
   }
+}
+template <typename T, int V, bool NT = (VAE_NT_LOAD != 0)>
+__device__ __forceinline__ void load_vec(const T* __restrict__ p, float (&out)[V]) {
+  if constexpr (V == 1) out[0] = to_f32(p[0]);
+  else unpack<T, V>(load_pack<T, V, NT>(p), out);
 }
 
 template <typename T, int V>

@@ -62,12 +62,30 @@ __global__ __launch_bounds__(kBlock) void nll_elbo_fwd_kernel(
         if (mi) m = to_f32(mi[row]);
       }
       for (int j0 = sub; j0 < nvec; j0 += G * U) {
+        // 16-bit Bernoulli: the packets wait as they are, 8 registers a pair of vectors and not 16, and are worked off
+        // one after the other; otherwise four pairs take 96 registers (B = 65536, D = 784 bf16: 52 us, occupancy 5)
+        constexpr bool kLate = NLL == VAE_NLL_BERNOULLI && sizeof(T) == 2 && V > 1;
         float xv[U][V], a[U][V], b[U][V];
-        load_chunk<T, V, U, kNtNllFwd>(xr, j0, G, nvec, xv);
-        load_chunk<T, V, U, kNtNllFwd>(rr, j0, G, nvec, a);
-        if constexpr (NLL != VAE_NLL_BERNOULLI) load_chunk<T, V, U, kNtNllFwd>(rr + D, j0, G, nvec, b);
+        typename PackOf<T, kLate ? V : VecOf<T>::n>::type xp[kLate ? U : 1], ap[kLate ? U : 1];
+        if constexpr (kLate) {
+#pragma unroll
+          for (int u = 0; u < U; ++u) {
+            const int j = j0 + u * G < nvec ? j0 + u * G : nvec - 1;
+            xp[u] = load_pack<T, V, kNtNllFwd>(xr + (int64_t)j * V);
+            ap[u] = load_pack<T, V, kNtNllFwd>(rr + (int64_t)j * V);
+          }
+        } else {
+          load_chunk<T, V, U, kNtNllFwd>(xr, j0, G, nvec, xv);
+          load_chunk<T, V, U, kNtNllFwd>(rr, j0, G, nvec, a);
+          if constexpr (NLL != VAE_NLL_BERNOULLI) load_chunk<T, V, U, kNtNllFwd>(rr + D, j0, G, nvec, b);
+        }
 #pragma unroll
         for (int u = 0; u < U; ++u) {
+          if constexpr (kLate) {
+            __builtin_amdgcn_sched_barrier(0);
+            unpack<T, V>(xp[u], xv[u]);
+            unpack<T, V>(ap[u], a[u]);
+          }
           float su = 0.f;
 #pragma unroll
           for (int i = 0; i < V; ++i) {
