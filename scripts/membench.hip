@@ -1,5 +1,5 @@
 // Streaming-ceiling probe for the hot path's byte mixes (tuning aid, not part of the library):
-//   hipcc -O3 --offload-arch=gfx950 scripts/membench.hip -o scripts/membench && scripts/membench
+//   hipcc -O3 --offload-arch=gfx950 -Xclang -target-feature -Xclang -packed-fp32-ops scripts/membench.hip -o scripts/membench && scripts/membench
 // Flat 16-B-per-lane kernels with R read streams and W write streams over buffers that rotate through
 // NSETS > 256 MiB of distinct memory, so the Infinity Cache never holds a pass's data (what the kernels of a
 // training step see).  Prints TB/s per variant: the rate a row kernel with the same mix can hope for.

@@ -3,7 +3,7 @@
 # A kernel with ScratchSize > 0 spills or indexes a private array dynamically: none should.   scripts/resource_scan.sh > profiles/rNN/kernel_resources.txt
 cd "$(dirname "$0")/../vae_amd/csrc" || exit 1
 for f in *.hip; do
-  /opt/rocm/bin/hipcc -O3 -std=c++17 --offload-arch=gfx950 -fno-gpu-rdc --cuda-device-only -c $f -o /dev/null \
+  /opt/rocm/bin/hipcc -O3 -std=c++17 --offload-arch=gfx950 -fno-gpu-rdc -Xclang -target-feature -Xclang -packed-fp32-ops --cuda-device-only -c $f -o /dev/null \
       -Rpass-analysis=kernel-resource-usage 2>&1 | python3 -c "
 import sys, re, subprocess
 name = None; res = {}
