@@ -67,10 +67,10 @@ __device__ __forceinline__ void gamma_small(float x, float& lg_nolog, float& P, 
   }
 }
 
-// gamma_small<LG, PSI, false> on TWO arguments at once, laid out for the packed-fp32 pipe (v_pk_fma_f32 /
-// v_pk_mul_f32 / v_pk_add_f32: two values per lane and instruction).  The forward KL is arithmetic-bound (r03:
-// ~110 full-rate + 14 quarter-rate instructions per element pair, 152 us where the bytes need 88): the polynomials are
-// two thirds of it and pack perfectly; the reciprocals and logs stay one per value.
+// gamma_small<LG, PSI, false> on TWO arguments at once: two independent chains for every instruction's latency.  The
+// forward KL is arithmetic-bound (B = 65536, L = 512: 147-154 us where the bytes need 88): the polynomials are two thirds of
+// it.  The build has no packed-FP32 instructions, which the pairs were laid out for and which took it to 137-145 us, so a
+// pair costs what two elements cost; the reciprocals and logs were one per value either way.
 typedef float f32x2 __attribute__((ext_vector_type(2)));
 __device__ __forceinline__ f32x2 rcp2(f32x2 v) { return f32x2{fast_rcp(v[0]), fast_rcp(v[1])}; }
 __device__ __forceinline__ f32x2 ln2_(f32x2 v) { return f32x2{log2_raw(v[0]), log2_raw(v[1])} * kLn2; }
@@ -84,7 +84,7 @@ __device__ __forceinline__ void gamma_small2(f32x2 x, f32x2& lg_nolog, f32x2& P,
   const f32x2 d1 = ((((6.0f * x + 75.0f) * x + 340.0f) * x + 675.0f) * x + 548.0f) * x + 120.0f;
   psi = ly - 0.5f * i - i2 * (1.0f / 12.0f - i2 * (1.0f / 120.0f - i2 * (1.0f / 252.0f))) - d1 * iP;
 }
-// The KL of TWO elements (a1[e], a0[e]), e = 0, 1, against the fixed prior Beta(b, b): three packed evaluations --
+// The KL of TWO elements (a1[e], a0[e]), e = 0, 1, against the fixed prior Beta(b, b): three evaluations of pairs --
 // {a1[0], a0[0]}, {a1[1], a0[1]}, {sp[0], sp[1]} -- where beta_kl_elem_small makes six scalar ones.  Returns
 // kl[0] + kl[1] (the caller sums over the row anyway).
 __device__ __forceinline__ float beta_kl_pair_small(float a1x, float a0x, float a1y, float a0y, float b, float lgq) {

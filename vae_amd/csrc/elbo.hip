@@ -248,7 +248,7 @@ __global__ __launch_bounds__(kBlock) void nll_elbo_fused_kernel(
   for (int64_t t = blockIdx.x; t < tiles; t += gridDim.x) {
     const int64_t row = t * rpb + rloc;
     float s = 0.f;
-    f32x2 s2 = {0.f, 0.f};   // Bernoulli: the packed pair of partial sums (nll_bern_value_grad)
+    f32x2 s2 = {0.f, 0.f};   // Bernoulli: a pair of partial sums (nll_bern_value_grad)
     // the [B] inputs of the row epilogue, requested with the row itself (behind the row sum they were a dependent
     // round trip with nothing else of the wave in flight)
     float k = 0.f, ad = 0.f, m = 0.f;

@@ -715,8 +715,8 @@ static void bn_colstats_launch(int NJ, int grid, hipStream_t st, const T* x, con
   // vectors of the 16-bit types (their registers hold twice the floats: NJ * R = 8 spilled 64-112 bytes per lane to
   // scratch there, -Rpass-analysis=kernel-resource-usage, r03)
   constexpr int R2 = V >= 8 ? 2 : 4;
-  // four 8-element vectors per lane do not fit either (the compiler pairs the 32 shift constants for packed
-  // arithmetic and parks them in scratch): wide 16-bit rows take windows of two vectors per lane instead
+  // four 8-element vectors per lane do not fit either (32 shift constants beside them): wide 16-bit rows take windows of
+  // two vectors per lane instead
   constexpr int NJW = V >= 8 ? 2 : 4;
   if (NJ == 1)
     hipLaunchKernelGGL((bn_colstats_kernel<T, V, 1, 4>), dim3(grid), dim3(kBlock), 0, st, x, gy, gld, mean, rstd, part,

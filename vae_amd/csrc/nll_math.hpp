@@ -30,11 +30,11 @@ __device__ __forceinline__ float nll_bern(float x, float l) {
 }
 __device__ __forceinline__ float nll_bern_grad(float x, float l) { return fast_rcp(1.0f + __expf(-l)) - x; }
 
-// Value AND gradient of V elements (V even), for the one-pass kernels.  At 2 bytes per element those are no longer
-// HBM-bound but co-bound by VALU issue (r03: 406 instructions per wave, ~25 per element), so the arithmetic is laid
-// out for the packed-fp32 pipe (v_pk_add / v_pk_mul / v_pk_fma_f32: two elements per lane and instruction):
+// Value AND gradient of V elements (V even), for the one-pass kernels.  At 2 bytes per element those are co-bound by VALU
+// issue, so the two share what they can, and two elements go side by side (the build has no packed-FP32 instructions: a
+// pair is two ordinary ones):
 //   e = exp(-|l|), p = 1 + e, r = 1/p, pos = [sign bit of l clear], d = pos - x
-//   value    = max(l,0) - l x + log1p(e) = l d + ln2 log2(p)                         (two packed fma into the sum)
+//   value    = max(l,0) - l x + log1p(e) = l d + ln2 log2(p)                         (two fma into the sum)
 //   gradient = sigmoid(l) - x            = d - copysign(e r, l)    (l >= 0: (1 - x) - e r; l < 0: e r - x: no
 //                                                                   cancellation at x = 1, as before)
 // One exponential serves both; `pos` and the copysign both read the SIGN BIT of l, so l = -0.0 is consistent
@@ -57,8 +57,7 @@ __device__ __forceinline__ void nll_bern_value_grad(const float (&x)[V], const f
   for (int i = 0; i + 1 < V; i += 2) {
     const f32x2 lv = {l[i], l[i + 1]}, xv = {x[i], x[i + 1]};
     // (element-wise on the scalars, not through lv[k]: hipcc 7.2 folded `bit_cast<int>(lv[k]) < 0` of both halves
-    // into the compare of the LOW half -- op_sel_hi:[0,1] on the packed subtract -- and every odd element took its
-    // neighbour's sign)
+    // into the compare of the LOW half, and every odd element took its neighbour's sign)
     const float p0 = __builtin_bit_cast(int, l[i]) < 0 ? 0.0f : 1.0f;
     const float p1 = __builtin_bit_cast(int, l[i + 1]) < 0 ? 0.0f : 1.0f;
     const f32x2 pos = {p0, p1};

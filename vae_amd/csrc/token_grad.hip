@@ -241,7 +241,9 @@ __global__ __launch_bounds__(BT) void token_bwd_kernel(GradArgs a) {
 // loss and gradient in one pass: a workgroup holds its row in registers, U vectors a thread, as every element's
 // exponential against the thread's own maximum: one exponential an element (AGAIN: two), the gradient is a product.
 // Bound by memory: 4096 x 131072 bf16 412 us (5.2 TB/s read + written), as a distillation too; 8144 x 65536 375 us (5.7);
-// 16384 x 16384 181 us (5.9); two passes over the logits instead 525, 584, 553 and 268.
+// 16384 x 16384 181 us (5.9); two passes instead 525 (584 as a distillation), 553 and 268.  fp32: 4096 x
+// 32768 192 us (5.6), 4096 x 65536 404 us (5.3), though 64 exponentials a thread beside the packets spill 60 bytes a lane (104
+// with a teacher, 221 and 424 us; bf16 with a teacher 12 and 40).
 // An exponential takes a register, 8 a 16-bit vector.  AGAIN: bf16 rows that do not fit so stay as their packets, 4
 // registers a vector, and the gradient forms its exponentials again: 4096 x 131072 412 us, 401 with them kept in binary16,
 // which lost bits of probabilities below 2^-29 of a thread's largest and left nothing of those below 2^-40.
