@@ -535,7 +535,8 @@ int vae_grad_scale(void* buf, const float* factor, int64_t n, int dtype, vae_str
 /* Distillation from a teacher's K <= VAE_MAX_TEACHER largest logits per row, both sides at `temperature` > 0:
  * q = softmax(t_logits / temperature) over the entries that are there (id >= 0 and logit > -inf), p = softmax(logits /
  * temperature) over V,  kl[r] = sum_k q_k (ln q_k - ln p[id_k]).  An id may come more than once.  No entry there: kl 0,
- * gradient 0, the row's logits are not read.  An id >= V: NaN, nothing is read out of range.
+ * gradient 0, the row's logits are not read.  An id >= V: NaN, nothing is read out of range; a teacher logit of NaN or
+ * +inf: NaN.
  * t_logits [N, K] in t_dtype and t_ids [N, K], rows t_stride / id_stride apart.  teacher: vae_distill_teacher_floats(N, K)
  * floats that the call fills (the teacher's softmax, each id once) and the backward reads.  mean (may be NULL):
  * mean_scale * sum of kl.  stats [N, 2] for the backward (may be NULL without glogits); glogits [N, V] != NULL: also

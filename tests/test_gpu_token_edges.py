@@ -346,3 +346,27 @@ def test_forward_and_backward_in_one_graph_keep_the_stored_gradient():
         g = replay()
         torch.cuda.synchronize()
         check_elements(g, (torch.softmax(z.double(), -1) - at.double()) * 2.0 / N, at, 2.0 / N, 2.0 ** -24)
+
+
+@pytest.mark.parametrize('dt,V', [('f32', 50), ('bf16', 9000), ('f16', 9000), ('bf16', 70000), ('f32', 70001)])
+@pytest.mark.parametrize('fuse', [True, False])
+def test_a_teacher_without_a_distribution_makes_its_row_nan(dt, V, fuse):
+    """NaN or +inf among the teacher's logits: kl and the whole row's gradient, (sum q) p - q, are NaN; the other rows are
+    what they are without it."""
+    from vae_amd import functional as F_
+    N = 5
+    z = torch.randn(N, V, generator=gen(V)).to(TYPES[dt])
+    ids = torch.stack([torch.randperm(V, generator=gen(i))[:4] for i in range(N)])
+    y = torch.randn(N, 4, generator=gen(1))
+    kl_r, grad_r, at = ref_distill(z.double(), y.double(), ids, 1.0)
+    y[1, 2] = float('nan')
+    y[3, 0] = float('inf')
+    bad, fine = [1, 3], [0, 2, 4]
+    x = z.to(DEV).requires_grad_(True)
+    kl, mean = F_.distill_top_logits(x, y.to(DEV), ids.to(DEV), fuse_backward=fuse)
+    assert bool(kl[bad].isnan().all()) and bool(mean.isnan())
+    torch.testing.assert_close(kl[fine].detach().double().cpu(), kl_r[fine], rtol=1e-6, atol=2e-5)
+    for out, up, scale in ((mean, torch.ones(()), 1.0 / N), (kl, torch.ones(N), 1.0)):
+        g, = torch.autograd.grad(out, x, up.to(DEV), retain_graph=True)
+        assert bool(g[bad].isnan().all())
+        check_elements(g[fine], grad_r[fine] * scale, at[fine], scale)

@@ -211,7 +211,7 @@ __device__ __forceinline__ float vec_max(const float (&v)[VN], float m) {
 
 // The teacher's entries as prepare_teacher (token_teacher.hip) leaves them: per row a state, and K entries of
 // id (-1: none), q and ln q; entries of one id are merged into the first of them.
-enum { kRowFine = 0, kRowEmpty = 1, kRowBad = 2 };  // nothing there | an id beyond the vocabulary
+enum { kRowFine = 0, kRowEmpty = 1, kRowBad = 2 };  // nothing there | an id beyond the vocabulary, a NaN or +inf logit
 struct Teacher {
   const int* state;       // [N]
   const int* id;          // [N, K]

@@ -53,7 +53,7 @@ __global__ __launch_bounds__(kBlock) void distill_teacher_kernel(const void* __r
 #pragma unroll
     for (int r = 0; r < R; ++r) {
       q[r] = id[r] >= 0 ? exp2_raw((y[r] - m) * scale2) : 0.f;
-      if (q[r] == 0.f) id[r] = -1;   // NaN keeps its id: the row comes out NaN
+      if (q[r] == 0.f) id[r] = -1;
       s += q[r];
     }
     s = group_sum(s, 64);
@@ -130,7 +130,7 @@ __global__ __launch_bounds__(kBlock) void distill_teacher_kernel(const void* __r
       q_out[row * K + k] = q[r];
       logq_out[row * K + k] = logq[r];
     }
-    const bool any_bad = __ballot(bad) != 0;
+    const bool any_bad = __ballot(bad) != 0 || s != s;   // NaN or +inf among the teacher's: no distribution either
     if (lane == 0) state[row] = any_bad ? kRowBad : (s == 0.f ? kRowEmpty : kRowFine);
   }
 }

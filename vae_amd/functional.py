@@ -852,7 +852,8 @@ def distill_top_logits(logits, teacher_logits, teacher_ids, temperature=1.0, inv
     loss is to be weighted so).  Differentiable with respect to `logits` only.
 
     A negative id or a teacher logit of -inf is no entry; a row without entries has kl 0 and gradient 0 and its logits
-    are not read; an id may come twice; an id beyond the vocabulary gives NaN.  `fuse_backward`: d(mean)/d(logits) is
+    are not read; an id may come twice; an id beyond the vocabulary, a teacher logit of NaN or +inf give NaN (kl and the
+    row's gradient).  `fuse_backward`: d(mean)/d(logits) is
     formed by the forward launch (one read of the logits per step instead of two); a gradient on `kl` takes the general
     kernel."""
     _check_vocab(logits, 'distill_top_logits')
