@@ -57,7 +57,8 @@ struct Terms {
 template <typename T, int BT>
 __global__ __launch_bounds__(BT) void token_elbo_fwd_kernel(
     const float* __restrict__ logp, int64_t len, Terms terms, float kl_beta, float inv_count, T* __restrict__ nll,
-    T* __restrict__ loss, T* __restrict__ elbo, float* __restrict__ means, MeansTo to, float* __restrict__ ws, int64_t B, int G) {
+    T* __restrict__ loss, T* __restrict__ elbo, float* __restrict__ means, MeansTo to, float* __restrict__ ws, int64_t B,
+    int G) {
   __shared__ float part[BT / 64][6];
   const int rpb = BT / G, sub = threadIdx.x % G, rloc = threadIdx.x / G;
   float acc[6] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
